@@ -524,6 +524,117 @@ int mtp_apply_logit_deltas(float* logits, long long ld, int rows, int V, const i
  * it to pin the lane layout the kernels assume). */
 int mtp_probe_mfma_layout(float* out, void* stream);
 
+/* ---- rotary positions -----------------------------------------------------
+ * Rows q [T, Hq, D] and k [T, Hkv, D] (k NULL with Hkv = 0: q alone) bf16,
+ * strides in elements, rotated at positions[t] into q_out / k_out:
+ *   y1 = gain (x1 cos a - x2 sin a), y2 = gain (x1 sin a + x2 cos a)
+ * over the first `dims` (even) elements of each head, in pairs (i, i + dims/2)
+ * or, traditional = 1, (2i, 2i + 1); the rest is copied. table[i] (uint64,
+ * dims/2 of them) is pair i's frequency in revolutions per position times
+ * 2^64: position * table[i] mod 2^64 is exact for every int32 position.
+ * The outputs may be the inputs unless traditional = 0 and dims % 16 != 0.
+ * D a multiple of 8 up to 256; bases 16-byte aligned, strides multiples of 8.
+ * (mx.fast.rope's dims / traditional / offset; tests/test_ragged_kv_cache.py:62-100
+ * of the reference calls it with per-row offsets.) */
+typedef struct mtp_rotary_args {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  const int32_t* positions; /* [T] */
+  const void* table;        /* uint64 [dims/2] */
+  int T, Hq, Hkv, D, dims, traditional;
+  float gain;
+  long long q_token, q_head, k_token, k_head, qo_token, qo_head, ko_token, ko_head;
+} mtp_rotary_args;
+int mtp_rotary(const mtp_rotary_args* args, void* stream);
+
+/* ---- paged KV cache ---------------------------------------------------------
+ * A pool of num_pages pages of page_size keys (a multiple of 32) for Hkv heads
+ * of D (64, 128, 256): k_pages / v_pages [num_pages][Hkv][page_size / 32]
+ * [32 * D] bf16 (bits = 16) or int8 (bits = 8) in the order in which the
+ * attention loads its operands; with 8 bits k_scales / v_scales
+ * [num_pages][Hkv][page_size] fp32. Request b's positions [i * page_size,
+ * (i + 1) * page_size) are in page block_table[b * width + i]; an entry
+ * outside [0, num_pages) is no page. Packed tokens: request b's are rows
+ * [row_off[b], row_off[b + 1]) (row_off NULL: T / B each), the first at
+ * position q_start[b]. Rows of no request are neither read nor written.
+ * `status` (int32 [1], may be NULL) gets bit 0 set where a position has no
+ * page; that row is skipped. Device arrays are never trusted with an access:
+ * row offsets are clamped to [0, T], pages to the pool.
+ *
+ * 8 bits, per token and head: A = max |x|, scale = A / 127,
+ * q = rint(x * (127 / A)) in fp32; a row below 2^-100 is zeros, one with a NaN
+ * or an infinity gets a NaN scale and reads as NaN.
+ *
+ * mtp_paged_write: k, v [T, Hkv, D] into the pages; dims > 0 rotates k at its
+ * positions first (as mtp_rotary, rounded to bf16), and q, if given, into
+ * q_out. max_rows (rows of the longest request, 0 unknown) sizes the grid only.
+ * Two tokens of one call must not share a slot.
+ * mtp_paged_read: positions [start[b], start[b] + count) (start NULL: 0) into
+ * k_out, v_out [B, Hkv, count, D] bf16; positions at or past lengths[b]
+ * (lengths NULL: none) and those without a page read as zeros, the latter set
+ * the status.
+ * mtp_paged_attn: q, out [T, Hq, D]; out = softmax(scale q k^T) v over
+ * positions 0 .. own; a row that sees no key is zeros. max_rows as above,
+ * it chooses the kernel (at most 32 query rows per kv head and request, or
+ * more) and not the result's meaning. A row's result depends on no key behind
+ * its own position, whatever its page holds. Hq = 1 to 32 times Hkv. */
+typedef struct mtp_paged_write_args {
+  const void* k;
+  const void* v;
+  const void* q;     /* may be NULL */
+  void* q_out;
+  const void* table; /* rotation table, as mtp_rotary_args */
+  void* k_pages;
+  void* v_pages;
+  void* k_scales;
+  void* v_scales;
+  const int32_t* block_table; /* [B, width] */
+  const int32_t* q_start;     /* [B] */
+  const int32_t* row_off;     /* [B + 1] or NULL */
+  int32_t* status;
+  int T, B, width, Hq, Hkv, D, page_size, num_pages, bits, dims, traditional, max_rows;
+  float gain;
+  long long k_token, k_head, v_token, v_head, q_token, q_head, qo_token, qo_head;
+} mtp_paged_write_args;
+int mtp_paged_write(const mtp_paged_write_args* args, void* stream);
+
+typedef struct mtp_paged_read_args {
+  const void* k_pages;
+  const void* v_pages;
+  const void* k_scales;
+  const void* v_scales;
+  const int32_t* block_table;
+  const int32_t* start;
+  const int32_t* lengths;
+  void* k_out;
+  void* v_out;
+  int32_t* status;
+  int B, width, count, Hkv, D, page_size, num_pages, bits;
+} mtp_paged_read_args;
+int mtp_paged_read(const mtp_paged_read_args* args, void* stream);
+
+typedef struct mtp_paged_attn_args {
+  const void* q;
+  void* out;
+  const void* k_pages;
+  const void* v_pages;
+  const void* k_scales;
+  const void* v_scales;
+  const int32_t* block_table;
+  const int32_t* q_start;
+  const int32_t* row_off;
+  int32_t* status;
+  void* ws;
+  size_t ws_bytes;
+  int T, B, width, Hq, Hkv, D, page_size, num_pages, bits, max_rows;
+  float scale;
+  long long q_token, q_head, out_token, out_head;
+} mtp_paged_attn_args;
+size_t mtp_paged_attn_workspace_bytes(int Hq, int Hkv, int D, int max_rows);
+int mtp_paged_attn(const mtp_paged_attn_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -79,6 +79,11 @@ SIGNATURES = {
     "mtp_attn_vt_workspace_bytes": (_sz, [_i, _i, _i]),
     "mtp_ragged_gqa_attn_rows_vt": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _vp, _sz, _vp]),
     "mtp_rope_qkv_to_cache_vt": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _vp, _vp]),
+    "mtp_rotary": (_i, [_vp, _vp]),
+    "mtp_paged_write": (_i, [_vp, _vp]),
+    "mtp_paged_read": (_i, [_vp, _vp]),
+    "mtp_paged_attn_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "mtp_paged_attn": (_i, [_vp, _vp]),
 }
 
 
@@ -142,6 +147,28 @@ class AttnBlocksArgs(C.Structure):
 def attn_blocks(stream, **fields) -> None:
     """Call ``mtp_ragged_gqa_attn_blocks``; tensor fields may be torch tensors or None."""
     call("mtp_ragged_gqa_attn_blocks", C.byref(_fill(AttnBlocksArgs(), fields)), stream)
+
+
+def _block(name: str, doc: str, *groups):
+    """An argument block: groups of (ctypes type, field names)."""
+    return type(name, (C.Structure,), {"__doc__": doc, "_fields_": [(n, t) for t, ns in groups for n in ns.split()]})
+
+
+_ll = C.c_longlong
+RotaryArgs = _block("RotaryArgs", "``mtp_rotary_args`` of include/mtplx_amd.h (same field order).",
+                    (_vp, "q k q_out k_out positions table"), (_i, "T Hq Hkv D dims traditional"), (_f, "gain"),
+                    (_ll, "q_token q_head k_token k_head qo_token qo_head ko_token ko_head"))
+PagedWriteArgs = _block("PagedWriteArgs", "``mtp_paged_write_args`` (same field order).",
+                        (_vp, "k v q q_out table k_pages v_pages k_scales v_scales block_table q_start row_off status"),
+                        (_i, "T B width Hq Hkv D page_size num_pages bits dims traditional max_rows"), (_f, "gain"),
+                        (_ll, "k_token k_head v_token v_head q_token q_head qo_token qo_head"))
+PagedReadArgs = _block("PagedReadArgs", "``mtp_paged_read_args`` (same field order).",
+                       (_vp, "k_pages v_pages k_scales v_scales block_table start lengths k_out v_out status"),
+                       (_i, "B width count Hkv D page_size num_pages bits"))
+PagedAttnArgs = _block("PagedAttnArgs", "``mtp_paged_attn_args`` (same field order).",
+                       (_vp, "q out k_pages v_pages k_scales v_scales block_table q_start row_off status ws"),
+                       (_sz, "ws_bytes"), (_i, "T B width Hq Hkv D page_size num_pages bits max_rows"), (_f, "scale"),
+                       (_ll, "q_token q_head out_token out_head"))
 
 
 class MtpError(RuntimeError):

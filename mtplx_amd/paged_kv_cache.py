@@ -1,0 +1,193 @@
+"""A paged KV cache on gfx950, in 16 or 8 bits.
+
+The reference's ragged cache (``mtplx/ragged_kv_cache.py:71``,
+:class:`mtplx_amd.ragged_kv_cache.RaggedBatchKVCache` here) holds one padded
+buffer for a batch. This one holds a pool of pages; a request's keys are in
+the pages that its row of a block table names, so requests of any length come
+and go without copies and may share the pages of a common prefix. Which page
+belongs to whom is the caller's: the cache stores, it does not allocate.
+
+Pages lie in the order in which :func:`mtplx_amd.paged_attention.paged_sdpa`
+loads them (``include/mtplx_amd.h``); :meth:`PagedKVCache.read` gives rows
+back in the reference's ``[B, Hkv, count, D]``.
+
+With ``bits=8`` each token's row of each head is stored as int8 and one fp32
+scale (``scale = max|x| / 127``, values rounded to nearest even): 0.52 of the
+bytes at head dim 128. The largest error of a value is half a step,
+``max|x| / 254``.
+"""
+
+from __future__ import annotations
+
+from typing import Any
+
+import torch
+
+from . import _lib
+from .rotary import RotaryTable, _call, _int32, _readable, _rows, _same_device, _writable, _overlaps
+
+__all__ = ["PagedKVCache"]
+
+
+class PagedKVCache:
+    """``num_pages`` pages of ``page_size`` keys for ``n_kv_heads`` heads."""
+
+    def __init__(self, num_pages: int, n_kv_heads: int, head_dim: int, *, page_size: int = 64, bits: int = 16,
+                 device: Any = "cuda") -> None:
+        if num_pages < 1 or n_kv_heads < 1:
+            raise ValueError(f"need at least one page and one kv head (got {num_pages}, {n_kv_heads})")
+        if head_dim not in (64, 128, 256):
+            raise ValueError(f"head_dim must be 64, 128 or 256 (got {head_dim})")
+        if page_size < 32 or page_size % 32:
+            raise ValueError(f"page_size must be a positive multiple of 32 (got {page_size})")
+        if bits not in (8, 16):
+            raise ValueError(f"bits must be 8 or 16 (got {bits})")
+        self.num_pages, self.n_kv_heads, self.head_dim = int(num_pages), int(n_kv_heads), int(head_dim)
+        self.page_size, self.bits = int(page_size), int(bits)
+        shape = (self.num_pages, self.n_kv_heads, self.page_size // 32, 32 * self.head_dim)
+        dtype = torch.int8 if bits == 8 else torch.bfloat16
+        self.k_pages = torch.zeros(shape, dtype=dtype, device=device)
+        self.v_pages = torch.zeros_like(self.k_pages)
+        self.k_scales = self.v_scales = None
+        if bits == 8:
+            self.k_scales = torch.zeros(shape[:2] + (self.page_size,), dtype=torch.float32, device=device)
+            self.v_scales = torch.zeros_like(self.k_scales)
+        self._status = torch.zeros(1, dtype=torch.int32, device=device)
+
+    @property
+    def device(self) -> torch.device:
+        return self.k_pages.device
+
+    @property
+    def nbytes(self) -> int:
+        held = (self.k_pages, self.v_pages, self.k_scales, self.v_scales)
+        return sum(t.numel() * t.element_size() for t in held if t is not None)
+
+    def status(self) -> torch.Tensor:
+        """Device status word (int32 [1]): nonzero once a call met a position
+        that the block table has no page for (its row was skipped)."""
+        return self._status
+
+    def check_status(self) -> None:
+        """Raise :class:`MtpError` if a call since the last check met a position
+        without a page (synchronises with the device)."""
+        if int(self._status.item()) != 0:
+            self._status.zero_()
+            raise _lib.MtpError("paged_kv_cache", -1, "a position without a page of the pool (status word set)")
+
+    # -- shared by the calls over this cache --------------------------------------
+    def _pages(self, block) -> None:
+        block.k_pages, block.v_pages = self.k_pages.data_ptr(), self.v_pages.data_ptr()
+        if self.bits == 8:
+            block.k_scales, block.v_scales = self.k_scales.data_ptr(), self.v_scales.data_ptr()
+        block.status = self._status.data_ptr()
+        block.Hkv, block.D, block.page_size = self.n_kv_heads, self.head_dim, self.page_size
+        block.num_pages, block.bits = self.num_pages, self.bits
+
+    def _table(self, block_table: Any) -> torch.Tensor:
+        t = _int32("block_table", block_table, self.device)
+        if t.dim() != 2 or t.shape[0] < 1 or t.shape[1] < 1:
+            raise ValueError(f"block_table must be [requests, pages] (got {list(t.shape)})")
+        if t.shape[1] * self.page_size > 0x7fffffff:
+            raise ValueError("block_table covers more than 2^31 - 1 positions")
+        return t
+
+    def _requests(self, tokens: int, B: int, q_start: Any, row_off: Any):
+        start = _int32("q_start", q_start, self.device, B)
+        if row_off is None:
+            if tokens % B:
+                raise ValueError(f"{tokens} tokens are no whole rows of {B} requests: give row_off")
+            return start, None
+        return start, _int32("row_off", row_off, self.device, B + 1)
+
+    # -- writes and reads ------------------------------------------------------------
+    def write(self, keys: torch.Tensor, values: torch.Tensor, block_table: Any, q_start: Any, row_off: Any = None, *,
+              max_rows: int | None = None, queries: torch.Tensor | None = None, rotary: RotaryTable | None = None,
+              out: torch.Tensor | None = None) -> torch.Tensor | None:
+        """Store the new tokens' ``keys`` / ``values`` [T, Hkv, D] bf16.
+
+        Request b's tokens are rows ``[row_off[b], row_off[b+1])`` (``row_off``
+        None: ``T / B`` each) at positions ``q_start[b]`` on, in the pages of
+        ``block_table[b]`` (int32 ``[B, pages]``, -1 where there is none). All
+        three may stay on the GPU. Rows past ``row_off[B]`` belong to nobody: they
+        are not stored, nor written in the returned tensor (undefined there).
+        ``max_rows``: the longest request's rows, if the caller knows (a hint
+        that sizes the launch). With ``rotary`` keys are rotated at their
+        positions on the way, and ``queries`` [T, Hq, D] into the returned
+        tensor (or ``out``), as :func:`apply_rotary` would. Without ``rotary``
+        ``queries`` has no meaning and is refused.
+
+        Two tokens of one call must not share a slot. A position without a
+        page is skipped and sets :meth:`status`."""
+        D, H = self.head_dim, self.n_kv_heads
+        k, v = _rows("keys", keys, H, D), _rows("values", values, H, D)
+        T = k.shape[0]
+        if v.shape[0] != T:
+            raise ValueError(f"keys have {T} tokens, values {v.shape[0]}")
+        if queries is not None and rotary is None:
+            raise ValueError("queries are taken to be rotated: give rotary with them")
+        if rotary is not None and rotary.dims > D:
+            raise ValueError(f"the rotary table's {rotary.dims} dims exceed the head dim {D}")
+        table = self._table(block_table)
+        B = table.shape[0]
+        start, off = self._requests(T, B, q_start, row_off)
+        _same_device(self.device, keys=k, values=v, queries=queries,
+                     rotary=None if rotary is None else rotary.phases)
+        q = qo = None
+        if queries is not None:
+            q = _rows("queries", queries, None, D)
+            if q.shape[0] != T:
+                raise ValueError(f"keys have {T} tokens, queries {q.shape[0]}")
+            if out is None:
+                qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            else:
+                qo = _writable("out", out, queries)
+                for name, x in (("keys", k), ("values", v)):
+                    if _overlaps(qo, x) and not _beside(qo, x):
+                        raise ValueError(f"out overlaps {name}")
+                if _overlaps(qo, q):
+                    same = qo.data_ptr() == q.data_ptr() and qo.stride() == q.stride()
+                    if not same or not (rotary.traditional or rotary.dims % 16 == 0):
+                        q = q.clone(memory_format=torch.contiguous_format)
+        if T == 0:
+            return qo
+        a = _lib.PagedWriteArgs(k=k.data_ptr(), v=v.data_ptr(), block_table=table.data_ptr(),
+                                q_start=start.data_ptr(), row_off=_lib.ptr(off), T=T, B=B, width=table.shape[1],
+                                max_rows=max(0, int(max_rows or 0)), k_token=k.stride(0), k_head=k.stride(1),
+                                v_token=v.stride(0), v_head=v.stride(1))
+        self._pages(a)
+        if rotary is not None:
+            a.table, a.dims, a.gain = rotary.phases.data_ptr(), rotary.dims, rotary.gain
+            a.traditional = int(rotary.traditional)
+        if q is not None and q.shape[1]:
+            a.q, a.q_out, a.Hq = q.data_ptr(), qo.data_ptr(), q.shape[1]
+            a.q_token, a.q_head, a.qo_token, a.qo_head = q.stride(0), q.stride(1), qo.stride(0), qo.stride(1)
+        _call("mtp_paged_write", a, self.device)
+        return qo
+
+    def read(self, block_table: Any, count: int, *, start: Any = None, lengths: Any = None):
+        """``(keys, values)`` bf16 ``[B, Hkv, count, D]`` of positions
+        ``start[b]`` (None: 0) on. Positions at or past ``lengths[b]`` (None:
+        all are live) read as zeros and touch no page; live positions without a
+        page read as zeros and set :meth:`status`."""
+        table = self._table(block_table)
+        B, count = table.shape[0], int(count)
+        if count < 0:
+            raise ValueError(f"count must not be negative (got {count})")
+        first = None if start is None else _int32("start", start, self.device, B)
+        ends = None if lengths is None else _int32("lengths", lengths, self.device, B)
+        shape = (B, self.n_kv_heads, count, self.head_dim)
+        k = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+        v = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+        if count:
+            a = _lib.PagedReadArgs(block_table=table.data_ptr(), start=_lib.ptr(first), lengths=_lib.ptr(ends),
+                                   k_out=k.data_ptr(), v_out=v.data_ptr(), B=B, width=table.shape[1], count=count)
+            self._pages(a)
+            _call("mtp_paged_read", a, self.device)
+        return k, v
+
+
+def _beside(a: torch.Tensor, b: torch.Tensor) -> bool:
+    from .rotary import _interleaved
+
+    return _interleaved(a, b)

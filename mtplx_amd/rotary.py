@@ -1,0 +1,245 @@
+"""Rotary positions on gfx950: pairs half a rotation apart or side by side,
+the whole head or part of it, frequencies as trained or scaled for longer
+contexts.
+
+The reference rotates with ``mx.fast.rope`` (``dims``, ``traditional``, a base
+and per-row offsets, ``tests/test_ragged_kv_cache.py:62-100``); here the
+frequencies are a table made once (:func:`rotary_table`) and any packed
+tokens are rotated at their own positions in one launch
+(:func:`apply_rotary`). ``PagedKVCache.write`` takes the same table and
+rotates on the way into the cache.
+
+For pair i of position p, with angle ``a = p f_i``::
+
+    y1 = gain (x1 cos a - x2 sin a)      y2 = gain (x1 sin a + x2 cos a)
+
+in fp32, rounded once to bf16. The angle is reduced exactly (64-bit
+fixed-point revolutions), so far positions are as precise as near ones.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from dataclasses import dataclass
+from typing import Any, Sequence
+
+import torch
+
+from . import _lib
+
+__all__ = ["RotaryTable", "rotary_table", "apply_rotary"]
+
+
+@dataclass(frozen=True)
+class RotaryTable:
+    """Frequencies of ``dims / 2`` pairs: ``frequencies`` in radians per
+    position (host, float64), ``phases`` the same as revolutions times 2^64
+    (device, the bits of a uint64), ``gain`` the factor of the rotated values."""
+
+    dims: int
+    traditional: bool
+    gain: float
+    frequencies: tuple
+    phases: torch.Tensor
+
+
+def rotary_frequencies(dims: int, *, base: float = 10000.0, scale: float = 1.0, scaling: str | None = None,
+                       factor: float = 1.0, trained_positions: int = 0, fast_turns: float = 32.0,
+                       slow_turns: float = 1.0) -> tuple[list[float], float]:
+    """``(radians per position of each pair, gain)``.
+
+    ``f_i = scale base^(-2 i / dims)``; ``scale`` below 1 squeezes positions
+    evenly (``mx.fast.rope``'s ``scale``). ``scaling``:
+
+    * ``"ntk"``: the base grows by ``factor^(dims / (dims - 2))``, so the
+      slowest pair turns ``factor`` times slower and the fastest as before;
+    * ``"yarn"``: pairs that make more than ``fast_turns`` turns over
+      ``trained_positions`` stay, those below ``slow_turns`` turn ``factor``
+      times slower, the pairs between are blended linearly in their index;
+      the gain is ``0.1 ln(factor) + 1``.
+    """
+    if dims < 2 or dims % 2:
+        raise ValueError(f"dims must be even and positive (got {dims})")
+    for name, value in (("base", base), ("scale", scale), ("factor", factor)):
+        if not (math.isfinite(value) and value > 0.0):
+            raise ValueError(f"{name} must be positive and finite (got {value})")
+    if scaling not in (None, "ntk", "yarn"):
+        raise ValueError(f"scaling must be None, 'ntk' or 'yarn' (got {scaling!r})")
+    if scaling is None and factor != 1.0:
+        raise ValueError("factor belongs to a scaling ('ntk' or 'yarn'); use scale to squeeze positions evenly")
+    if scaling == "ntk":
+        if dims == 2:
+            raise ValueError("ntk scaling needs more than one pair")
+        base = base * factor ** (dims / (dims - 2))
+    freqs = [scale * base ** (-2.0 * i / dims) for i in range(dims // 2)]
+    if scaling != "yarn":
+        return freqs, 1.0
+    if trained_positions < 1 or not fast_turns > slow_turns > 0.0 or base <= 1.0 or factor < 1.0:
+        raise ValueError("yarn scaling needs trained_positions >= 1, fast_turns > slow_turns > 0, base > 1 and "
+                         "factor >= 1")
+
+    def pair_of(turns: float) -> float:   # index (in dims / 2 pairs) of the pair that makes so many turns
+        return dims * math.log(trained_positions / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
+
+    low, high = max(math.floor(pair_of(fast_turns)), 0), min(math.ceil(pair_of(slow_turns)), dims - 1)
+    for i, f in enumerate(freqs):
+        ramp = min(max((i - low) / max(high - low, 0.001), 0.0), 1.0)
+        freqs[i] = f * (1.0 - ramp) + f / factor * ramp
+    return freqs, 0.1 * math.log(factor) + 1.0
+
+
+def rotary_table(dims: int, *, base: float = 10000.0, traditional: bool = False, scale: float = 1.0,
+                 scaling: str | None = None, factor: float = 1.0, trained_positions: int = 0,
+                 fast_turns: float = 32.0, slow_turns: float = 1.0, frequencies: Sequence[float] | None = None,
+                 gain: float | None = None, device: Any = "cuda") -> RotaryTable:
+    """The frequencies of :func:`rotary_frequencies`, or ``frequencies`` as
+    given (radians per position, ``dims / 2`` of them, at most pi each), on
+    ``device``. ``gain`` replaces the scaling's own."""
+    if frequencies is None:
+        freqs, own_gain = rotary_frequencies(dims, base=base, scale=scale, scaling=scaling, factor=factor,
+                                             trained_positions=trained_positions, fast_turns=fast_turns,
+                                             slow_turns=slow_turns)
+    else:
+        if dims < 2 or dims % 2:
+            raise ValueError(f"dims must be even and positive (got {dims})")
+        freqs, own_gain = [float(f) for f in frequencies], 1.0
+        if len(freqs) != dims // 2:
+            raise ValueError(f"expected {dims // 2} frequencies for dims={dims}, got {len(freqs)}")
+    if dims > 256:
+        raise ValueError(f"dims={dims} exceeds the largest head dim (256)")
+    if not all(math.isfinite(f) and 0.0 <= f <= math.pi for f in freqs):
+        raise ValueError("frequencies must lie in [0, pi] radians per position")
+    gain = own_gain if gain is None else float(gain)
+    if not math.isfinite(gain):
+        raise ValueError("gain must be finite")
+    # At most half a revolution each: the fixed-point value stays below 2^63.
+    fixed = [min(round(f / (2.0 * math.pi) * 2.0 ** 64), 2 ** 63 - 1) for f in freqs]
+    return RotaryTable(int(dims), bool(traditional), gain, tuple(freqs),
+                       torch.tensor(fixed, dtype=torch.int64).to(device))
+
+
+def _rows(name: str, x: torch.Tensor, heads: int | None = None, dim: int | None = None) -> torch.Tensor:
+    """``x`` [T, H, D] bf16 on the GPU as the kernels read it: 16-byte aligned
+    rows, strides of whole 16 bytes (other views are copied)."""
+    if not x.is_cuda:
+        raise RuntimeError(f"{name}: the paged operators run on the GPU only")
+    if x.dtype != torch.bfloat16:
+        raise TypeError(f"{name} must be bfloat16 (got {x.dtype})")
+    if x.dim() != 3 or (heads is not None and x.shape[1] != heads) or (dim is not None and x.shape[2] != dim):
+        raise ValueError(f"{name} must be [tokens, {heads or 'heads'}, {dim or 'dim'}] (got {list(x.shape)})")
+    return x if _readable(x) else x.clone(memory_format=torch.contiguous_format)
+
+
+def _readable(x: torch.Tensor) -> bool:
+    t, h, d = x.stride()
+    return d == 1 and t >= 0 and t % 8 == 0 and h % 8 == 0 and h >= x.shape[2] and x.data_ptr() % 16 == 0
+
+
+def _writable(name: str, out: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
+    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
+        raise ValueError(f"{name} must be {list(like.shape)} {like.dtype} on {like.device}")
+    if not _readable(out) or out.stride(0) < out.stride(1) * (out.shape[1] - 1) + out.shape[2]:
+        raise ValueError(f"{name} must have 16-byte aligned rows that do not overlap")
+    return out
+
+
+def _int32(name: str, value: Any, device, numel: int | None = None) -> torch.Tensor:
+    t = value if isinstance(value, torch.Tensor) else torch.as_tensor(value)
+    if t.dtype != torch.int32 or t.device != device:
+        t = t.to(device=device, dtype=torch.int32)
+    t = t.contiguous()
+    if numel is not None and t.numel() != numel:
+        raise ValueError(f"{name} must hold {numel} values (got {t.numel()})")
+    return t
+
+
+def _same_device(device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, the call's other tensors on {device}")
+
+
+def _call(name: str, block: ctypes.Structure, device) -> None:
+    """Run an argument-block entry point on ``device``'s current stream (the
+    kernels of a call go to the current HIP device)."""
+    if torch.cuda.current_device() == device.index:
+        _lib.call(name, ctypes.byref(block), _lib.stream_handle(device))
+        return
+    with torch.cuda.device(device):
+        _lib.call(name, ctypes.byref(block), _lib.stream_handle(device))
+
+
+def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
+    if a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr():
+        return False
+
+    def span(x):
+        lo = x.storage_offset()
+        return lo, lo + sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1
+
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def apply_rotary(table: RotaryTable, queries: torch.Tensor, keys: torch.Tensor | None, positions: Any, *,
+                 out: tuple | None = None):
+    """Rotate ``queries`` [T, Hq, D] and ``keys`` [T, Hkv, D] (or None) bf16 at
+    ``positions`` [T] (int32; may stay on the GPU). Returns ``(queries, keys)``
+    rotated, in new tensors or in ``out`` (a pair; the inputs themselves for in
+    place). Views of a fused projection are read where they are."""
+    q = _rows("queries", queries)
+    T, Hq, D = q.shape
+    device = q.device
+    k = None if keys is None else _rows("keys", keys, None, D)
+    if k is not None and k.shape[0] != T:
+        raise ValueError(f"queries have {T} tokens, keys {k.shape[0]}")
+    if D % 8 or D > 256 or table.dims > D:
+        raise ValueError(f"head dim {D} must be a multiple of 8 up to 256 and hold the table's {table.dims} dims")
+    pos = _int32("positions", positions, device, T)
+    _same_device(device, keys=k, table=table.phases)
+    if out is None:
+        qo = torch.empty((T, Hq, D), dtype=q.dtype, device=device)
+        ko = None if k is None else torch.empty((T, k.shape[1], D), dtype=q.dtype, device=device)
+    else:
+        qo = _writable("out[0]", out[0], queries)
+        ko = None if k is None else _writable("out[1]", out[1], keys)
+        # The kernel reads a row's parts where it writes them only as far as
+        # the very same view goes.
+        exact = table.traditional or table.dims % 16 == 0
+        for dst in (qo, ko):
+            if dst is None:
+                continue
+            for src in (q, k):
+                if src is not None and _overlaps(dst, src):
+                    same = exact and dst.data_ptr() == src.data_ptr() and dst.stride() == src.stride() \
+                        and dst.shape == src.shape
+                    if not same:
+                        if src is q:
+                            q = q.clone(memory_format=torch.contiguous_format)
+                        else:
+                            k = k.clone(memory_format=torch.contiguous_format)
+        if ko is not None and _overlaps(qo, ko) and not _interleaved(qo, ko):
+            raise ValueError("the two outputs overlap")
+    if T == 0 or Hq == 0:
+        return qo, ko
+    a = _lib.RotaryArgs(q=q.data_ptr(), q_out=qo.data_ptr(), positions=pos.data_ptr(), table=table.phases.data_ptr(),
+                        T=T, Hq=Hq, D=D, dims=table.dims, traditional=int(table.traditional), gain=table.gain,
+                        q_token=q.stride(0), q_head=q.stride(1), qo_token=qo.stride(0), qo_head=qo.stride(1))
+    if k is not None and k.shape[1]:
+        a.k, a.k_out, a.Hkv = k.data_ptr(), ko.data_ptr(), k.shape[1]
+        a.k_token, a.k_head, a.ko_token, a.ko_head = k.stride(0), k.stride(1), ko.stride(0), ko.stride(1)
+    _call("mtp_rotary", a, device)
+    return qo, ko
+
+
+def _interleaved(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two views of one buffer of rows lie side by side in each row
+    (the parts of a fused projection): equal token strides, disjoint columns."""
+    if a.stride(0) != b.stride(0) or a.stride(0) <= 0:
+        return False
+    wide = a.stride(0)
+    (a0, an), (b0, bn) = ((x.storage_offset(), (x.shape[1] - 1) * x.stride(1) + x.shape[2]) for x in (a, b))
+    first, n, second = (a0, an, b0) if a0 <= b0 else (b0, bn, a0)
+    gap = second - first
+    return gap < wide and n <= gap and gap + (bn if first == a0 else an) <= wide
