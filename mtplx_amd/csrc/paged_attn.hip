@@ -27,6 +27,7 @@
 // workgroup, and attn_join adds them in the line's order. The split depends on
 // lengths alone, so results do not depend on timing.
 #include "paged.hpp"
+#include "qmv_common.hpp"
 
 namespace mtp {
 
@@ -47,6 +48,7 @@ struct PAttn {
   int32_t* status;
   float* part_o;    // [2 G][rows of a tile][D]
   float* part_ml;   // [2 G][rows of a tile][2]
+  int4* begun;      // [G]: the tile that workgroup g began and others finish
   int T, B, width, Hq, Hkv, rep, bpp, num_pages;
   int P;            // tokens of a row tile
   int G;            // most workgroups
@@ -82,64 +84,87 @@ __device__ __forceinline__ long long head_len(const PAttn& p, long long start, i
 }
 
 __device__ __forceinline__ long long shfl64(long long v, int src) { return __shfl(v, src, 64); }
-
-// Total length of the line, and the request that holds line position x (by
-// scans of 64 requests at a time; every wave for itself).
-__device__ __forceinline__ long long line_total(const PAttn& p, int lane) {
-  long long sum = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
-    long long v = 0;
-    const int b = b0 + lane;
-    if (b < p.B) v = p.Hkv * head_len(p, p.q_start[b], req_rows(p.row_off, b, p.B, p.T).n);
-    sum += v;
-  }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-  return sum;
+__device__ __forceinline__ long long uniform64(long long v) {
+  const unsigned lo = __builtin_amdgcn_readfirstlane((int)v), hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
+  return (long long)((unsigned long long)hi << 32 | lo);
 }
 
-__device__ __forceinline__ int find_req(const PAttn& p, int lane, long long x, Req& r) {
-  long long carry = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
-    const int b = b0 + lane;
-    long long len = 0, start = 0;
-    ReqRows rr = {0, 0};
-    if (b < p.B) {
-      rr = req_rows(p.row_off, b, p.B, p.T);
-      start = p.q_start[b];
-      len = head_len(p, start, rr.n);
-    }
-    long long incl = p.Hkv * len;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const long long t = __shfl_up(incl, off, 64);
-      if (lane >= off) incl += t;
-    }
-    const unsigned long long m = __ballot(len > 0 && x < carry + incl);   // the first whose end lies behind x
-    if (m) {
-      const int src = __ffsll((long long)m) - 1;
-      r.lo = __builtin_amdgcn_readfirstlane(__shfl(rr.lo, src, 64));
-      r.n = __builtin_amdgcn_readfirstlane(__shfl(rr.n, src, 64));
-      r.start = shfl64(start, src);
-      r.head = shfl64(len, src);
-      r.base = carry + shfl64(incl, src) - p.Hkv * r.head;
-      return __builtin_amdgcn_readfirstlane(b0 + src);
-    }
-    carry += shfl64(incl, 63);
-  }
-  return -1;
+// a / b for a quotient below 2^31 (and a, b below 2^52), by one fp64 division
+// instead of the integer one's long sequence.
+__device__ __forceinline__ int div_small(long long a, long long b) {
+  int q = (int)((double)a / (double)b);
+  if ((long long)q * b > a) --q;
+  if ((long long)(q + 1) * b <= a) ++q;
+  return q;
 }
 
-// Shares of the line: workgroup g of G takes [lo(g), lo(g + 1)).
-struct Shares {
-  long long W;
+// A lane's request of the line (64 requests at a time), its rows and length.
+struct LaneReq {
+  ReqRows rows;
+  long long start, len;   // len: one head
+};
+__device__ __forceinline__ LaneReq lane_req(const PAttn& p, int b) {
+  LaneReq r = {{0, 0}, 0, 0};
+  if (b < p.B) {
+    r.rows = req_rows(p.row_off, b, p.B, p.T);
+    r.start = p.q_start[b];
+    r.len = head_len(p, r.start, r.rows.n);
+  }
+  return r;
+}
+__device__ __forceinline__ long long scan64(long long v, int lane) {
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const long long t = __shfl_up(v, off, 64);
+    if (lane >= off) v += t;
+  }
+  return v;
+}
+
+// The line as a wave sees it: its total length W, cut into G shares of S; of
+// up to 64 requests the lanes keep their own.
+struct Line {
+  LaneReq mine;
+  long long incl;   // line position where the lane's request ends
+  long long W, S;
   int G;
-  __device__ Shares(long long W_, int most, int min_share) : W(W_) {
-    const long long n = W_ / min_share;
-    G = n < 1 ? 1 : n < most ? (int)n : most;
+  __device__ __forceinline__ Line(const PAttn& p, int lane) {
+    mine = lane_req(p, lane);
+    incl = scan64(p.Hkv * mine.len, lane);
+    W = shfl64(incl, 63);
+    for (int b0 = 64; b0 < p.B; b0 += 64) W += shfl64(scan64(p.Hkv * lane_req(p, b0 + lane).len, lane), 63);
+    W = uniform64(W);
+    // Equal shares, a whole number of steps each, no shorter than min_share.
+    const long long s = (long long)ceil((double)W / (double)p.G);
+    S = (s > p.min_share ? (s + kStep - 1) / kStep : p.min_share / kStep) * kStep;
+    G = W > 0 ? div_small(W - 1, S) + 1 : 0;
   }
-  __device__ long long lo(int g) const { return (long long)g * W / G; }
-  __device__ int owner(long long x) const { return (int)(((x + 1) * G - 1) / W); }
+  static constexpr int kStep = 64;
+  __device__ __forceinline__ long long lo(int g) const { return g * S; }
+  __device__ __forceinline__ long long hi(int g) const { return g + 1 < G ? (g + 1) * S : W; }
+  __device__ __forceinline__ int owner(long long x) const { return div_small(x, S); }
+  // The request that holds line position x.
+  __device__ __forceinline__ int find(const PAttn& p, int lane, long long x, Req& r) const {
+    LaneReq q = mine;
+    long long end = incl, carry = 0;
+    for (int b0 = 0;;) {
+      const unsigned long long m = __ballot(q.len > 0 && x < carry + end);   // the first whose end lies behind x
+      if (m) {
+        const int src = __ffsll((long long)m) - 1;
+        r.lo = __builtin_amdgcn_readfirstlane(__shfl(q.rows.lo, src, 64));
+        r.n = __builtin_amdgcn_readfirstlane(__shfl(q.rows.n, src, 64));
+        r.start = uniform64(shfl64(q.start, src));
+        r.head = uniform64(shfl64(q.len, src));
+        r.base = uniform64(carry + shfl64(end, src)) - p.Hkv * r.head;
+        return __builtin_amdgcn_readfirstlane(b0 + src);
+      }
+      carry += shfl64(end, 63);
+      b0 += 64;
+      if (b0 >= p.B) return -1;   // (not reached: x < W)
+      q = lane_req(p, b0 + lane);
+      end = scan64(p.Hkv * q.len, lane);
+    }
+  }
 };
 
 // One row tile of one head: where it lies on the line and what it is.
@@ -153,7 +178,7 @@ struct Tile {
 __device__ __forceinline__ Tile tile_at(const PAttn& p, const Req& r, long long x) {
   Tile u;
   const long long y = x - r.base;
-  u.h = (int)(y / r.head);
+  u.h = div_small(y, r.head);
   const long long z = y - u.h * r.head;
   const long long q0 = clamp_start(p, r.start);
   int a = 0, b = (r.n + p.P - 1) / p.P - 1;   // the last tile that begins at or before z
@@ -196,8 +221,8 @@ struct RowState {
   int bound[NB];   // last key that the lane's row sees; -1: no row here
 };
 
-// Keys (bit k: key kt + k) of a 16-bit V block with a NaN or an infinity in
-// any element; the same in every lane.
+// Keys (bit k: key k of the block) of a 16-bit V block with a NaN or an
+// infinity in any element; the same in every lane.
 template <int D, class VO>
 __device__ __forceinline__ uint32_t odd_keys(VO vop, int h2) {
   // An exponent of all ones plus one carries into the sign's place, half by half.
@@ -219,35 +244,67 @@ __device__ __forceinline__ uint32_t odd_keys(VO vop, int h2) {
   return __builtin_amdgcn_readfirstlane((int)keys);
 }
 
-// kop(i), vop(t, jj): operands (bf16, the latter as their 16 bytes); ks(r), vs(r): scales of the lane's key of
-// score register r (8 bits), ks already times scale_log2. Keys kt..kt+31.
-template <int D, int BITS, int NB, bool MASK, class KO, class VO, class KS, class VS>
-__device__ __forceinline__ void attend(RowState<D, NB>& s, int kt, int h2, float scale_log2, KO kop, VO vop, KS ks,
-                                       VS vs) {
-  f32x16 st[NB];
+// KB blocks of 32 keys from kt on. kop(j, i), vop(j, t, jj): block j's operands
+// (as 16 bytes of bf16); ks(j, r), vs(j, r): scales of the lane's key of score
+// register r (8 bits), ks already times scale_log2. MASK: rows see keys up to
+// their bound, none at or past end;
+// what lies there in V is no number.
+// AHEAD: the operands come from LDS; a phase's are all asked for before it
+// begins, V's before the softmax (left to itself, the compiler reads each right
+// before the product that waits for it).
+template <int D, int BITS, int NB, int KB, bool MASK, bool AHEAD, class KO, class VO, class KS, class VS>
+__device__ __forceinline__ void attend(RowState<D, NB>& s, int kt, int end, int h2, float scale_log2,
+                                       KO kop, VO vop, KS ks, VS vs) {
+  f32x16 st[KB][NB];
+  u32x4 ka[KB][D / 16], va[KB][D / 16];
+  if (AHEAD) {
 #pragma unroll
-  for (int n = 0; n < NB; ++n) st[n] = f32x16{};
+    for (int j = 0; j < KB; ++j)
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i) {
-    const bf16x8 k = kop(i);
-#pragma unroll
-    for (int n = 0; n < NB; ++n) st[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, s.q[n][i], st[n], 0, 0, 0);
+      for (int i = 0; i < D / 16; ++i) ka[j][i] = kop(j, i);
+    __builtin_amdgcn_sched_barrier(0);
   }
-  bf16x8 w[NB][2];
+#pragma unroll
+  for (int j = 0; j < KB; ++j) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n) st[j][n] = f32x16{};
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      const bf16x8 k = __builtin_bit_cast(bf16x8, AHEAD ? ka[j][i] : kop(j, i));
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+        st[j][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, s.q[n][i], st[j][n], 0, 0, 0);
+    }
+  }
+  if (AHEAD) {
+#pragma unroll
+    for (int j = 0; j < KB; ++j)
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) va[j][i] = vop(j, i >> 1, i & 1);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  u32x4 w[KB][NB][2];
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
-    float x[16];
+    // 16 bits without a mask: the maximum is taken before the scale (positive),
+    // and scale and maximum go into one FMA.
+    constexpr bool RAW = BITS == 16 && !MASK;
     float top = -INFINITY;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      x[r] = BITS == 8 ? st[n][r] * ks(r) : st[n][r] * scale_log2;
-      if (MASK) {
-        const int key = kt + 8 * (r >> 2) + 4 * h2 + (r & 3);
-        x[r] = key <= s.bound[n] ? x[r] : -INFINITY;
+    for (int j = 0; j < KB; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float x = st[j][n][r];
+        if (!RAW) x *= BITS == 8 ? ks(j, r) : scale_log2;
+        if (MASK) {
+          const int key = kt + 32 * j + 8 * (r >> 2) + 4 * h2 + (r & 3);
+          x = key <= s.bound[n] && key < end ? x : -INFINITY;
+        }
+        st[j][n][r] = x;
+        top = __builtin_elementwise_maximum(top, x);   // (no quieting of each x; a NaN makes its row NaN)
       }
-      top = fmaxf(top, x[r]);
-    }
     top = max_halves(top);
+    if (RAW) top *= scale_log2;
     if (__any(top > s.m[n] + 8.f)) {
       // Only the rows that passed: the others' bits do not turn on their neighbours.
       const float m_new = top > s.m[n] + 8.f ? top : s.m[n];
@@ -261,69 +318,110 @@ __device__ __forceinline__ void attend(RowState<D, NB>& s, int kt, int h2, float
     }
     const float m = s.m[n] == -INFINITY ? 0.f : s.m[n];
     float sum = 0.f;
-    uint32_t pk[8];
 #pragma unroll
-    for (int r = 0; r < 16; r += 2) {
-      float a = exp2_fast(x[r] - m), b = exp2_fast(x[r + 1] - m);
-      sum += a + b;
-      if (BITS == 8) {
-        const float va = vs(r), vb = vs(r + 1);
-        a = MASK && a == 0.f ? 0.f : a * va;   // a hidden key's scale may be NaN
-        b = MASK && b == 0.f ? 0.f : b * vb;
+    for (int j = 0; j < KB; ++j) {
+      uint32_t pk[8];
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        auto weight = [&](int rr) {
+          const float x = st[j][n][rr];
+          return exp2_fast(RAW ? __fmaf_rn(x, scale_log2, -m) : x - m);
+        };
+        float a = weight(r), b = weight(r + 1);
+        sum += a + b;
+        if (BITS == 8) {
+          const float va = vs(j, r), vb = vs(j, r + 1);
+          a = MASK && a == 0.f ? 0.f : a * va;   // a hidden key's scale may be NaN
+          b = MASK && b == 0.f ? 0.f : b * vb;
+        }
+        pk[r / 2] = f2bf2(a, b);
       }
-      pk[r / 2] = f2bf2(a, b);
+      w[j][n][0] = u32x4{pk[0], pk[1], pk[2], pk[3]};
+      w[j][n][1] = u32x4{pk[4], pk[5], pk[6], pk[7]};
     }
     s.l[n] += sum;
-#pragma unroll
-    for (int jj = 0; jj < 2; ++jj)
-      w[n][jj] = __builtin_bit_cast(bf16x8, u32x4{pk[4 * jj], pk[4 * jj + 1], pk[4 * jj + 2], pk[4 * jj + 3]});
   }
-  // A hidden key's weight is 0, but 0 times a NaN or an infinity in its value is
-  // not: in blocks with hidden keys (MASK), keys whose values are not all
-  // finite leave the product and are added one by one, to the rows that see them.
-  // (8-bit values are integers; their scale went into the weight.)
-  u32x4 keep0 = {}, keep1 = {};
-  uint32_t odd = 0;
-  if (MASK && BITS == 16) {
-    odd = odd_keys<D>(vop, h2);
-    auto word = [&](int jj, int i) {
-      return (odd >> (16 * jj + v_slot_key(h2, 2 * i)) & 1 ? 0u : 0x0000ffffu) |
-             (odd >> (16 * jj + v_slot_key(h2, 2 * i + 1)) & 1 ? 0u : 0xffff0000u);
-    };
-    keep0 = u32x4{word(0, 0), word(0, 1), word(0, 2), word(0, 3)};
-    keep1 = u32x4{word(1, 0), word(1, 1), word(1, 2), word(1, 3)};
-  }
+  __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-  for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-    for (int jj = 0; jj < 2; ++jj) {
-      u32x4 v = vop(t, jj);
-      if (MASK && BITS == 16) v &= jj ? keep1 : keep0;
-#pragma unroll
-      for (int n = 0; n < NB; ++n)
-        s.o[n][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v), w[n][jj], s.o[n][t], 0, 0, 0);
+  for (int j = 0; j < KB; ++j) {
+    // A hidden key's weight is 0, but 0 times a NaN or an infinity in its value
+    // is not: in blocks with hidden keys (MASK), keys whose values are not all
+    // finite leave the product and are added one by one, to the rows that see
+    // them. (8-bit values are integers; their scale went into the weight.)
+    u32x4 keep0 = {}, keep1 = {};
+    uint32_t odd = 0;
+    auto vj = [&](int t, int jj) { return AHEAD ? va[j][2 * t + jj] : vop(j, t, jj); };
+    if (MASK && BITS == 16) {
+      const int n = end - kt - 32 * j;   // keys that exist
+      const uint32_t have = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+      odd = odd_keys<D>(vj, h2) & have;
+      const uint32_t in = have & ~odd;
+      auto word = [&](int jj, int i) {
+        return (in >> (16 * jj + v_slot_key(h2, 2 * i)) & 1 ? 0x0000ffffu : 0u) |
+               (in >> (16 * jj + v_slot_key(h2, 2 * i + 1)) & 1 ? 0xffff0000u : 0u);
+      };
+      keep0 = u32x4{word(0, 0), word(0, 1), word(0, 2), word(0, 3)};
+      keep1 = u32x4{word(1, 0), word(1, 1), word(1, 2), word(1, 3)};
     }
-  if (MASK && BITS == 16) {
-    for (; odd; odd &= odd - 1) {
-      const int key = __ffs((int)odd) - 1, r = key & 15;
-      const int e = r < 8 ? (r & 3) : 4 + (r & 3);
-      const uint32_t half = h2 != (r & 7) >> 2 ? 0u : e & 1 ? 0xffff0000u : 0x0000ffffu;
-      const int word = e >> 1;
-      const u32x4 only = {word == 0 ? half : 0u, word == 1 ? half : 0u, word == 2 ? half : 0u, word == 3 ? half : 0u};
 #pragma unroll
-      for (int t = 0; t < D / 32; ++t) {
-        const u32x4 v = (key < 16 ? vop(t, 0) : vop(t, 1)) & only;
+    for (int t = 0; t < D / 32; ++t)
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          const bf16x8 wn = key < 16 ? w[n][0] : w[n][1];
-          const f32x16 add = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v), wn, f32x16{}, 0, 0, 0);
+      for (int jj = 0; jj < 2; ++jj) {
+        u32x4 v = vj(t, jj);
+        if (MASK && BITS == 16) v &= jj ? keep1 : keep0;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) s.o[n][t][i] += kt + key <= s.bound[n] ? add[i] : 0.f;
+        for (int n = 0; n < NB; ++n)
+          s.o[n][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v),
+                                                              __builtin_bit_cast(bf16x8, w[j][n][jj]), s.o[n][t], 0, 0, 0);
+      }
+    if (MASK && BITS == 16) {
+      for (; odd; odd &= odd - 1) {
+        const int key = __ffs((int)odd) - 1, r = key & 15;
+        const int e = r < 8 ? (r & 3) : 4 + (r & 3);
+        const uint32_t half = h2 != (r & 7) >> 2 ? 0u : e & 1 ? 0xffff0000u : 0x0000ffffu;
+        const uint32_t low = key < 16 ? 0xffffffffu : 0u;
+        const int word = e >> 1;
+        const u32x4 only = {word == 0 ? half : 0u, word == 1 ? half : 0u, word == 2 ? half : 0u,
+                            word == 3 ? half : 0u};
+#pragma unroll
+        for (int t = 0; t < D / 32; ++t) {
+          const u32x4 v = ((vj(t, 0) & low) | (vj(t, 1) & ~low)) & only;
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            const u32x4 wn = (w[j][n][0] & low) | (w[j][n][1] & ~low);
+            const f32x16 add = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                __builtin_bit_cast(bf16x8, v), __builtin_bit_cast(bf16x8, wn), f32x16{}, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s.o[n][t][i] += kt + 32 * j + key <= s.bound[n] ? add[i] : 0.f;
+          }
         }
       }
     }
   }
 }
+
+// Bases (elements) of the blocks of a request's key range, 64 at a time: lane l
+// keeps block `first` + l's, so the key loop looks nothing up in memory (a
+// load there would wait for every tile in flight). -1: no page.
+struct BlockList {
+  long long at;
+  int first;
+  __device__ __forceinline__ void fill(const PAttn& p, int b, int h, int blk, int end, int lane, int elems) {
+    first = blk;
+    at = blk + lane < end ? page_block(p.table, p.width, b, blk + lane, p.bpp, p.num_pages, p.Hkv, h, elems) : -1;
+    if (p.status && blk + lane < end && at < 0) atomicOr(p.status, kStatusPage);
+  }
+  // Leading blocks of the list that have a page.
+  __device__ __forceinline__ int present() const {
+    const unsigned long long gone = __ballot(at < 0);
+    return gone ? __ffsll((long long)gone) - 1 : 64;
+  }
+  __device__ __forceinline__ long long get(int blk) const {
+    const int l = blk - first;
+    const unsigned lo = __builtin_amdgcn_readlane((int)at, l), hi = __builtin_amdgcn_readlane((int)(at >> 32), l);
+    return (long long)((unsigned long long)hi << 32 | lo);
+  }
+};
 
 // Rows of the wave's NB blocks of 32: query operands, bounds; every row of the
 // list is (token r / rep, head r % rep).
@@ -362,9 +460,16 @@ __device__ __forceinline__ void store4(uint16_t* dst, float a, float b, float c,
   *reinterpret_cast<uint2*>(dst) = make_uint2(f2bf2(a, b), f2bf2(c, d));
 }
 
-__device__ __forceinline__ uint16_t* out_row(const PAttn& p, const Req& rq, const Tile& u, int r) {
+// Row r of the tile whose first token is `token` (packed), of kv head h.
+__device__ __forceinline__ uint16_t* out_row(const PAttn& p, int token, int h, int r) {
   const int i = r / p.rep, g = r - i * p.rep;
-  return p.out + (rq.lo + (long long)u.t * p.P + i) * p.out_token + (long long)(u.h * p.rep + g) * p.out_head;
+  return p.out + ((long long)token + i) * p.out_token + (long long)(h * p.rep + g) * p.out_head;
+}
+
+// What the join needs to know of the tile that workgroup g begins and others
+// finish (at most one).
+__device__ __forceinline__ void note_begun(const PAttn& p, const Line& line, const Req& rq, const Tile& u, int g) {
+  p.begun[g] = make_int4(u.n * p.rep, line.owner(u.begin + u.len - 1) - g + 1, rq.lo + u.t * p.P, u.h);
 }
 
 // Eight bytes of integers -> eight bf16 (exact).
@@ -375,147 +480,205 @@ __device__ __forceinline__ u32x4 widen8(uint32_t a, uint32_t b) {
   return u32x4{pair(a, 0), pair(a, 2), pair(b, 0), pair(b, 2)};
 }
 
-// V operand registers (keys 16 jj + v_slot_key(h2, .) of block key kt) with the keys at
-// or past nk zeroed: stale bits of a page's tail are no numbers.
-__device__ __forceinline__ u32x4 cut_tail(u32x4 v, int key0, int h2, int nk) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t lo = key0 + v_slot_key(h2, 2 * i) < nk ? 0x0000ffffu : 0u;
-    const uint32_t hi = key0 + v_slot_key(h2, 2 * i + 1) < nk ? 0xffff0000u : 0u;
-    v[i] &= lo | hi;
-  }
-  return v;
-}
-
-// -- chunks: row tiles of 128 NB rows, K and V tiles shared through LDS ----------
+// -- chunks: row tiles of 32 NB rows a wave, K and V tiles shared through LDS ----
 
 constexpr int kStepKeys = 64;
 
-template <int D, int BITS, int NB>
-__global__ __launch_bounds__(kPT, 1) void attn_chunk_kernel(PAttn p) {
-  constexpr int RT = 4 * 32 * NB;
-  constexpr int BE = kBlk * D;                    // elements of a block
-  constexpr int CB = BE * (BITS / 8) / 16;        // 16-byte chunks of a block
-  constexpr int LD = 2 * CB / kPT;                // a thread's, of a step's two blocks
-  __shared__ __attribute__((aligned(16))) uint16_t kbuf[2][2 * BE];
-  __shared__ __attribute__((aligned(16))) uint16_t vbuf[2][2 * BE];
+// Waves and row blocks of a wave by head dim: two waves of 32 rows on a SIMD,
+// so one's softmax runs beside the other's products; at D = 256 one (its
+// accumulators and queries take 192 registers).
+template <int D>
+constexpr int chunk_waves() { return D == 256 ? 4 : 8; }
+
+template <int D, int BITS>
+__global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn p) {
+  constexpr int NW = chunk_waves<D>(), NT = 64 * NW, NB = 1;
+  constexpr int RT = NW * 32 * NB;
+  constexpr int BE = kBlk * D;                      // elements of a block
+  constexpr int NBUF = BITS == 8 || D == 256 ? 2 : 3;
+  constexpr int CB = BE * (BITS / 8) / 16;          // 16-byte chunks of a block
+  constexpr int LD = 2 * CB / NT > 0 ? 2 * CB / NT : 1;   // a thread's, of a step's two blocks
+  __shared__ __attribute__((aligned(16))) uint16_t kbuf[NBUF][2 * BE];
+  __shared__ __attribute__((aligned(16))) uint16_t vbuf[NBUF][2 * BE];
   __shared__ __attribute__((aligned(16))) float ksc[2][kStepKeys], vsc[2][kStepKeys];
   const int tid = threadIdx.x, lane = tid & 63, h2 = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Shares sh(line_total(p, lane), p.G, p.min_share);
+  const Line line(p, lane);
   const int g = blockIdx.x;
-  if (sh.W == 0 || g >= sh.G) return;
-  const long long lo = sh.lo(g), hi = sh.lo(g + 1);
+  if (tid == 0) p.begun[g] = make_int4(0, 0, 0, 0);
+  if (g >= line.G) return;
+  const long long lo = line.lo(g), hi = line.hi(g);
   Req rq;
-  int b = find_req(p, lane, lo, rq);
+  int b = line.find(p, lane, lo, rq);
   for (long long x = lo; x < hi;) {
-    if (x >= rq.base + p.Hkv * rq.head) b = find_req(p, lane, x, rq);
+    if (x >= rq.base + p.Hkv * rq.head) b = line.find(p, lane, x, rq);
     const Tile u = tile_at(p, rq, x);
     const long long end = hi < u.begin + u.len ? hi : u.begin + u.len;
     const int ka = key_at(u, x - u.begin, kStepKeys), kb = key_at(u, end - u.begin, kStepKeys);
     const bool starts = x == u.begin, ends = end == u.begin + u.len;
     x = end;
+    if (starts && !ends && tid == 0) note_begun(p, line, rq, u, g);
     const int row0 = wave * 32 * NB;
     const int rows = u.n * p.rep;   // of the tile
     RowState<D, NB> s;
     load_rows<D, NB>(s, p, rq, u, row0, lane);
-    // Bounds of the wave's rows: blocks behind wmax are skipped, blocks up to
+    // Bounds of the wave's rows: steps behind wmax are skipped, steps up to
     // wmin need no mask (rows past the list are computed on zeros, and dropped).
     const int last = (row0 + 32 * NB < rows ? row0 + 32 * NB : rows) - 1;
-    long long wmin = u.pos + row0 / p.rep, wmax = row0 < rows ? u.pos + last / p.rep : -1;
+    long long wmin = u.pos + row0 / p.rep;
+    const long long wmax = row0 < rows ? u.pos + last / p.rep : -1;
     if (wmin > u.nk - 1) wmin = u.nk - 1;
 
-    u32x4 kr[LD], vr[LD];
-    float kscale = 0.f, vscale = 0.f;
-    long long at[2], nat[2];
-    auto lookup = [&](int kt, long long (&a)[2]) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        a[j] = kt + 32 * j < kb ? page_block(p.table, p.width, b, (kt >> 5) + j, p.bpp, p.num_pages, p.Hkv, u.h, BE)
-                                : -2;
+    BlockList blocks;
+    blocks.fill(p, b, u.h, ka >> 5, (kb + 31) >> 5, lane, BE);
+    const int nstep = (kb - ka + kStepKeys - 1) / kStepKeys;
+    // Steps st .. of 32 a list: bases of step st's blocks (-1 past the end).
+    auto base = [&](int st, int j) {
+      const int blk = (ka >> 5) + 2 * st + j;
+      return 32 * blk < kb ? blocks.get(blk) : -1LL;
     };
-    auto load = [&](const long long (&a)[2]) {
+    u32x4 kr[LD], vr[LD];   // 8 bits: a step on its way to LDS
+    float kscale = 0.f, vscale = 0.f;
+    auto load = [&](int st, int buf) {
+      const long long a0 = base(st, 0), a1 = base(st, 1);
+      if constexpr (BITS == 16) {
+        // Straight into LDS: each wave instruction 1 KB of a block. (Absent blocks: page 0's, never used.)
 #pragma unroll
-      for (int i = 0; i < LD; ++i) {
-        const int c = i * kPT + tid;
-        const long long at_j = c / CB ? a[1] : a[0];
-        const size_t o = (size_t)(at_j < 0 ? 0 : at_j) * (BITS / 8) + (size_t)(c % CB) * 16;
-        kr[i] = *reinterpret_cast<const u32x4*>(p.k_pages + o);
-        vr[i] = *reinterpret_cast<const u32x4*>(p.v_pages + o);
-      }
-      if constexpr (BITS == 8) {
+        for (int i = 0; i < 4 * CB / NT; ++i) {
+          const int c = (i * NW + wave) * 64;   // first chunk: K's 2 CB, then V's
+          const bool isv = c >= 2 * CB;
+          const int cs = isv ? c - 2 * CB : c;
+          const long long at = cs >= CB ? a1 : a0;
+          const unsigned char* src = (isv ? p.v_pages : p.k_pages) +
+                                     ((size_t)(at < 0 ? 0 : at) * 2 + (size_t)(cs >= CB ? cs - CB : cs) * 16);
+          dma16(src, lane * 16, lds_addr((isv ? vbuf[buf] : kbuf[buf]) + cs * 8));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+          const int c = i * NT + tid;
+          if (c >= 2 * CB) break;
+          const long long at = c >= CB ? a1 : a0;
+          const size_t o = (size_t)(at < 0 ? 0 : at) + (size_t)(c >= CB ? c - CB : c) * 16;
+          kr[i] = *reinterpret_cast<const u32x4*>(p.k_pages + o);
+          vr[i] = *reinterpret_cast<const u32x4*>(p.v_pages + o);
+        }
         if (tid < kStepKeys) {
-          const long long a0 = tid < 32 ? a[0] : a[1];
-          const size_t o = (size_t)(a0 < 0 ? 0 : a0) / D + (tid & 31);
-          kscale = p.k_scales[o] * p.scale_log2;
+          const long long at = tid >= 32 ? a1 : a0;
+          const size_t o = (size_t)(at < 0 ? 0 : at) / D + (tid & 31);
+          kscale = p.k_scales[o];
           vscale = p.v_scales[o];
         }
       }
     };
-    auto store = [&](int buf, int kt) {
+    auto store = [&](int buf) {   // 8 bits
 #pragma unroll
       for (int i = 0; i < LD; ++i) {
-        const int c = i * kPT + tid, j = c / CB, cb = c % CB;
-        if constexpr (BITS == 16) {
-          *reinterpret_cast<u32x4*>(&kbuf[buf][c * 8]) = kr[i];
-          u32x4 v = vr[i];
-          if (kt + kStepKeys > u.nk) v = cut_tail(v, kt + 32 * j + 16 * ((cb >> 6) & 1), (cb >> 5) & 1, u.nk);
-          *reinterpret_cast<u32x4*>(&vbuf[buf][c * 8]) = v;
-        } else {
-          const int o = j * BE + (2 * (cb >> 6) * 64 + (cb & 63)) * 8;
-          *reinterpret_cast<u32x4*>(&kbuf[buf][o]) = widen8(kr[i].x, kr[i].y);
-          *reinterpret_cast<u32x4*>(&kbuf[buf][o + 512]) = widen8(kr[i].z, kr[i].w);
-          *reinterpret_cast<u32x4*>(&vbuf[buf][o]) = widen8(vr[i].x, vr[i].y);
-          *reinterpret_cast<u32x4*>(&vbuf[buf][o + 512]) = widen8(vr[i].z, vr[i].w);
-        }
+        const int c = i * NT + tid;
+        if (c >= 2 * CB) break;
+        const int cb = c >= CB ? c - CB : c;
+        const int o = (c >= CB ? BE : 0) + (2 * (cb >> 6) * 64 + (cb & 63)) * 8;
+        *reinterpret_cast<u32x4*>(&kbuf[buf][o]) = widen8(kr[i].x, kr[i].y);
+        *reinterpret_cast<u32x4*>(&kbuf[buf][o + 512]) = widen8(kr[i].z, kr[i].w);
+        *reinterpret_cast<u32x4*>(&vbuf[buf][o]) = widen8(vr[i].x, vr[i].y);
+        *reinterpret_cast<u32x4*>(&vbuf[buf][o + 512]) = widen8(vr[i].z, vr[i].w);
       }
-      if constexpr (BITS == 8) {
-        if (tid < kStepKeys) {
-          ksc[buf][tid] = kscale;
-          vsc[buf][tid] = vscale;
-        }
+      if (tid < kStepKeys) {
+        ksc[buf][tid] = kscale * p.scale_log2;
+        vsc[buf][tid] = vscale;
       }
     };
-    if (ka < kb) {
-      lookup(ka, at);
-      load(at);
-      lookup(ka + kStepKeys, nat);
-      store(0, ka);
-      __syncthreads();
-      int buf = 0;
-      for (int kt = ka; kt < kb; kt += kStepKeys) {
-        const bool more = kt + kStepKeys < kb;
-        const long long cur0 = at[0], cur1 = at[1];
-        if (more) {
-          at[0] = nat[0];
-          at[1] = nat[1];
-          load(at);
-          lookup(kt + 2 * kStepKeys, nat);
-        }
+    // Steps [0, nfull) hide no key from any of the wave's rows and have all
+    // their pages: they run in a loop of their own.
+    int nfull = 0;
+    if (row0 < rows && wmin + 1 - ka >= kStepKeys) nfull = (int)((wmin + 1 - ka) / kStepKeys);
+    if (nfull > nstep) nfull = nstep;
+    auto cut = [&](int st) {   // the list begins at step st: its steps before the first absent block
+      const int lead = st + (blocks.present() >> 1);
+      if (lead < nfull && lead < st + 32) nfull = lead;
+    };
+    cut(0);
+    auto full = [&](int buf) {
+      constexpr int KB = BITS == 8 || D == 256 ? 1 : 2;   // blocks at a time, as registers allow
+      const uint16_t* kl = &kbuf[buf][lane * 8];
+      const uint16_t* vl = &vbuf[buf][lane * 8];
+      const float* kss = &ksc[buf & 1][4 * h2];
+      const float* vss = &vsc[buf & 1][4 * h2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int k0 = kt + 32 * j;
-          const long long here = j ? cur1 : cur0;
-          if (here == -1 && p.status && tid == 0 && k0 < kb) atomicOr(p.status, kStatusPage);
-          if (here < 0 || k0 > wmax) continue;   // uniform over the wave
-          const uint16_t* kl = &kbuf[buf][j * BE + lane * 8];
-          const uint16_t* vl = &vbuf[buf][j * BE + lane * 8];
-          const float* kss = &ksc[buf][32 * j + 4 * h2];
-          const float* vss = &vsc[buf][32 * j + 4 * h2];
-          auto kop = [&](int i) { return __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(kl + i * 512)); };
-          auto vop = [&](int t, int jj) {
-            return *reinterpret_cast<const u32x4*>(vl + (2 * t + jj) * 512);
-          };
-          auto ks = [&](int r) { return kss[8 * (r >> 2) + (r & 3)]; };
-          auto vs = [&](int r) { return vss[8 * (r >> 2) + (r & 3)]; };
-          if (k0 + 31 <= wmin)
-            attend<D, BITS, NB, false>(s, k0, h2, p.scale_log2, kop, vop, ks, vs);
-          else
-            attend<D, BITS, NB, true>(s, k0, h2, p.scale_log2, kop, vop, ks, vs);
-        }
-        if (more) store(buf ^ 1, kt + kStepKeys);
+      for (int j0 = 0; j0 < 2; j0 += KB)
+        attend<D, BITS, NB, KB, false, D < 256>(
+            s, 0, 0, h2, p.scale_log2,
+            [&](int j, int i) { return *reinterpret_cast<const u32x4*>(kl + (j0 + j) * BE + i * 512); },
+            [&](int j, int t, int jj) { return *reinterpret_cast<const u32x4*>(vl + (j0 + j) * BE + (2 * t + jj) * 512); },
+            [&](int j, int r) { return kss[32 * (j0 + j) + 8 * (r >> 2) + (r & 3)]; },
+            [&](int j, int r) { return vss[32 * (j0 + j) + 8 * (r >> 2) + (r & 3)]; });
+    };
+    auto masked = [&](int st, int buf) {
+      const int kt = ka + st * kStepKeys;
+      const uint16_t* kl = &kbuf[buf][lane * 8];
+      const uint16_t* vl = &vbuf[buf][lane * 8];
+      const float* kss = &ksc[buf & 1][4 * h2];
+      const float* vss = &vsc[buf & 1][4 * h2];
+#pragma unroll 1
+      for (int j = 0; j < 2; ++j) {
+        if (kt + 32 * j > wmax || base(st, j) < 0) continue;
+        attend<D, BITS, NB, 1, true, D < 256>(
+            s, kt + 32 * j, u.nk, h2, p.scale_log2,
+            [&](int, int i) { return *reinterpret_cast<const u32x4*>(kl + j * BE + i * 512); },
+            [&](int, int t, int jj) { return *reinterpret_cast<const u32x4*>(vl + j * BE + (2 * t + jj) * 512); },
+            [&](int, int r) { return kss[32 * j + 8 * (r >> 2) + (r & 3)]; },
+            [&](int, int r) { return vss[32 * j + 8 * (r >> 2) + (r & 3)]; });
+      }
+    };
+    // The list is replaced while step st still uses it: lists overlap by the steps in flight.
+    auto load_ahead = [&](int st, int next, int buf) {
+      const int blk = (ka >> 5) + 2 * next;
+      if (blk + 2 > blocks.first + 64) {
+        blocks.fill(p, b, u.h, (ka >> 5) + 2 * st, (kb + 31) >> 5, lane, BE);
+        cut(st);
+      }
+      load(next, buf);
+    };
+    __syncthreads();   // the previous piece's reads are done
+    if constexpr (BITS == 16) {
+      constexpr int PER = 4 * CB / NT;   // loads of a wave per step
+      for (int i = 0; i < NBUF - 1 && i < nstep; ++i) load(i, i);
+      int buf = 0;
+      auto meet = [&](int st) {   // step st is in LDS, of every wave; the one before it is read
+        if (NBUF == 3 && st + 1 < nstep) wait_vm<PER>();
+        else wait_vm<0>();
+        lds_barrier();
+        if (st + NBUF - 1 < nstep) load_ahead(st, st + NBUF - 1, buf == 0 ? NBUF - 1 : buf - 1);
+      };
+      for (int st = 0; st < nfull; ++st) {
+        meet(st);
+        full(buf);
+        buf = buf == NBUF - 1 ? 0 : buf + 1;
+      }
+      for (int st = nfull; st < nstep; ++st) {
+        meet(st);
+        masked(st, buf);
+        buf = buf == NBUF - 1 ? 0 : buf + 1;
+      }
+    } else {
+      if (nstep > 0) {
+        load(0, 0);
+        store(0);
+      }
+      __syncthreads();
+      auto next = [&](int st) {
+        if (st + 1 < nstep) store((st + 1) & 1);
         __syncthreads();
-        buf ^= 1;
+      };
+      for (int st = 0; st < nfull; ++st) {
+        if (st + 1 < nstep) load_ahead(st, st + 1, 0);
+        full(st & 1);
+        next(st);
+      }
+      for (int st = nfull; st < nstep; ++st) {
+        if (st + 1 < nstep) load_ahead(st, st + 1, 0);
+        masked(st, st & 1);
+        next(st);
       }
     }
     // Out: the whole tile's rows, or this piece's partial.
@@ -528,14 +691,14 @@ __global__ __launch_bounds__(kPT, 1) void attn_chunk_kernel(PAttn p) {
       const float l = s.l[n] + __shfl_xor(s.l[n], 32, 64);
       if (whole) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        uint16_t* dst = out_row(p, rq, u, r);
+        uint16_t* dst = out_row(p, rq.lo + u.t * p.P, u.h, r);
 #pragma unroll
         for (int t = 0; t < D / 32; ++t)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             store4(dst + 32 * t + 8 * j + 4 * h2, s.o[n][t][4 * j] * inv, s.o[n][t][4 * j + 1] * inv,
                    s.o[n][t][4 * j + 2] * inv, s.o[n][t][4 * j + 3] * inv);
-      } else if (ka < kb) {
+      } else {   // (a piece without keys leaves m = -infinity, l = 0, and its o is not read)
         float* po = p.part_o + ((size_t)slot * RT + r) * D;
 #pragma unroll
         for (int t = 0; t < D / 32; ++t)
@@ -565,19 +728,21 @@ __global__ __launch_bounds__(kPT) void attn_few_kernel(PAttn p) {
   __shared__ float s_m[4][32], s_l[4][32];
   const int tid = threadIdx.x, lane = tid & 63, c32 = lane & 31, h2 = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Shares sh(line_total(p, lane), p.G, p.min_share);
+  const Line line(p, lane);
   const int g = blockIdx.x;
-  if (sh.W == 0 || g >= sh.G) return;
-  const long long lo = sh.lo(g), hi = sh.lo(g + 1);
+  if (tid == 0) p.begun[g] = make_int4(0, 0, 0, 0);
+  if (g >= line.G) return;
+  const long long lo = line.lo(g), hi = line.hi(g);
   Req rq;
-  int b = find_req(p, lane, lo, rq);
+  int b = line.find(p, lane, lo, rq);
   for (long long x = lo; x < hi;) {
-    if (x >= rq.base + p.Hkv * rq.head) b = find_req(p, lane, x, rq);
+    if (x >= rq.base + p.Hkv * rq.head) b = line.find(p, lane, x, rq);
     const Tile u = tile_at(p, rq, x);
     const long long end = hi < u.begin + u.len ? hi : u.begin + u.len;
     const int ka = key_at(u, x - u.begin, kBlk), kb = key_at(u, end - u.begin, kBlk);
     const bool starts = x == u.begin, ends = end == u.begin + u.len;
     x = end;
+    if (starts && !ends && tid == 0) note_begun(p, line, rq, u, g);
     const int rows = u.n * p.rep;
     RowState<D, 1> s;
     load_rows<D, 1>(s, p, rq, u, 0, lane);
@@ -588,9 +753,8 @@ __global__ __launch_bounds__(kPT) void attn_few_kernel(PAttn p) {
     const int k1 = e1 < kb ? e1 : kb;
     u32x4 kr[LD], vr[LD];
     float4 kq[4], vq[4];   // scales of the lane's keys
-    auto lookup = [&](int kt) {
-      return kt < k1 ? page_block(p.table, p.width, b, kt >> 5, p.bpp, p.num_pages, p.Hkv, u.h, BE) : -2;
-    };
+    BlockList blocks;
+    if (k0 < k1) blocks.fill(p, b, u.h, k0 >> 5, (k1 + 31) >> 5, lane, BE);
     auto load = [&](long long at) {
       const size_t o = (size_t)(at < 0 ? 0 : at);
 #pragma unroll
@@ -606,39 +770,31 @@ __global__ __launch_bounds__(kPT) void attn_few_kernel(PAttn p) {
       }
     };
     if (k0 < k1) {
-      long long at = lookup(k0);
+      long long at = blocks.get(k0 >> 5);
       load(at);
-      long long nat = lookup(k0 + kBlk);
       for (int kt = k0; kt < k1; kt += kBlk) {
         if (at >= 0) {   // uniform
-          if (BITS == 16 && kt + kBlk > u.nk) {
-#pragma unroll
-            for (int i = 0; i < LD; ++i) vr[i] = cut_tail(vr[i], kt + 16 * (i & 1), h2, u.nk);
-          }
-          auto kop = [&](int i) {
-            if constexpr (BITS == 16) return __builtin_bit_cast(bf16x8, kr[i]);
-            else
-              return __builtin_bit_cast(bf16x8, (i & 1) ? widen8(kr[i >> 1].z, kr[i >> 1].w)
-                                                        : widen8(kr[i >> 1].x, kr[i >> 1].y));
+          auto kop = [&](int, int i) {
+            if constexpr (BITS == 16) return kr[i];
+            else return (i & 1) ? widen8(kr[i >> 1].z, kr[i >> 1].w) : widen8(kr[i >> 1].x, kr[i >> 1].y);
           };
-          auto vop = [&](int t, int jj) {
+          auto vop = [&](int, int t, int jj) {
             if constexpr (BITS == 16) return vr[2 * t + jj];
             else return jj ? widen8(vr[t].z, vr[t].w) : widen8(vr[t].x, vr[t].y);
           };
           auto part = [](const float4& f, int e) { return e == 0 ? f.x : e == 1 ? f.y : e == 2 ? f.z : f.w; };
-          auto ks = [&](int r) { return part(kq[r >> 2], r & 3) * p.scale_log2; };
-          auto vs = [&](int r) { return part(vq[r >> 2], r & 3); };
+          auto ks = [&](int, int r) { return part(kq[r >> 2], r & 3) * p.scale_log2; };
+          auto vs = [&](int, int r) { return part(vq[r >> 2], r & 3); };
           if (kt + 31 <= wmin)
-            attend<D, BITS, 1, false>(s, kt, h2, p.scale_log2, kop, vop, ks, vs);
+            attend<D, BITS, 1, 1, false, false>(s, kt, u.nk, h2, p.scale_log2, kop, vop, ks, vs);
           else
-            attend<D, BITS, 1, true>(s, kt, h2, p.scale_log2, kop, vop, ks, vs);
-        } else if (p.status && lane == 0) {
-          atomicOr(p.status, kStatusPage);
+            attend<D, BITS, 1, 1, true, false>(s, kt, u.nk, h2, p.scale_log2, kop, vop, ks, vs);
         }
         if (kt + kBlk < k1) {
-          at = nat;
+          const int blk = (kt >> 5) + 1;
+          if (blk >= blocks.first + 64) blocks.fill(p, b, u.h, blk, (k1 + 31) >> 5, lane, BE);
+          at = blocks.get(blk);
           load(at);
-          nat = lookup(kt + 2 * kBlk);
         }
       }
     }
@@ -658,7 +814,6 @@ __global__ __launch_bounds__(kPT) void attn_few_kernel(PAttn p) {
     __syncthreads();
     const int slot = 2 * g + (starts ? 1 : 0);
     const bool whole = starts && ends;
-    if (!whole && ka >= kb) continue;
     for (int idx = 4 * tid; idx < rows * D; idx += 4 * kPT) {
       const int r = idx / D, d = idx % D;
       float m = s_m[0][r];
@@ -678,7 +833,7 @@ __global__ __launch_bounds__(kPT) void attn_few_kernel(PAttn p) {
       }
       if (whole) {
         const float inv = ls == 0.f ? 0.f : 1.f / ls;
-        store4(out_row(p, rq, u, r) + d, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+        store4(out_row(p, rq.lo + u.t * p.P, u.h, r) + d, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
       } else {
         *reinterpret_cast<float4*>(p.part_o + ((size_t)slot * RT + r) * D + d) = v;
         if (d == 0) {
@@ -694,50 +849,95 @@ __global__ __launch_bounds__(kPT) void attn_few_kernel(PAttn p) {
 // -- join: the tiles that fell to more than one workgroup ------------------------
 
 // Workgroup (g, y): rows [y RB, y RB + RB) of the tile that workgroup g began
-// and others finished.
+// and others finished. The pieces' weights 2^(m - max) first, one per (row,
+// piece) in LDS, kJoin pieces at a time; then GR groups of threads sum every
+// GR-th piece's rows, their loads independent, and meet in LDS in order.
+constexpr int kJoin = 64;
+
 template <int D, int RT, int RB>
-__global__ __launch_bounds__(kPT) void attn_join_kernel(PAttn p, int step) {
-  const int tid = threadIdx.x, lane = tid & 63;
-  const Shares sh(line_total(p, lane), p.G, p.min_share);
+__global__ __launch_bounds__(kPT) void attn_join_kernel(PAttn p) {
+  constexpr int TR = RB * D / 4;   // threads of a group
+  constexpr int GR = kPT / TR;
+  static_assert(TR * GR == kPT, "whole groups");
+  __shared__ float s_w[kJoin][RB], s_m[RB], s_l[RB];
+  __shared__ __attribute__((aligned(16))) float4 s_v[GR][TR];
+  const int tid = threadIdx.x;
   const int g = blockIdx.x;
-  if (sh.W == 0 || g + 1 >= sh.G) return;
-  const long long hi = sh.lo(g + 1);   // the tile that crosses this line position
-  Req rq;
-  find_req(p, lane, hi, rq);
-  const Tile u = tile_at(p, rq, hi);
-  if (u.begin >= hi || u.begin < sh.lo(g)) return;   // none, or begun before g
-  const int gl = sh.owner(u.begin + u.len - 1);
-  const int rows = u.n * p.rep;
+  const int4 t = p.begun[g];   // rows (0: none), pieces, first token, kv head
+  const int rows = t.x, np = t.y;
   const int r0 = blockIdx.y * RB;
   if (r0 >= rows) return;
-  const int r1 = r0 + RB < rows ? r0 + RB : rows;
-  for (int idx = 4 * tid; idx < (r1 - r0) * D; idx += 4 * kPT) {
-    const int r = r0 + idx / D, d = idx % D;
-    float m = -INFINITY, l = 0.f;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int w = g; w <= gl; ++w) {
-      const long long a = w == g ? 0 : sh.lo(w) - u.begin;
-      const int ka = key_at(u, a, step), kb = key_at(u, sh.lo(w + 1) - u.begin, step);
-      if (ka >= kb) continue;   // an empty piece left nothing
-      const size_t row = (size_t)(2 * w + (w == g ? 1 : 0)) * RT + r;
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + row * 2);
-      if (ml.x == -INFINITY) {   // no finite score yet: l is 0 or NaN
-        l += ml.y;
-        continue;
-      }
-      const float4 a4 = *reinterpret_cast<const float4*>(p.part_o + row * D + d);
-      const float mn = fmaxf(m, ml.x);
-      const float cm = m == -INFINITY ? 0.f : exp2_fast(m - mn), cw = exp2_fast(ml.x - mn);
-      m = mn;
-      l = l * cm + ml.y * cw;
-      v.x = v.x * cm + a4.x * cw;
-      v.y = v.y * cm + a4.y * cw;
-      v.z = v.z * cm + a4.z * cw;
-      v.w = v.w * cm + a4.w * cw;
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    store4(out_row(p, rq, u, r) + d, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+  // Piece k's slot: the one that begins the tile is g's second.
+  auto slot = [&](int k) { return (size_t)(2 * (g + k) + (k == 0 ? 1 : 0)) * RT; };
+  const int gr = tid / TR, rr = tid % TR / (D / 4), d = tid % (D / 4) * 4;
+  const bool in = r0 + rr < rows;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (tid < RB) {
+    s_m[tid] = -INFINITY;
+    s_l[tid] = 0.f;
   }
+  for (int k0 = 0; k0 < np; k0 += kJoin) {
+    const int n = np - k0 < kJoin ? np - k0 : kJoin;
+    __syncthreads();
+    const float m_old = s_m[rr];
+    __syncthreads();   // read before it is replaced
+    // Row tid / 32's weights by 32 lanes, two pieces each.
+    for (int row = tid >> 5; row < RB; row += kPT / 32) {
+      const int x = tid & 31;
+      const bool live = r0 + row < rows;
+      float2 a = make_float2(-INFINITY, 0.f), b = a;
+      if (live && x < n) a = *reinterpret_cast<const float2*>(p.part_ml + (slot(k0 + x) + r0 + row) * 2);
+      if (live && x + 32 < n) b = *reinterpret_cast<const float2*>(p.part_ml + (slot(k0 + x + 32) + r0 + row) * 2);
+      const float old = s_m[row];
+      float m = fmaxf(old, fmaxf(a.x, b.x));
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+      const float wa = a.x == -INFINITY ? 0.f : exp2_fast(a.x - m), wb = b.x == -INFINITY ? 0.f : exp2_fast(b.x - m);
+      float l = (a.x == -INFINITY ? a.y : a.y * wa) + (b.x == -INFINITY ? b.y : b.y * wb);   // no score: 0 or NaN
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) l += __shfl_xor(l, off, 64);
+      s_w[x][row] = wa;
+      s_w[x + 32][row] = wb;
+      if (x == 0) {
+        s_l[row] = s_l[row] * (old == -INFINITY ? 1.f : exp2_fast(old - m)) + l;
+        s_m[row] = m;
+      }
+    }
+    __syncthreads();
+    if (in) {
+      const float c = m_old == -INFINITY ? 0.f : exp2_fast(m_old - s_m[rr]);
+      v.x *= c;
+      v.y *= c;
+      v.z *= c;
+      v.w *= c;
+#pragma unroll 8
+      for (int k = gr; k < n; k += GR) {
+        const float w = s_w[k][rr];
+        if (w == 0.f) continue;   // nothing there, or nothing beside the others
+        const float4 a = *reinterpret_cast<const float4*>(p.part_o + (slot(k0 + k) + r0 + rr) * D + d);
+        v.x += a.x * w;
+        v.y += a.y * w;
+        v.z += a.z * w;
+        v.w += a.w * w;
+      }
+    }
+  }
+  if (GR > 1) {
+    s_v[gr][tid % TR] = v;
+    __syncthreads();
+    if (gr) return;
+#pragma unroll
+    for (int k = 1; k < GR; ++k) {
+      const float4 a = s_v[k][tid];
+      v.x += a.x;
+      v.y += a.y;
+      v.z += a.z;
+      v.w += a.w;
+    }
+  }
+  if (!in) return;
+  const float l = s_l[rr], inv = l == 0.f ? 0.f : 1.f / l;
+  store4(out_row(p, t.z, t.w, r0 + rr) + d, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
 }
 
 // Which kernel runs, and its tiles: calls of at most 32 query rows per kv head
@@ -745,15 +945,14 @@ __global__ __launch_bounds__(kPT) void attn_join_kernel(PAttn p, int step) {
 // them straight into registers; others share K and V tiles through LDS.
 struct AttnPlan {
   bool few;
-  int RT, P, G, min_share, step;
+  int RT, P, G, min_share;
 };
 inline AttnPlan attn_plan(int Hq, int Hkv, int D, int max_rows) {
   const int rep = Hq / Hkv;
   AttnPlan a;
   a.few = max_rows > 0 && (long long)max_rows * rep <= 32;
-  a.RT = a.few ? 32 : D == 256 ? 128 : 256;
+  a.RT = a.few ? 32 : D == 256 ? 128 : 256;   // chunk_waves<D>() * 32
   a.P = a.RT / rep;
-  a.step = a.few ? kBlk : kStepKeys;
   a.G = device_cus();
   a.min_share = a.few ? 4 * kBlk : 2 * kStepKeys;
   return a;
@@ -761,17 +960,20 @@ inline AttnPlan attn_plan(int Hq, int Hkv, int D, int max_rows) {
 
 template <int D, int BITS>
 int launch_attn(const PAttn& p, const AttnPlan& a, hipStream_t st) {
-  constexpr int NB = D == 256 ? 1 : 2;
+  constexpr int NW = chunk_waves<D>();
   if (a.few)
     hipLaunchKernelGGL((attn_few_kernel<D, BITS>), dim3((unsigned)p.G), dim3(kPT), 0, st, p);
   else
-    hipLaunchKernelGGL((attn_chunk_kernel<D, BITS, NB>), dim3((unsigned)p.G), dim3(kPT), 0, st, p);
+    hipLaunchKernelGGL((attn_chunk_kernel<D, BITS>), dim3((unsigned)p.G), dim3(64 * NW), 0, st, p);
   const int rc = launch_check("mtp_paged_attn");
   if (rc) return rc;
+  constexpr int RF = 256 / D < 1 ? 1 : 256 / D;    // few rows: four groups of threads to a join
+  constexpr int RC = 1024 / D;                     // chunks: one
   if (a.few)
-    hipLaunchKernelGGL((attn_join_kernel<D, 32, 8>), dim3((unsigned)p.G, 4), dim3(kPT), 0, st, p, a.step);
+    hipLaunchKernelGGL((attn_join_kernel<D, 32, RF>), dim3((unsigned)p.G, cdiv(a.P * p.rep, RF)), dim3(kPT), 0, st, p);
   else
-    hipLaunchKernelGGL((attn_join_kernel<D, 128 * NB, 16>), dim3((unsigned)p.G, 8 * NB), dim3(kPT), 0, st, p, a.step);
+    hipLaunchKernelGGL((attn_join_kernel<D, 32 * NW, RC>), dim3((unsigned)p.G, cdiv(a.P * p.rep, RC)), dim3(kPT), 0,
+                       st, p);
   return launch_check("mtp_paged_attn");
 }
 
@@ -782,7 +984,7 @@ using namespace mtp;
 MTP_API size_t mtp_paged_attn_workspace_bytes(int Hq, int Hkv, int D, int max_rows) {
   if (Hkv < 1 || Hq < Hkv || Hq % Hkv || D < 1) return 0;
   const AttnPlan a = attn_plan(Hq, Hkv, D, max_rows);
-  return (size_t)2 * a.G * a.RT * (D + 2) * sizeof(float);
+  return (size_t)2 * a.G * a.RT * (D + 2) * sizeof(float) + (size_t)a.G * 16;
 }
 
 MTP_API int mtp_paged_attn(const mtp_paged_attn_args* a, void* stream) {
@@ -832,6 +1034,7 @@ MTP_API int mtp_paged_attn(const mtp_paged_attn_args* a, void* stream) {
   p.status = a->status;
   p.part_o = (float*)a->ws;
   p.part_ml = p.part_o + (size_t)2 * plan.G * plan.RT * a->D;
+  p.begun = reinterpret_cast<int4*>(p.part_ml + (size_t)2 * plan.G * plan.RT * 2);
   p.T = a->T;
   p.B = a->B;
   p.width = a->width;
