@@ -29,11 +29,14 @@
 #include "paged.hpp"
 #include "qmv_common.hpp"
 
+#include <type_traits>
+
 namespace mtp {
 
 constexpr int kPT = 256;   // threads: four waves
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 
 struct PAttn {
   const uint16_t* q;
@@ -121,18 +124,15 @@ __device__ __forceinline__ long long scan64(long long v, int lane) {
   return v;
 }
 
-// The line as a wave sees it: its total length W, cut into G shares of S; of
-// up to 64 requests the lanes keep their own.
+// The line as a wave sees it: its total length W, cut into G shares of S.
 struct Line {
-  LaneReq mine;
-  long long incl;   // line position where the lane's request ends
   long long W, S;
   int G;
   __device__ __forceinline__ Line(const PAttn& p, int lane) {
-    mine = lane_req(p, lane);
-    incl = scan64(p.Hkv * mine.len, lane);
-    W = shfl64(incl, 63);
-    for (int b0 = 64; b0 < p.B; b0 += 64) W += shfl64(scan64(p.Hkv * lane_req(p, b0 + lane).len, lane), 63);
+    W = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 64) W += p.Hkv * lane_req(p, b0 + lane).len;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) W += __shfl_xor(W, off, 64);
     W = uniform64(W);
     // Equal shares, a whole number of steps each, no shorter than min_share.
     const long long s = (long long)ceil((double)W / (double)p.G);
@@ -145,9 +145,10 @@ struct Line {
   __device__ __forceinline__ int owner(long long x) const { return div_small(x, S); }
   // The request that holds line position x.
   __device__ __forceinline__ int find(const PAttn& p, int lane, long long x, Req& r) const {
-    LaneReq q = mine;
-    long long end = incl, carry = 0;
-    for (int b0 = 0;;) {
+    long long carry = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+      const LaneReq q = lane_req(p, b0 + lane);
+      const long long end = scan64(p.Hkv * q.len, lane);
       const unsigned long long m = __ballot(q.len > 0 && x < carry + end);   // the first whose end lies behind x
       if (m) {
         const int src = __ffsll((long long)m) - 1;
@@ -159,11 +160,8 @@ struct Line {
         return __builtin_amdgcn_readfirstlane(b0 + src);
       }
       carry += shfl64(end, 63);
-      b0 += 64;
-      if (b0 >= p.B) return -1;   // (not reached: x < W)
-      q = lane_req(p, b0 + lane);
-      end = scan64(p.Hkv * q.len, lane);
     }
+    return -1;   // (not reached: x < W)
   }
 };
 
@@ -213,12 +211,14 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 // Maximum with lane + 32's.
 __device__ __forceinline__ float max_halves(float x) { return fmaxf(x, __shfl_xor(x, 32, 64)); }
 
-template <int D, int NB>
+// A lane's query row (lane % 32 of the wave's 32): operands, running output,
+// maximum and sum.
+template <int D>
 struct RowState {
-  bf16x8 q[NB][D / 16];
-  f32x16 o[NB][D / 32];
-  float m[NB], l[NB];
-  int bound[NB];   // last key that the lane's row sees; -1: no row here
+  bf16x8 q[D / 16];
+  f32x16 o[D / 32];
+  float m, l;
+  int bound;   // last key that the row sees; -1: none, or no row here
 };
 
 // Keys (bit k: key k of the block) of a 16-bit V block with a NaN or an
@@ -244,210 +244,176 @@ __device__ __forceinline__ uint32_t odd_keys(VO vop, int h2) {
   return __builtin_amdgcn_readfirstlane((int)keys);
 }
 
-// KB blocks of 32 keys from kt on. kop(j, i), vop(j, t, jj): block j's operands
-// (as 16 bytes of bf16); ks(j, r), vs(j, r): scales of the lane's key of score
-// register r (8 bits), ks already times scale_log2. MASK: rows see keys up to
-// their bound, none at or past end;
-// what lies there in V is no number.
-// AHEAD: the operands come from LDS; a phase's are all asked for before it
-// begins, V's before the softmax (left to itself, the compiler reads each right
-// before the product that waits for it).
-template <int D, int BITS, int NB, int KB, bool MASK, bool AHEAD, class KO, class VO, class KS, class VS>
-__device__ __forceinline__ void attend(RowState<D, NB>& s, int kt, int end, int h2, float scale_log2,
-                                       KO kop, VO vop, KS ks, VS vs) {
-  f32x16 st[KB][NB];
-  u32x4 ka[KB][D / 16], va[KB][D / 16];
-  if (AHEAD) {
-#pragma unroll
-    for (int j = 0; j < KB; ++j)
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) ka[j][i] = kop(j, i);
-    __builtin_amdgcn_sched_barrier(0);
-  }
+// A step's KB blocks of 32 keys from kt on go through three phases, each with
+// its operands from where the caller keeps them (as 16 bytes of bf16).
+
+// S^T = K Q^T. kop(j, i): operand i of block j.
+template <int D, int KB, class KO>
+__device__ __forceinline__ void scores(const RowState<D>& s, f32x16 (&st)[KB], KO kop) {
 #pragma unroll
   for (int j = 0; j < KB; ++j) {
+    st[j] = f32x16{};
 #pragma unroll
-    for (int n = 0; n < NB; ++n) st[j][n] = f32x16{};
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      const bf16x8 k = __builtin_bit_cast(bf16x8, AHEAD ? ka[j][i] : kop(j, i));
-#pragma unroll
-      for (int n = 0; n < NB; ++n)
-        st[j][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, s.q[n][i], st[j][n], 0, 0, 0);
-    }
+    for (int i = 0; i < D / 16; ++i)
+      st[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kop(j, i)), s.q[i], st[j], 0, 0, 0);
   }
-  if (AHEAD) {
+}
+
+// Scores to weights (the second product's operand), the running maximum and
+// sum. ks(j, r), vs(j, r): scales of the lane's key of score register r (8
+// bits), ks already times scale_log2. MASK: the row sees keys up to its bound,
+// of block j none at or past end[j].
+template <int D, int BITS, int KB, bool MASK, class KS, class VS>
+__device__ __forceinline__ void soften(RowState<D>& s, f32x16 (&st)[KB], u32x4 (&w)[KB][2], int kt,
+                                       const int (&end)[KB], int h2, float scale_log2, KS ks, VS vs) {
+  // 16 bits without a mask: the maximum is taken before the scale (positive),
+  // and scale and maximum go into one FMA.
+  constexpr bool RAW = BITS == 16 && !MASK;
+  float top = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < KB; ++j)
+  for (int j = 0; j < KB; ++j)
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) va[j][i] = vop(j, i >> 1, i & 1);
-  }
-  __builtin_amdgcn_sched_barrier(0);
-  u32x4 w[KB][NB][2];
-#pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    // 16 bits without a mask: the maximum is taken before the scale (positive),
-    // and scale and maximum go into one FMA.
-    constexpr bool RAW = BITS == 16 && !MASK;
-    float top = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < KB; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        float x = st[j][n][r];
-        if (!RAW) x *= BITS == 8 ? ks(j, r) : scale_log2;
-        if (MASK) {
-          const int key = kt + 32 * j + 8 * (r >> 2) + 4 * h2 + (r & 3);
-          x = key <= s.bound[n] && key < end ? x : -INFINITY;
-        }
-        st[j][n][r] = x;
-        top = __builtin_elementwise_maximum(top, x);   // (no quieting of each x; a NaN makes its row NaN)
+    for (int r = 0; r < 16; ++r) {
+      float x = st[j][r];
+      if (!RAW) x *= BITS == 8 ? ks(j, r) : scale_log2;
+      if (MASK) {
+        const int key = kt + 32 * j + 8 * (r >> 2) + 4 * h2 + (r & 3);
+        x = key <= s.bound && key < end[j] ? x : -INFINITY;
       }
-    top = max_halves(top);
-    if (RAW) top *= scale_log2;
-    if (__any(top > s.m[n] + 8.f)) {
-      // Only the rows that passed: the others' bits do not turn on their neighbours.
-      const float m_new = top > s.m[n] + 8.f ? top : s.m[n];
-      const float corr = s.m[n] == -INFINITY ? 0.f : exp2_fast(s.m[n] - m_new);
-      s.m[n] = m_new;
-      s.l[n] *= corr;
-#pragma unroll
-      for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s.o[n][t][r] *= corr;
+      st[j][r] = x;
+      top = __builtin_elementwise_maximum(top, x);   // (no quieting of each x; a NaN makes its row NaN)
     }
-    const float m = s.m[n] == -INFINITY ? 0.f : s.m[n];
-    float sum = 0.f;
-#pragma unroll
-    for (int j = 0; j < KB; ++j) {
-      uint32_t pk[8];
-#pragma unroll
-      for (int r = 0; r < 16; r += 2) {
-        auto weight = [&](int rr) {
-          const float x = st[j][n][rr];
-          return exp2_fast(RAW ? __fmaf_rn(x, scale_log2, -m) : x - m);
-        };
-        float a = weight(r), b = weight(r + 1);
-        sum += a + b;
-        if (BITS == 8) {
-          const float va = vs(j, r), vb = vs(j, r + 1);
-          a = MASK && a == 0.f ? 0.f : a * va;   // a hidden key's scale may be NaN
-          b = MASK && b == 0.f ? 0.f : b * vb;
-        }
-        pk[r / 2] = f2bf2(a, b);
-      }
-      w[j][n][0] = u32x4{pk[0], pk[1], pk[2], pk[3]};
-      w[j][n][1] = u32x4{pk[4], pk[5], pk[6], pk[7]};
-    }
-    s.l[n] += sum;
-  }
-  __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-  for (int j = 0; j < KB; ++j) {
-    // A hidden key's weight is 0, but 0 times a NaN or an infinity in its value
-    // is not: in blocks with hidden keys (MASK), keys whose values are not all
-    // finite leave the product and are added one by one, to the rows that see
-    // them. (8-bit values are integers; their scale went into the weight.)
-    u32x4 keep0 = {}, keep1 = {};
-    uint32_t odd = 0;
-    auto vj = [&](int t, int jj) { return AHEAD ? va[j][2 * t + jj] : vop(j, t, jj); };
-    if (MASK && BITS == 16) {
-      const int n = end - kt - 32 * j;   // keys that exist
-      const uint32_t have = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
-      odd = odd_keys<D>(vj, h2) & have;
-      const uint32_t in = have & ~odd;
-      auto word = [&](int jj, int i) {
-        return (in >> (16 * jj + v_slot_key(h2, 2 * i)) & 1 ? 0x0000ffffu : 0u) |
-               (in >> (16 * jj + v_slot_key(h2, 2 * i + 1)) & 1 ? 0xffff0000u : 0u);
-      };
-      keep0 = u32x4{word(0, 0), word(0, 1), word(0, 2), word(0, 3)};
-      keep1 = u32x4{word(1, 0), word(1, 1), word(1, 2), word(1, 3)};
-    }
+  top = max_halves(top);
+  if (RAW) top *= scale_log2;
+  if (__any(top > s.m + 8.f)) {
+    // Only the rows that passed: the others' bits do not turn on their neighbours.
+    const float m_new = top > s.m + 8.f ? top : s.m;
+    const float corr = s.m == -INFINITY ? 0.f : exp2_fast(s.m - m_new);
+    s.m = m_new;
+    s.l *= corr;
 #pragma unroll
     for (int t = 0; t < D / 32; ++t)
 #pragma unroll
-      for (int jj = 0; jj < 2; ++jj) {
-        u32x4 v = vj(t, jj);
-        if (MASK && BITS == 16) v &= jj ? keep1 : keep0;
+      for (int r = 0; r < 16; ++r) s.o[t][r] *= corr;
+  }
+  const float m = s.m == -INFINITY ? 0.f : s.m;
+  float sum = 0.f;
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
-          s.o[n][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v),
-                                                              __builtin_bit_cast(bf16x8, w[j][n][jj]), s.o[n][t], 0, 0, 0);
+  for (int j = 0; j < KB; ++j) {
+    uint32_t pk[8];
+#pragma unroll
+    for (int r = 0; r < 16; r += 2) {
+      auto weight = [&](int rr) {
+        const float x = st[j][rr];
+        return exp2_fast(RAW ? __fmaf_rn(x, scale_log2, -m) : x - m);
+      };
+      float a = weight(r), b = weight(r + 1);
+      sum += a + b;
+      if (BITS == 8) {
+        const float va = vs(j, r), vb = vs(j, r + 1);
+        a = MASK && a == 0.f ? 0.f : a * va;   // a hidden key's scale may be NaN
+        b = MASK && b == 0.f ? 0.f : b * vb;
       }
-    if (MASK && BITS == 16) {
-      for (; odd; odd &= odd - 1) {
-        const int key = __ffs((int)odd) - 1, r = key & 15;
-        const int e = r < 8 ? (r & 3) : 4 + (r & 3);
-        const uint32_t half = h2 != (r & 7) >> 2 ? 0u : e & 1 ? 0xffff0000u : 0x0000ffffu;
-        const uint32_t low = key < 16 ? 0xffffffffu : 0u;
-        const int word = e >> 1;
-        const u32x4 only = {word == 0 ? half : 0u, word == 1 ? half : 0u, word == 2 ? half : 0u,
-                            word == 3 ? half : 0u};
+      pk[r / 2] = f2bf2(a, b);
+    }
+    w[j][0] = u32x4{pk[0], pk[1], pk[2], pk[3]};
+    w[j][1] = u32x4{pk[4], pk[5], pk[6], pk[7]};
+  }
+  s.l += sum;
+}
+
+// O^T += V^T P^T of block j's weights w. vop(t, jj): its operands. MASK, 16
+// bits: a hidden key's weight is 0, but 0 times a NaN or an infinity in its
+// value is not: keys whose values are not all finite leave the product and are
+// added one by one, to the rows that see them; at or past `end` there is
+// nothing. (8-bit values are integers; their scale went into the weight.)
+template <int D, int BITS, bool MASK, class VO>
+__device__ __forceinline__ void add_values(RowState<D>& s, const u32x4 (&w)[2], int kt, int end, int h2, VO vop) {
+  u32x4 keep0 = {}, keep1 = {};
+  uint32_t odd = 0;
+  if (MASK && BITS == 16) {
+    const int n = end - kt;   // keys that exist
+    const uint32_t have = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+    odd = odd_keys<D>(vop, h2) & have;
+    const uint32_t in = have & ~odd;
+    auto word = [&](int jj, int i) {
+      return (in >> (16 * jj + v_slot_key(h2, 2 * i)) & 1 ? 0x0000ffffu : 0u) |
+             (in >> (16 * jj + v_slot_key(h2, 2 * i + 1)) & 1 ? 0xffff0000u : 0u);
+    };
+    keep0 = u32x4{word(0, 0), word(0, 1), word(0, 2), word(0, 3)};
+    keep1 = u32x4{word(1, 0), word(1, 1), word(1, 2), word(1, 3)};
+  }
 #pragma unroll
-        for (int t = 0; t < D / 32; ++t) {
-          const u32x4 v = ((vj(t, 0) & low) | (vj(t, 1) & ~low)) & only;
+  for (int t = 0; t < D / 32; ++t)
 #pragma unroll
-          for (int n = 0; n < NB; ++n) {
-            const u32x4 wn = (w[j][n][0] & low) | (w[j][n][1] & ~low);
-            const f32x16 add = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                __builtin_bit_cast(bf16x8, v), __builtin_bit_cast(bf16x8, wn), f32x16{}, 0, 0, 0);
+    for (int jj = 0; jj < 2; ++jj) {
+      u32x4 v = vop(t, jj);
+      if (MASK && BITS == 16) v &= jj ? keep1 : keep0;
+      s.o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v), __builtin_bit_cast(bf16x8, w[jj]),
+                                                       s.o[t], 0, 0, 0);
+    }
+  if (MASK && BITS == 16) {
+    for (; odd; odd &= odd - 1) {
+      const int key = __ffs((int)odd) - 1, r = key & 15;
+      const int e = r < 8 ? (r & 3) : 4 + (r & 3);
+      const uint32_t half = h2 != (r & 7) >> 2 ? 0u : e & 1 ? 0xffff0000u : 0x0000ffffu;
+      const uint32_t low = key < 16 ? 0xffffffffu : 0u;
+      const int word = e >> 1;
+      const u32x4 only = {word == 0 ? half : 0u, word == 1 ? half : 0u, word == 2 ? half : 0u, word == 3 ? half : 0u};
+      const u32x4 wn = (w[0] & low) | (w[1] & ~low);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s.o[n][t][i] += kt + 32 * j + key <= s.bound[n] ? add[i] : 0.f;
-          }
-        }
+      for (int t = 0; t < D / 32; ++t) {
+        const u32x4 v = ((vop(t, 0) & low) | (vop(t, 1) & ~low)) & only;
+        const f32x16 add = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v),
+                                                                   __builtin_bit_cast(bf16x8, wn), f32x16{}, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s.o[t][i] += kt + key <= s.bound ? add[i] : 0.f;
       }
     }
   }
 }
 
-// Bases (elements) of the blocks of a request's key range, 64 at a time: lane l
-// keeps block `first` + l's, so the key loop looks nothing up in memory (a
-// load there would wait for every tile in flight). -1: no page.
+// Where the blocks of a request's key range lie in the pool (block ordinals),
+// 64 at a time: lane l keeps block `first` + l's, so the key loop looks nothing
+// up in memory (a load there would wait for every tile in flight). Blocks
+// without a page (bits of `gone`) are given ordinal 0: what is read there is
+// never used.
 struct BlockList {
-  long long at;
-  int first;
-  __device__ __forceinline__ void fill(const PAttn& p, int b, int h, int blk, int end, int lane, int elems) {
+  unsigned long long gone;
+  int at, first;
+  __device__ __forceinline__ void fill(const PAttn& p, int b, int h, int blk, int end, int lane) {
     first = blk;
-    at = blk + lane < end ? page_block(p.table, p.width, b, blk + lane, p.bpp, p.num_pages, p.Hkv, h, elems) : -1;
+    at = blk + lane < end ? (int)page_block(p.table, p.width, b, blk + lane, p.bpp, p.num_pages, p.Hkv, h, 1) : -1;
     if (p.status && blk + lane < end && at < 0) atomicOr(p.status, kStatusPage);
+    gone = __ballot(at < 0);
+    if (at < 0) at = 0;
   }
+  __device__ __forceinline__ int get(int blk) const { return __builtin_amdgcn_readlane(at, blk - first); }
+  __device__ __forceinline__ bool absent(int blk) const { return gone >> (blk - first) & 1; }
   // Leading blocks of the list that have a page.
-  __device__ __forceinline__ int present() const {
-    const unsigned long long gone = __ballot(at < 0);
-    return gone ? __ffsll((long long)gone) - 1 : 64;
-  }
-  __device__ __forceinline__ long long get(int blk) const {
-    const int l = blk - first;
-    const unsigned lo = __builtin_amdgcn_readlane((int)at, l), hi = __builtin_amdgcn_readlane((int)(at >> 32), l);
-    return (long long)((unsigned long long)hi << 32 | lo);
-  }
+  __device__ __forceinline__ int present() const { return gone ? __ffsll((long long)gone) - 1 : 64; }
 };
 
-// Rows of the wave's NB blocks of 32: query operands, bounds; every row of the
-// list is (token r / rep, head r % rep).
-template <int D, int NB>
-__device__ __forceinline__ void load_rows(RowState<D, NB>& s, const PAttn& p, const Req& rq, const Tile& u, int row0,
+// Rows row0 .. of a tile (row r of the list: token r / rep, head r % rep).
+template <int D>
+__device__ __forceinline__ void load_rows(RowState<D>& s, const PAttn& p, const Req& rq, const Tile& u, int row0,
                                           int lane) {
-  const int c = lane & 31, h2 = lane >> 5;
+  const int h2 = lane >> 5, r = row0 + (lane & 31);
+  const int i = r / p.rep, g = r - i * p.rep;
+  const bool valid = i < u.n;
+  const long long pos = u.pos + i;
+  s.bound = !valid || pos < 0 ? -1 : pos < u.nk ? (int)pos : u.nk - 1;
+  const long long tok = rq.lo + (long long)u.t * p.P + (valid ? i : 0);
+  const uint16_t* row = p.q + tok * p.q_token + (long long)(u.h * p.rep + (valid ? g : 0)) * p.q_head;
 #pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    const int r = row0 + 32 * n + c;
-    const int i = r / p.rep, g = r - i * p.rep;
-    const bool valid = i < u.n;
-    const long long pos = u.pos + i;
-    s.bound[n] = !valid || pos < 0 ? -1 : pos < u.nk ? (int)pos : u.nk - 1;
-    const long long tok = rq.lo + (long long)u.t * p.P + (valid ? i : 0);
-    const uint16_t* row = p.q + tok * p.q_token + (long long)(u.h * p.rep + (valid ? g : 0)) * p.q_head;
-#pragma unroll
-    for (int j = 0; j < D / 16; ++j) {
-      const u32x4 raw = *reinterpret_cast<const u32x4*>(row + (D / 2) * h2 + 8 * j);
-      s.q[n][j] = __builtin_bit_cast(bf16x8, valid ? raw : u32x4{0, 0, 0, 0});
-    }
-#pragma unroll
-    for (int t = 0; t < D / 32; ++t) s.o[n][t] = f32x16{};
-    s.m[n] = -INFINITY;
-    s.l[n] = 0.f;
+  for (int j = 0; j < D / 16; ++j) {
+    const u32x4 raw = *reinterpret_cast<const u32x4*>(row + (D / 2) * h2 + 8 * j);
+    s.q[j] = __builtin_bit_cast(bf16x8, valid ? raw : u32x4{0, 0, 0, 0});
   }
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t) s.o[t] = f32x16{};
+  s.m = -INFINITY;
+  s.l = 0.f;
 }
 
 // 16 bytes read once per launch (non-temporal, as ld_stream).
@@ -484,30 +450,47 @@ __device__ __forceinline__ u32x4 widen8(uint32_t a, uint32_t b) {
 
 constexpr int kStepKeys = 64;
 
-// Waves and row blocks of a wave by head dim: two waves of 32 rows on a SIMD,
-// so one's softmax runs beside the other's products; at D = 256 one (its
-// accumulators and queries take 192 registers).
+// Two waves of 32 rows on a SIMD; at D = 256 one (its accumulators and queries
+// take 192 registers).
 template <int D>
 constexpr int chunk_waves() { return D == 256 ? 4 : 8; }
 
+// Between two barriers a wave computes a step's products (PV of step n - 1, then
+// QK of n) and a softmax, and the two waves of a SIMD (w and w + 4) do so in
+// turn: the first four products(n), softmax(n), the others softmax(n - 1),
+// products(n), so one's matrix instructions run beside the other's exponentials.
+//
+// With step n's products a wave also stores its share of K and V of step n + 1,
+// loaded a step before, and loads those of n + 2: V(n) lies there a step before
+// its product, whose first operands are read ahead of the barrier. (Loads
+// straight into LDS stall the wave that issues them, 600 to 1000 cycles of a
+// step.)
 template <int D, int BITS>
 __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn p) {
-  constexpr int NW = chunk_waves<D>(), NT = 64 * NW, NB = 1;
-  constexpr int RT = NW * 32 * NB;
+  constexpr int NW = chunk_waves<D>(), NT = 64 * NW;
+  constexpr int RT = NW * 32;
   constexpr int BE = kBlk * D;                      // elements of a block
-  constexpr int NBUF = BITS == 8 || D == 256 ? 2 : 3;
   constexpr int CB = BE * (BITS / 8) / 16;          // 16-byte chunks of a block
   constexpr int LD = 2 * CB / NT > 0 ? 2 * CB / NT : 1;   // a thread's, of a step's two blocks
-  __shared__ __attribute__((aligned(16))) uint16_t kbuf[NBUF][2 * BE];
-  __shared__ __attribute__((aligned(16))) uint16_t vbuf[NBUF][2 * BE];
-  __shared__ __attribute__((aligned(16))) float ksc[2][kStepKeys], vsc[2][kStepKeys];
+  // K of a step lives for two phases and is written in the two before; V lives
+  // for four (at D = 256, where no wave runs half a step behind, for two).
+  constexpr int KR = 2, VR = D == 256 ? 2 : 3;
+  __shared__ __attribute__((aligned(16))) uint16_t kbuf[KR][2 * BE];
+  __shared__ __attribute__((aligned(16))) uint16_t vbuf[VR][2 * BE];
+  __shared__ __attribute__((aligned(16))) float ksc[4][kStepKeys], vsc[4][kStepKeys];   // (of step n - 1 to n + 1)
   const int tid = threadIdx.x, lane = tid & 63, h2 = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Line line(p, lane);
-  const int g = blockIdx.x;
+  if (tid == 0 && (int)blockIdx.x >= line.G) p.begun[blockIdx.x] = make_int4(0, 0, 0, 0);
+  // Neighbours on the line share a head's keys: they go to one XCD (workgroups
+  // are dealt to the eight in turn), whose L2 then serves them.
+  const int per = cdiv(line.G, 8);
+  const int g = ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);
+  if ((int)blockIdx.x >> 3 >= per || g >= line.G) return;
   if (tid == 0) p.begun[g] = make_int4(0, 0, 0, 0);
-  if (g >= line.G) return;
   const long long lo = line.lo(g), hi = line.hi(g);
+  const int turn = NW == 8 && wave >= 4 ? 1 : 0;
+  const uint32_t klds = lds_addr(kbuf), vlds = lds_addr(vbuf);
   Req rq;
   int b = line.find(p, lane, lo, rq);
   for (long long x = lo; x < hi;) {
@@ -518,199 +501,270 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
     const bool starts = x == u.begin, ends = end == u.begin + u.len;
     x = end;
     if (starts && !ends && tid == 0) note_begun(p, line, rq, u, g);
-    const int row0 = wave * 32 * NB;
+    const int row0 = wave * 32;
     const int rows = u.n * p.rep;   // of the tile
-    RowState<D, NB> s;
-    load_rows<D, NB>(s, p, rq, u, row0, lane);
+    RowState<D> s;
+    load_rows<D>(s, p, rq, u, row0, lane);
     // Bounds of the wave's rows: steps behind wmax are skipped, steps up to
     // wmin need no mask (rows past the list are computed on zeros, and dropped).
-    const int last = (row0 + 32 * NB < rows ? row0 + 32 * NB : rows) - 1;
+    const int last = (row0 + 32 < rows ? row0 + 32 : rows) - 1;
     long long wmin = u.pos + row0 / p.rep;
     const long long wmax = row0 < rows ? u.pos + last / p.rep : -1;
     if (wmin > u.nk - 1) wmin = u.nk - 1;
 
     BlockList blocks;
-    blocks.fill(p, b, u.h, ka >> 5, (kb + 31) >> 5, lane, BE);
+    blocks.fill(p, b, u.h, ka >> 5, (kb + 31) >> 5, lane);
     const int nstep = (kb - ka + kStepKeys - 1) / kStepKeys;
-    // Steps st .. of 32 a list: bases of step st's blocks (-1 past the end).
-    auto base = [&](int st, int j) {
-      const int blk = (ka >> 5) + 2 * st + j;
-      return 32 * blk < kb ? blocks.get(blk) : -1LL;
-    };
-    u32x4 kr[LD], vr[LD];   // 8 bits: a step on its way to LDS
-    float kscale = 0.f, vscale = 0.f;
-    auto load = [&](int st, int buf) {
-      const long long a0 = base(st, 0), a1 = base(st, 1);
-      if constexpr (BITS == 16) {
-        // Straight into LDS: each wave instruction 1 KB of a block. (Absent blocks: page 0's, never used.)
-#pragma unroll
-        for (int i = 0; i < 4 * CB / NT; ++i) {
-          const int c = (i * NW + wave) * 64;   // first chunk: K's 2 CB, then V's
-          const bool isv = c >= 2 * CB;
-          const int cs = isv ? c - 2 * CB : c;
-          const long long at = cs >= CB ? a1 : a0;
-          const unsigned char* src = (isv ? p.v_pages : p.k_pages) +
-                                     ((size_t)(at < 0 ? 0 : at) * 2 + (size_t)(cs >= CB ? cs - CB : cs) * 16);
-          dma16(src, lane * 16, lds_addr((isv ? vbuf[buf] : kbuf[buf]) + cs * 8));
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < LD; ++i) {
-          const int c = i * NT + tid;
-          if (c >= 2 * CB) break;
-          const long long at = c >= CB ? a1 : a0;
-          const size_t o = (size_t)(at < 0 ? 0 : at) + (size_t)(c >= CB ? c - CB : c) * 16;
-          kr[i] = *reinterpret_cast<const u32x4*>(p.k_pages + o);
-          vr[i] = *reinterpret_cast<const u32x4*>(p.v_pages + o);
-        }
-        if (tid < kStepKeys) {
-          const long long at = tid >= 32 ? a1 : a0;
-          const size_t o = (size_t)(at < 0 ? 0 : at) / D + (tid & 31);
-          kscale = p.k_scales[o];
-          vscale = p.v_scales[o];
-        }
-      }
-    };
-    auto store = [&](int buf) {   // 8 bits
-#pragma unroll
-      for (int i = 0; i < LD; ++i) {
-        const int c = i * NT + tid;
-        if (c >= 2 * CB) break;
-        const int cb = c >= CB ? c - CB : c;
-        const int o = (c >= CB ? BE : 0) + (2 * (cb >> 6) * 64 + (cb & 63)) * 8;
-        *reinterpret_cast<u32x4*>(&kbuf[buf][o]) = widen8(kr[i].x, kr[i].y);
-        *reinterpret_cast<u32x4*>(&kbuf[buf][o + 512]) = widen8(kr[i].z, kr[i].w);
-        *reinterpret_cast<u32x4*>(&vbuf[buf][o]) = widen8(vr[i].x, vr[i].y);
-        *reinterpret_cast<u32x4*>(&vbuf[buf][o + 512]) = widen8(vr[i].z, vr[i].w);
-      }
-      if (tid < kStepKeys) {
-        ksc[buf][tid] = kscale * p.scale_log2;
-        vsc[buf][tid] = vscale;
-      }
-    };
     // Steps [0, nfull) hide no key from any of the wave's rows and have all
-    // their pages: they run in a loop of their own.
-    int nfull = 0;
-    if (row0 < rows && wmin + 1 - ka >= kStepKeys) nfull = (int)((wmin + 1 - ka) / kStepKeys);
-    if (nfull > nstep) nfull = nstep;
+    // their pages; [nfull, nlive) hide some; the rest hides all.
+    int nfull = 0, nlive = 0;
+    if (wmax >= ka) nlive = wmax >= kb ? nstep : (int)((wmax - ka) / kStepKeys) + 1;
+    if (nlive > 0 && wmin + 1 - ka >= kStepKeys) nfull = (int)((wmin + 1 - ka) / kStepKeys);
+    if (nfull > nlive) nfull = nlive;
     auto cut = [&](int st) {   // the list begins at step st: its steps before the first absent block
       const int lead = st + (blocks.present() >> 1);
       if (lead < nfull && lead < st + 32) nfull = lead;
     };
     cut(0);
-    auto full = [&](int buf) {
-      constexpr int KB = BITS == 8 || D == 256 ? 1 : 2;   // blocks at a time, as registers allow
-      const uint16_t* kl = &kbuf[buf][lane * 8];
-      const uint16_t* vl = &vbuf[buf][lane * 8];
-      const float* kss = &ksc[buf & 1][4 * h2];
-      const float* vss = &vsc[buf & 1][4 * h2];
+    // A list that step st ends is replaced while steps from `from` on still use
+    // it: lists overlap.
+    const int blk0 = ka >> 5, blk1 = (kb + 31) >> 5;
+    auto cover = [&](int from, int st) {
+      if (blk0 + 2 * st + 2 > blocks.first + 64) {
+        blocks.fill(p, b, u.h, blk0 + 2 * from, blk1, lane);
+        cut(from);
+      }
+    };
+    u32x4 kr[LD], vr[LD];   // a step's K and V on their way to LDS
+    float kscale = 0.f, vscale = 0.f;
+    // The thread's share of K and V of step st (past the last: the last one's
+    // again, never used).
+    auto load = [&](int st, bool isv) {
+      const int blk = blk0 + 2 * (st < nstep ? st : nstep - 1);
+      const int a0 = blocks.get(blk), a1 = blocks.get(blk + 1);
+      const unsigned char* pool = isv ? p.v_pages : p.k_pages;
 #pragma unroll
-      for (int j0 = 0; j0 < 2; j0 += KB)
-        attend<D, BITS, NB, KB, false, D < 256>(
-            s, 0, 0, h2, p.scale_log2,
-            [&](int j, int i) { return *reinterpret_cast<const u32x4*>(kl + (j0 + j) * BE + i * 512); },
-            [&](int j, int t, int jj) { return *reinterpret_cast<const u32x4*>(vl + (j0 + j) * BE + (2 * t + jj) * 512); },
-            [&](int j, int r) { return kss[32 * (j0 + j) + 8 * (r >> 2) + (r & 3)]; },
-            [&](int j, int r) { return vss[32 * (j0 + j) + 8 * (r >> 2) + (r & 3)]; });
-    };
-    auto masked = [&](int st, int buf) {
-      const int kt = ka + st * kStepKeys;
-      const uint16_t* kl = &kbuf[buf][lane * 8];
-      const uint16_t* vl = &vbuf[buf][lane * 8];
-      const float* kss = &ksc[buf & 1][4 * h2];
-      const float* vss = &vsc[buf & 1][4 * h2];
-#pragma unroll 1
-      for (int j = 0; j < 2; ++j) {
-        if (kt + 32 * j > wmax || base(st, j) < 0) continue;
-        attend<D, BITS, NB, 1, true, D < 256>(
-            s, kt + 32 * j, u.nk, h2, p.scale_log2,
-            [&](int, int i) { return *reinterpret_cast<const u32x4*>(kl + j * BE + i * 512); },
-            [&](int, int t, int jj) { return *reinterpret_cast<const u32x4*>(vl + j * BE + (2 * t + jj) * 512); },
-            [&](int, int r) { return kss[32 * j + 8 * (r >> 2) + (r & 3)]; },
-            [&](int, int r) { return vss[32 * j + 8 * (r >> 2) + (r & 3)]; });
+      for (int i = 0; i < LD; ++i) {
+        const int c = i * NT + wave * 64;   // the wave's first chunk: uniform, 64 chunks lie in one block
+        if (2 * CB % NT && c >= 2 * CB) break;
+        const bool second = CB % NT ? c >= CB : i * NT >= CB;
+        const unsigned char* src = pool + (size_t)(second ? a1 : a0) * (CB * 16) + (second ? c - CB : c) * 16;
+        const u32x4 r = *reinterpret_cast<const u32x4*>(src + (uint32_t)(lane * 16));
+        if (isv) vr[i] = r; else kr[i] = r;
+      }
+      if (BITS == 8 && !isv && tid < kStepKeys) {
+        const size_t o = (size_t)(tid >= 32 ? a1 : a0) * kBlk + (tid & 31);
+        kscale = p.k_scales[o];
+        vscale = p.v_scales[o];
       }
     };
-    // The list is replaced while step st still uses it: lists overlap by the steps in flight.
-    auto load_ahead = [&](int st, int next, int buf) {
-      const int blk = (ka >> 5) + 2 * next;
-      if (blk + 2 > blocks.first + 64) {
-        blocks.fill(p, b, u.h, (ka >> 5) + 2 * st, (kb + 31) >> 5, lane, BE);
-        cut(st);
-      }
-      load(next, buf);
+    auto load_next = [&](int n) {   // with step n's products
+      load(n + 2, false);
+      load(n + VR - 1, true);
     };
-    __syncthreads();   // the previous piece's reads are done
-    if constexpr (BITS == 16) {
-      constexpr int PER = 4 * CB / NT;   // loads of a wave per step
-      for (int i = 0; i < NBUF - 1 && i < nstep; ++i) load(i, i);
-      int buf = 0;
-      auto meet = [&](int st) {   // step st is in LDS, of every wave; the one before it is read
-        if (NBUF == 3 && st + 1 < nstep) wait_vm<PER>();
-        else wait_vm<0>();
-        lds_barrier();
-        if (st + NBUF - 1 < nstep) load_ahead(st, st + NBUF - 1, buf == 0 ? NBUF - 1 : buf - 1);
+    auto put = [&](uint32_t dst, const u32x4 (&r)[LD]) {   // LDS addresses
+#pragma unroll
+      for (int i = 0; i < LD; ++i) {
+        const int c = i * NT + wave * 64;
+        if (2 * CB % NT && c >= 2 * CB) break;
+        lds_u32x4* d = reinterpret_cast<lds_u32x4*>(dst + lane * 16 + c * (BITS == 16 ? 16 : 32));
+        if constexpr (BITS == 16) {
+          d[0] = r[i];
+        } else {   // 64 chunks of 16 integers to two operands of 64 x 8
+          d[0] = widen8(r[i].x, r[i].y);
+          d[64] = widen8(r[i].z, r[i].w);
+        }
+      }
+    };
+    // Ring slots: K of steps n and n + 1; V of n - 1, n and (of three) n + 1.
+    int k0 = 0, k1 = 1, v0 = VR - 1, v1 = 0, v2 = 1;
+    auto turn_ring = [&] {
+      const int k = k0, v = v0;
+      k0 = k1;
+      k1 = k;
+      v0 = v1;
+      v1 = VR == 3 ? v2 : v;
+      v2 = v;
+    };
+    auto store_k = [&](int n) {   // of step n (slot k1 when n is the next step)
+      put(klds + k1 * (4 * BE), kr);
+      if (BITS == 8 && tid < kStepKeys) {
+        ksc[n & 3][tid] = kscale * p.scale_log2;
+        vsc[n & 3][tid] = vscale;
+      }
+    };
+    auto store_v = [&] { put(vlds + (VR == 3 ? v2 : v1) * (4 * BE), vr); };   // of step n + 1 (two slots: n)
+    f32x16 st[2];
+    u32x4 w[2][2];
+    u32x4 op[2][D / 16];
+    // Operands from a ring slot: one address, offsets in the instructions.
+    auto operands = [&](uint32_t lds, int ring) {
+      uint32_t a = lds + ring * (4 * BE) + lane * 16;
+      asm("" : "+v"(a));
+      return reinterpret_cast<const lds_u32x4*>(a);
+    };
+    auto ask = [&](u32x4 (&to)[D / 16], const lds_u32x4* from, int j) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) to[i] = from[(j * (D / 16) + i) * 64];
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    auto keys = [&] {
+      const lds_u32x4* k = operands(klds, k0);
+      scores<D, 2>(s, st, [&](int j, int i) { return k[(j * (D / 16) + i) * 64]; });
+    };
+    auto ends2 = [&](int n, int j) { return blocks.absent(blk0 + 2 * n + j) ? 0 : u.nk; };
+    auto values = [&](int n) {   // of step n, masked; slot v0 when n is the last step
+      const lds_u32x4* v = operands(vlds, v0);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        add_values<D, BITS, true>(s, w[j], ka + n * kStepKeys + 32 * j, ends2(n, j), h2,
+                                  [&](int t, int jj) { return v[(j * (D / 16) + 2 * t + jj) * 64]; });
+    };
+    // Both products of step n, no key hidden: each eight operands are asked for
+    // eight matrix instructions ahead (left alone, the compiler reads one, waits
+    // for it and multiplies); op[0] is in hand.
+    auto products = [&](int n) {
+      const lds_u32x4* v = operands(vlds, v0);
+      const lds_u32x4* k = operands(klds, k0);
+      auto add = [&](const u32x4 (&from)[D / 16], int j) {
+        add_values<D, BITS, false>(s, w[j], 0, 0, h2, [&](int t, int jj) { return from[2 * t + jj]; });
+        __builtin_amdgcn_sched_barrier(0);
       };
-      for (int st = 0; st < nfull; ++st) {
-        meet(st);
-        full(buf);
-        buf = buf == NBUF - 1 ? 0 : buf + 1;
-      }
-      for (int st = nfull; st < nstep; ++st) {
-        meet(st);
-        masked(st, buf);
-        buf = buf == NBUF - 1 ? 0 : buf + 1;
-      }
-    } else {
-      if (nstep > 0) {
-        load(0, 0);
-        store(0);
-      }
-      __syncthreads();
-      auto next = [&](int st) {
-        if (st + 1 < nstep) store((st + 1) & 1);
-        __syncthreads();
+      auto score = [&](const u32x4 (&from)[D / 16], int j) {
+        f32x16 one[1];
+        scores<D, 1>(s, one, [&](int, int i) { return from[i]; });
+        st[j] = one[0];
+        __builtin_amdgcn_sched_barrier(0);
       };
-      for (int st = 0; st < nfull; ++st) {
-        if (st + 1 < nstep) load_ahead(st, st + 1, 0);
-        full(st & 1);
-        next(st);
+      if (VR == 2) ask(op[0], v, 0);
+      ask(op[1], v, 1);
+      add(op[0], 0);
+      ask(op[0], k, 0);
+      store_k(n + 1);
+      add(op[1], 1);
+      ask(op[1], k, 1);
+      store_v();
+      score(op[0], 0);
+      load_next(n);
+      score(op[1], 1);
+    };
+    // Scores to weights. (They are not to be touched before the barrier that ends
+    // the products phase: moved ahead of it, the softmax would keep the other
+    // waves waiting.)
+    auto weights = [&](int n, auto mask) {
+      constexpr bool MASK = decltype(mask)::value;
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("" : "+v"(st[0]), "+v"(st[1]));
+      const float* kss = &ksc[n & 3][4 * h2];
+      const float* vss = &vsc[n & 3][4 * h2];
+      const int end[2] = {MASK ? ends2(n, 0) : 0, MASK ? ends2(n, 1) : 0};
+      soften<D, BITS, 2, MASK>(
+          s, st, w, ka + n * kStepKeys, end, h2, p.scale_log2,
+          [&](int j, int r) { return kss[32 * j + 8 * (r >> 2) + (r & 3)]; },
+          [&](int j, int r) { return vss[32 * j + 8 * (r >> 2) + (r & 3)]; });
+    };
+    auto look_ahead = [&] {   // the next products' first operands: V of the step just softened
+      if (VR == 3) ask(op[0], operands(vlds, v0), 0);
+    };
+    constexpr std::true_type yes;
+    constexpr std::false_type no;
+    lds_barrier();   // the previous piece's reads are done
+    if (nstep > 0) {
+      // Step 0 in LDS (its V on the way, of two slots), step 1 on its way.
+      load(0, false);
+      load(0, true);
+      put(klds, kr);
+      if (BITS == 8 && tid < kStepKeys) {
+        ksc[0][tid] = kscale * p.scale_log2;
+        vsc[0][tid] = vscale;
       }
-      for (int st = nfull; st < nstep; ++st) {
-        if (st + 1 < nstep) load_ahead(st, st + 1, 0);
-        masked(st, st & 1);
-        next(st);
+      load(1, false);
+      if (VR == 3) {
+        put(vlds, vr);
+        load(1, true);
+      }
+      lds_barrier();
+      auto stage = [&](int n) {   // what goes with step n's products
+        store_k(n + 1);
+        store_v();
+        cover(n > 0 ? n - 1 : 0, n + 2);
+        load_next(n);
+      };
+      auto between = [&] {   // products and softmax
+        if (turn) lds_barrier();
+      };
+      auto after = [&] {
+        turn_ring();
+        if (!turn) lds_barrier();
+      };
+      // Full steps, then steps that may hide keys, then (for the other waves)
+      // staging alone; straight lines between, so the accumulators stay where
+      // they are.
+      int n = 0;
+      if (nfull > 0) {
+        keys();
+        stage(0);
+        between();
+        weights(0, no);
+        after();
+        look_ahead();
+        for (n = 1; n < nfull; ++n) {
+          cover(n - 1, n + 2);
+          products(n);
+          between();
+          weights(n, no);
+          after();
+          look_ahead();
+        }
+      } else if (nlive > 0) {
+        keys();
+        stage(0);
+        between();
+        weights(0, yes);
+        after();
+        n = 1;
+      }
+      for (; n < nlive; ++n) {
+        values(n - 1);
+        keys();
+        stage(n);
+        between();
+        weights(n, yes);
+        after();
+      }
+      if (nlive > 0) values(nlive - 1);
+      for (; n < nstep; ++n) {
+        stage(n);
+        between();
+        after();
       }
     }
     // Out: the whole tile's rows, or this piece's partial.
     const int slot = 2 * g + (starts ? 1 : 0);
-    const bool whole = starts && ends;
+    const int r = row0 + (lane & 31);
+    const float l = s.l + __shfl_xor(s.l, 32, 64);
+    if (r >= rows) continue;
+    if (starts && ends) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      uint16_t* dst = out_row(p, rq.lo + u.t * p.P, u.h, r);
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      const int r = row0 + 32 * n + (lane & 31);
-      if (r >= rows) continue;
-      const float l = s.l[n] + __shfl_xor(s.l[n], 32, 64);
-      if (whole) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        uint16_t* dst = out_row(p, rq.lo + u.t * p.P, u.h, r);
+      for (int t = 0; t < D / 32; ++t)
 #pragma unroll
-        for (int t = 0; t < D / 32; ++t)
+        for (int j = 0; j < 4; ++j)
+          store4(dst + 32 * t + 8 * j + 4 * h2, s.o[t][4 * j] * inv, s.o[t][4 * j + 1] * inv, s.o[t][4 * j + 2] * inv,
+                 s.o[t][4 * j + 3] * inv);
+    } else {   // (a piece without keys leaves m = -infinity, l = 0, and its o is not read)
+      float* po = p.part_o + ((size_t)slot * RT + r) * D;
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            store4(dst + 32 * t + 8 * j + 4 * h2, s.o[n][t][4 * j] * inv, s.o[n][t][4 * j + 1] * inv,
-                   s.o[n][t][4 * j + 2] * inv, s.o[n][t][4 * j + 3] * inv);
-      } else {   // (a piece without keys leaves m = -infinity, l = 0, and its o is not read)
-        float* po = p.part_o + ((size_t)slot * RT + r) * D;
+      for (int t = 0; t < D / 32; ++t)
 #pragma unroll
-        for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<float4*>(po + 32 * t + 8 * j + 4 * h2) =
-                make_float4(s.o[n][t][4 * j], s.o[n][t][4 * j + 1], s.o[n][t][4 * j + 2], s.o[n][t][4 * j + 3]);
-        if (h2 == 0) {
-          float* ml = p.part_ml + ((size_t)slot * RT + r) * 2;
-          ml[0] = s.m[n];
-          ml[1] = l;
-        }
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<float4*>(po + 32 * t + 8 * j + 4 * h2) =
+              make_float4(s.o[t][4 * j], s.o[t][4 * j + 1], s.o[t][4 * j + 2], s.o[t][4 * j + 3]);
+      if (h2 == 0) {
+        float* ml = p.part_ml + ((size_t)slot * RT + r) * 2;
+        ml[0] = s.m;
+        ml[1] = l;
       }
     }
   }
@@ -744,8 +798,8 @@ __global__ __launch_bounds__(kPT) void attn_few_kernel(PAttn p) {
     x = end;
     if (starts && !ends && tid == 0) note_begun(p, line, rq, u, g);
     const int rows = u.n * p.rep;
-    RowState<D, 1> s;
-    load_rows<D, 1>(s, p, rq, u, 0, lane);
+    RowState<D> s;
+    load_rows<D>(s, p, rq, u, 0, lane);
     const long long wmin = u.pos < u.nk - 1 ? u.pos : u.nk - 1;   // blocks up to it hide no key
     const int nblk = (kb - ka + kBlk - 1) / kBlk;
     const int k0 = ka + (nblk * wave / 4) * kBlk;
@@ -754,9 +808,9 @@ __global__ __launch_bounds__(kPT) void attn_few_kernel(PAttn p) {
     u32x4 kr[LD], vr[LD];
     float4 kq[4], vq[4];   // scales of the lane's keys
     BlockList blocks;
-    if (k0 < k1) blocks.fill(p, b, u.h, k0 >> 5, (k1 + 31) >> 5, lane, BE);
-    auto load = [&](long long at) {
-      const size_t o = (size_t)(at < 0 ? 0 : at);
+    if (k0 < k1) blocks.fill(p, b, u.h, k0 >> 5, (k1 + 31) >> 5, lane);
+    auto load = [&](int at) {
+      const size_t o = (size_t)at * BE;
 #pragma unroll
       for (int i = 0; i < LD; ++i) kr[i] = ld_nt(p.k_pages + o * (BITS / 8) + (size_t)(i * 64 + lane) * 16);
 #pragma unroll
@@ -770,39 +824,44 @@ __global__ __launch_bounds__(kPT) void attn_few_kernel(PAttn p) {
       }
     };
     if (k0 < k1) {
-      long long at = blocks.get(k0 >> 5);
-      load(at);
+      load(blocks.get(k0 >> 5));
       for (int kt = k0; kt < k1; kt += kBlk) {
-        if (at >= 0) {   // uniform
+        if (!blocks.absent(kt >> 5)) {   // uniform
           auto kop = [&](int, int i) {
             if constexpr (BITS == 16) return kr[i];
             else return (i & 1) ? widen8(kr[i >> 1].z, kr[i >> 1].w) : widen8(kr[i >> 1].x, kr[i >> 1].y);
           };
-          auto vop = [&](int, int t, int jj) {
+          auto vop = [&](int t, int jj) {
             if constexpr (BITS == 16) return vr[2 * t + jj];
             else return jj ? widen8(vr[t].z, vr[t].w) : widen8(vr[t].x, vr[t].y);
           };
           auto part = [](const float4& f, int e) { return e == 0 ? f.x : e == 1 ? f.y : e == 2 ? f.z : f.w; };
           auto ks = [&](int, int r) { return part(kq[r >> 2], r & 3) * p.scale_log2; };
           auto vs = [&](int, int r) { return part(vq[r >> 2], r & 3); };
-          if (kt + 31 <= wmin)
-            attend<D, BITS, 1, 1, false, false>(s, kt, u.nk, h2, p.scale_log2, kop, vop, ks, vs);
-          else
-            attend<D, BITS, 1, 1, true, false>(s, kt, u.nk, h2, p.scale_log2, kop, vop, ks, vs);
+          f32x16 st[1];
+          u32x4 w[1][2];
+          const int end[1] = {u.nk};
+          scores<D, 1>(s, st, kop);
+          if (kt + 31 <= wmin) {
+            soften<D, BITS, 1, false>(s, st, w, kt, end, h2, p.scale_log2, ks, vs);
+            add_values<D, BITS, false>(s, w[0], kt, u.nk, h2, vop);
+          } else {
+            soften<D, BITS, 1, true>(s, st, w, kt, end, h2, p.scale_log2, ks, vs);
+            add_values<D, BITS, true>(s, w[0], kt, u.nk, h2, vop);
+          }
         }
         if (kt + kBlk < k1) {
           const int blk = (kt >> 5) + 1;
-          if (blk >= blocks.first + 64) blocks.fill(p, b, u.h, blk, (k1 + 31) >> 5, lane, BE);
-          at = blocks.get(blk);
-          load(at);
+          if (blk >= blocks.first + 64) blocks.fill(p, b, u.h, blk, (k1 + 31) >> 5, lane);
+          load(blocks.get(blk));
         }
       }
     }
     // The waves' parts, in wave order.
-    const float l = s.l[0] + __shfl_xor(s.l[0], 32, 64);
+    const float l = s.l + __shfl_xor(s.l, 32, 64);
     __syncthreads();   // the previous piece's reads are done
     if (h2 == 0) {
-      s_m[wave][c32] = s.m[0];
+      s_m[wave][c32] = s.m;
       s_l[wave][c32] = l;
     }
 #pragma unroll
@@ -810,7 +869,7 @@ __global__ __launch_bounds__(kPT) void attn_few_kernel(PAttn p) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         *reinterpret_cast<float4*>(&s_o[wave][c32 * OS + 32 * t + 8 * j + 4 * h2]) =
-            make_float4(s.o[0][t][4 * j], s.o[0][t][4 * j + 1], s.o[0][t][4 * j + 2], s.o[0][t][4 * j + 3]);
+            make_float4(s.o[t][4 * j], s.o[t][4 * j + 1], s.o[t][4 * j + 2], s.o[t][4 * j + 3]);
     __syncthreads();
     const int slot = 2 * g + (starts ? 1 : 0);
     const bool whole = starts && ends;
