@@ -53,12 +53,23 @@ struct PAttn {
   float* part_ml;   // [2 G][rows of a tile][2]
   int4* begun;      // [G]: the tile that workgroup g began and others finish
   int T, B, width, Hq, Hkv, rep, bpp, num_pages;
+  uint32_t rep_inv;   // row / rep = row * rep_inv >> 16 for rows below 2048
   int P;            // tokens of a row tile
   int G;            // most workgroups
   int min_share;    // least keys of a workgroup's share
   float scale_log2;
   long long q_token, q_head, out_token, out_head;
 };
+
+// Token and head (of those that share a kv head) of a row of a tile's list.
+__device__ __forceinline__ int row_token(const PAttn& p, int r) { return (int)(((uint32_t)r * p.rep_inv) >> 16); }
+
+// The same value, computed here: what follows from it is not kept in registers
+// across the key loop (a spill's reload waits for every load in flight).
+__device__ __forceinline__ int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
 
 // -- the line of work -------------------------------------------------------------
 
@@ -194,6 +205,23 @@ __device__ __forceinline__ Tile tile_at(const PAttn& p, const Req& r, long long 
   const long long e = u.pos + u.n;
   u.nk = (int)(e < 0 ? 0 : e > cap ? cap : e);
   return u;
+}
+
+// The tile after u on the line, in the same request.
+__device__ __forceinline__ void next_tile(const PAttn& p, const Req& r, Tile& u) {
+  u.begin += u.len;
+  ++u.t;
+  if (u.t * p.P >= r.n) {
+    u.t = 0;
+    ++u.h;
+  }
+  const int left = r.n - u.t * p.P;
+  u.n = left < p.P ? left : p.P;
+  u.len = clamp_start(p, r.start) + kTileCost + u.t * p.P + u.n;
+  u.pos = r.start + (long long)u.t * p.P;
+  const long long cap = (long long)p.width * p.bpp * kBlk;
+  const long long e = u.pos + u.n;
+  u.nk = (int)(e < 0 ? 0 : e > cap ? cap : e);
 }
 
 // Keys [0, key_at(x)) of the tile lie before offset x of its line: whole steps
@@ -394,26 +422,60 @@ struct BlockList {
   __device__ __forceinline__ int present() const { return gone ? __ffsll((long long)gone) - 1 : 64; }
 };
 
-// Rows row0 .. of a tile (row r of the list: token r / rep, head r % rep).
+// Rows row0 .. of a tile (row r of the list: token r / rep, head r % rep), 32 of
+// a wave. A lane's operands lie all over its row, so the rows come whole, 16
+// bytes a lane, and turn through LDS (RB bytes a row, the wave's own).
 template <int D>
-__device__ __forceinline__ void load_rows(RowState<D>& s, const PAttn& p, const Req& rq, const Tile& u, int row0,
-                                          int lane) {
+constexpr int row_bytes() { return D * 2 + 16; }   // (reads of 8 rows hit distinct banks)
+
+template <int D>
+struct RowLoads {
+  u32x4 r[D / 16];
+};
+template <int D>
+__device__ __forceinline__ void ask_rows(RowLoads<D>& q, const PAttn& p, const Req& rq, const Tile& u, int row0,
+                                         int lane) {
+  constexpr int LPR = D / 8;   // lanes of a row
+  lane = fresh(lane);
+#pragma unroll
+  for (int j = 0; j < D / 16; ++j) {
+    const int r = row0 + j * (64 / LPR) + lane / LPR;
+    int i = row_token(p, r), g = r - i * p.rep;
+    if (i >= u.n) i = g = 0;   // no row here: any
+    const long long tok = rq.lo + (long long)u.t * p.P + i;
+    q.r[j] = *reinterpret_cast<const u32x4*>(p.q + tok * p.q_token + (long long)(u.h * p.rep + g) * p.q_head +
+                                             lane % LPR * 8);
+  }
+}
+template <int D>
+__device__ __forceinline__ void take_rows(RowState<D>& s, const RowLoads<D>& q, const PAttn& p, const Tile& u, int row0,
+                                          int lane, unsigned char* lds) {
+  constexpr int LPR = D / 8, RB = row_bytes<D>();
+  lane = fresh(lane);
+#pragma unroll
+  for (int j = 0; j < D / 16; ++j)
+    *reinterpret_cast<u32x4*>(lds + (j * (64 / LPR) + lane / LPR) * RB + lane % LPR * 16) = q.r[j];
   const int h2 = lane >> 5, r = row0 + (lane & 31);
-  const int i = r / p.rep, g = r - i * p.rep;
+  const int i = row_token(p, r);
   const bool valid = i < u.n;
   const long long pos = u.pos + i;
   s.bound = !valid || pos < 0 ? -1 : pos < u.nk ? (int)pos : u.nk - 1;
-  const long long tok = rq.lo + (long long)u.t * p.P + (valid ? i : 0);
-  const uint16_t* row = p.q + tok * p.q_token + (long long)(u.h * p.rep + (valid ? g : 0)) * p.q_head;
 #pragma unroll
   for (int j = 0; j < D / 16; ++j) {
-    const u32x4 raw = *reinterpret_cast<const u32x4*>(row + (D / 2) * h2 + 8 * j);
+    const u32x4 raw = *reinterpret_cast<const u32x4*>(lds + (lane & 31) * RB + D * h2 + 16 * j);
     s.q[j] = __builtin_bit_cast(bf16x8, valid ? raw : u32x4{0, 0, 0, 0});
   }
 #pragma unroll
   for (int t = 0; t < D / 32; ++t) s.o[t] = f32x16{};
   s.m = -INFINITY;
   s.l = 0.f;
+}
+
+// Partials: float4 e of (32 rows, 32 d) block (row block, t) is row e % 32 and
+// d = 4 (e / 32): the registers' own order, 1 KB a store.
+template <int D>
+__device__ __forceinline__ float4* part_block(const PAttn& p, size_t slot, int RT, int rb, int t) {
+  return reinterpret_cast<float4*>(p.part_o) + ((slot * (RT / 32) + rb) * (D / 32) + t) * 256;
 }
 
 // 16 bytes read once per launch (non-temporal, as ld_stream).
@@ -428,7 +490,7 @@ __device__ __forceinline__ void store4(uint16_t* dst, float a, float b, float c,
 
 // Row r of the tile whose first token is `token` (packed), of kv head h.
 __device__ __forceinline__ uint16_t* out_row(const PAttn& p, int token, int h, int r) {
-  const int i = r / p.rep, g = r - i * p.rep;
+  const int i = row_token(p, r), g = r - i * p.rep;
   return p.out + ((long long)token + i) * p.out_token + (long long)(h * p.rep + g) * p.out_head;
 }
 
@@ -475,8 +537,8 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
   // K of a step lives for two phases and is written in the two before; V lives
   // for four (at D = 256, where no wave runs half a step behind, for two).
   constexpr int KR = 2, VR = D == 256 ? 2 : 3;
-  __shared__ __attribute__((aligned(16))) uint16_t kbuf[KR][2 * BE];
-  __shared__ __attribute__((aligned(16))) uint16_t vbuf[VR][2 * BE];
+  __shared__ __attribute__((aligned(16))) unsigned char lds[(KR + VR) * 4 * BE];   // K slots, then V's
+  static_assert(NW * 32 * row_bytes<D>() <= (KR + VR) * 4 * BE, "a wave's rows turn in the slots' place");
   __shared__ __attribute__((aligned(16))) float ksc[4][kStepKeys], vsc[4][kStepKeys];   // (of step n - 1 to n + 1)
   const int tid = threadIdx.x, lane = tid & 63, h2 = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -490,12 +552,17 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
   if (tid == 0) p.begun[g] = make_int4(0, 0, 0, 0);
   const long long lo = line.lo(g), hi = line.hi(g);
   const int turn = NW == 8 && wave >= 4 ? 1 : 0;
-  const uint32_t klds = lds_addr(kbuf), vlds = lds_addr(vbuf);
+  const uint32_t klds = lds_addr(lds), vlds = klds + KR * 4 * BE;
   Req rq;
   int b = line.find(p, lane, lo, rq);
+  Tile u = tile_at(p, rq, lo);
   for (long long x = lo; x < hi;) {
-    if (x >= rq.base + p.Hkv * rq.head) b = line.find(p, lane, x, rq);
-    const Tile u = tile_at(p, rq, x);
+    if (x >= rq.base + p.Hkv * rq.head) {
+      b = line.find(p, lane, x, rq);
+      u = tile_at(p, rq, x);
+    } else if (x >= u.begin + u.len) {
+      next_tile(p, rq, u);
+    }
     const long long end = hi < u.begin + u.len ? hi : u.begin + u.len;
     const int ka = key_at(u, x - u.begin, kStepKeys), kb = key_at(u, end - u.begin, kStepKeys);
     const bool starts = x == u.begin, ends = end == u.begin + u.len;
@@ -503,13 +570,13 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
     if (starts && !ends && tid == 0) note_begun(p, line, rq, u, g);
     const int row0 = wave * 32;
     const int rows = u.n * p.rep;   // of the tile
-    RowState<D> s;
-    load_rows<D>(s, p, rq, u, row0, lane);
+    RowLoads<D> ql;
+    ask_rows<D>(ql, p, rq, u, row0, lane);
     // Bounds of the wave's rows: steps behind wmax are skipped, steps up to
     // wmin need no mask (rows past the list are computed on zeros, and dropped).
     const int last = (row0 + 32 < rows ? row0 + 32 : rows) - 1;
-    long long wmin = u.pos + row0 / p.rep;
-    const long long wmax = row0 < rows ? u.pos + last / p.rep : -1;
+    long long wmin = u.pos + row_token(p, row0);
+    const long long wmax = row0 < rows ? u.pos + row_token(p, last) : -1;
     if (wmin > u.nk - 1) wmin = u.nk - 1;
 
     BlockList blocks;
@@ -594,6 +661,13 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
       }
     };
     auto store_v = [&] { put(vlds + (VR == 3 ? v2 : v1) * (4 * BE), vr); };   // of step n + 1 (two slots: n)
+    if (nstep > 0) {   // step 0 in LDS (its V on the way, of two slots), step 1 on its way
+      load(0, false);
+      load(0, true);
+    }
+    unsigned char* const mine = lds + wave * (32 * row_bytes<D>());   // (of no step: between pieces)
+    RowState<D> s;
+    take_rows<D>(s, ql, p, u, row0, lane, mine);
     f32x16 st[2];
     u32x4 w[2][2];
     u32x4 op[2][D / 16];
@@ -668,11 +742,8 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
     };
     constexpr std::true_type yes;
     constexpr std::false_type no;
-    lds_barrier();   // the previous piece's reads are done
+    lds_barrier();   // every wave has its rows
     if (nstep > 0) {
-      // Step 0 in LDS (its V on the way, of two slots), step 1 on its way.
-      load(0, false);
-      load(0, true);
       put(klds, kr);
       if (BITS == 8 && tid < kStepKeys) {
         ksc[0][tid] = kscale * p.scale_log2;
@@ -739,30 +810,37 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
         after();
       }
     }
-    // Out: the whole tile's rows, or this piece's partial.
-    const int slot = 2 * g + (starts ? 1 : 0);
-    const int r = row0 + (lane & 31);
+    // Out: the whole tile's rows (turned through LDS, as they came), or this
+    // piece's partial (without keys: m = -infinity, l = 0, and its o is not read).
     const float l = s.l + __shfl_xor(s.l, 32, 64);
-    if (r >= rows) continue;
+    lds_barrier();   // every wave is done with the slots
+    const int ln = fresh(lane);
     if (starts && ends) {
+      constexpr int LPR = D / 8, RB = row_bytes<D>();
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      uint16_t* dst = out_row(p, rq.lo + u.t * p.P, u.h, r);
 #pragma unroll
       for (int t = 0; t < D / 32; ++t)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          store4(dst + 32 * t + 8 * j + 4 * h2, s.o[t][4 * j] * inv, s.o[t][4 * j + 1] * inv, s.o[t][4 * j + 2] * inv,
-                 s.o[t][4 * j + 3] * inv);
-    } else {   // (a piece without keys leaves m = -infinity, l = 0, and its o is not read)
-      float* po = p.part_o + ((size_t)slot * RT + r) * D;
+          store4(reinterpret_cast<uint16_t*>(mine + (ln & 31) * RB) + 32 * t + 8 * j + 4 * (ln >> 5), s.o[t][4 * j] * inv,
+                 s.o[t][4 * j + 1] * inv, s.o[t][4 * j + 2] * inv, s.o[t][4 * j + 3] * inv);
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        const int r = j * (64 / LPR) + ln / LPR;
+        const u32x4 v = *reinterpret_cast<const u32x4*>(mine + r * RB + ln % LPR * 16);
+        if (row0 + r < rows)
+          *reinterpret_cast<u32x4*>(out_row(p, rq.lo + u.t * p.P, u.h, row0 + r) + ln % LPR * 8) = v;
+      }
+    } else if (row0 < rows) {
+      const size_t slot = 2 * (size_t)g + (starts ? 1 : 0);
 #pragma unroll
       for (int t = 0; t < D / 32; ++t)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          *reinterpret_cast<float4*>(po + 32 * t + 8 * j + 4 * h2) =
+          part_block<D>(p, slot, RT, wave, t)[j * 64 + ln] =
               make_float4(s.o[t][4 * j], s.o[t][4 * j + 1], s.o[t][4 * j + 2], s.o[t][4 * j + 3]);
-      if (h2 == 0) {
-        float* ml = p.part_ml + ((size_t)slot * RT + r) * 2;
+      if (ln < 32) {
+        float* ml = p.part_ml + (slot * RT + row0 + ln) * 2;
         ml[0] = s.m;
         ml[1] = l;
       }
@@ -789,9 +867,14 @@ __global__ __launch_bounds__(kPT) void attn_few_kernel(PAttn p) {
   const long long lo = line.lo(g), hi = line.hi(g);
   Req rq;
   int b = line.find(p, lane, lo, rq);
+  Tile u = tile_at(p, rq, lo);
   for (long long x = lo; x < hi;) {
-    if (x >= rq.base + p.Hkv * rq.head) b = line.find(p, lane, x, rq);
-    const Tile u = tile_at(p, rq, x);
+    if (x >= rq.base + p.Hkv * rq.head) {
+      b = line.find(p, lane, x, rq);
+      u = tile_at(p, rq, x);
+    } else if (x >= u.begin + u.len) {
+      next_tile(p, rq, u);
+    }
     const long long end = hi < u.begin + u.len ? hi : u.begin + u.len;
     const int ka = key_at(u, x - u.begin, kBlk), kb = key_at(u, end - u.begin, kBlk);
     const bool starts = x == u.begin, ends = end == u.begin + u.len;
@@ -799,7 +882,12 @@ __global__ __launch_bounds__(kPT) void attn_few_kernel(PAttn p) {
     if (starts && !ends && tid == 0) note_begun(p, line, rq, u, g);
     const int rows = u.n * p.rep;
     RowState<D> s;
-    load_rows<D>(s, p, rq, u, 0, lane);
+    {
+      RowLoads<D> q;
+      ask_rows<D>(q, p, rq, u, 0, lane);
+      __syncthreads();   // the previous piece's reads of s_o are done
+      take_rows<D>(s, q, p, u, 0, lane, reinterpret_cast<unsigned char*>(s_o[wave]));
+    }
     const long long wmin = u.pos < u.nk - 1 ? u.pos : u.nk - 1;   // blocks up to it hide no key
     const int nblk = (kb - ka + kBlk - 1) / kBlk;
     const int k0 = ka + (nblk * wave / 4) * kBlk;
@@ -859,7 +947,6 @@ __global__ __launch_bounds__(kPT) void attn_few_kernel(PAttn p) {
     }
     // The waves' parts, in wave order.
     const float l = s.l + __shfl_xor(s.l, 32, 64);
-    __syncthreads();   // the previous piece's reads are done
     if (h2 == 0) {
       s_m[wave][c32] = s.m;
       s_l[wave][c32] = l;
@@ -873,8 +960,9 @@ __global__ __launch_bounds__(kPT) void attn_few_kernel(PAttn p) {
     __syncthreads();
     const int slot = 2 * g + (starts ? 1 : 0);
     const bool whole = starts && ends;
-    for (int idx = 4 * tid; idx < rows * D; idx += 4 * kPT) {
-      const int r = idx / D, d = idx % D;
+    for (int e = tid; e < 8 * D; e += kPT) {   // (row e % 32, d = 4 (e / 32): the partials' order)
+      const int r = e & 31, d = e >> 5 << 2;
+      if (r >= rows) continue;
       float m = s_m[0][r];
 #pragma unroll
       for (int w = 1; w < 4; ++w) m = fmaxf(m, s_m[w][r]);
@@ -894,7 +982,7 @@ __global__ __launch_bounds__(kPT) void attn_few_kernel(PAttn p) {
         const float inv = ls == 0.f ? 0.f : 1.f / ls;
         store4(out_row(p, rq.lo + u.t * p.P, u.h, r) + d, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
       } else {
-        *reinterpret_cast<float4*>(p.part_o + ((size_t)slot * RT + r) * D + d) = v;
+        part_block<D>(p, slot, RT, 0, 0)[e] = v;
         if (d == 0) {
           float* ml = p.part_ml + ((size_t)slot * RT + r) * 2;
           ml[0] = m;
@@ -907,73 +995,79 @@ __global__ __launch_bounds__(kPT) void attn_few_kernel(PAttn p) {
 
 // -- join: the tiles that fell to more than one workgroup ------------------------
 
-// Workgroup (g, y): rows [y RB, y RB + RB) of the tile that workgroup g began
-// and others finished. The pieces' weights 2^(m - max) first, one per (row,
-// piece) in LDS, kJoin pieces at a time; then GR groups of threads sum every
-// GR-th piece's rows, their loads independent, and meet in LDS in order.
-constexpr int kJoin = 64;
+// Workgroup (g, y): one (32 rows, 32 d) block of the tile that workgroup g began
+// and others finished; a thread sums one float4 of it over the pieces, eight
+// loads at a time, with the pieces' weights 2^(m - max) from LDS.
+constexpr int kJoin = 64;   // pieces whose weights LDS holds
 
-template <int D, int RT, int RB>
+template <int D, int RT>
 __global__ __launch_bounds__(kPT) void attn_join_kernel(PAttn p) {
-  constexpr int TR = RB * D / 4;   // threads of a group
-  constexpr int GR = kPT / TR;
-  static_assert(TR * GR == kPT, "whole groups");
-  __shared__ float s_w[kJoin][RB], s_m[RB], s_l[RB];
-  __shared__ __attribute__((aligned(16))) float4 s_v[GR][TR];
+  __shared__ float s_w[kJoin][32], s_m[32], s_l[32];
+  __shared__ __attribute__((aligned(16))) uint16_t s_out[32][32 + 8];
   const int tid = threadIdx.x;
   const int g = blockIdx.x;
-  const int4 t = p.begun[g];   // rows (0: none), pieces, first token, kv head
-  const int rows = t.x, np = t.y;
-  const int r0 = blockIdx.y * RB;
+  const int4 tile = p.begun[g];   // rows (0: none), pieces, first token, kv head
+  const int rows = tile.x, np = tile.y;
+  const int rb = blockIdx.y / (D / 32), t = blockIdx.y % (D / 32);
+  const int r0 = 32 * rb;
   if (r0 >= rows) return;
   // Piece k's slot: the one that begins the tile is g's second.
-  auto slot = [&](int k) { return (size_t)(2 * (g + k) + (k == 0 ? 1 : 0)) * RT; };
-  const int gr = tid / TR, rr = tid % TR / (D / 4), d = tid % (D / 4) * 4;
-  const bool in = r0 + rr < rows;
+  auto slot = [&](int k) { return (size_t)(2 * (g + k) + (k == 0 ? 1 : 0)); };
+  const int row = tid & 31;
+  const bool in = r0 + row < rows;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (tid < RB) {
+  if (tid < 32) {
     s_m[tid] = -INFINITY;
     s_l[tid] = 0.f;
   }
   for (int k0 = 0; k0 < np; k0 += kJoin) {
     const int n = np - k0 < kJoin ? np - k0 : kJoin;
     __syncthreads();
-    const float m_old = s_m[rr];
+    const float m_old = s_m[row];
     __syncthreads();   // read before it is replaced
-    // Row tid / 32's weights by 32 lanes, two pieces each.
-    for (int row = tid >> 5; row < RB; row += kPT / 32) {
-      const int x = tid & 31;
-      const bool live = r0 + row < rows;
-      float2 a = make_float2(-INFINITY, 0.f), b = a;
-      if (live && x < n) a = *reinterpret_cast<const float2*>(p.part_ml + (slot(k0 + x) + r0 + row) * 2);
-      if (live && x + 32 < n) b = *reinterpret_cast<const float2*>(p.part_ml + (slot(k0 + x + 32) + r0 + row) * 2);
-      const float old = s_m[row];
-      float m = fmaxf(old, fmaxf(a.x, b.x));
+    // A row's weights by 8 lanes, eight pieces each at most.
+    {
+      const int rr = tid >> 3, x = tid & 7;
+      const bool live = r0 + rr < rows;
+      float2 a[kJoin / 8];
+      const float old = s_m[rr];
+      float m = old;
 #pragma unroll
-      for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-      const float wa = a.x == -INFINITY ? 0.f : exp2_fast(a.x - m), wb = b.x == -INFINITY ? 0.f : exp2_fast(b.x - m);
-      float l = (a.x == -INFINITY ? a.y : a.y * wa) + (b.x == -INFINITY ? b.y : b.y * wb);   // no score: 0 or NaN
+      for (int i = 0; i < kJoin / 8; ++i) {
+        const int k = 8 * i + x;
+        a[i] = make_float2(-INFINITY, 0.f);
+        if (live && k < n) a[i] = *reinterpret_cast<const float2*>(p.part_ml + (slot(k0 + k) * RT + r0 + rr) * 2);
+      }
 #pragma unroll
-      for (int off = 16; off > 0; off >>= 1) l += __shfl_xor(l, off, 64);
-      s_w[x][row] = wa;
-      s_w[x + 32][row] = wb;
+      for (int i = 0; i < kJoin / 8; ++i) m = fmaxf(m, a[i].x);
+#pragma unroll
+      for (int off = 1; off < 8; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+      float l = 0.f;
+#pragma unroll
+      for (int i = 0; i < kJoin / 8; ++i) {
+        const float w = a[i].x == -INFINITY ? 0.f : exp2_fast(a[i].x - m);
+        l += a[i].x == -INFINITY ? a[i].y : a[i].y * w;   // (no score: 0 or NaN)
+        s_w[8 * i + x][rr] = w;
+      }
+#pragma unroll
+      for (int off = 1; off < 8; off <<= 1) l += __shfl_xor(l, off, 64);
       if (x == 0) {
-        s_l[row] = s_l[row] * (old == -INFINITY ? 1.f : exp2_fast(old - m)) + l;
-        s_m[row] = m;
+        s_l[rr] = s_l[rr] * (old == -INFINITY ? 1.f : exp2_fast(old - m)) + l;
+        s_m[rr] = m;
       }
     }
     __syncthreads();
     if (in) {
-      const float c = m_old == -INFINITY ? 0.f : exp2_fast(m_old - s_m[rr]);
+      const float c = m_old == -INFINITY ? 0.f : exp2_fast(m_old - s_m[row]);
       v.x *= c;
       v.y *= c;
       v.z *= c;
       v.w *= c;
 #pragma unroll 8
-      for (int k = gr; k < n; k += GR) {
-        const float w = s_w[k][rr];
+      for (int k = 0; k < n; ++k) {
+        const float w = s_w[k][row];
         if (w == 0.f) continue;   // nothing there, or nothing beside the others
-        const float4 a = *reinterpret_cast<const float4*>(p.part_o + (slot(k0 + k) + r0 + rr) * D + d);
+        const float4 a = part_block<D>(p, slot(k0 + k), RT, rb, t)[tid];
         v.x += a.x * w;
         v.y += a.y * w;
         v.z += a.z * w;
@@ -981,22 +1075,13 @@ __global__ __launch_bounds__(kPT) void attn_join_kernel(PAttn p) {
       }
     }
   }
-  if (GR > 1) {
-    s_v[gr][tid % TR] = v;
-    __syncthreads();
-    if (gr) return;
-#pragma unroll
-    for (int k = 1; k < GR; ++k) {
-      const float4 a = s_v[k][tid];
-      v.x += a.x;
-      v.y += a.y;
-      v.z += a.z;
-      v.w += a.w;
-    }
-  }
-  if (!in) return;
-  const float l = s_l[rr], inv = l == 0.f ? 0.f : 1.f / l;
-  store4(out_row(p, t.z, t.w, r0 + rr) + d, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+  const float l = s_l[row], inv = l == 0.f ? 0.f : 1.f / l;
+  store4(&s_out[row][4 * (tid >> 5)], v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+  __syncthreads();
+  if (tid >= 128) return;
+  const int r = tid >> 2, d = tid % 4 * 8;   // 64 bytes a row
+  if (r0 + r < rows)
+    *reinterpret_cast<u32x4*>(out_row(p, tile.z, tile.w, r0 + r) + 32 * t + d) = *reinterpret_cast<const u32x4*>(&s_out[r][d]);
 }
 
 // Which kernel runs, and its tiles: calls of at most 32 query rows per kv head
@@ -1026,13 +1111,11 @@ int launch_attn(const PAttn& p, const AttnPlan& a, hipStream_t st) {
     hipLaunchKernelGGL((attn_chunk_kernel<D, BITS>), dim3((unsigned)p.G), dim3(64 * NW), 0, st, p);
   const int rc = launch_check("mtp_paged_attn");
   if (rc) return rc;
-  constexpr int RF = 256 / D < 1 ? 1 : 256 / D;    // few rows: four groups of threads to a join
-  constexpr int RC = 1024 / D;                     // chunks: one
+  const int blocks = cdiv(a.P * p.rep, 32) * (D / 32);
   if (a.few)
-    hipLaunchKernelGGL((attn_join_kernel<D, 32, RF>), dim3((unsigned)p.G, cdiv(a.P * p.rep, RF)), dim3(kPT), 0, st, p);
+    hipLaunchKernelGGL((attn_join_kernel<D, 32>), dim3((unsigned)p.G, blocks), dim3(kPT), 0, st, p);
   else
-    hipLaunchKernelGGL((attn_join_kernel<D, 32 * NW, RC>), dim3((unsigned)p.G, cdiv(a.P * p.rep, RC)), dim3(kPT), 0,
-                       st, p);
+    hipLaunchKernelGGL((attn_join_kernel<D, 32 * NW>), dim3((unsigned)p.G, blocks), dim3(kPT), 0, st, p);
   return launch_check("mtp_paged_attn");
 }
 
@@ -1100,6 +1183,7 @@ MTP_API int mtp_paged_attn(const mtp_paged_attn_args* a, void* stream) {
   p.Hq = a->Hq;
   p.Hkv = a->Hkv;
   p.rep = a->Hq / a->Hkv;
+  p.rep_inv = 65536u / (uint32_t)p.rep + 1;   // (exact while row * rep < 65536)
   p.bpp = a->page_size / kBlk;
   p.num_pages = a->num_pages;
   p.P = plan.P;
