@@ -57,6 +57,8 @@ struct PAttn {
   int P;            // tokens of a row tile
   int G;            // most workgroups
   int min_share;    // least keys of a workgroup's share
+  int step;         // shares are whole numbers of steps
+  int tile_cost;
   float scale_log2;
   long long q_token, q_head, out_token, out_head;
 };
@@ -73,7 +75,6 @@ __device__ __forceinline__ int fresh(int x) {
 
 // -- the line of work -------------------------------------------------------------
 
-constexpr int kTileCost = 64;   // keys' worth of a row tile's own cost (Q in, O out)
 
 struct Req {
   int lo, n;          // packed rows
@@ -84,14 +85,15 @@ struct Req {
 
 // Line length of a request's first t row tiles (one head).
 __device__ __forceinline__ long long tiles_len(long long q0, int n, int P, long long t) {
-  // sum over tiles x < t of q0 + min((x + 1) P, n) + kTileCost
+  // sum over tiles x < t of q0 + min((x + 1) P, n)
   const long long full = n / P;
   const long long f = t < full ? t : full;
-  return t * (q0 + kTileCost) + P * (f * (f + 1) / 2) + (t - f) * n;
+  return t * q0 + P * (f * (f + 1) / 2) + (t - f) * n;
 }
+// (A tile's own cost, Q in and O out, counts as tile_cost keys.)
 __device__ __forceinline__ long long clamp_start(const PAttn& p, long long s) {
   const long long cap = (long long)p.width * p.bpp * kBlk;
-  return s < 0 ? 0 : s > cap ? cap : s;
+  return (s < 0 ? 0 : s > cap ? cap : s) + p.tile_cost;
 }
 __device__ __forceinline__ long long head_len(const PAttn& p, long long start, int n) {
   return tiles_len(clamp_start(p, start), n, p.P, (n + p.P - 1) / p.P);
@@ -103,10 +105,14 @@ __device__ __forceinline__ long long uniform64(long long v) {
   return (long long)((unsigned long long)hi << 32 | lo);
 }
 
-// a / b for a quotient below 2^31 (and a, b below 2^52), by one fp64 division
-// instead of the integer one's long sequence.
+// a / b for a quotient below 2^31 (and a, b below 2^52), by an fp64 reciprocal
+// with one Newton step (within one of it, then put right) instead of the integer
+// division's long sequence.
 __device__ __forceinline__ int div_small(long long a, long long b) {
-  int q = (int)((double)a / (double)b);
+  const double d = (double)b;
+  double r = __builtin_amdgcn_rcp(d);
+  r = fma(fma(-d, r, 1.0), r, r);
+  int q = (int)((double)a * r);
   if ((long long)q * b > a) --q;
   if ((long long)(q + 1) * b <= a) ++q;
   return q;
@@ -146,11 +152,10 @@ struct Line {
     for (int off = 32; off > 0; off >>= 1) W += __shfl_xor(W, off, 64);
     W = uniform64(W);
     // Equal shares, a whole number of steps each, no shorter than min_share.
-    const long long s = (long long)ceil((double)W / (double)p.G);
-    S = (s > p.min_share ? (s + kStep - 1) / kStep : p.min_share / kStep) * kStep;
+    const long long s = W > 0 ? div_small(W - 1, p.G) + 1LL : 0;   // (W / G below 2^31: a share's keys)
+    S = s > p.min_share ? (s + p.step - 1) & -(long long)p.step : p.min_share;
     G = W > 0 ? div_small(W - 1, S) + 1 : 0;
   }
-  static constexpr int kStep = 64;
   __device__ __forceinline__ long long lo(int g) const { return g * S; }
   __device__ __forceinline__ long long hi(int g) const { return g + 1 < G ? (g + 1) * S : W; }
   __device__ __forceinline__ int owner(long long x) const { return div_small(x, S); }
@@ -217,7 +222,7 @@ __device__ __forceinline__ void next_tile(const PAttn& p, const Req& r, Tile& u)
   }
   const int left = r.n - u.t * p.P;
   u.n = left < p.P ? left : p.P;
-  u.len = clamp_start(p, r.start) + kTileCost + u.t * p.P + u.n;
+  u.len = clamp_start(p, r.start) + u.t * p.P + u.n;
   u.pos = r.start + (long long)u.t * p.P;
   const long long cap = (long long)p.width * p.bpp * kBlk;
   const long long e = u.pos + u.n;
@@ -500,12 +505,22 @@ __device__ __forceinline__ void note_begun(const PAttn& p, const Line& line, con
   p.begun[g] = make_int4(u.n * p.rep, line.owner(u.begin + u.len - 1) - g + 1, rq.lo + u.t * p.P, u.h);
 }
 
+// Byte I of w, signed, as a float: one instruction (the compiler takes two, a
+// bit field and a conversion).
+template <int I>
+__device__ __forceinline__ float byte_f32(uint32_t w) {
+  float f;
+  if constexpr (I == 0) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0" : "=v"(f) : "v"(w));
+  if constexpr (I == 1) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(f) : "v"(w));
+  if constexpr (I == 2) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(f) : "v"(w));
+  if constexpr (I == 3) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(f) : "v"(w));
+  return f;
+}
+
 // Eight bytes of integers -> eight bf16 (exact).
 __device__ __forceinline__ u32x4 widen8(uint32_t a, uint32_t b) {
-  auto pair = [](uint32_t w, int i) {
-    return f2bf2((float)(int8_t)(w >> (8 * i)), (float)(int8_t)(w >> (8 * i + 8)));
-  };
-  return u32x4{pair(a, 0), pair(a, 2), pair(b, 0), pair(b, 2)};
+  return u32x4{f2bf2(byte_f32<0>(a), byte_f32<1>(a)), f2bf2(byte_f32<2>(a), byte_f32<3>(a)),
+               f2bf2(byte_f32<0>(b), byte_f32<1>(b)), f2bf2(byte_f32<2>(b), byte_f32<3>(b))};
 }
 
 // -- chunks: row tiles of 32 NB rows a wave, K and V tiles shared through LDS ----
@@ -850,12 +865,15 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
 
 // -- few rows: one tile of 32 rows, the four waves share a piece by keys ---------
 
+// Blocks go straight from the pages into a wave's registers, RING of them in
+// flight (8-bit blocks are half as large: two).
 template <int D, int BITS>
-__global__ __launch_bounds__(kPT) void attn_few_kernel(PAttn p) {
+__global__ __launch_bounds__(kPT, D == 256 ? 1 : 2) void attn_few_kernel(PAttn p) {
   constexpr int RT = 32;
   constexpr int BE = kBlk * D;
   constexpr int LD = D / 16 * (BITS / 8) / 2;   // 16-byte loads of a lane per block
   constexpr int OS = D + 4;                     // padded row: lanes of one store hit distinct banks
+  constexpr int RING = 1;
   __shared__ __attribute__((aligned(16))) float s_o[4][32 * OS];
   __shared__ float s_m[4][32], s_l[4][32];
   const int tid = threadIdx.x, lane = tid & 63, c32 = lane & 31, h2 = lane >> 5;
@@ -881,69 +899,84 @@ __global__ __launch_bounds__(kPT) void attn_few_kernel(PAttn p) {
     x = end;
     if (starts && !ends && tid == 0) note_begun(p, line, rq, u, g);
     const int rows = u.n * p.rep;
-    RowState<D> s;
-    {
-      RowLoads<D> q;
-      ask_rows<D>(q, p, rq, u, 0, lane);
-      __syncthreads();   // the previous piece's reads of s_o are done
-      take_rows<D>(s, q, p, u, 0, lane, reinterpret_cast<unsigned char*>(s_o[wave]));
-    }
+    RowLoads<D> q;
+    ask_rows<D>(q, p, rq, u, 0, lane);
     const long long wmin = u.pos < u.nk - 1 ? u.pos : u.nk - 1;   // blocks up to it hide no key
     const int nblk = (kb - ka + kBlk - 1) / kBlk;
-    const int k0 = ka + (nblk * wave / 4) * kBlk;
-    const int e1 = ka + (nblk * (wave + 1) / 4) * kBlk;
-    const int k1 = e1 < kb ? e1 : kb;
-    u32x4 kr[LD], vr[LD];
-    float4 kq[4], vq[4];   // scales of the lane's keys
+    const int b0 = (ka >> 5) + nblk * wave / 4, b1 = (ka >> 5) + nblk * (wave + 1) / 4;   // the wave's blocks
     BlockList blocks;
-    if (k0 < k1) blocks.fill(p, b, u.h, k0 >> 5, (k1 + 31) >> 5, lane);
-    auto load = [&](int at) {
-      const size_t o = (size_t)at * BE;
+    if (b0 < b1) blocks.fill(p, b, u.h, b0, b1, lane);
+    u32x4 kr[RING][LD], vr[RING][LD];
+    float sc[RING];   // 8 bits: lane l's key's scale, of K (l < 32) and of V
+    auto load = [&](int slot, int blk) {
+      const size_t o = (size_t)blocks.get(blk < b1 ? blk : b1 - 1) * BE;   // (past the last: the last again, never used)
+      const unsigned char* k = p.k_pages + o * (BITS / 8);
+      const unsigned char* v = p.v_pages + o * (BITS / 8);
 #pragma unroll
-      for (int i = 0; i < LD; ++i) kr[i] = ld_nt(p.k_pages + o * (BITS / 8) + (size_t)(i * 64 + lane) * 16);
+      for (int i = 0; i < LD; ++i) kr[slot][i] = ld_nt(k + (uint32_t)(i * 1024 + lane * 16));
 #pragma unroll
-      for (int i = 0; i < LD; ++i) vr[i] = ld_nt(p.v_pages + o * (BITS / 8) + (size_t)(i * 64 + lane) * 16);
-      if constexpr (BITS == 8) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          kq[j] = *reinterpret_cast<const float4*>(p.k_scales + o / D + 8 * j + 4 * h2);
-          vq[j] = *reinterpret_cast<const float4*>(p.v_scales + o / D + 8 * j + 4 * h2);
-        }
-      }
+      for (int i = 0; i < LD; ++i) vr[slot][i] = ld_nt(v + (uint32_t)(i * 1024 + lane * 16));
+      if constexpr (BITS == 8) sc[slot] = (h2 ? p.v_scales : p.k_scales)[o / D + c32];
     };
-    if (k0 < k1) {
-      load(blocks.get(k0 >> 5));
-      for (int kt = k0; kt < k1; kt += kBlk) {
-        if (!blocks.absent(kt >> 5)) {   // uniform
-          auto kop = [&](int, int i) {
-            if constexpr (BITS == 16) return kr[i];
-            else return (i & 1) ? widen8(kr[i >> 1].z, kr[i >> 1].w) : widen8(kr[i >> 1].x, kr[i >> 1].y);
-          };
-          auto vop = [&](int t, int jj) {
-            if constexpr (BITS == 16) return vr[2 * t + jj];
-            else return jj ? widen8(vr[t].z, vr[t].w) : widen8(vr[t].x, vr[t].y);
-          };
-          auto part = [](const float4& f, int e) { return e == 0 ? f.x : e == 1 ? f.y : e == 2 ? f.z : f.w; };
-          auto ks = [&](int, int r) { return part(kq[r >> 2], r & 3) * p.scale_log2; };
-          auto vs = [&](int, int r) { return part(vq[r >> 2], r & 3); };
-          f32x16 st[1];
-          u32x4 w[1][2];
-          const int end[1] = {u.nk};
-          scores<D, 1>(s, st, kop);
-          if (kt + 31 <= wmin) {
-            soften<D, BITS, 1, false>(s, st, w, kt, end, h2, p.scale_log2, ks, vs);
-            add_values<D, BITS, false>(s, w[0], kt, u.nk, h2, vop);
-          } else {
-            soften<D, BITS, 1, true>(s, st, w, kt, end, h2, p.scale_log2, ks, vs);
-            add_values<D, BITS, true>(s, w[0], kt, u.nk, h2, vop);
-          }
+    if (b0 < b1) {
+#pragma unroll
+      for (int i = 0; i < RING; ++i) load(i, b0 + i);
+    }
+    RowState<D> s;
+    __syncthreads();   // the previous piece's reads of s_o are done
+    take_rows<D>(s, q, p, u, 0, lane, reinterpret_cast<unsigned char*>(s_o[wave]));
+    float* const scales = s_o[wave];   // 8 bits: a block's scales, on their way to the lanes that need them
+    auto block = [&](int slot, int blk, auto mask) {
+      constexpr bool MASK = decltype(mask)::value;
+      const int kt = 32 * blk;
+      if constexpr (BITS == 8) scales[lane] = h2 ? sc[slot] : sc[slot] * p.scale_log2;
+      auto scale = [&](int r) { return scales[8 * (r >> 2) + 4 * h2 + (r & 3)]; };
+      f32x16 st[1];
+      u32x4 w[1][2];
+      const int end1[1] = {u.nk};
+      scores<D, 1>(s, st, [&](int, int i) {
+        if constexpr (BITS == 16) return kr[slot][i];
+        else return (i & 1) ? widen8(kr[slot][i >> 1].z, kr[slot][i >> 1].w) : widen8(kr[slot][i >> 1].x, kr[slot][i >> 1].y);
+      });
+      soften<D, BITS, 1, MASK>(
+          s, st, w, kt, end1, h2, p.scale_log2, [&](int, int r) { return scale(r); },
+          [&](int, int r) { return scale(r + 16); });
+      if (BITS == 8) __builtin_amdgcn_sched_barrier(0);   // (V's integers are not widened before their turn)
+      add_values<D, BITS, MASK>(s, w[0], kt, u.nk, h2, [&](int t, int jj) {
+        if constexpr (BITS == 16) return vr[slot][2 * t + jj];
+        else return jj ? widen8(vr[slot][t].z, vr[slot][t].w) : widen8(vr[slot][t].x, vr[slot][t].y);
+      });
+    };
+    auto next = [&](int slot, int blk) {   // block blk + RING into the slot that blk leaves
+      if (blk + RING >= blocks.first + 64 && blk + RING < b1) blocks.fill(p, b, u.h, blk + 1, b1, lane);
+      load(slot, blk + RING);
+    };
+    // Blocks [b0, bf) hide no key and have their pages.
+    int bf = wmin + 1 >= 0 ? (int)((wmin + 1) >> 5) : 0;
+    if (bf > b1) bf = b1;
+    int blk = b0;
+    while (blk < b1) {
+      // As far as this list knows; RING at a time, so each stays in its registers.
+      int to = blocks.first + blocks.present();
+      if (to > bf) to = bf;
+#pragma unroll 1
+      for (; blk + RING <= to; blk += RING) {
+#pragma unroll
+        for (int i = 0; i < RING; ++i) {
+          block(i, blk + i, std::false_type());
+          next(i, blk + i);
         }
-        if (kt + kBlk < k1) {
-          const int blk = (kt >> 5) + 1;
-          if (blk >= blocks.first + 64) blocks.fill(p, b, u.h, blk, (k1 + 31) >> 5, lane);
-          load(blocks.get(blk));
+        to = blocks.first + blocks.present() < bf ? blocks.first + blocks.present() : bf;
+      }
+      if (blk >= b1) break;
+#pragma unroll
+      for (int i = 0; i < RING; ++i) {
+        if (blk + i < b1) {
+          if (!blocks.absent(blk + i)) block(i, blk + i, std::true_type());
+          next(i, blk + i);
         }
       }
+      blk += RING;
     }
     // The waves' parts, in wave order.
     const float l = s.l + __shfl_xor(s.l, 32, 64);
@@ -1014,8 +1047,14 @@ __global__ __launch_bounds__(kPT) void attn_join_kernel(PAttn p) {
   // Piece k's slot: the one that begins the tile is g's second.
   auto slot = [&](int k) { return (size_t)(2 * (g + k) + (k == 0 ? 1 : 0)); };
   const int row = tid & 31;
-  const bool in = r0 + row < rows;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  constexpr int B8 = 8;   // pieces whose blocks are in flight together
+  float4 a8[B8];
+  auto ask = [&](int k) {   // (the last piece again past the last: never used)
+#pragma unroll
+    for (int i = 0; i < B8; ++i) a8[i] = part_block<D>(p, slot(k + i < np ? k + i : np - 1), RT, rb, t)[tid];
+  };
+  ask(0);
   if (tid < 32) {
     s_m[tid] = -INFINITY;
     s_l[tid] = 0.f;
@@ -1057,22 +1096,22 @@ __global__ __launch_bounds__(kPT) void attn_join_kernel(PAttn p) {
       }
     }
     __syncthreads();
-    if (in) {
-      const float c = m_old == -INFINITY ? 0.f : exp2_fast(m_old - s_m[row]);
-      v.x *= c;
-      v.y *= c;
-      v.z *= c;
-      v.w *= c;
-#pragma unroll 8
-      for (int k = 0; k < n; ++k) {
-        const float w = s_w[k][row];
-        if (w == 0.f) continue;   // nothing there, or nothing beside the others
-        const float4 a = part_block<D>(p, slot(k0 + k), RT, rb, t)[tid];
-        v.x += a.x * w;
-        v.y += a.y * w;
-        v.z += a.z * w;
-        v.w += a.w * w;
+    const float c = m_old == -INFINITY ? 0.f : exp2_fast(m_old - s_m[row]);
+    v.x *= c;
+    v.y *= c;
+    v.z *= c;
+    v.w *= c;
+    for (int k = 0; k < n; k += B8) {
+#pragma unroll
+      for (int i = 0; i < B8; ++i) {
+        const float w = k + i < n ? s_w[k + i][row] : 0.f;
+        // (weight 0: a piece without keys wrote no block, or one that is nothing beside the others)
+        v.x += w == 0.f ? 0.f : a8[i].x * w;
+        v.y += w == 0.f ? 0.f : a8[i].y * w;
+        v.z += w == 0.f ? 0.f : a8[i].z * w;
+        v.w += w == 0.f ? 0.f : a8[i].w * w;
       }
+      if (k0 + k + B8 < np) ask(k0 + k + B8);
     }
   }
   const float l = s_l[row], inv = l == 0.f ? 0.f : 1.f / l;
@@ -1089,7 +1128,7 @@ __global__ __launch_bounds__(kPT) void attn_join_kernel(PAttn p) {
 // them straight into registers; others share K and V tiles through LDS.
 struct AttnPlan {
   bool few;
-  int RT, P, G, min_share;
+  int RT, P, G, min_share, step, tile_cost;
 };
 inline AttnPlan attn_plan(int Hq, int Hkv, int D, int max_rows) {
   const int rep = Hq / Hkv;
@@ -1099,6 +1138,8 @@ inline AttnPlan attn_plan(int Hq, int Hkv, int D, int max_rows) {
   a.P = a.RT / rep;
   a.G = device_cus();
   a.min_share = a.few ? 4 * kBlk : 2 * kStepKeys;
+  a.step = a.few ? kBlk : kStepKeys;
+  a.tile_cost = a.few ? 0 : 2 * kStepKeys;
   return a;
 }
 
@@ -1189,6 +1230,8 @@ MTP_API int mtp_paged_attn(const mtp_paged_attn_args* a, void* stream) {
   p.P = plan.P;
   p.G = plan.G;
   p.min_share = plan.min_share;
+  p.step = plan.step;
+  p.tile_cost = plan.tile_cost;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.q_token = a->q_token;
   p.q_head = a->q_head;
