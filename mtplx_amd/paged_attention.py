@@ -17,7 +17,7 @@ import torch
 
 from . import _lib
 from .paged_kv_cache import PagedKVCache
-from .rotary import _call, _rows, _same_device, _writable, _overlaps
+from .rotary import _call, _on, _overlaps, _rows, _stream, _writable
 
 __all__ = ["paged_sdpa"]
 
@@ -36,34 +36,58 @@ def paged_sdpa(queries: torch.Tensor, cache: PagedKVCache, block_table: Any, q_s
     (without ``out``: undefined). Rows that see no key are zeros;
     positions without a page count as absent and set ``cache.status()``.
     ``scale`` is positive; default ``1 / sqrt(D)``."""
-    q = _rows("queries", queries, None, cache.head_dim)
-    T, Hq, D = q.shape
+    q, T, Hq, D, qt, qh = _rows("queries", queries, None, cache.head_dim)
     Hkv = cache.n_kv_heads
     if Hq % Hkv or not 1 <= Hq // Hkv <= 32:
         raise ValueError(f"query heads ({Hq}) must be 1 to 32 times the cache's kv heads ({Hkv})")
+    device = cache.device
+    _on(device, "queries", q)
     table = cache._table(block_table)
-    B = table.shape[0]
+    B, width = table.shape
     start, off = cache._requests(T, B, q_start, row_off)
-    _same_device(cache.device, queries=q)
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError(f"scale must be positive and finite (got {scale})")
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
+        out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=device)
+        ot, oh = Hq * D, D
     else:
         out = _writable("out", out, queries)
         if _overlaps(out, q):
             q = q.clone(memory_format=torch.contiguous_format)
+            qt, qh = Hq * D, D
+        ot, oh = out.stride()[:2]
     if T == 0:
         return out
-    rows = T // B if off is None else max(0, int(max_rows or 0))
-    with torch.cuda.device(cache.device):
-        nb = _lib.query("mtp_paged_attn_workspace_bytes", Hq, Hkv, D, rows)
-    ws = _lib.WORKSPACES.get(nb, "paged_attn", cache.device)
-    a = _lib.PagedAttnArgs(q=q.data_ptr(), out=out.data_ptr(), block_table=table.data_ptr(), q_start=start.data_ptr(),
-                           row_off=_lib.ptr(off), ws=ws.data_ptr(), ws_bytes=ws.numel(), T=T, B=B,
-                           width=table.shape[1], Hq=Hq, max_rows=rows, scale=scale, q_token=q.stride(0),
-                           q_head=q.stride(1), out_token=out.stride(0), out_head=out.stride(1))
-    cache._pages(a)
-    _call("mtp_paged_attn", a, cache.device)
+    rows = T // B if off is None else 0 if max_rows is None else min(max(0, int(max_rows)), T)
+    ws = _workspace(device, Hq, Hkv, D, rows)
+    a = cache._block(_lib.PagedAttnArgs)
+    a.q, a.out, a.block_table, a.q_start = q.data_ptr(), out.data_ptr(), table.data_ptr(), start.data_ptr()
+    if off is not None:
+        a.row_off = off.data_ptr()
+    a.ws, a.ws_bytes = ws.data_ptr(), ws.numel()
+    a.T, a.B, a.width, a.Hq, a.max_rows, a.scale = T, B, width, Hq, rows, scale
+    a.q_token, a.q_head, a.out_token, a.out_head = qt, qh, ot, oh
+    _call("mtp_paged_attn", a, device)
     return out
+
+
+_SPACES: dict = {}
+
+
+def _workspace(device, Hq: int, Hkv: int, D: int, rows: int) -> torch.Tensor:
+    """The partials' buffer of this device, stream and kind of call, looked up
+    once (the pool keeps what it gave out allocated). A call that is being
+    captured takes the graph's own memory: graphs captured on one stream may be
+    replayed on two at once."""
+    if torch.cuda.is_current_stream_capturing():
+        with torch.cuda.device(device):
+            nb = _lib.query("mtp_paged_attn_workspace_bytes", Hq, Hkv, D, rows)
+        return torch.empty(nb, dtype=torch.uint8, device=device)
+    key = (device.index, _stream(device), Hq, Hkv, D, 0 < rows * (Hq // Hkv) <= 32)
+    ws = _SPACES.get(key)
+    if ws is None:
+        with torch.cuda.device(device):
+            nb = _lib.query("mtp_paged_attn_workspace_bytes", Hq, Hkv, D, rows)
+        ws = _SPACES[key] = _lib.WORKSPACES.get(nb, "paged_attn", device)
+    return ws

@@ -24,7 +24,7 @@ from typing import Any
 import torch
 
 from . import _lib
-from .rotary import RotaryTable, _call, _int32, _readable, _rows, _same_device, _writable, _overlaps
+from .rotary import RotaryTable, _call, _int32, _interleaved, _on, _overlaps, _rows, _writable
 
 __all__ = ["PagedKVCache"]
 
@@ -46,21 +46,41 @@ class PagedKVCache:
         self.page_size, self.bits = int(page_size), int(bits)
         shape = (self.num_pages, self.n_kv_heads, self.page_size // 32, 32 * self.head_dim)
         dtype = torch.int8 if bits == 8 else torch.bfloat16
-        self.k_pages = torch.zeros(shape, dtype=dtype, device=device)
-        self.v_pages = torch.zeros_like(self.k_pages)
-        self.k_scales = self.v_scales = None
+        self._k = torch.zeros(shape, dtype=dtype, device=device)
+        self._v = torch.zeros_like(self._k)
+        self._ks = self._vs = None
         if bits == 8:
-            self.k_scales = torch.zeros(shape[:2] + (self.page_size,), dtype=torch.float32, device=device)
-            self.v_scales = torch.zeros_like(self.k_scales)
+            self._ks = torch.zeros(shape[:2] + (self.page_size,), dtype=torch.float32, device=device)
+            self._vs = torch.zeros_like(self._ks)
         self._status = torch.zeros(1, dtype=torch.int32, device=device)
+        self.device = self._k.device
+        # What every call over this cache passes, filled in once.
+        held = dict(k_pages=self._k.data_ptr(), v_pages=self._v.data_ptr(), k_scales=_lib.ptr(self._ks),
+                    v_scales=_lib.ptr(self._vs), status=self._status.data_ptr(), Hkv=self.n_kv_heads, D=self.head_dim,
+                    page_size=self.page_size, num_pages=self.num_pages, bits=self.bits)
+        self._blocks = {cls: cls(**held) for cls in (_lib.PagedWriteArgs, _lib.PagedReadArgs, _lib.PagedAttnArgs)}
+
+    # The pool's tensors (their contents may be copied in and out; the cache
+    # keeps the tensors themselves).
+    @property
+    def k_pages(self) -> torch.Tensor:
+        return self._k
 
     @property
-    def device(self) -> torch.device:
-        return self.k_pages.device
+    def v_pages(self) -> torch.Tensor:
+        return self._v
+
+    @property
+    def k_scales(self) -> torch.Tensor | None:
+        return self._ks
+
+    @property
+    def v_scales(self) -> torch.Tensor | None:
+        return self._vs
 
     @property
     def nbytes(self) -> int:
-        held = (self.k_pages, self.v_pages, self.k_scales, self.v_scales)
+        held = (self._k, self._v, self._ks, self._vs)
         return sum(t.numel() * t.element_size() for t in held if t is not None)
 
     def status(self) -> torch.Tensor:
@@ -76,13 +96,8 @@ class PagedKVCache:
             raise _lib.MtpError("paged_kv_cache", -1, "a position without a page of the pool (status word set)")
 
     # -- shared by the calls over this cache --------------------------------------
-    def _pages(self, block) -> None:
-        block.k_pages, block.v_pages = self.k_pages.data_ptr(), self.v_pages.data_ptr()
-        if self.bits == 8:
-            block.k_scales, block.v_scales = self.k_scales.data_ptr(), self.v_scales.data_ptr()
-        block.status = self._status.data_ptr()
-        block.Hkv, block.D, block.page_size = self.n_kv_heads, self.head_dim, self.page_size
-        block.num_pages, block.bits = self.num_pages, self.bits
+    def _block(self, cls):
+        return cls.from_buffer_copy(self._blocks[cls])
 
     def _table(self, block_table: Any) -> torch.Tensor:
         t = _int32("block_table", block_table, self.device)
@@ -120,49 +135,58 @@ class PagedKVCache:
         Two tokens of one call must not share a slot. A position without a
         page is skipped and sets :meth:`status`."""
         D, H = self.head_dim, self.n_kv_heads
-        k, v = _rows("keys", keys, H, D), _rows("values", values, H, D)
-        T = k.shape[0]
-        if v.shape[0] != T:
-            raise ValueError(f"keys have {T} tokens, values {v.shape[0]}")
+        k, T, _, _, kt, kh = _rows("keys", keys, H, D)
+        v, Tv, _, _, vt, vh = _rows("values", values, H, D)
+        if Tv != T:
+            raise ValueError(f"keys have {T} tokens, values {Tv}")
+        device = self.device
+        _on(device, "keys", k)
+        _on(device, "values", v)
         if queries is not None and rotary is None:
             raise ValueError("queries are taken to be rotated: give rotary with them")
-        if rotary is not None and rotary.dims > D:
-            raise ValueError(f"the rotary table's {rotary.dims} dims exceed the head dim {D}")
+        if rotary is not None:
+            if rotary.dims > D:
+                raise ValueError(f"the rotary table's {rotary.dims} dims exceed the head dim {D}")
+            _on(device, "rotary", rotary.phases)
         table = self._table(block_table)
-        B = table.shape[0]
+        B, width = table.shape
         start, off = self._requests(T, B, q_start, row_off)
-        _same_device(self.device, keys=k, values=v, queries=queries,
-                     rotary=None if rotary is None else rotary.phases)
         q = qo = None
         if queries is not None:
-            q = _rows("queries", queries, None, D)
-            if q.shape[0] != T:
-                raise ValueError(f"keys have {T} tokens, queries {q.shape[0]}")
+            q, Tq, Hq, _, qt, qh = _rows("queries", queries, None, D)
+            if Tq != T:
+                raise ValueError(f"keys have {T} tokens, queries {Tq}")
+            _on(device, "queries", q)
             if out is None:
-                qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+                qo = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=device)
+                qot, qoh = Hq * D, D
             else:
                 qo = _writable("out", out, queries)
                 for name, x in (("keys", k), ("values", v)):
-                    if _overlaps(qo, x) and not _beside(qo, x):
+                    if _overlaps(qo, x) and not _interleaved(qo, x):
                         raise ValueError(f"out overlaps {name}")
                 if _overlaps(qo, q):
                     same = qo.data_ptr() == q.data_ptr() and qo.stride() == q.stride()
                     if not same or not (rotary.traditional or rotary.dims % 16 == 0):
                         q = q.clone(memory_format=torch.contiguous_format)
+                        qt, qh = Hq * D, D
+                qot, qoh = qo.stride()[:2]
         if T == 0:
             return qo
-        a = _lib.PagedWriteArgs(k=k.data_ptr(), v=v.data_ptr(), block_table=table.data_ptr(),
-                                q_start=start.data_ptr(), row_off=_lib.ptr(off), T=T, B=B, width=table.shape[1],
-                                max_rows=max(0, int(max_rows or 0)), k_token=k.stride(0), k_head=k.stride(1),
-                                v_token=v.stride(0), v_head=v.stride(1))
-        self._pages(a)
+        a = self._block(_lib.PagedWriteArgs)
+        a.k, a.v, a.k_token, a.k_head, a.v_token, a.v_head = k.data_ptr(), v.data_ptr(), kt, kh, vt, vh
+        a.block_table, a.q_start, a.T, a.B, a.width = table.data_ptr(), start.data_ptr(), T, B, width
+        if off is not None:
+            a.row_off = off.data_ptr()
+            if max_rows is not None and max_rows > 0:
+                a.max_rows = min(int(max_rows), T)
         if rotary is not None:
             a.table, a.dims, a.gain = rotary.phases.data_ptr(), rotary.dims, rotary.gain
-            a.traditional = int(rotary.traditional)
-        if q is not None and q.shape[1]:
-            a.q, a.q_out, a.Hq = q.data_ptr(), qo.data_ptr(), q.shape[1]
-            a.q_token, a.q_head, a.qo_token, a.qo_head = q.stride(0), q.stride(1), qo.stride(0), qo.stride(1)
-        _call("mtp_paged_write", a, self.device)
+            a.traditional = rotary.traditional
+        if q is not None and Hq:
+            a.q, a.q_out, a.Hq = q.data_ptr(), qo.data_ptr(), Hq
+            a.q_token, a.q_head, a.qo_token, a.qo_head = qt, qh, qot, qoh
+        _call("mtp_paged_write", a, device)
         return qo
 
     def read(self, block_table: Any, count: int, *, start: Any = None, lengths: Any = None):
@@ -180,14 +204,9 @@ class PagedKVCache:
         k = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
         v = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
         if count:
-            a = _lib.PagedReadArgs(block_table=table.data_ptr(), start=_lib.ptr(first), lengths=_lib.ptr(ends),
-                                   k_out=k.data_ptr(), v_out=v.data_ptr(), B=B, width=table.shape[1], count=count)
-            self._pages(a)
+            a = self._block(_lib.PagedReadArgs)
+            a.block_table, a.k_out, a.v_out = table.data_ptr(), k.data_ptr(), v.data_ptr()
+            a.start, a.lengths = _lib.ptr(first), _lib.ptr(ends)
+            a.B, a.width, a.count = B, table.shape[1], count
             _call("mtp_paged_read", a, self.device)
         return k, v
-
-
-def _beside(a: torch.Tensor, b: torch.Tensor) -> bool:
-    from .rotary import _interleaved
-
-    return _interleaved(a, b)

@@ -119,16 +119,27 @@ def rotary_table(dims: int, *, base: float = 10000.0, traditional: bool = False,
                        torch.tensor(fixed, dtype=torch.int64).to(device))
 
 
-def _rows(name: str, x: torch.Tensor, heads: int | None = None, dim: int | None = None) -> torch.Tensor:
-    """``x`` [T, H, D] bf16 on the GPU as the kernels read it: 16-byte aligned
-    rows, strides of whole 16 bytes (other views are copied)."""
+def _rows(name: str, x: torch.Tensor, heads: int | None = None, dim: int | None = None):
+    """``(x, tokens, heads, dim, token stride, head stride)`` of rows ``x``
+    [T, H, D] bf16 on the GPU as the kernels read them: 16-byte aligned, strides
+    of whole 16 bytes (other views are copied)."""
     if not x.is_cuda:
         raise RuntimeError(f"{name}: the paged operators run on the GPU only")
-    if x.dtype != torch.bfloat16:
+    if x.dtype is not torch.bfloat16:
         raise TypeError(f"{name} must be bfloat16 (got {x.dtype})")
-    if x.dim() != 3 or (heads is not None and x.shape[1] != heads) or (dim is not None and x.shape[2] != dim):
-        raise ValueError(f"{name} must be [tokens, {heads or 'heads'}, {dim or 'dim'}] (got {list(x.shape)})")
-    return x if _readable(x) else x.clone(memory_format=torch.contiguous_format)
+    shape = x.shape
+    if len(shape) != 3 or (heads is not None and shape[1] != heads) or (dim is not None and shape[2] != dim):
+        raise ValueError(f"{name} must be [tokens, {heads or 'heads'}, {dim or 'dim'}] (got {list(shape)})")
+    T, H, D = shape
+    t, h, d = x.stride()
+    if d != 1 or t < 0 or t & 7 or h & 7 or h < D or x.data_ptr() & 15:
+        x = x.clone(memory_format=torch.contiguous_format)
+        t, h, d = x.stride()
+        if T == 1 or H == 1:   # (a single row's stride is anything)
+            t, h = H * D, D
+            if D & 7:
+                raise ValueError(f"{name}: a row of {D} elements is no whole 16 bytes")
+    return x, T, H, D, t, h
 
 
 def _readable(x: torch.Tensor) -> bool:
@@ -146,28 +157,35 @@ def _writable(name: str, out: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
 
 def _int32(name: str, value: Any, device, numel: int | None = None) -> torch.Tensor:
     t = value if isinstance(value, torch.Tensor) else torch.as_tensor(value)
-    if t.dtype != torch.int32 or t.device != device:
-        t = t.to(device=device, dtype=torch.int32)
-    t = t.contiguous()
+    if t.dtype is not torch.int32 or t.device != device or not t.is_contiguous():
+        t = t.to(device=device, dtype=torch.int32).contiguous()
     if numel is not None and t.numel() != numel:
         raise ValueError(f"{name} must hold {numel} values (got {t.numel()})")
     return t
 
 
-def _same_device(device, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, the call's other tensors on {device}")
+def _on(device, name: str, t: torch.Tensor) -> None:
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the call's other tensors on {device}")
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream(device) -> int:
+    """The current stream of ``device`` (as :func:`_lib.stream_handle`, without
+    making a stream object where torch offers the handle itself)."""
+    return _raw_stream(device.index) if _raw_stream is not None else _lib.stream_handle(device)
 
 
 def _call(name: str, block: ctypes.Structure, device) -> None:
     """Run an argument-block entry point on ``device``'s current stream (the
     kernels of a call go to the current HIP device)."""
     if torch.cuda.current_device() == device.index:
-        _lib.call(name, ctypes.byref(block), _lib.stream_handle(device))
+        _lib.call(name, ctypes.byref(block), _stream(device))
         return
     with torch.cuda.device(device):
-        _lib.call(name, ctypes.byref(block), _lib.stream_handle(device))
+        _lib.call(name, ctypes.byref(block), _stream(device))
 
 
 def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -188,19 +206,25 @@ def apply_rotary(table: RotaryTable, queries: torch.Tensor, keys: torch.Tensor |
     ``positions`` [T] (int32; may stay on the GPU). Returns ``(queries, keys)``
     rotated, in new tensors or in ``out`` (a pair; the inputs themselves for in
     place). Views of a fused projection are read where they are."""
-    q = _rows("queries", queries)
-    T, Hq, D = q.shape
+    q, T, Hq, D, qt, qh = _rows("queries", queries)
     device = q.device
-    k = None if keys is None else _rows("keys", keys, None, D)
-    if k is not None and k.shape[0] != T:
-        raise ValueError(f"queries have {T} tokens, keys {k.shape[0]}")
+    k, Hkv, kt, kh = None, 0, 0, 0
+    if keys is not None:
+        k, Tk, Hkv, _, kt, kh = _rows("keys", keys, None, D)
+        if Tk != T:
+            raise ValueError(f"queries have {T} tokens, keys {Tk}")
+        _on(device, "keys", k)
     if D % 8 or D > 256 or table.dims > D:
         raise ValueError(f"head dim {D} must be a multiple of 8 up to 256 and hold the table's {table.dims} dims")
     pos = _int32("positions", positions, device, T)
-    _same_device(device, keys=k, table=table.phases)
+    _on(device, "table", table.phases)
+    ko = None
     if out is None:
-        qo = torch.empty((T, Hq, D), dtype=q.dtype, device=device)
-        ko = None if k is None else torch.empty((T, k.shape[1], D), dtype=q.dtype, device=device)
+        qo = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=device)
+        qot, qoh = Hq * D, D
+        if k is not None:
+            ko = torch.empty((T, Hkv, D), dtype=torch.bfloat16, device=device)
+        kot, koh = Hkv * D, D
     else:
         qo = _writable("out[0]", out[0], queries)
         ko = None if k is None else _writable("out[1]", out[1], keys)
@@ -217,19 +241,22 @@ def apply_rotary(table: RotaryTable, queries: torch.Tensor, keys: torch.Tensor |
                     if not same:
                         if src is q:
                             q = q.clone(memory_format=torch.contiguous_format)
+                            qt, qh = Hq * D, D
                         else:
                             k = k.clone(memory_format=torch.contiguous_format)
+                            kt, kh = Hkv * D, D
         if ko is not None and _overlaps(qo, ko) and not _interleaved(qo, ko):
             raise ValueError("the two outputs overlap")
+        qot, qoh = qo.stride()[:2]
+        kot, koh = (0, 0) if ko is None else ko.stride()[:2]
     if T == 0 or Hq == 0:
         return qo, ko
-    a = _lib.RotaryArgs(q=q.data_ptr(), q_out=qo.data_ptr(), positions=pos.data_ptr(), table=table.phases.data_ptr(),
-                        T=T, Hq=Hq, D=D, dims=table.dims, traditional=int(table.traditional), gain=table.gain,
-                        q_token=q.stride(0), q_head=q.stride(1), qo_token=qo.stride(0), qo_head=qo.stride(1))
-    if k is not None and k.shape[1]:
-        a.k, a.k_out, a.Hkv = k.data_ptr(), ko.data_ptr(), k.shape[1]
-        a.k_token, a.k_head, a.ko_token, a.ko_head = k.stride(0), k.stride(1), ko.stride(0), ko.stride(1)
-    _call("mtp_rotary", a, device)
+    if not Hkv:
+        k = None
+    _call("mtp_rotary", _lib.RotaryArgs(
+        q.data_ptr(), None if k is None else k.data_ptr(), qo.data_ptr(), None if k is None else ko.data_ptr(),
+        pos.data_ptr(), table.phases.data_ptr(), T, Hq, Hkv, D, table.dims, table.traditional, table.gain, qt, qh, kt, kh,
+        qot, qoh, kot, koh), device)
     return qo, ko
 
 

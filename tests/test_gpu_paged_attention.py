@@ -317,3 +317,36 @@ def test_streams_and_captured_steps(gpu):
         got = step(c, *parts[1])
     side.synchronize()
     assert torch.equal(got, step(e, *parts[1]))
+
+
+def test_captured_steps_at_once(gpu):
+    """Steps captured on one stream hold workspaces of their own: replayed on
+    two streams at the same time they give what they give in turn."""
+    rng = np.random.default_rng(18)
+    H, Hq, D, page, B = 2, 16, 128, 64, 2
+    table, pages = tables(rng, [9000] * B, page)
+    c = PagedKVCache(pages, H, D, page_size=page)
+    for b in range(B):
+        c.write(rows(rng, 9000, H, D), rows(rng, 9000, H, D), table[b:b + 1], i32([0]))
+    start = i32([8900, 5000])
+    qs = [rows(rng, B * n, Hq, D) for n in (4, 4, 100, 100)]
+    want = [paged_sdpa(q, c, table, start) for q in qs]
+    side, streams = torch.cuda.Stream(), [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for q in qs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            outs.append(paged_sdpa(q, c, table, start))
+        graphs.append(g)
+    for _ in range(3):
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                for _ in range(4):
+                    g.replay()
+        torch.cuda.synchronize()
+        for out, w in zip(outs, want):
+            assert torch.equal(out, w)
