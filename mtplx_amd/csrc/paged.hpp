@@ -71,6 +71,8 @@ struct mtp_paged_attn_args {
 
 namespace mtp {
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
 // Pages hold [Hkv][page_size / 32] blocks of 32 keys x D, each in the order
 // in which an attention wave loads its v_mfma_f32_32x32x16_bf16 operands: 64
 // lanes x 16 contiguous bytes, so an operand is one 1 KB load and V needs no
@@ -95,6 +97,15 @@ __device__ __forceinline__ int page_k_index(int key, int d) {
 
 // Key (of 16) in slot e (of 8) of lane half h2.
 __device__ __forceinline__ int v_slot_key(int h2, int e) { return e < 4 ? 4 * h2 + e : 4 + 4 * h2 + e; }
+
+// And the half and the slot of a key of 16.
+__device__ __forceinline__ int v_key_half(int k) { return (k >> 2) & 1; }
+__device__ __forceinline__ int v_key_slot(int k) { return (k & 3) + (k >> 3) * 4; }
+template <int D, int BITS>
+__device__ __forceinline__ int page_v_index(int key, int d) {
+  const int lane = 32 * v_key_half(key & 15) + d % 32, e = v_key_slot(key & 15);
+  return BITS == 8 ? (d / 32 * 64 + lane) * 16 + 8 * (key >> 4) + e : ((2 * (d / 32) + (key >> 4)) * 64 + lane) * 8 + e;
+}
 
 // Status bits: a position outside the block table (or a page outside the
 // pool) was asked for; that row was not written, or reads as absent.

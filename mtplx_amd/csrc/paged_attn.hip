@@ -35,7 +35,6 @@ namespace mtp {
 
 constexpr int kPT = 256;   // threads: four waves
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 
 struct PAttn {

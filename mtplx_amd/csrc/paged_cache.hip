@@ -26,7 +26,7 @@ __device__ __forceinline__ void rotate_rows(const RotRows& q, int Hq, const RotR
     const RotRows& s = isq ? q : k;
     const int hh = isq ? h : h - Hq;
     uint16_t* dst = s.dst + (t0 + t) * s.dt + hh * s.dh;
-    rot_item(it, s.src + (t0 + t) * s.st + hh * s.sh, r.dims, r.trad, cs + t * half,
+    rot_item(it, s.src + (t0 + t) * s.st + hh * s.sh, r.dims, r.trad, [&](int i) { return cs[t * half + i]; },
              [&](int d, uint4 v) { *reinterpret_cast<uint4*>(dst + d) = v; });
   }
 }
@@ -75,204 +75,269 @@ __device__ __forceinline__ int touched_blocks(long long start, int n) {
   return n > 0 ? (int)(floor_blk(start + n - 1) - floor_blk(start)) + 1 : 0;
 }
 
-// The request and block that write unit u is, and the number of units in all.
-// With row offsets every wave scans the requests' block counts, 64 at a time.
-__device__ __forceinline__ bool find_unit(const WriteParams& p, long long u, int lane, int& b, int& blk,
-                                          long long& total) {
+// A wave's work: one block of 32 positions of one request, one head, K and V.
+struct Unit {
+  ReqRows rows;
+  long long start, blk;   // first position of the request, block of positions
+  int b;
+};
+
+// Unit u (of one head) of the call. With row offsets every wave scans the
+// requests' block counts, 64 at a time. False behind the last one.
+__device__ __forceinline__ bool find_unit(const WriteParams& p, long long u, int lane, Unit& w) {
   if (!p.row_off) {
-    total = (long long)p.B * p.nb_uniform;
-    b = (int)(u / p.nb_uniform);
-    blk = (int)(u % p.nb_uniform);
-    return u < total;
+    if (u >= (long long)p.B * p.nb_uniform) return false;
+    w.b = (int)(u / p.nb_uniform);
+    w.rows = req_rows(nullptr, w.b, p.B, p.T);
+    w.start = p.q_start[w.b];
+    w.blk = floor_blk(w.start) + (int)(u % p.nb_uniform);
+    return true;
   }
   long long carry = 0;
-  bool found = false;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
     const int bb = b0 + lane;
-    int cnt = 0;
-    if (bb < p.B) cnt = touched_blocks(p.q_start[bb], req_rows(p.row_off, bb, p.B, p.T).n);
+    ReqRows r = {0, 0};
+    int start = 0, cnt = 0;
+    if (bb < p.B) {
+      r = req_rows(p.row_off, bb, p.B, p.T);
+      start = p.q_start[bb];
+      cnt = touched_blocks(start, r.n);
+    }
     int incl = cnt;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
       const int t = __shfl_up(incl, off, 64);
       if (lane >= off) incl += t;
     }
-    const bool mine = !found && u >= carry + incl - cnt && u < carry + incl;
-    const unsigned long long m = __ballot(mine);
+    const unsigned long long m = __ballot(u < carry + incl);   // the first whose end lies behind u
     if (m) {
       const int src = __ffsll((long long)m) - 1;
-      b = b0 + src;
-      blk = (int)(u - carry) - __shfl(incl - cnt, src, 64);
-      found = true;
+      w.b = __builtin_amdgcn_readfirstlane(b0 + src);
+      w.rows.lo = __builtin_amdgcn_readlane(r.lo, src);
+      w.rows.n = __builtin_amdgcn_readlane(r.n, src);
+      w.start = __builtin_amdgcn_readlane(start, src);
+      w.blk = floor_blk(w.start) + (int)(u - carry) - __builtin_amdgcn_readlane(incl - cnt, src);
+      return true;
     }
-    carry += __shfl(incl, 63, 64);
+    carry += __builtin_amdgcn_readlane(incl, 63);
   }
-  total = carry;
-  b = __builtin_amdgcn_readfirstlane(b);
-  blk = __builtin_amdgcn_readfirstlane(blk);
-  return found;
+  return false;
 }
 
-// One unit: a block of 32 positions of one request, one head, K or V. The new
-// rows in it go through LDS (K rotated, rounded to bf16 as the standalone
-// rotation rounds) and out in the page's order, whole 16-byte chunks wherever
-// all their keys are new.
+// What a wave's lanes left in LDS is there for its other lanes (one wave's LDS
+// accesses complete in order; this keeps the compiler's order).
+__device__ __forceinline__ void wave_lds() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
+// LDS of a wave: 32 rows, padded so that 16-byte accesses of 8 rows hit
+// distinct banks; 8-bit rows take their place.
+template <int D>
+constexpr int row16() { return D + 8; }    // elements
+template <int D>
+constexpr int row8() { return D + 16; }    // bytes
+template <int D>
+constexpr int cache_waves() { return D == 256 ? 2 : 4; }
+
+// Lane l's half (l / 32) of row l % 32.
+template <int D>
+__device__ __forceinline__ void half_row(const uint16_t* rows, int lane, u32x4 (&x)[D / 16]) {
+  const uint16_t* row = rows + (lane & 31) * row16<D>() + (lane >> 5) * (D / 2);
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) x[i] = reinterpret_cast<const u32x4*>(row)[i];
+}
+
+// The row's scale (in both its lanes), and its elements as bytes. Largest
+// magnitude A, by the bits of bf16; then 127 / A and A / 127 (one correctly
+// rounded division each) and q = rint(x (127 / A)): adding 1.5 2^23 rounds to
+// an integer in the low bits, |x (127 / A)| < 127.5. A row with a NaN or an
+// infinity gets a NaN scale, so it reads as NaN instead of as wrong numbers;
+// one below 2^-100 gets zeros (127 / A would overflow, A / 127 go subnormal).
+template <int D>
+__device__ __forceinline__ float quantise(const u32x4 (&x)[D / 16], uint32_t (&w)[D / 8]) {
+#pragma clang fp contract(off)   // (the product is rounded before the sum)
+  u16x2 mx = {0, 0};
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) mx = __builtin_elementwise_max(mx, __builtin_bit_cast(u16x2, x[i][j] & 0x7fff7fffu));
+  }
+  int m = mx.x > mx.y ? mx.x : mx.y;
+  const int other = __shfl_xor(m, 32, 64);
+  m = m > other ? m : other;
+  const float a = __uint_as_float((uint32_t)m << 16);
+  const bool bad = m >= 0x7f80, tiny = a < 0x1p-100f;
+  const float inv = bad || tiny ? 0.f : 127.f / a;
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    const Chunk8 c = unpack8(__builtin_bit_cast(uint4, x[i]));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t q[4];   // (NaN has zeros in its low byte)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) q[j] = __float_as_uint(c.v[4 * h + j] * inv + 12582912.f);
+      w[2 * i + h] = __builtin_amdgcn_perm(q[1], q[0], 0x0c0c0400u) | __builtin_amdgcn_perm(q[3], q[2], 0x04000c0cu);
+    }
+  }
+  return bad ? __uint_as_float(0x7fc00000u) : tiny ? 0.f : a / 127.f;
+}
+
+// Bytes j of four words, as the j-th word.
+__device__ __forceinline__ void turn4(const uint32_t (&a)[4], uint32_t (&t)[4]) {
+  const uint32_t lo01 = __builtin_amdgcn_perm(a[1], a[0], 0x05010400u), hi01 = __builtin_amdgcn_perm(a[1], a[0], 0x07030602u);
+  const uint32_t lo23 = __builtin_amdgcn_perm(a[3], a[2], 0x05010400u), hi23 = __builtin_amdgcn_perm(a[3], a[2], 0x07030602u);
+  t[0] = __builtin_amdgcn_perm(lo23, lo01, 0x05040100u);
+  t[1] = __builtin_amdgcn_perm(lo23, lo01, 0x07060302u);
+  t[2] = __builtin_amdgcn_perm(hi23, hi01, 0x05040100u);
+  t[3] = __builtin_amdgcn_perm(hi23, hi01, 0x07060302u);
+}
+
+// One unit by one wave, in its own LDS: rows come whole, turn in LDS and leave
+// in the page's order, 16 bytes a lane; keys of a block that is not all new go
+// out element by element (V) or chunk by chunk (K).
 template <int D, int BITS>
-__device__ __forceinline__ void write_unit(const WriteParams& p, int b, int blk, int h, bool isk, unsigned char* lds) {
-  constexpr int RS = D + 8;   // LDS row: 16-byte reads of 8 rows hit distinct banks
-  uint16_t* rows = reinterpret_cast<uint16_t*>(lds);                 // [32][RS]
-  float2* cs = reinterpret_cast<float2*>(lds + 32 * RS * 2);         // [32][dims / 2]
-  float* sc = reinterpret_cast<float*>(lds + 32 * RS * 2 + 32 * (D / 2) * 8);   // [32] inverse scales
-  const int tid = threadIdx.x;
-  const ReqRows rq = req_rows(p.row_off, b, p.B, p.T);
-  const long long start = p.q_start[b];
-  const long long ablk = floor_blk(start) + blk, base = ablk * kBlk;
+__device__ __forceinline__ void write_unit(const WriteParams& p, const Unit& w, int h, int lane, uint16_t* rows) {
+  constexpr int RS = row16<D>(), NC = D / 16, BS = row8<D>();   // 16-byte loads of a lane
+  constexpr bool AHEAD = D < 256;   // V is asked for before K is done
+  const long long base = w.blk * kBlk;
   // Keys [klo, khi) of the block are new; token of key kk: first + kk.
-  const int klo = start > base ? (int)(start - base) : 0;
-  const long long end = start + rq.n - base;
+  const int klo = w.start > base ? (int)(w.start - base) : 0;
+  const long long end = w.start + w.rows.n - base;
   const int khi = end < kBlk ? (int)end : kBlk;
-  if (klo >= khi) return;   // uniform (a request of no rows)
-  const long long first = rq.lo + (base - start);
-  const long long at = page_block(p.block_table, p.width, b, ablk, p.bpp, p.num_pages, p.Hkv, h, kBlk * D);
+  if (klo >= khi) return;   // (a request of no rows)
+  const long long first = w.rows.lo + (base - w.start);
+  u32x4 kx[NC], vx[NC];
+  auto ask = [&](u32x4 (&x)[NC], const uint16_t* src, long long st) {   // (other keys' rows: the nearest new one's)
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = i * 64 + lane;
+      int kk = c / (D / 8);
+      kk = kk < klo ? klo : kk >= khi ? khi - 1 : kk;
+      x[i] = *reinterpret_cast<const u32x4*>(src + (first + kk) * st + c % (D / 8) * 8);
+    }
+  };
+  auto put = [&](const u32x4 (&x)[NC]) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = i * 64 + lane;
+      *reinterpret_cast<u32x4*>(rows + c / (D / 8) * RS + c % (D / 8) * 8) = x[i];
+    }
+    wave_lds();
+  };
+  ask(kx, p.k + h * p.k_head, p.k_token);
+  if (AHEAD) ask(vx, p.v + h * p.v_head, p.v_token);
+  const long long at = page_block(p.block_table, p.width, w.b, w.blk, p.bpp, p.num_pages, p.Hkv, h, kBlk * D);
   if (at < 0) {
-    if (p.status && tid == 0) atomicOr(p.status, kStatusPage);
+    if (p.status && lane == 0) atomicOr(p.status, kStatusPage);
     return;
   }
-  const int half = p.r.dims / 2, n = khi - klo;
-  if (isk && half) {
-    for (int x = tid; x < n * half; x += kNT)
-      cs[x] = rot_angle(base + klo + x / half, p.r.table[x % half], p.r.gain);
-    __syncthreads();
-  }
-  const uint16_t* src = isk ? p.k + h * p.k_head : p.v + h * p.v_head;
-  const long long st = isk ? p.k_token : p.v_token;
-  if (isk && half) {
-    const int ipr = rot_items(D, p.r.dims, p.r.trad);
-    for (int x = tid; x < n * ipr; x += kNT) {
-      const int kk = x / ipr;
-      uint16_t* dst = rows + (klo + kk) * RS;
-      rot_item(x % ipr, src + (first + klo + kk) * st, p.r.dims, p.r.trad, cs + kk * half,
-               [&](int d, uint4 v) { *reinterpret_cast<uint4*>(dst + d) = v; });
-    }
-  } else {
-    for (int x = tid; x < n * (D / 8); x += kNT) {
-      const int kk = klo + x / (D / 8), d = (x % (D / 8)) * 8;
-      *reinterpret_cast<uint4*>(rows + kk * RS + d) = *reinterpret_cast<const uint4*>(src + (first + kk) * st + d);
-    }
-  }
-  __syncthreads();
-  unsigned char* pool = isk ? p.k_pages : p.v_pages;
-  if constexpr (BITS == 8) {
-    // Eight lanes a row: its largest magnitude, then 127 / A and A / 127 (one
-    // correctly rounded division each). A row with a NaN or an infinity gets a
-    // NaN scale, so it reads as NaN instead of as wrong numbers; one below
-    // 2^-100 gets zeros (127 / A would overflow, A / 127 go subnormal).
-    const int kk = tid >> 3, part = tid & 7;
-    float a = 0.f;
-    bool bad = false;
-    if (kk >= klo && kk < khi) {
-#pragma unroll
-      for (int e = 0; e < D / 8; e += 8) {
-        const Chunk8 c = unpack8(*reinterpret_cast<const uint4*>(rows + kk * RS + part * (D / 8) + e));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          a = fmaxf(a, fabsf(c.v[i]));
-          bad |= !(fabsf(c.v[i]) <= 3.4e38f);
-        }
-      }
-    }
-#pragma unroll
-    for (int off = 1; off < 8; off <<= 1) {
-      a = fmaxf(a, __shfl_xor(a, off, 64));
-      bad |= (bool)__shfl_xor((int)bad, off, 64);
-    }
-    if (part == 0 && kk >= klo && kk < khi) {
-      const bool tiny = a < 0x1p-100f;
-      sc[kk] = bad || tiny ? 0.f : 127.f / a;
-      float* scales = (isk ? p.k_scales : p.v_scales) + at / D;   // [page][head][slot]
-      scales[kk] = bad ? __uint_as_float(0x7fc00000u) : tiny ? 0.f : a / 127.f;
-    }
-    __syncthreads();
-  }
-  auto quant = [&](float x, float inv) -> uint32_t {
-    // inv = 0 for a row of NaN scale: NaN and inf * 0 count as 0.
-    const float q = rintf(__fmul_rn(x, inv));
-    return (uint32_t)(q >= -127.f && q <= 127.f ? (int)q : q > 127.f ? 127 : q < -127.f ? -127 : 0) & 0xffu;
-  };
-  if (isk) {
-    constexpr int CH = BITS == 8 ? 16 : 8;
-    for (int x = tid; x < 32 * (D / CH); x += kNT) {   // chunk x: key x % 32, the order of the page
-      const int kk = x & 31, ih = x >> 5;
+  unsigned char* kd = p.k_pages + (size_t)at * (BITS / 8);
+  unsigned char* vd = p.v_pages + (size_t)at * (BITS / 8);
+  const int key = lane & 31;
+  const bool mine = key >= klo && key < khi;   // the lane's row
+  put(kx);
+  if (p.r.dims) {   // in place: an item reads what it stores, or the source
+    const int np = rot_paired(p.r.dims, p.r.trad) ? p.r.dims / 16 : (p.r.dims + 7) / 8;
+    const bool inplace = p.r.trad || rot_paired(p.r.dims, p.r.trad);
+    for (int x = lane; x < 32 * np; x += 64) {
+      const int kk = x / np;
       if (kk < klo || kk >= khi) continue;
-      const int d = (ih & 1) * (D / 2) + (ih >> 1) * CH;
-      const uint16_t* row = rows + kk * RS + d;
-      uint4 o;
-      if constexpr (BITS == 16) {
-        o = *reinterpret_cast<const uint4*>(row);
-      } else {
-        const float inv = sc[kk];
-        uint32_t w[4];
+      const int pos = (int)(base + kk);
+      uint16_t* row = rows + kk * RS;
+      auto angles = [&](int i) { return rot_angle(pos, p.r.table[i], p.r.gain); };
+      auto store = [&](int d, uint4 v) { *reinterpret_cast<uint4*>(row + d) = v; };
+      if (inplace)
+        rot_item(x % np, row, p.r.dims, p.r.trad, angles, store);
+      else
+        rot_item(x % np, p.k + h * p.k_head + (first + kk) * p.k_token, p.r.dims, p.r.trad, angles, store);
+    }
+    wave_lds();
+  }
+  half_row<D>(rows, lane, kx);
+  if constexpr (BITS == 16) {
+    if (mine) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const Chunk8 c = unpack8(*reinterpret_cast<const uint4*>(row + 8 * j));
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            w[2 * j + i] = quant(c.v[4 * i], inv) | quant(c.v[4 * i + 1], inv) << 8 |
-                           quant(c.v[4 * i + 2], inv) << 16 | quant(c.v[4 * i + 3], inv) << 24;
-        }
-        o = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-      *reinterpret_cast<uint4*>(pool + (size_t)at * (BITS / 8) + (size_t)x * 16) = o;
+      for (int i = 0; i < NC; ++i) *reinterpret_cast<u32x4*>(kd + (i * 64 + lane) * 16) = kx[i];
     }
   } else {
-    constexpr int JJ = BITS == 8 ? 1 : 2;   // 16-bit chunks hold the keys of one 16, 8-bit chunks of both
-    for (int x = tid; x < JJ * D * 2; x += kNT) {
-      const int c = x & 31, h2 = (x >> 5) & 1, tj = x >> 6;
-      const int d = 32 * (tj / JJ) + c;
-      unsigned char* dst = pool + (size_t)at * (BITS / 8) + (size_t)x * 16;
-      if constexpr (BITS == 16) {
-        const int k16 = 16 * (tj & 1);
-        uint16_t e[8];
-        bool all = true;
+    uint32_t q[D / 8];
+    const float s = quantise<D>(kx, q);
+    if (mine) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int kk = k16 + v_slot_key(h2, i);
-          const bool in = kk >= klo && kk < khi;
-          all &= in;
-          e[i] = in ? rows[kk * RS + d] : 0;
-        }
-        if (all) {
-          *reinterpret_cast<uint4*>(dst) = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16,
-                                                      e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
-        } else {
+      for (int i = 0; i < NC / 2; ++i)
+        *reinterpret_cast<u32x4*>(kd + (i * 64 + lane) * 16) = u32x4{q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]};
+      if (lane < 32) (p.k_scales + at / D)[key] = s;   // [page][head][slot]
+    }
+  }
+  wave_lds();
+  if (!AHEAD) ask(vx, p.v + h * p.v_head, p.v_token);
+  put(vx);
+  const bool all = klo == 0 && khi == kBlk;
+  if constexpr (BITS == 16) {
+    if (all) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int kk = k16 + v_slot_key(h2, i);
-            if (kk >= klo && kk < khi) reinterpret_cast<uint16_t*>(dst)[i] = e[i];
-          }
-        }
-      } else {
-        uint32_t w[4] = {0, 0, 0, 0};
-        bool all = true;
+      for (int i = 0; i < 2 * D / 64; ++i) {   // two columns, the eight keys of a chunk each
+        const int x = i * 64 + lane, c = x % 16 * 2, hh = (x >> 4) & 1, tj = x >> 5;
+        const uint16_t* col = rows + 16 * (tj & 1) * RS + 32 * (tj >> 1) + c;
+        uint32_t a[8];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int kk = 16 * (i >> 3) + v_slot_key(h2, i & 7);
-          const bool in = kk >= klo && kk < khi;
-          all &= in;
-          if (in) w[i >> 2] |= quant(bf2f(rows[kk * RS + d]), sc[kk]) << (8 * (i & 3));
-        }
-        if (all) {
-          *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-        } else {
+        for (int e = 0; e < 8; ++e) a[e] = *reinterpret_cast<const uint32_t*>(col + v_slot_key(hh, e) * RS);
+        uint32_t lo[4], hi[4];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int kk = 16 * (i >> 3) + v_slot_key(h2, i & 7);
-            if (kk >= klo && kk < khi) dst[i] = (unsigned char)(w[i >> 2] >> (8 * (i & 3)));
-          }
+        for (int e = 0; e < 4; ++e) {
+          lo[e] = __builtin_amdgcn_perm(a[2 * e + 1], a[2 * e], 0x05040100u);
+          hi[e] = __builtin_amdgcn_perm(a[2 * e + 1], a[2 * e], 0x07060302u);
         }
+        u32x4* dst = reinterpret_cast<u32x4*>(vd) + tj * 64 + hh * 32 + c;
+        dst[0] = u32x4{lo[0], lo[1], lo[2], lo[3]};
+        dst[1] = u32x4{hi[0], hi[1], hi[2], hi[3]};
+      }
+    } else {
+      for (int x = lane; x < (khi - klo) * D; x += 64) {
+        const int kk = klo + x / D, d = x % D;
+        reinterpret_cast<uint16_t*>(vd)[page_v_index<D, 16>(kk, d)] = rows[kk * RS + d];
+      }
+    }
+  } else {
+    uint32_t q[D / 8];
+    half_row<D>(rows, lane, vx);
+    const float s = quantise<D>(vx, q);
+    if (mine && lane < 32) (p.v_scales + at / D)[key] = s;
+    wave_lds();
+    unsigned char* bytes = reinterpret_cast<unsigned char*>(rows);
+#pragma unroll
+    for (int i = 0; i < NC / 2; ++i)
+      *reinterpret_cast<u32x4*>(bytes + key * BS + (lane >> 5) * (D / 2) + 16 * i) =
+          u32x4{q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]};
+    wave_lds();
+    if (all) {
+      for (int x = lane; x < D / 2; x += 64) {   // four columns, the sixteen keys of a chunk each
+        const int c = x % 8 * 4, hh = (x >> 3) & 1, t = x >> 4;
+        uint32_t o[4][4];   // [keys][column]
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t a[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            a[e] = *reinterpret_cast<const uint32_t*>(bytes + (16 * (j >> 1) + v_slot_key(hh, 4 * (j & 1) + e)) * BS + 32 * t + c);
+          turn4(a, o[j]);
+        }
+        u32x4* dst = reinterpret_cast<u32x4*>(vd) + t * 64 + hh * 32 + c;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dst[e] = u32x4{o[0][e], o[1][e], o[2][e], o[3][e]};
+      }
+    } else {
+      for (int x = lane; x < (khi - klo) * D; x += 64) {
+        const int kk = klo + x / D, d = x % D;
+        vd[page_v_index<D, 8>(kk, d)] = bytes[kk * BS + d];
       }
     }
   }
+  wave_lds();
 }
 
 // Request of packed token t: the b with row_off[b] <= t < row_off[b + 1], or
@@ -296,16 +361,12 @@ __device__ __forceinline__ int token_request(const WriteParams& p, int t, long l
 }
 
 template <int D, int BITS>
-constexpr size_t write_lds_bytes() {
-  return (size_t)32 * (D + 8) * 2 + (size_t)32 * (D / 2) * 8 + 32 * 4;
-}
-
-template <int D, int BITS>
-__global__ __launch_bounds__(kNT) void paged_write_kernel(WriteParams p) {
-  __shared__ __attribute__((aligned(16))) unsigned char lds[write_lds_bytes<D, BITS>()];
+__global__ __launch_bounds__(64 * cache_waves<D>(), D == 256 ? 1 : 4) void paged_write_kernel(WriteParams p) {
+  constexpr int NT = 64 * cache_waves<D>();
+  __shared__ __attribute__((aligned(16))) uint16_t lds[cache_waves<D>()][32 * row16<D>()];
   const int lane = threadIdx.x & 63;
   if ((int)blockIdx.x >= p.kv_groups) {   // rotate queries, q_tokens at a time
-    float2* cs = reinterpret_cast<float2*>(lds);
+    float2* cs = reinterpret_cast<float2*>(&lds[0][0]);
     __shared__ int s_live[kRotTokens];
     const int half = p.r.dims / 2, ipr = rot_items(D, p.r.dims, p.r.trad);
     const int stride = ((int)gridDim.x - p.kv_groups) * p.q_tokens;
@@ -315,15 +376,16 @@ __global__ __launch_bounds__(kNT) void paged_write_kernel(WriteParams p) {
         long long pos = 0;
         const int b = token_request(p, t0 + t, &pos);   // the same in every thread
         if (threadIdx.x == 0) s_live[t] = b >= 0;
-        for (int x = threadIdx.x; x < half; x += kNT) cs[t * half + x] = rot_angle(pos, p.r.table[x], p.r.gain);
+        for (int x = threadIdx.x; x < half; x += NT) cs[t * half + x] = rot_angle(pos, p.r.table[x], p.r.gain);
       }
       __syncthreads();
-      for (int x = threadIdx.x; x < n * p.Hq * ipr; x += kNT) {
+      for (int x = threadIdx.x; x < n * p.Hq * ipr; x += NT) {
         const int it = x % ipr, th = x / ipr;
         const int h = th % p.Hq, t = th / p.Hq;
         if (!s_live[t]) continue;   // rows behind the last request stay as they are
         uint16_t* dst = p.q.dst + (t0 + t) * p.q.dt + h * p.q.dh;
-        rot_item(it, p.q.src + (t0 + t) * p.q.st + h * p.q.sh, p.r.dims, p.r.trad, cs + t * half,
+        rot_item(it, p.q.src + (t0 + t) * p.q.st + h * p.q.sh, p.r.dims, p.r.trad,
+                 [&](int i) { return cs[t * half + i]; },
                  [&](int d, uint4 v) { *reinterpret_cast<uint4*>(dst + d) = v; });
       }
       __syncthreads();
@@ -331,14 +393,11 @@ __global__ __launch_bounds__(kNT) void paged_write_kernel(WriteParams p) {
     }
     return;
   }
-  const long long per = 2LL * p.Hkv;
-  for (long long x = blockIdx.x;; x += p.kv_groups) {
-    int b = 0, blk = 0;
-    long long total = 0;
-    if (!find_unit(p, x / per, lane, b, blk, total)) return;   // the same in every thread
-    const int hk = (int)(x % per);
-    write_unit<D, BITS>(p, b, blk, hk >> 1, (hk & 1) == 0, lds);
-    __syncthreads();
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  for (long long x = (long long)blockIdx.x * cache_waves<D>() + wave;; x += (long long)p.kv_groups * cache_waves<D>()) {
+    Unit w;
+    if (!find_unit(p, x / p.Hkv, lane, w)) return;   // (no barrier follows)
+    write_unit<D, BITS>(p, w, (int)(x % p.Hkv), lane, lds[wave]);
   }
 }
 
@@ -356,88 +415,132 @@ struct ReadParams {
   int B, width, count, Hkv, bpp, num_pages, nb;
 };
 
-// One workgroup: a block of 32 positions of one request, one head, K or V,
-// back into rows [B, Hkv, count, D].
+// One wave: a block of 32 positions of one request, one head, K and V, from the
+// page's order through its LDS back into rows [B, Hkv, count, D]. 8-bit
+// elements turn as bytes and are widened on their way out.
 template <int D, int BITS>
-__global__ __launch_bounds__(kNT) void paged_read_kernel(ReadParams p) {
-  constexpr int RS = D + 8;
-  __shared__ __attribute__((aligned(16))) uint16_t rows[32 * RS];
-  __shared__ float sc[32];
-  const int tid = threadIdx.x;
-  const long long units = 2LL * p.B * p.Hkv * p.nb;
-  for (long long u = blockIdx.x; u < units; u += gridDim.x) {
-    const bool isk = (u & 1) == 0;
-    const long long v = u >> 1;
-    const int blk = (int)(v % p.nb);
-    const int h = (int)(v / p.nb % p.Hkv);
-    const int b = (int)(v / p.nb / p.Hkv);
-    const long long start = p.start ? p.start[b] : 0;
-    const long long ablk = floor_blk(start) + blk, base = ablk * kBlk;
-    const int klo = start > base ? (int)(start - base) : 0;
-    const long long end = start + p.count - base;
-    const int khi = end < kBlk ? (int)end : kBlk;
-    if (klo < khi) {   // uniform
-      const long long len = p.lengths ? (long long)p.lengths[b] - base : kBlk;
-      int live = len < khi ? (len < 0 ? 0 : (int)len) : khi;   // keys [klo, live) are read, [live, khi) are zeros
-      if (live < klo) live = klo;
-      if (live > klo) {
-        const long long at = page_block(p.block_table, p.width, b, ablk, p.bpp, p.num_pages, p.Hkv, h, kBlk * D);
-        if (at < 0) {
-          if (p.status && tid == 0) atomicOr(p.status, kStatusPage);
-          live = klo;
-        } else {
-          const unsigned char* pool = (isk ? p.k_pages : p.v_pages) + (size_t)at * (BITS / 8);
-          if constexpr (BITS == 8) {
-            if (tid < 32) sc[tid] = ((isk ? p.k_scales : p.v_scales) + at / D)[tid];
-            __syncthreads();
-          }
-          auto put8 = [&](uint32_t byte, float s) { return f2bf(__fmul_rn((float)(int8_t)byte, s)); };
-          constexpr int CH = BITS == 8 ? 16 : 8;
-          for (int x = tid; x < 32 * (D / CH); x += kNT) {
-            const uint4 c = *reinterpret_cast<const uint4*>(pool + (size_t)x * 16);
-            const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-            if (isk) {
-              const int kk = x & 31, ih = x >> 5;
-              uint16_t* dst = rows + kk * RS + (ih & 1) * (D / 2) + (ih >> 1) * CH;
-              if constexpr (BITS == 16) {
-                *reinterpret_cast<uint4*>(dst) = c;
-              } else {
-                const float s = sc[kk];
+__device__ __forceinline__ void read_unit(const ReadParams& p, int b, int h, int blk, int lane, unsigned char* lds) {
+  constexpr int NC = D * BITS / 256;   // 16-byte loads of a lane
+  constexpr int RS = BITS == 8 ? row8<D>() : row16<D>() * 2;   // bytes of a row
+  constexpr bool AHEAD = NC <= 8;
+  const long long start = p.start ? p.start[b] : 0;
+  const long long ablk = floor_blk(start) + blk, base = ablk * kBlk;
+  const int klo = start > base ? (int)(start - base) : 0;
+  const long long end = start + p.count - base;
+  const int khi = end < kBlk ? (int)end : kBlk;
+  if (klo >= khi) return;
+  const long long len = p.lengths ? (long long)p.lengths[b] - base : kBlk;
+  int live = len < khi ? (len < 0 ? 0 : (int)len) : khi;   // keys [klo, live) are read, [live, khi) are zeros
+  if (live < klo) live = klo;
+  long long at = -1;
+  if (live > klo) {
+    at = page_block(p.block_table, p.width, b, ablk, p.bpp, p.num_pages, p.Hkv, h, kBlk * D);
+    if (at < 0) {
+      if (p.status && lane == 0) atomicOr(p.status, kStatusPage);
+      live = klo;
+    }
+  }
+  constexpr int W = BITS == 8 ? 4 : 2, NV = NC < W ? W : NC;   // (D = 64, 8 bits: half the lanes hold all of V)
+  u32x4 kx[NC], vx[NV];
+  float ks = 0.f, vs = 0.f;   // lane l: key l % 32's
+  auto ask = [&](u32x4 (&x)[NC], const unsigned char* pool) {
+    const unsigned char* src = pool + (size_t)at * (BITS / 8);
 #pragma unroll
-                for (int i = 0; i < 16; i += 2)
-                  *reinterpret_cast<uint32_t*>(dst + i) =
-                      put8(w[i >> 2] >> (8 * (i & 3)), s) |
-                      (uint32_t)put8(w[i >> 2] >> (8 * (i & 3) + 8), s) << 16;
-              }
-            } else {
-              const int cc = x & 31, h2 = (x >> 5) & 1, tj = x >> 6;
-              if constexpr (BITS == 16) {
-                const int d = 32 * (tj >> 1) + cc, k16 = 16 * (tj & 1);
+    for (int i = 0; i < NC; ++i) x[i] = *reinterpret_cast<const u32x4*>(src + (i * 64 + lane) * 16);
+  };
+  // V's chunks by what turns together: four columns of 16 keys, or two of 8.
+  auto ask_v = [&]() {
+    const u32x4* src = reinterpret_cast<const u32x4*>(p.v_pages + (size_t)at * (BITS / 8));
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                  rows[(k16 + v_slot_key(h2, i)) * RS + d] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
-              } else {
-                const int d = 32 * tj + cc;
+    for (int i = 0; i < NV; ++i) {
+      const int x = (i / W) * 64 + lane;
+      const int c = BITS == 8 ? x / 8 * 32 + x % 8 * 4 : x / 16 * 32 + x % 16 * 2;
+      if (x * W < D * BITS / 4) vx[i] = src[c + i % W];
+    }
+  };
+  if (at >= 0) {
+    ask(kx, p.k_pages);
+    if (AHEAD) ask_v();
+    if constexpr (BITS == 8) {
+      ks = (p.k_scales + at / D)[lane & 31];
+      vs = (p.v_scales + at / D)[lane & 31];
+    }
+  }
+  auto leave = [&](uint16_t* dst, float s) {   // rows [klo, khi): whole 16-byte chunks
+    dst += (((size_t)b * p.Hkv + h) * p.count) * D;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  const int kk = 16 * (i >> 3) + v_slot_key(h2, i & 7);
-                  rows[kk * RS + d] = put8(w[i >> 2] >> (8 * (i & 3)), sc[kk]);
-                }
-              }
-            }
-          }
+    for (int i = 0; i < D / 16; ++i) {
+      const int c = i * 64 + lane, kk = c / (D / 8), d = c % (D / 8) * 8;
+      u32x4 o;
+      if constexpr (BITS == 8) {
+        const uint2 w = *reinterpret_cast<const uint2*>(lds + kk * RS + d);
+        const float sk = __shfl(s, kk, 64);
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          y[e] = __fmul_rn((float)(int8_t)(w.x >> (8 * e)), sk);
+          y[e + 4] = __fmul_rn((float)(int8_t)(w.y >> (8 * e)), sk);
+        }
+        o = __builtin_bit_cast(u32x4, pack8(y));
+      } else {
+        o = *reinterpret_cast<const u32x4*>(lds + kk * RS + d * 2);
+      }
+      if (kk >= live) o = u32x4{0, 0, 0, 0};
+      if (kk >= klo && kk < khi) *reinterpret_cast<u32x4*>(dst + (base + kk - start) * D + d) = o;
+    }
+    wave_lds();
+  };
+  if (at >= 0) {   // lane l: its half of row l % 32
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      *reinterpret_cast<u32x4*>(lds + (lane & 31) * RS + (lane >> 5) * (D * BITS / 16) + 16 * i) = kx[i];
+    wave_lds();
+  }
+  leave(p.k_out, ks);
+  if (at >= 0) {
+    if (!AHEAD) ask_v();
+    if constexpr (BITS == 8) {
+#pragma unroll
+      for (int i = 0; i < NV; i += 4) {
+        const int x = i / 4 * 64 + lane, c = x % 8 * 4, hh = (x >> 3) & 1, t = x >> 4;
+        if (x >= D / 2) continue;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t a[4] = {vx[i][j], vx[i + 1][j], vx[i + 2][j], vx[i + 3][j]};
+          uint32_t o[4];
+          turn4(a, o);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<uint32_t*>(lds + (16 * (j >> 1) + v_slot_key(hh, 4 * (j & 1) + e)) * RS + 32 * t + c) = o[e];
         }
       }
-      __syncthreads();
-      uint16_t* out = (isk ? p.k_out : p.v_out) + (((size_t)b * p.Hkv + h) * p.count) * D;
-      for (int x = tid; x < (khi - klo) * (D / 8); x += kNT) {
-        const int kk = klo + x / (D / 8), d = (x % (D / 8)) * 8;
-        const size_t j = (size_t)(base + kk - start);
-        *reinterpret_cast<uint4*>(out + j * D + d) =
-            kk < live ? *reinterpret_cast<const uint4*>(rows + kk * RS + d) : make_uint4(0, 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; i += 2) {
+        const int x = i / 2 * 64 + lane, c = x % 16 * 2, hh = (x >> 4) & 1, tj = x >> 5;
+        unsigned char* col = lds + 16 * (tj & 1) * RS + (32 * (tj >> 1) + c) * 2;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t a = vx[i][e], bb = vx[i + 1][e];
+          *reinterpret_cast<uint32_t*>(col + v_slot_key(hh, 2 * e) * RS) = __builtin_amdgcn_perm(bb, a, 0x05040100u);
+          *reinterpret_cast<uint32_t*>(col + v_slot_key(hh, 2 * e + 1) * RS) = __builtin_amdgcn_perm(bb, a, 0x07060302u);
+        }
       }
     }
-    __syncthreads();
+    wave_lds();
+  }
+  leave(p.v_out, vs);
+}
+
+template <int D, int BITS>
+__global__ __launch_bounds__(64 * cache_waves<D>()) void paged_read_kernel(ReadParams p) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[cache_waves<D>()][32 * (BITS == 8 ? row8<D>() : row16<D>() * 2)];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long long units = (long long)p.B * p.Hkv * p.nb, step = (long long)gridDim.x * cache_waves<D>();
+  for (long long u = (long long)blockIdx.x * cache_waves<D>() + wave; u < units; u += step) {
+    const long long v = u / p.nb;
+    read_unit<D, BITS>(p, (int)(v / p.Hkv), (int)(v % p.Hkv), (int)(u % p.nb), lane, lds[wave]);
   }
 }
 
@@ -455,11 +558,11 @@ inline int rot_tokens(int T) { return T >= 8 * 256 ? 8 : T >= 4 * 256 ? 4 : T >=
 
 template <int D, int BITS>
 void launch_write(const WriteParams& p, int groups, hipStream_t st) {
-  hipLaunchKernelGGL((paged_write_kernel<D, BITS>), dim3((unsigned)groups), dim3(kNT), 0, st, p);
+  hipLaunchKernelGGL((paged_write_kernel<D, BITS>), dim3((unsigned)groups), dim3(64 * cache_waves<D>()), 0, st, p);
 }
 template <int D, int BITS>
 void launch_read(const ReadParams& p, int groups, hipStream_t st) {
-  hipLaunchKernelGGL((paged_read_kernel<D, BITS>), dim3((unsigned)groups), dim3(kNT), 0, st, p);
+  hipLaunchKernelGGL((paged_read_kernel<D, BITS>), dim3((unsigned)groups), dim3(64 * cache_waves<D>()), 0, st, p);
 }
 
 }  // namespace mtp
@@ -550,7 +653,8 @@ MTP_API int mtp_paged_write(const mtp_paged_write_args* a, void* stream) {
     p.nb_uniform = (int)most(a->T / a->B);
     units = (long long)a->B * p.nb_uniform;
   }
-  long long groups = units * 2 * a->Hkv;
+  const int waves = a->D == 256 ? cache_waves<256>() : cache_waves<128>();
+  long long groups = (units * a->Hkv + waves - 1) / waves;
   if (groups > 1 << 20) groups = 1 << 20;
   p.kv_groups = (int)groups;
   if (a->q) {
@@ -588,7 +692,8 @@ MTP_API int mtp_paged_read(const mtp_paged_read_args* a, void* stream) {
                   (const float*)a->v_scales, a->block_table, a->start, a->lengths, (uint16_t*)a->k_out,
                   (uint16_t*)a->v_out, a->status, a->B, a->width, a->count, a->Hkv, a->page_size / kBlk,
                   a->num_pages, (int)(((long long)a->count + 30) / kBlk + 1)};
-  long long groups = 2LL * a->B * a->Hkv * p.nb;
+  const int waves = a->D == 256 ? cache_waves<256>() : cache_waves<128>();
+  long long groups = ((long long)a->B * a->Hkv * p.nb + waves - 1) / waves;
   if (groups > 1 << 20) groups = 1 << 20;
   hipStream_t st = (hipStream_t)stream;
   switch (a->D * 100 + a->bits) {

@@ -11,7 +11,6 @@
 // take revolutions; both are within 2^-20 of the true values over all
 // fractions (bf16 rounds at 2^-9), for 8 issue slots instead of the ~40 that
 // sincosf spends on its own reduction.
-// (-> test_gpu_rotary.py measures that bound through the operator.)
 #pragma once
 
 #include "common.hpp"
@@ -61,13 +60,12 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
   return make_uint4(f2bf2(v[0], v[1]), f2bf2(v[2], v[3]), f2bf2(v[4], v[5]), f2bf2(v[6], v[7]));
 }
 
-// Item `it` of one head's row (16-byte aligned), cs its token's cos/sin of
-// each pair; store(d, chunk) takes 8 finished elements from d on. An item
+// Item `it` of one head's row (16-byte aligned), cs(i) its token's cos/sin of
+// pair i; store(d, chunk) takes 8 finished elements from d on. An item
 // reads all it needs before it stores, and only what it stores, unless the
 // halves are no whole chunks (then partners are read from other items' rows).
-template <class Store>
-__device__ __forceinline__ void rot_item(int it, const uint16_t* row, int dims, int trad, const float2* cs,
-                                         Store store) {
+template <class Angles, class Store>
+__device__ __forceinline__ void rot_item(int it, const uint16_t* row, int dims, int trad, Angles cs, Store store) {
   if (rot_paired(dims, trad)) {
     const int np = dims / 16;
     if (it < np) {
@@ -77,7 +75,7 @@ __device__ __forceinline__ void rot_item(int it, const uint16_t* row, int dims, 
       float y1[8], y2[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float2 w = cs[d + e];
+        const float2 w = cs(d + e);
         y1[e] = rot_first(a.v[e], b.v[e], w);
         y2[e] = rot_second(a.v[e], b.v[e], w);
       }
@@ -101,7 +99,7 @@ __device__ __forceinline__ void rot_item(int it, const uint16_t* row, int dims, 
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {   // dims is even: a pair rotates or passes as a whole
       const bool in = d + e < dims;
-      const float2 w = in ? cs[(d + e) >> 1] : make_float2(1.f, 0.f);
+      const float2 w = in ? cs((d + e) >> 1) : make_float2(1.f, 0.f);
       y[e] = in ? rot_first(a.v[e], a.v[e + 1], w) : a.v[e];
       y[e + 1] = in ? rot_second(a.v[e], a.v[e + 1], w) : a.v[e + 1];
     }
@@ -113,9 +111,9 @@ __device__ __forceinline__ void rot_item(int it, const uint16_t* row, int dims, 
       if (dd >= dims)
         y[e] = a.v[e];
       else if (dd < half)
-        y[e] = rot_first(a.v[e], bf2f(row[dd + half]), cs[dd]);
+        y[e] = rot_first(a.v[e], bf2f(row[dd + half]), cs(dd));
       else
-        y[e] = rot_second(bf2f(row[dd - half]), a.v[e], cs[dd - half]);
+        y[e] = rot_second(bf2f(row[dd - half]), a.v[e], cs(dd - half));
     }
   }
   store(d, pack8(y));
