@@ -107,6 +107,18 @@ __device__ __forceinline__ int page_v_index(int key, int d) {
   return BITS == 8 ? (d / 32 * 64 + lane) * 16 + 8 * (key >> 4) + e : ((2 * (d / 32) + (key >> 4)) * 64 + lane) * 8 + e;
 }
 
+// The same value, computed here: what follows from it is not kept in registers
+// across a loop (a spill's reload waits for every load in flight).
+__device__ __forceinline__ int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// a / b of a >= 0, b > 0; 32-bit division where that does.
+__device__ __forceinline__ long long div_pos(long long a, int b) {
+  return a >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+}
+
 // Status bits: a position outside the block table (or a page outside the
 // pool) was asked for; that row was not written, or reads as absent.
 constexpr int kStatusPage = 1;
@@ -116,9 +128,10 @@ constexpr int kStatusPage = 1;
 __device__ __forceinline__ long long page_block(const int32_t* table, int width, int b, long long blk, int bpp,
                                                 int num_pages, int Hkv, int h, int elems) {
   if (blk < 0 || blk >= (long long)width * bpp) return -1;
-  const int id = table[(size_t)b * width + (int)(blk / bpp)];
+  const uint32_t page = (uint32_t)blk / (uint32_t)bpp;   // (width * page_size < 2^31)
+  const int id = table[(size_t)b * width + page];
   if (id < 0 || id >= num_pages) return -1;
-  return (((long long)id * Hkv + h) * bpp + (int)(blk % bpp)) * elems;
+  return (((long long)id * Hkv + h) * bpp + (int)((uint32_t)blk - page * (uint32_t)bpp)) * elems;
 }
 
 // Rows [lo, hi) of the packed tokens that belong to request b, whatever the

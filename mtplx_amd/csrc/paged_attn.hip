@@ -65,13 +65,6 @@ struct PAttn {
 // Token and head (of those that share a kv head) of a row of a tile's list.
 __device__ __forceinline__ int row_token(const PAttn& p, int r) { return (int)(((uint32_t)r * p.rep_inv) >> 16); }
 
-// The same value, computed here: what follows from it is not kept in registers
-// across the key loop (a spill's reload waits for every load in flight).
-__device__ __forceinline__ int fresh(int x) {
-  asm volatile("" : "+v"(x));
-  return x;
-}
-
 // -- the line of work -------------------------------------------------------------
 
 
@@ -1029,7 +1022,9 @@ __global__ __launch_bounds__(kPT, D == 256 ? 1 : 2) void attn_few_kernel(PAttn p
 
 // Workgroup (g, y): one (32 rows, 32 d) block of the tile that workgroup g began
 // and others finished; a thread sums one float4 of it over the pieces, eight
-// loads at a time, with the pieces' weights 2^(m - max) from LDS.
+// loads at a time, with the pieces' weights 2^(m - max) from LDS. Lanes without
+// a row (a decode step's tile holds few) take a share of the pieces instead:
+// with NR rows' lanes, lane r + NR s adds pieces s, s + 32 / NR, .. of row r.
 constexpr int kJoin = 64;   // pieces whose weights LDS holds
 
 template <int D, int RT>
@@ -1045,13 +1040,18 @@ __global__ __launch_bounds__(kPT) void attn_join_kernel(PAttn p) {
   if (r0 >= rows) return;
   // Piece k's slot: the one that begins the tile is g's second.
   auto slot = [&](int k) { return (size_t)(2 * (g + k) + (k == 0 ? 1 : 0)); };
-  const int row = tid & 31;
+  int NR = 32;   // (chunks' tiles: always, so that the loop below is a plain one)
+  while (RT == 32 && NR > 4 && rows - r0 <= NR / 2) NR >>= 1;
+  const int SP = 32 / NR, row = tid & (NR - 1), share = (tid & 31) / NR;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   constexpr int B8 = 8;   // pieces whose blocks are in flight together
   float4 a8[B8];
   auto ask = [&](int k) {   // (the last piece again past the last: never used)
 #pragma unroll
-    for (int i = 0; i < B8; ++i) a8[i] = part_block<D>(p, slot(k + i < np ? k + i : np - 1), RT, rb, t)[tid];
+    for (int i = 0; i < B8; ++i) {
+      const int kk = k + SP * i + share;
+      a8[i] = part_block<D>(p, slot(kk < np ? kk : np - 1), RT, rb, t)[(tid & ~31) + row];
+    }
   };
   ask(0);
   if (tid < 32) {
@@ -1100,18 +1100,25 @@ __global__ __launch_bounds__(kPT) void attn_join_kernel(PAttn p) {
     v.y *= c;
     v.z *= c;
     v.w *= c;
-    for (int k = 0; k < n; k += B8) {
+    for (int k = 0; k < n; k += B8 * SP) {   // (B8 SP divides kJoin)
 #pragma unroll
       for (int i = 0; i < B8; ++i) {
-        const float w = k + i < n ? s_w[k + i][row] : 0.f;
+        const int kk = k + SP * i + share;
+        const float w = kk < n ? s_w[kk][row] : 0.f;
         // (weight 0: a piece without keys wrote no block, or one that is nothing beside the others)
         v.x += w == 0.f ? 0.f : a8[i].x * w;
         v.y += w == 0.f ? 0.f : a8[i].y * w;
         v.z += w == 0.f ? 0.f : a8[i].z * w;
         v.w += w == 0.f ? 0.f : a8[i].w * w;
       }
-      if (k0 + k + B8 < np) ask(k0 + k + B8);
+      if (k0 + k + B8 * SP < np) ask(k0 + k + B8 * SP);
     }
+  }
+  for (int off = NR; off < 32; off <<= 1) {
+    v.x += __shfl_xor(v.x, off, 64);
+    v.y += __shfl_xor(v.y, off, 64);
+    v.z += __shfl_xor(v.z, off, 64);
+    v.w += __shfl_xor(v.w, off, 64);
   }
   const float l = s_l[row], inv = l == 0.f ? 0.f : 1.f / l;
   store4(&s_out[row][4 * (tid >> 5)], v.x * inv, v.y * inv, v.z * inv, v.w * inv);

@@ -67,7 +67,7 @@ struct WriteParams {
   int nb_uniform;                // blocks of each request where row_off is null
 };
 
-__device__ __forceinline__ long long floor_blk(long long p) { return p >= 0 ? p / kBlk : -((-p + kBlk - 1) / kBlk); }
+__device__ __forceinline__ long long floor_blk(long long p) { return p >> 5; }   // (blocks of 32)
 
 // Blocks of 32 positions that request b's new tokens fall into, from the
 // block of the first one on.
@@ -87,10 +87,10 @@ struct Unit {
 __device__ __forceinline__ bool find_unit(const WriteParams& p, long long u, int lane, Unit& w) {
   if (!p.row_off) {
     if (u >= (long long)p.B * p.nb_uniform) return false;
-    w.b = (int)(u / p.nb_uniform);
+    w.b = (int)div_pos(u, p.nb_uniform);
     w.rows = req_rows(nullptr, w.b, p.B, p.T);
     w.start = p.q_start[w.b];
-    w.blk = floor_blk(w.start) + (int)(u % p.nb_uniform);
+    w.blk = floor_blk(w.start) + (u - (long long)w.b * p.nb_uniform);
     return true;
   }
   long long carry = 0;
@@ -151,39 +151,51 @@ __device__ __forceinline__ void half_row(const uint16_t* rows, int lane, u32x4 (
   for (int i = 0; i < D / 16; ++i) x[i] = reinterpret_cast<const u32x4*>(row)[i];
 }
 
-// The row's scale (in both its lanes), and its elements as bytes. Largest
-// magnitude A, by the bits of bf16; then 127 / A and A / 127 (one correctly
-// rounded division each) and q = rint(x (127 / A)): adding 1.5 2^23 rounds to
-// an integer in the low bits, |x (127 / A)| < 127.5. A row with a NaN or an
-// infinity gets a NaN scale, so it reads as NaN instead of as wrong numbers;
-// one below 2^-100 gets zeros (127 / A would overflow, A / 127 go subnormal).
-template <int D>
-__device__ __forceinline__ float quantise(const u32x4 (&x)[D / 16], uint32_t (&w)[D / 8]) {
-#pragma clang fp contract(off)   // (the product is rounded before the sum)
-  u16x2 mx = {0, 0};
+// 8-bit rows. Largest magnitude A, by the bits of bf16 (m: of each two
+// elements); then 127 / A and A / 127, one correctly rounded division each, and
+// q = rint(x (127 / A)): adding 1.5 2^23 rounds to an integer in the low bits,
+// |x (127 / A)| < 127.5. A row with a NaN or an infinity gets a NaN scale, so it
+// reads as NaN instead of as wrong numbers; one below 2^-100 gets zeros
+// (127 / A would overflow, A / 127 go subnormal).
+__device__ __forceinline__ u16x2 max_bits(u16x2 m, u32x4 x) {
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i) {
-    #pragma unroll
-    for (int j = 0; j < 4; ++j) mx = __builtin_elementwise_max(mx, __builtin_bit_cast(u16x2, x[i][j] & 0x7fff7fffu));
-  }
-  int m = mx.x > mx.y ? mx.x : mx.y;
-  const int other = __shfl_xor(m, 32, 64);
-  m = m > other ? m : other;
+  for (int j = 0; j < 4; ++j) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, x[j] & 0x7fff7fffu));
+  return m;
+}
+struct RowScale {
+  float inv, scale;
+};
+__device__ __forceinline__ RowScale row_scale(int m) {
   const float a = __uint_as_float((uint32_t)m << 16);
   const bool bad = m >= 0x7f80, tiny = a < 0x1p-100f;
-  const float inv = bad || tiny ? 0.f : 127.f / a;
+  return {bad || tiny ? 0.f : 127.f / a, bad ? __uint_as_float(0x7fc00000u) : tiny ? 0.f : a / 127.f};
+}
+__device__ __forceinline__ uint2 bytes8(u32x4 x, float inv) {
+#pragma clang fp contract(off)   // (the product is rounded before the sum)
+  const Chunk8 c = unpack8(__builtin_bit_cast(uint4, x));
+  uint32_t q[8];   // (NaN has zeros in its low byte)
+#pragma unroll
+  for (int j = 0; j < 8; ++j) q[j] = __float_as_uint(c.v[j] * inv + 12582912.f);
+  return make_uint2(__builtin_amdgcn_perm(q[1], q[0], 0x0c0c0400u) | __builtin_amdgcn_perm(q[3], q[2], 0x04000c0cu),
+                    __builtin_amdgcn_perm(q[5], q[4], 0x0c0c0400u) | __builtin_amdgcn_perm(q[7], q[6], 0x04000c0cu));
+}
+
+// Lane l's half row (half_row) as bytes; the row's scale, in both its lanes.
+template <int D>
+__device__ __forceinline__ float quantise(const u32x4 (&x)[D / 16], uint32_t (&w)[D / 8]) {
+  u16x2 mx = {0, 0};
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) mx = max_bits(mx, x[i]);
+  int m = mx.x > mx.y ? mx.x : mx.y;
+  const int other = __shfl_xor(m, 32, 64);
+  const RowScale s = row_scale(m > other ? m : other);
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) {
-    const Chunk8 c = unpack8(__builtin_bit_cast(uint4, x[i]));
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t q[4];   // (NaN has zeros in its low byte)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) q[j] = __float_as_uint(c.v[4 * h + j] * inv + 12582912.f);
-      w[2 * i + h] = __builtin_amdgcn_perm(q[1], q[0], 0x0c0c0400u) | __builtin_amdgcn_perm(q[3], q[2], 0x04000c0cu);
-    }
+    const uint2 q = bytes8(x[i], s.inv);
+    w[2 * i] = q.x;
+    w[2 * i + 1] = q.y;
   }
-  return bad ? __uint_as_float(0x7fc00000u) : tiny ? 0.f : a / 127.f;
+  return s.scale;
 }
 
 // Bytes j of four words, as the j-th word.
@@ -194,6 +206,77 @@ __device__ __forceinline__ void turn4(const uint32_t (&a)[4], uint32_t (&t)[4]) 
   t[1] = __builtin_amdgcn_perm(lo23, lo01, 0x07060302u);
   t[2] = __builtin_amdgcn_perm(hi23, hi01, 0x05040100u);
   t[3] = __builtin_amdgcn_perm(hi23, hi01, 0x07060302u);
+}
+
+// Keys [klo, khi) of a block, few of them (a decode or verify step's): a lane
+// has one 16-byte chunk of a row, its elements go where they belong.
+template <int D, int BITS>
+__device__ __forceinline__ void write_few(const WriteParams& p, int h, int lane, long long base, long long first,
+                                          long long at, int klo, int khi) {
+  constexpr int CPR = D / 8;   // lanes of a row
+  const int dims = p.r.dims;
+  const bool paired = rot_paired(dims, p.r.trad);
+#pragma unroll 1
+  for (int k0 = klo; k0 < khi; k0 += 64 / CPR) {
+    lane = fresh(lane);
+    const int c = lane % CPR, key = k0 + lane / CPR;
+    const bool mine = key < khi;
+    const long long token = first + (mine ? key : khi - 1);
+    const int pos = (int)(base + key);
+    const uint16_t* krow = p.k + h * p.k_head + token * p.k_token;
+    u32x4 x[2];
+    x[1] = *reinterpret_cast<const u32x4*>(p.v + h * p.v_head + token * p.v_token + 8 * c);
+    auto angles = [&](int i) { return rot_angle(pos, p.r.table[i], p.r.gain); };
+    if (paired && 8 * c < dims) {
+      const int half = dims / 2, d = 8 * c < half ? 8 * c : 8 * c - half;
+      const Chunk8 a = unpack8(*reinterpret_cast<const uint4*>(krow + d));
+      const Chunk8 b = unpack8(*reinterpret_cast<const uint4*>(krow + d + half));
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float2 w = angles(d + e);
+        y[e] = 8 * c < half ? rot_first(a.v[e], b.v[e], w) : rot_second(a.v[e], b.v[e], w);
+      }
+      x[0] = __builtin_bit_cast(u32x4, pack8(y));
+    } else if (!paired && 8 * c < dims) {
+      rot_item(c, krow, dims, p.r.trad, angles, [&](int, uint4 v) { x[0] = __builtin_bit_cast(u32x4, v); });
+    } else {
+      x[0] = *reinterpret_cast<const u32x4*>(krow + 8 * c);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      unsigned char* dst = (i ? p.v_pages : p.k_pages) + (size_t)at * (BITS / 8);
+      if constexpr (BITS == 16) {
+        if (!mine) continue;
+        if (i == 0) {
+          *reinterpret_cast<u32x4*>(dst + 2 * page_k_index<D, BITS>(key, 8 * c)) = x[i];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            reinterpret_cast<uint16_t*>(dst)[page_v_index<D, BITS>(key, 8 * c + e)] = (uint16_t)(x[i][e / 2] >> (16 * (e & 1)));
+        }
+      } else {
+        const u16x2 mx = max_bits(u16x2{0, 0}, x[i]);
+        int m = mx.x > mx.y ? mx.x : mx.y;
+#pragma unroll
+        for (int off = 1; off < CPR; off <<= 1) {
+          const int o = __shfl_xor(m, off, 64);
+          m = m > o ? m : o;
+        }
+        const RowScale s = row_scale(m);
+        const uint2 q = bytes8(x[i], s.inv);
+        if (!mine) continue;
+        if (c == 0) ((i ? p.v_scales : p.k_scales) + at / D)[key] = s.scale;
+        if (i == 0) {
+          *reinterpret_cast<uint2*>(dst + page_k_index<D, BITS>(key, 8 * c)) = q;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            dst[page_v_index<D, BITS>(key, 8 * c + e)] = (unsigned char)((e < 4 ? q.x : q.y) >> (8 * (e & 3)));
+        }
+      }
+    }
+  }
 }
 
 // One unit by one wave, in its own LDS: rows come whole, turn in LDS and leave
@@ -210,6 +293,15 @@ __device__ __forceinline__ void write_unit(const WriteParams& p, const Unit& w, 
   const int khi = end < kBlk ? (int)end : kBlk;
   if (klo >= khi) return;   // (a request of no rows)
   const long long first = w.rows.lo + (base - w.start);
+  const long long at = page_block(p.block_table, p.width, w.b, w.blk, p.bpp, p.num_pages, p.Hkv, h, kBlk * D);
+  if (at < 0) {
+    if (p.status && lane == 0) atomicOr(p.status, kStatusPage);
+    return;
+  }
+  if (khi - klo <= 1024 / D) {
+    write_few<D, BITS>(p, h, lane, base, first, at, klo, khi);
+    return;
+  }
   u32x4 kx[NC], vx[NC];
   auto ask = [&](u32x4 (&x)[NC], const uint16_t* src, long long st) {   // (other keys' rows: the nearest new one's)
 #pragma unroll
@@ -230,11 +322,6 @@ __device__ __forceinline__ void write_unit(const WriteParams& p, const Unit& w, 
   };
   ask(kx, p.k + h * p.k_head, p.k_token);
   if (AHEAD) ask(vx, p.v + h * p.v_head, p.v_token);
-  const long long at = page_block(p.block_table, p.width, w.b, w.blk, p.bpp, p.num_pages, p.Hkv, h, kBlk * D);
-  if (at < 0) {
-    if (p.status && lane == 0) atomicOr(p.status, kStatusPage);
-    return;
-  }
   unsigned char* kd = p.k_pages + (size_t)at * (BITS / 8);
   unsigned char* vd = p.v_pages + (size_t)at * (BITS / 8);
   const int key = lane & 31;
@@ -396,8 +483,9 @@ __global__ __launch_bounds__(64 * cache_waves<D>(), D == 256 ? 1 : 4) void paged
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   for (long long x = (long long)blockIdx.x * cache_waves<D>() + wave;; x += (long long)p.kv_groups * cache_waves<D>()) {
     Unit w;
-    if (!find_unit(p, x / p.Hkv, lane, w)) return;   // (no barrier follows)
-    write_unit<D, BITS>(p, w, (int)(x % p.Hkv), lane, lds[wave]);
+    const long long u = div_pos(x, p.Hkv);
+    if (!find_unit(p, u, lane, w)) return;   // (no barrier follows)
+    write_unit<D, BITS>(p, w, (int)(x - u * p.Hkv), fresh(lane), lds[wave]);
   }
 }
 
@@ -539,8 +627,8 @@ __global__ __launch_bounds__(64 * cache_waves<D>()) void paged_read_kernel(ReadP
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const long long units = (long long)p.B * p.Hkv * p.nb, step = (long long)gridDim.x * cache_waves<D>();
   for (long long u = (long long)blockIdx.x * cache_waves<D>() + wave; u < units; u += step) {
-    const long long v = u / p.nb;
-    read_unit<D, BITS>(p, (int)(v / p.Hkv), (int)(v % p.Hkv), (int)(u % p.nb), lane, lds[wave]);
+    const long long v = div_pos(u, p.nb), b = div_pos(v, p.Hkv);
+    read_unit<D, BITS>(p, (int)b, (int)(v - b * p.Hkv), (int)(u - v * p.nb), lane, lds[wave]);
   }
 }
 
