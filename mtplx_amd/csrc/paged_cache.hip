@@ -75,7 +75,7 @@ __device__ __forceinline__ int touched_blocks(long long start, int n) {
   return n > 0 ? (int)(floor_blk(start + n - 1) - floor_blk(start)) + 1 : 0;
 }
 
-// A wave's work: one block of 32 positions of one request, one head, K and V.
+// A wave's work: one block of 32 positions of one request, one head, K or V.
 struct Unit {
   ReqRows rows;
   long long start, blk;   // first position of the request, block of positions
@@ -211,8 +211,8 @@ __device__ __forceinline__ void turn4(const uint32_t (&a)[4], uint32_t (&t)[4]) 
 // Keys [klo, khi) of a block, few of them (a decode or verify step's): a lane
 // has one 16-byte chunk of a row, its elements go where they belong.
 template <int D, int BITS>
-__device__ __forceinline__ void write_few(const WriteParams& p, int h, int lane, long long base, long long first,
-                                          long long at, int klo, int khi) {
+__device__ __forceinline__ void write_few(const WriteParams& p, int h, bool isk, int lane, long long base,
+                                          long long first, long long at, int klo, int khi) {
   constexpr int CPR = D / 8;   // lanes of a row
   const int dims = p.r.dims;
   const bool paired = rot_paired(dims, p.r.trad);
@@ -223,57 +223,53 @@ __device__ __forceinline__ void write_few(const WriteParams& p, int h, int lane,
     const bool mine = key < khi;
     const long long token = first + (mine ? key : khi - 1);
     const int pos = (int)(base + key);
-    const uint16_t* krow = p.k + h * p.k_head + token * p.k_token;
-    u32x4 x[2];
-    x[1] = *reinterpret_cast<const u32x4*>(p.v + h * p.v_head + token * p.v_token + 8 * c);
+    const uint16_t* row = isk ? p.k + h * p.k_head + token * p.k_token : p.v + h * p.v_head + token * p.v_token;
+    u32x4 x;
     auto angles = [&](int i) { return rot_angle(pos, p.r.table[i], p.r.gain); };
-    if (paired && 8 * c < dims) {
+    if (isk && paired && 8 * c < dims) {
       const int half = dims / 2, d = 8 * c < half ? 8 * c : 8 * c - half;
-      const Chunk8 a = unpack8(*reinterpret_cast<const uint4*>(krow + d));
-      const Chunk8 b = unpack8(*reinterpret_cast<const uint4*>(krow + d + half));
+      const Chunk8 a = unpack8(*reinterpret_cast<const uint4*>(row + d));
+      const Chunk8 b = unpack8(*reinterpret_cast<const uint4*>(row + d + half));
       float y[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float2 w = angles(d + e);
         y[e] = 8 * c < half ? rot_first(a.v[e], b.v[e], w) : rot_second(a.v[e], b.v[e], w);
       }
-      x[0] = __builtin_bit_cast(u32x4, pack8(y));
-    } else if (!paired && 8 * c < dims) {
-      rot_item(c, krow, dims, p.r.trad, angles, [&](int, uint4 v) { x[0] = __builtin_bit_cast(u32x4, v); });
+      x = __builtin_bit_cast(u32x4, pack8(y));
+    } else if (isk && !paired && 8 * c < dims) {
+      rot_item(c, row, dims, p.r.trad, angles, [&](int, uint4 v) { x = __builtin_bit_cast(u32x4, v); });
     } else {
-      x[0] = *reinterpret_cast<const u32x4*>(krow + 8 * c);
+      x = *reinterpret_cast<const u32x4*>(row + 8 * c);
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      unsigned char* dst = (i ? p.v_pages : p.k_pages) + (size_t)at * (BITS / 8);
-      if constexpr (BITS == 16) {
-        if (!mine) continue;
-        if (i == 0) {
-          *reinterpret_cast<u32x4*>(dst + 2 * page_k_index<D, BITS>(key, 8 * c)) = x[i];
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            reinterpret_cast<uint16_t*>(dst)[page_v_index<D, BITS>(key, 8 * c + e)] = (uint16_t)(x[i][e / 2] >> (16 * (e & 1)));
-        }
+    unsigned char* dst = (isk ? p.k_pages : p.v_pages) + (size_t)at * (BITS / 8);
+    if constexpr (BITS == 16) {
+      if (!mine) continue;
+      if (isk) {
+        *reinterpret_cast<u32x4*>(dst + 2 * page_k_index<D, BITS>(key, 8 * c)) = x;
       } else {
-        const u16x2 mx = max_bits(u16x2{0, 0}, x[i]);
-        int m = mx.x > mx.y ? mx.x : mx.y;
 #pragma unroll
-        for (int off = 1; off < CPR; off <<= 1) {
-          const int o = __shfl_xor(m, off, 64);
-          m = m > o ? m : o;
-        }
-        const RowScale s = row_scale(m);
-        const uint2 q = bytes8(x[i], s.inv);
-        if (!mine) continue;
-        if (c == 0) ((i ? p.v_scales : p.k_scales) + at / D)[key] = s.scale;
-        if (i == 0) {
-          *reinterpret_cast<uint2*>(dst + page_k_index<D, BITS>(key, 8 * c)) = q;
-        } else {
+        for (int e = 0; e < 8; ++e)
+          reinterpret_cast<uint16_t*>(dst)[page_v_index<D, BITS>(key, 8 * c + e)] = (uint16_t)(x[e / 2] >> (16 * (e & 1)));
+      }
+    } else {
+      const u16x2 mx = max_bits(u16x2{0, 0}, x);
+      int m = mx.x > mx.y ? mx.x : mx.y;
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            dst[page_v_index<D, BITS>(key, 8 * c + e)] = (unsigned char)((e < 4 ? q.x : q.y) >> (8 * (e & 3)));
-        }
+      for (int off = 1; off < CPR; off <<= 1) {
+        const int o = __shfl_xor(m, off, 64);
+        m = m > o ? m : o;
+      }
+      const RowScale s = row_scale(m);
+      const uint2 q = bytes8(x, s.inv);
+      if (!mine) continue;
+      if (c == 0) ((isk ? p.k_scales : p.v_scales) + at / D)[key] = s.scale;   // [page][head][slot]
+      if (isk) {
+        *reinterpret_cast<uint2*>(dst + page_k_index<D, BITS>(key, 8 * c)) = q;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          dst[page_v_index<D, BITS>(key, 8 * c + e)] = (unsigned char)((e < 4 ? q.x : q.y) >> (8 * (e & 3)));
       }
     }
   }
@@ -283,9 +279,9 @@ __device__ __forceinline__ void write_few(const WriteParams& p, int h, int lane,
 // in the page's order, 16 bytes a lane; keys of a block that is not all new go
 // out element by element (V) or chunk by chunk (K).
 template <int D, int BITS>
-__device__ __forceinline__ void write_unit(const WriteParams& p, const Unit& w, int h, int lane, uint16_t* rows) {
+__device__ __forceinline__ void write_unit(const WriteParams& p, const Unit& w, int h, bool isk, int lane,
+                                           uint16_t* rows) {
   constexpr int RS = row16<D>(), NC = D / 16, BS = row8<D>();   // 16-byte loads of a lane
-  constexpr bool AHEAD = D < 256;   // V is asked for before K is done
   const long long base = w.blk * kBlk;
   // Keys [klo, khi) of the block are new; token of key kk: first + kk.
   const int klo = w.start > base ? (int)(w.start - base) : 0;
@@ -293,41 +289,38 @@ __device__ __forceinline__ void write_unit(const WriteParams& p, const Unit& w, 
   const int khi = end < kBlk ? (int)end : kBlk;
   if (klo >= khi) return;   // (a request of no rows)
   const long long first = w.rows.lo + (base - w.start);
+  u32x4 x[NC];
+  const bool few = khi - klo <= 1024 / D;
+  if (!few) {
+    const uint16_t* src = isk ? p.k + h * p.k_head : p.v + h * p.v_head;
+    const long long st = isk ? p.k_token : p.v_token;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = i * 64 + lane;
+      int kk = c / (D / 8);
+      kk = kk < klo ? klo : kk >= khi ? khi - 1 : kk;   // (other keys' rows: the nearest new one's)
+      x[i] = *reinterpret_cast<const u32x4*>(src + (first + kk) * st + c % (D / 8) * 8);
+    }
+  }
   const long long at = page_block(p.block_table, p.width, w.b, w.blk, p.bpp, p.num_pages, p.Hkv, h, kBlk * D);
   if (at < 0) {
     if (p.status && lane == 0) atomicOr(p.status, kStatusPage);
     return;
   }
-  if (khi - klo <= 1024 / D) {
-    write_few<D, BITS>(p, h, lane, base, first, at, klo, khi);
+  if (few) {
+    write_few<D, BITS>(p, h, isk, lane, base, first, at, klo, khi);
     return;
   }
-  u32x4 kx[NC], vx[NC];
-  auto ask = [&](u32x4 (&x)[NC], const uint16_t* src, long long st) {   // (other keys' rows: the nearest new one's)
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int c = i * 64 + lane;
-      int kk = c / (D / 8);
-      kk = kk < klo ? klo : kk >= khi ? khi - 1 : kk;
-      x[i] = *reinterpret_cast<const u32x4*>(src + (first + kk) * st + c % (D / 8) * 8);
-    }
-  };
-  auto put = [&](const u32x4 (&x)[NC]) {
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int c = i * 64 + lane;
-      *reinterpret_cast<u32x4*>(rows + c / (D / 8) * RS + c % (D / 8) * 8) = x[i];
-    }
-    wave_lds();
-  };
-  ask(kx, p.k + h * p.k_head, p.k_token);
-  if (AHEAD) ask(vx, p.v + h * p.v_head, p.v_token);
-  unsigned char* kd = p.k_pages + (size_t)at * (BITS / 8);
-  unsigned char* vd = p.v_pages + (size_t)at * (BITS / 8);
+  for (int i = 0; i < NC; ++i) {
+    const int c = i * 64 + lane;
+    *reinterpret_cast<u32x4*>(rows + c / (D / 8) * RS + c % (D / 8) * 8) = x[i];
+  }
+  wave_lds();
+  unsigned char* dst = (isk ? p.k_pages : p.v_pages) + (size_t)at * (BITS / 8);
   const int key = lane & 31;
   const bool mine = key >= klo && key < khi;   // the lane's row
-  put(kx);
-  if (p.r.dims) {   // in place: an item reads what it stores, or the source
+  if (isk && p.r.dims) {   // in place: an item reads what it stores, or the source
     const int np = rot_paired(p.r.dims, p.r.trad) ? p.r.dims / 16 : (p.r.dims + 7) / 8;
     const bool inplace = p.r.trad || rot_paired(p.r.dims, p.r.trad);
     for (int x = lane; x < 32 * np; x += 64) {
@@ -344,25 +337,27 @@ __device__ __forceinline__ void write_unit(const WriteParams& p, const Unit& w, 
     }
     wave_lds();
   }
-  half_row<D>(rows, lane, kx);
-  if constexpr (BITS == 16) {
-    if (mine) {
-#pragma unroll
-      for (int i = 0; i < NC; ++i) *reinterpret_cast<u32x4*>(kd + (i * 64 + lane) * 16) = kx[i];
-    }
-  } else {
-    uint32_t q[D / 8];
-    const float s = quantise<D>(kx, q);
-    if (mine) {
-#pragma unroll
-      for (int i = 0; i < NC / 2; ++i)
-        *reinterpret_cast<u32x4*>(kd + (i * 64 + lane) * 16) = u32x4{q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]};
-      if (lane < 32) (p.k_scales + at / D)[key] = s;   // [page][head][slot]
-    }
+  uint32_t q[D / 8];   // 8 bits: the lane's half row
+  if constexpr (BITS == 8) {
+    half_row<D>(rows, lane, x);
+    const float s = quantise<D>(x, q);
+    if (mine && lane < 32) ((isk ? p.k_scales : p.v_scales) + at / D)[key] = s;   // [page][head][slot]
   }
-  wave_lds();
-  if (!AHEAD) ask(vx, p.v + h * p.v_head, p.v_token);
-  put(vx);
+  if (isk) {
+    if constexpr (BITS == 16) half_row<D>(rows, lane, x);
+    if (mine) {
+      if constexpr (BITS == 16) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) *reinterpret_cast<u32x4*>(dst + (i * 64 + lane) * 16) = x[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < NC / 2; ++i)
+          *reinterpret_cast<u32x4*>(dst + (i * 64 + lane) * 16) = u32x4{q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]};
+      }
+    }
+    wave_lds();
+    return;
+  }
   const bool all = klo == 0 && khi == kBlk;
   if constexpr (BITS == 16) {
     if (all) {
@@ -379,21 +374,17 @@ __device__ __forceinline__ void write_unit(const WriteParams& p, const Unit& w, 
           lo[e] = __builtin_amdgcn_perm(a[2 * e + 1], a[2 * e], 0x05040100u);
           hi[e] = __builtin_amdgcn_perm(a[2 * e + 1], a[2 * e], 0x07060302u);
         }
-        u32x4* dst = reinterpret_cast<u32x4*>(vd) + tj * 64 + hh * 32 + c;
-        dst[0] = u32x4{lo[0], lo[1], lo[2], lo[3]};
-        dst[1] = u32x4{hi[0], hi[1], hi[2], hi[3]};
+        u32x4* to = reinterpret_cast<u32x4*>(dst) + tj * 64 + hh * 32 + c;
+        to[0] = u32x4{lo[0], lo[1], lo[2], lo[3]};
+        to[1] = u32x4{hi[0], hi[1], hi[2], hi[3]};
       }
     } else {
       for (int x = lane; x < (khi - klo) * D; x += 64) {
         const int kk = klo + x / D, d = x % D;
-        reinterpret_cast<uint16_t*>(vd)[page_v_index<D, 16>(kk, d)] = rows[kk * RS + d];
+        reinterpret_cast<uint16_t*>(dst)[page_v_index<D, 16>(kk, d)] = rows[kk * RS + d];
       }
     }
   } else {
-    uint32_t q[D / 8];
-    half_row<D>(rows, lane, vx);
-    const float s = quantise<D>(vx, q);
-    if (mine && lane < 32) (p.v_scales + at / D)[key] = s;
     wave_lds();
     unsigned char* bytes = reinterpret_cast<unsigned char*>(rows);
 #pragma unroll
@@ -413,14 +404,14 @@ __device__ __forceinline__ void write_unit(const WriteParams& p, const Unit& w, 
             a[e] = *reinterpret_cast<const uint32_t*>(bytes + (16 * (j >> 1) + v_slot_key(hh, 4 * (j & 1) + e)) * BS + 32 * t + c);
           turn4(a, o[j]);
         }
-        u32x4* dst = reinterpret_cast<u32x4*>(vd) + t * 64 + hh * 32 + c;
+        u32x4* to = reinterpret_cast<u32x4*>(dst) + t * 64 + hh * 32 + c;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) dst[e] = u32x4{o[0][e], o[1][e], o[2][e], o[3][e]};
+        for (int e = 0; e < 4; ++e) to[e] = u32x4{o[0][e], o[1][e], o[2][e], o[3][e]};
       }
     } else {
       for (int x = lane; x < (khi - klo) * D; x += 64) {
         const int kk = klo + x / D, d = x % D;
-        vd[page_v_index<D, 8>(kk, d)] = bytes[kk * BS + d];
+        dst[page_v_index<D, 8>(kk, d)] = bytes[kk * BS + d];
       }
     }
   }
@@ -483,9 +474,9 @@ __global__ __launch_bounds__(64 * cache_waves<D>(), D == 256 ? 1 : 4) void paged
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   for (long long x = (long long)blockIdx.x * cache_waves<D>() + wave;; x += (long long)p.kv_groups * cache_waves<D>()) {
     Unit w;
-    const long long u = div_pos(x, p.Hkv);
+    const long long u = div_pos(x >> 1, p.Hkv);
     if (!find_unit(p, u, lane, w)) return;   // (no barrier follows)
-    write_unit<D, BITS>(p, w, (int)(x - u * p.Hkv), fresh(lane), lds[wave]);
+    write_unit<D, BITS>(p, w, (int)((x >> 1) - u * p.Hkv), (x & 1) == 0, fresh(lane), lds[wave]);
   }
 }
 
@@ -742,7 +733,7 @@ MTP_API int mtp_paged_write(const mtp_paged_write_args* a, void* stream) {
     units = (long long)a->B * p.nb_uniform;
   }
   const int waves = a->D == 256 ? cache_waves<256>() : cache_waves<128>();
-  long long groups = (units * a->Hkv + waves - 1) / waves;
+  long long groups = (units * 2 * a->Hkv + waves - 1) / waves;
   if (groups > 1 << 20) groups = 1 << 20;
   p.kv_groups = (int)groups;
   if (a->q) {
