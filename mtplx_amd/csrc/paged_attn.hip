@@ -1025,10 +1025,12 @@ __global__ __launch_bounds__(kPT, D == 256 ? 1 : 2) void attn_few_kernel(PAttn p
 // loads at a time, with the pieces' weights 2^(m - max) from LDS. Lanes without
 // a row (a decode step's tile holds few) take a share of the pieces instead:
 // with NR rows' lanes, lane r + NR s adds pieces s, s + 32 / NR, .. of row r.
-constexpr int kJoin = 64;   // pieces whose weights LDS holds
+template <int RT>
+constexpr int join_round() { return RT == 32 ? 64 : 16; }   // pieces whose weights LDS holds
 
 template <int D, int RT>
 __global__ __launch_bounds__(kPT) void attn_join_kernel(PAttn p) {
+  constexpr int kJoin = join_round<RT>();
   __shared__ float s_w[kJoin][32], s_m[32], s_l[32];
   __shared__ __attribute__((aligned(16))) uint16_t s_out[32][32 + 8];
   const int tid = threadIdx.x;
@@ -1044,7 +1046,7 @@ __global__ __launch_bounds__(kPT) void attn_join_kernel(PAttn p) {
   while (RT == 32 && NR > 4 && rows - r0 <= NR / 2) NR >>= 1;
   const int SP = 32 / NR, row = tid & (NR - 1), share = (tid & 31) / NR;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  constexpr int B8 = 8;   // pieces whose blocks are in flight together
+  constexpr int B8 = RT == 32 ? 8 : 4;   // pieces whose blocks are in flight together
   float4 a8[B8];
   auto ask = [&](int k) {   // (the last piece again past the last: never used)
 #pragma unroll
