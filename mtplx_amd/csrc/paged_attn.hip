@@ -53,9 +53,10 @@ struct PAttn {
   int4* begun;      // [G]: the tile that workgroup g began and others finish
   int T, B, width, Hq, Hkv, rep, bpp, num_pages;
   uint32_t rep_inv;   // row / rep = row * rep_inv >> 16 for rows below 2048
-  int P;            // tokens of a row tile
+  int P;            // tokens that the rows of a tile may belong to
   int G;            // most workgroups
   int min_share;    // least keys of a workgroup's share
+  int rt_log2;      // rows of a tile
   int step;         // shares are whole numbers of steps
   int tile_cost;
   float scale_log2;
@@ -77,7 +78,8 @@ struct Req {
 
 // Line length of a request's first t row tiles (one head).
 __device__ __forceinline__ long long tiles_len(long long q0, int n, int P, long long t) {
-  // sum over tiles x < t of q0 + min((x + 1) P, n)
+  // sum over tiles x < t of q0 + min((x + 1) P, n): a tile's last row sees at
+  // most that many keys (P: tokens that a tile's rows may belong to)
   const long long full = n / P;
   const long long f = t < full ? t : full;
   return t * q0 + P * (f * (f + 1) / 2) + (t - f) * n;
@@ -87,8 +89,12 @@ __device__ __forceinline__ long long clamp_start(const PAttn& p, long long s) {
   const long long cap = (long long)p.width * p.bpp * kBlk;
   return (s < 0 ? 0 : s > cap ? cap : s) + p.tile_cost;
 }
+// Row tiles of n tokens.
+__device__ __forceinline__ int tile_count(const PAttn& p, int n) {
+  return (int)(((long long)n * p.rep + (1 << p.rt_log2) - 1) >> p.rt_log2);
+}
 __device__ __forceinline__ long long head_len(const PAttn& p, long long start, int n) {
-  return tiles_len(clamp_start(p, start), n, p.P, (n + p.P - 1) / p.P);
+  return tiles_len(clamp_start(p, start), n, p.P, tile_count(p, n));
 }
 
 __device__ __forceinline__ long long shfl64(long long v, int src) { return __shfl(v, src, 64); }
@@ -144,7 +150,7 @@ struct Line {
     for (int off = 32; off > 0; off >>= 1) W += __shfl_xor(W, off, 64);
     W = uniform64(W);
     // Equal shares, a whole number of steps each, no shorter than min_share.
-    const long long s = W > 0 ? div_small(W - 1, p.G) + 1LL : 0;   // (W / G below 2^31: a share's keys)
+    const long long s = W > 0 ? (W - 1) / p.G + 1 : 0;
     S = s > p.min_share ? (s + p.step - 1) & -(long long)p.step : p.min_share;
     G = W > 0 ? div_small(W - 1, S) + 1 : 0;
   }
@@ -173,34 +179,43 @@ struct Line {
   }
 };
 
-// One row tile of one head: where it lies on the line and what it is.
+// One row tile of one head: where it lies on the line and what it is. Tiles are
+// whole whatever the heads of a kv head: a token's rows may lie in two of them.
 struct Tile {
   long long begin, len;   // line
   int h, t;               // kv head, row tile
-  int n;                  // its tokens
+  int tok, off, rows;     // its first row: token of the request, head of that token; its rows
   long long pos;          // position of its first token
   int nk;                 // keys it sees: [0, nk)
 };
+// All but begin and h, from t.
+__device__ __forceinline__ void set_tile(const PAttn& p, const Req& r, Tile& u) {
+  const int first = u.t << p.rt_log2;   // (rows of a call: below 2^31)
+  const int left = r.n * p.rep - first;
+  u.rows = left >> p.rt_log2 ? 1 << p.rt_log2 : left;
+  u.tok = (int)((uint32_t)first / (uint32_t)p.rep);
+  u.off = first - u.tok * p.rep;
+  const long long cost = (long long)(u.t + 1) * p.P;
+  u.len = clamp_start(p, r.start) + (cost < r.n ? cost : r.n);
+  u.pos = r.start + u.tok;
+  const long long cap = (long long)p.width * p.bpp * kBlk;
+  const long long e = u.pos + row_token(p, u.off + u.rows - 1) + 1;
+  u.nk = (int)(e < 0 ? 0 : e > cap ? cap : e);
+}
 __device__ __forceinline__ Tile tile_at(const PAttn& p, const Req& r, long long x) {
   Tile u;
   const long long y = x - r.base;
   u.h = div_small(y, r.head);
   const long long z = y - u.h * r.head;
   const long long q0 = clamp_start(p, r.start);
-  int a = 0, b = (r.n + p.P - 1) / p.P - 1;   // the last tile that begins at or before z
+  int a = 0, b = tile_count(p, r.n) - 1;   // the last tile that begins at or before z
   while (a < b) {
     const int m = (a + b + 1) >> 1;
     if (tiles_len(q0, r.n, p.P, m) <= z) a = m; else b = m - 1;
   }
   u.t = a;
-  const long long z0 = tiles_len(q0, r.n, p.P, a);
-  u.begin = r.base + u.h * r.head + z0;
-  u.len = tiles_len(q0, r.n, p.P, a + 1) - z0;
-  u.n = r.n - a * p.P < p.P ? r.n - a * p.P : p.P;
-  u.pos = r.start + (long long)a * p.P;
-  const long long cap = (long long)p.width * p.bpp * kBlk;
-  const long long e = u.pos + u.n;
-  u.nk = (int)(e < 0 ? 0 : e > cap ? cap : e);
+  u.begin = r.base + u.h * r.head + tiles_len(q0, r.n, p.P, a);
+  set_tile(p, r, u);
   return u;
 }
 
@@ -208,17 +223,11 @@ __device__ __forceinline__ Tile tile_at(const PAttn& p, const Req& r, long long 
 __device__ __forceinline__ void next_tile(const PAttn& p, const Req& r, Tile& u) {
   u.begin += u.len;
   ++u.t;
-  if (u.t * p.P >= r.n) {
+  if (u.t == tile_count(p, r.n)) {
     u.t = 0;
     ++u.h;
   }
-  const int left = r.n - u.t * p.P;
-  u.n = left < p.P ? left : p.P;
-  u.len = clamp_start(p, r.start) + u.t * p.P + u.n;
-  u.pos = r.start + (long long)u.t * p.P;
-  const long long cap = (long long)p.width * p.bpp * kBlk;
-  const long long e = u.pos + u.n;
-  u.nk = (int)(e < 0 ? 0 : e > cap ? cap : e);
+  set_tile(p, r, u);
 }
 
 // Keys [0, key_at(x)) of the tile lie before offset x of its line: whole steps
@@ -437,9 +446,9 @@ __device__ __forceinline__ void ask_rows(RowLoads<D>& q, const PAttn& p, const R
 #pragma unroll
   for (int j = 0; j < D / 16; ++j) {
     const int r = row0 + j * (64 / LPR) + lane / LPR;
-    int i = row_token(p, r), g = r - i * p.rep;
-    if (i >= u.n) i = g = 0;   // no row here: any
-    const long long tok = rq.lo + (long long)u.t * p.P + i;
+    int i = row_token(p, r + u.off), g = r + u.off - i * p.rep;
+    if (r >= u.rows) i = g = 0;   // no row here: any
+    const long long tok = (long long)rq.lo + u.tok + i;
     q.r[j] = *reinterpret_cast<const u32x4*>(p.q + tok * p.q_token + (long long)(u.h * p.rep + g) * p.q_head +
                                              lane % LPR * 8);
   }
@@ -453,8 +462,8 @@ __device__ __forceinline__ void take_rows(RowState<D>& s, const RowLoads<D>& q, 
   for (int j = 0; j < D / 16; ++j)
     *reinterpret_cast<u32x4*>(lds + (j * (64 / LPR) + lane / LPR) * RB + lane % LPR * 16) = q.r[j];
   const int h2 = lane >> 5, r = row0 + (lane & 31);
-  const int i = row_token(p, r);
-  const bool valid = i < u.n;
+  const int i = row_token(p, r + u.off);
+  const bool valid = r < u.rows;
   const long long pos = u.pos + i;
   s.bound = !valid || pos < 0 ? -1 : pos < u.nk ? (int)pos : u.nk - 1;
 #pragma unroll
@@ -485,7 +494,7 @@ __device__ __forceinline__ void store4(uint16_t* dst, float a, float b, float c,
   *reinterpret_cast<uint2*>(dst) = make_uint2(f2bf2(a, b), f2bf2(c, d));
 }
 
-// Row r of the tile whose first token is `token` (packed), of kv head h.
+// Row r (from the first head of token `token`, packed, on) of kv head h.
 __device__ __forceinline__ uint16_t* out_row(const PAttn& p, int token, int h, int r) {
   const int i = row_token(p, r), g = r - i * p.rep;
   return p.out + ((long long)token + i) * p.out_token + (long long)(h * p.rep + g) * p.out_head;
@@ -494,7 +503,8 @@ __device__ __forceinline__ uint16_t* out_row(const PAttn& p, int token, int h, i
 // What the join needs to know of the tile that workgroup g begins and others
 // finish (at most one).
 __device__ __forceinline__ void note_begun(const PAttn& p, const Line& line, const Req& rq, const Tile& u, int g) {
-  p.begun[g] = make_int4(u.n * p.rep, line.owner(u.begin + u.len - 1) - g + 1, rq.lo + u.t * p.P, u.h);
+  const int last = line.owner(u.begin + u.len - 1);
+  p.begun[g] = make_int4(u.rows | u.off << 16, (last < line.G ? last : line.G - 1) - g + 1, rq.lo + u.tok, u.h);
 }
 
 // Byte I of w, signed, as a float: one instruction (the compiler takes two, a
@@ -576,14 +586,14 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
     x = end;
     if (starts && !ends && tid == 0) note_begun(p, line, rq, u, g);
     const int row0 = wave * 32;
-    const int rows = u.n * p.rep;   // of the tile
+    const int rows = u.rows;
     RowLoads<D> ql;
     ask_rows<D>(ql, p, rq, u, row0, lane);
     // Bounds of the wave's rows: steps behind wmax are skipped, steps up to
     // wmin need no mask (rows past the list are computed on zeros, and dropped).
     const int last = (row0 + 32 < rows ? row0 + 32 : rows) - 1;
-    long long wmin = u.pos + row_token(p, row0);
-    const long long wmax = row0 < rows ? u.pos + row_token(p, last) : -1;
+    long long wmin = u.pos + row_token(p, row0 + u.off);
+    const long long wmax = row0 < rows ? u.pos + row_token(p, last + u.off) : -1;
     if (wmin > u.nk - 1) wmin = u.nk - 1;
 
     BlockList blocks;
@@ -836,7 +846,7 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
         const int r = j * (64 / LPR) + ln / LPR;
         const u32x4 v = *reinterpret_cast<const u32x4*>(mine + r * RB + ln % LPR * 16);
         if (row0 + r < rows)
-          *reinterpret_cast<u32x4*>(out_row(p, rq.lo + u.t * p.P, u.h, row0 + r) + ln % LPR * 8) = v;
+          *reinterpret_cast<u32x4*>(out_row(p, rq.lo + u.tok, u.h, row0 + r + u.off) + ln % LPR * 8) = v;
       }
     } else if (row0 < rows) {
       const size_t slot = 2 * (size_t)g + (starts ? 1 : 0);
@@ -890,7 +900,7 @@ __global__ __launch_bounds__(kPT, D == 256 ? 1 : 2) void attn_few_kernel(PAttn p
     const bool starts = x == u.begin, ends = end == u.begin + u.len;
     x = end;
     if (starts && !ends && tid == 0) note_begun(p, line, rq, u, g);
-    const int rows = u.n * p.rep;
+    const int rows = u.rows;
     RowLoads<D> q;
     ask_rows<D>(q, p, rq, u, 0, lane);
     const long long wmin = u.pos < u.nk - 1 ? u.pos : u.nk - 1;   // blocks up to it hide no key
@@ -1005,7 +1015,7 @@ __global__ __launch_bounds__(kPT, D == 256 ? 1 : 2) void attn_few_kernel(PAttn p
       }
       if (whole) {
         const float inv = ls == 0.f ? 0.f : 1.f / ls;
-        store4(out_row(p, rq.lo + u.t * p.P, u.h, r) + d, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+        store4(out_row(p, rq.lo + u.tok, u.h, r + u.off) + d, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
       } else {
         part_block<D>(p, slot, RT, 0, 0)[e] = v;
         if (d == 0) {
@@ -1035,8 +1045,8 @@ __global__ __launch_bounds__(kPT) void attn_join_kernel(PAttn p) {
   __shared__ __attribute__((aligned(16))) uint16_t s_out[32][32 + 8];
   const int tid = threadIdx.x;
   const int g = blockIdx.x;
-  const int4 tile = p.begun[g];   // rows (0: none), pieces, first token, kv head
-  const int rows = tile.x, np = tile.y;
+  const int4 tile = p.begun[g];   // rows (0: none) and first head, pieces, first token, kv head
+  const int rows = tile.x & 0xffff, head0 = tile.x >> 16, np = tile.y;
   const int rb = blockIdx.y / (D / 32), t = blockIdx.y % (D / 32);
   const int r0 = 32 * rb;
   if (r0 >= rows) return;
@@ -1128,7 +1138,7 @@ __global__ __launch_bounds__(kPT) void attn_join_kernel(PAttn p) {
   if (tid >= 128) return;
   const int r = tid >> 2, d = tid % 4 * 8;   // 64 bytes a row
   if (r0 + r < rows)
-    *reinterpret_cast<u32x4*>(out_row(p, tile.z, tile.w, r0 + r) + 32 * t + d) = *reinterpret_cast<const u32x4*>(&s_out[r][d]);
+    *reinterpret_cast<u32x4*>(out_row(p, tile.z, tile.w, r0 + r + head0) + 32 * t + d) = *reinterpret_cast<const u32x4*>(&s_out[r][d]);
 }
 
 // Which kernel runs, and its tiles: calls of at most 32 query rows per kv head
@@ -1143,7 +1153,7 @@ inline AttnPlan attn_plan(int Hq, int Hkv, int D, int max_rows) {
   AttnPlan a;
   a.few = max_rows > 0 && (long long)max_rows * rep <= 32;
   a.RT = a.few ? 32 : D == 256 ? 128 : 256;   // chunk_waves<D>() * 32
-  a.P = a.RT / rep;
+  a.P = (a.RT + rep - 2) / rep + 1;
   a.G = device_cus() * (a.few && D < 256 ? 2 : 1);
   a.min_share = a.few ? 4 * kBlk : 2 * kStepKeys;
   a.step = a.few ? kBlk : kStepKeys;
@@ -1160,7 +1170,7 @@ int launch_attn(const PAttn& p, const AttnPlan& a, hipStream_t st) {
     hipLaunchKernelGGL((attn_chunk_kernel<D, BITS>), dim3((unsigned)p.G), dim3(64 * NW), 0, st, p);
   const int rc = launch_check("mtp_paged_attn");
   if (rc) return rc;
-  const int blocks = cdiv(a.P * p.rep, 32) * (D / 32);
+  const int blocks = a.RT / 32 * (D / 32);
   if (a.few)
     hipLaunchKernelGGL((attn_join_kernel<D, 32>), dim3((unsigned)p.G, blocks), dim3(kPT), 0, st, p);
   else
@@ -1194,6 +1204,10 @@ MTP_API int mtp_paged_attn(const mtp_paged_attn_args* a, void* stream) {
   if (!a->row_off && a->T % a->B) {
     set_error("%s: %d tokens are no whole rows of %d requests (give row_off)", who, a->T, a->B);
     return MTP_ERR_ARG;
+  }
+  if ((long long)a->T * a->Hq > 0x7fffffffLL) {
+    set_error("%s: %d tokens of %d heads are more than 2^31 - 1 rows", who, a->T, a->Hq);
+    return MTP_ERR_UNSUPPORTED;
   }
   if (!(a->scale > 0.f) || !(a->scale < 3.0e38f)) {
     set_error("%s: the scale must be positive and finite", who);
@@ -1236,6 +1250,7 @@ MTP_API int mtp_paged_attn(const mtp_paged_attn_args* a, void* stream) {
   p.bpp = a->page_size / kBlk;
   p.num_pages = a->num_pages;
   p.P = plan.P;
+  p.rt_log2 = plan.RT == 32 ? 5 : plan.RT == 128 ? 7 : 8;
   p.G = plan.G;
   p.min_share = plan.min_share;
   p.step = plan.step;
