@@ -38,8 +38,9 @@ FLAGS = [
     "-mllvm", "-amdgpu-mfma-vgpr-form=1",
     "-I", CSRC,
 ]
-# Sources compiled without that option (the compiler fails on one of their
-# kernels with it; those with two waves per SIMD use no AGPRs either way).
+# Sources compiled without that option: the compiler crashes on
+# attn_chunk_kernel<256, 16> with it. Kernels of two waves per SIMD hold 256
+# registers and use no AGPRs either way.
 AGPR_SOURCES = {"paged_attn.hip"}
 
 

@@ -10,8 +10,10 @@
 // blocks cost no pass over o.
 //
 // The query rows of the heads that share a kv head are one list per request
-// (row r = token r / rep, head r % rep), so K and V are read once for all of
-// them. S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_32x32x16_bf16: a lane
+// (row r = token r / rep, head r % rep), cut into tiles of 32, 128 or 256 rows
+// wherever that falls, so K and V are read once for all of them and 512 tokens
+// of five heads are ten tiles (whole tokens, 51 a tile, took eleven: a chunk of
+// 512 at 16k 202 us, now 184). S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_32x32x16_bf16: a lane
 // holds one query row's scores, so the maximum and sum over keys are its own
 // registers' and one exchange with lane + 32, and P^T is already laid out as
 // the second product's operand.
@@ -26,6 +28,17 @@
 // one workgroup leaves one partial (o, m, l) per piece, at most two per
 // workgroup, and attn_join adds them in the line's order. The split depends on
 // lengths alone, so results do not depend on timing.
+//
+// What bounds it, on an MI355X (5.17 TB/s a large copy, 1350 TFLOP/s a large
+// bf16 product), 40 query heads over 8 kv heads of 128:
+//   sixteen requests' four verify rows up to 32k, 8 bits: 124 us, the pages at
+//     the rate of the copy;
+//   a chunk of 512 over 16k: 184 us, 890 TFLOP/s of what the mask leaves; whole
+//     prompts of 4096: 510 us, 745 (diagonal blocks are computed whole). The
+//     softmax's instructions (an exponential, a product, a maximum, a sum and
+//     half a conversion a score) take as many cycles of a SIMD as the MFMAs,
+//     and the two waves of a SIMD take them in turn;
+//   one token over 4k: 17.6 us, two launches and a chain of dependent loads.
 #include "paged.hpp"
 #include "qmv_common.hpp"
 
@@ -867,8 +880,10 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
 
 // -- few rows: one tile of 32 rows, the four waves share a piece by keys ---------
 
-// Blocks go straight from the pages into a wave's registers, RING of them in
-// flight (8-bit blocks are half as large: two).
+// Blocks go straight from the pages into a wave's registers, the next one asked
+// for as soon as this one's operands are used up (RING 1). Two workgroups a CU
+// where their registers allow (D < 256): sixteen requests' verify rows at 8 bits
+// take 120 us, with one 149.
 template <int D, int BITS>
 __global__ __launch_bounds__(kPT, D == 256 ? 1 : 2) void attn_few_kernel(PAttn p) {
   constexpr int RT = 32;

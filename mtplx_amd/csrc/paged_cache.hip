@@ -1,5 +1,18 @@
 // Rotary positions of packed tokens, and the paged KV cache's writes (rotating
-// and quantising on the way) and reads. All of them move bytes once.
+// and quantising on the way) and reads. All of them move bytes once, and long
+// calls are bound by that (a large copy reaches 5.17 TB/s on an MI355X):
+//
+//   rotation of 8192 tokens, 40 + 8 heads of 128: 34 us (201 MB, 5.9 TB/s: part
+//     of it stays in the last-level cache);
+//   write of the same at 8 bits, queries rotated: 52 us (218 MB, 4.2 TB/s);
+//   its read back: 11 us (50 MB); eight requests' prefixes: 73 us (349 MB, 4.8).
+//
+// Writes and reads go by blocks of 32 positions of one head. A wave has a block
+// to itself (writes: K or V of it, reads both): 8 or 16 KB of loads are under
+// way before it waits, and nothing waits for another wave. With a workgroup of
+// four waves and barriers per block the same calls took 75, 15 and 103 us.
+// V's transposition is done on 32-bit words of LDS rows (two bf16 or four
+// bytes of a key) and byte permutes, not element by element.
 #include "paged.hpp"
 #include "rotary.hpp"
 
@@ -31,6 +44,8 @@ __device__ __forceinline__ void rotate_rows(const RotRows& q, int Hq, const RotR
   }
 }
 
+// A workgroup rotates up to eight tokens, all heads of each: the angles are
+// computed once per token (64 pairs, not 48 heads x 64) and stay in LDS.
 constexpr int kRotTokens = 8;    // most tokens of a workgroup
 constexpr int kMaxPairs = 128;   // head dim 256 at most
 
@@ -209,7 +224,9 @@ __device__ __forceinline__ void turn4(const uint32_t (&a)[4], uint32_t (&t)[4]) 
 }
 
 // Keys [klo, khi) of a block, few of them (a decode or verify step's): a lane
-// has one 16-byte chunk of a row, its elements go where they belong.
+// has one 16-byte chunk of a row, its elements go where they belong. Up to two
+// rounds of it; as whole blocks through LDS a decode step of sixteen requests
+// took 10.4 us, this way 5.7.
 template <int D, int BITS>
 __device__ __forceinline__ void write_few(const WriteParams& p, int h, bool isk, int lane, long long base,
                                           long long first, long long at, int klo, int khi) {
