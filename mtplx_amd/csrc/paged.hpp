@@ -123,6 +123,15 @@ __device__ __forceinline__ long long div_pos(long long a, int b) {
 // pool) was asked for; that row was not written, or reads as absent.
 constexpr int kStatusPage = 1;
 
+// Keys [lo, hi) of the block from position `base` on that lie in [from, to).
+struct KeyRange {
+  int lo, hi;
+};
+__device__ __forceinline__ KeyRange block_keys(long long base, long long from, long long to) {
+  const long long a = from - base, b = to - base;
+  return {a < 0 ? 0 : a < kBlk ? (int)a : kBlk, b < 0 ? 0 : b < kBlk ? (int)b : kBlk};
+}
+
 // First element of block `blk` (of a request's positions) of head h, or -1
 // where the table holds no page of the pool for it.
 __device__ __forceinline__ long long page_block(const int32_t* table, int width, int b, long long blk, int bpp,

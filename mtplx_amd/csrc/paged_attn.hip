@@ -1169,7 +1169,8 @@ inline AttnPlan attn_plan(int Hq, int Hkv, int D, int max_rows) {
   a.few = max_rows > 0 && (long long)max_rows * rep <= 32;
   a.RT = a.few ? 32 : D == 256 ? 128 : 256;   // chunk_waves<D>() * 32
   a.P = (a.RT + rep - 2) / rep + 1;
-  a.G = device_cus() * (a.few && D < 256 ? 2 : 1);
+  a.G = a.few ? device_cus() * (D < 256 ? 2 : 1) : device_cus() / 8 * 8;   // (chunks: dealt to eight XCDs)
+  if (a.G < 8) a.G = 8;
   a.min_share = a.few ? 4 * kBlk : 2 * kStepKeys;
   a.step = a.few ? kBlk : kStepKeys;
   a.tile_cost = a.few ? 0 : 2 * kStepKeys;

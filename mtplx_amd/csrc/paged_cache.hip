@@ -301,9 +301,8 @@ __device__ __forceinline__ void write_unit(const WriteParams& p, const Unit& w, 
   constexpr int RS = row16<D>(), NC = D / 16, BS = row8<D>();   // 16-byte loads of a lane
   const long long base = w.blk * kBlk;
   // Keys [klo, khi) of the block are new; token of key kk: first + kk.
-  const int klo = w.start > base ? (int)(w.start - base) : 0;
-  const long long end = w.start + w.rows.n - base;
-  const int khi = end < kBlk ? (int)end : kBlk;
+  const KeyRange range = block_keys(base, w.start, w.start + w.rows.n);
+  const int klo = range.lo, khi = range.hi;
   if (klo >= khi) return;   // (a request of no rows)
   const long long first = w.rows.lo + (base - w.start);
   u32x4 x[NC];
@@ -521,9 +520,8 @@ __device__ __forceinline__ void read_unit(const ReadParams& p, int b, int h, int
   constexpr bool AHEAD = NC <= 8;
   const long long start = p.start ? p.start[b] : 0;
   const long long ablk = floor_blk(start) + blk, base = ablk * kBlk;
-  const int klo = start > base ? (int)(start - base) : 0;
-  const long long end = start + p.count - base;
-  const int khi = end < kBlk ? (int)end : kBlk;
+  const KeyRange range = block_keys(base, start, start + p.count);
+  const int klo = range.lo, khi = range.hi;
   if (klo >= khi) return;
   const long long len = p.lengths ? (long long)p.lengths[b] - base : kBlk;
   int live = len < khi ? (len < 0 ? 0 : (int)len) : khi;   // keys [klo, live) are read, [live, khi) are zeros

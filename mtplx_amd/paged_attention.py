@@ -11,6 +11,7 @@ prompts run together.
 from __future__ import annotations
 
 import math
+import threading
 from typing import Any
 
 import torch
@@ -68,11 +69,13 @@ def paged_sdpa(queries: torch.Tensor, cache: PagedKVCache, block_table: Any, q_s
     a.ws, a.ws_bytes = ws.data_ptr(), ws.numel()
     a.T, a.B, a.width, a.Hq, a.max_rows, a.scale = T, B, width, Hq, rows, scale
     a.q_token, a.q_head, a.out_token, a.out_head = qt, qh, ot, oh
-    _call("mtp_paged_attn", a, device)
+    with _LAUNCH:   # (its launches stay together: host threads may share a stream and so its workspace)
+        _call("mtp_paged_attn", a, device)
     return out
 
 
 _SPACES: dict = {}
+_LAUNCH = threading.Lock()
 
 
 def _workspace(device, Hq: int, Hkv: int, D: int, rows: int) -> torch.Tensor:
@@ -80,14 +83,15 @@ def _workspace(device, Hq: int, Hkv: int, D: int, rows: int) -> torch.Tensor:
     once (the pool keeps what it gave out allocated). A call that is being
     captured takes the graph's own memory: graphs captured on one stream may be
     replayed on two at once."""
-    if torch.cuda.is_current_stream_capturing():
+    if torch.cuda.current_device() != device.index:
         with torch.cuda.device(device):
-            nb = _lib.query("mtp_paged_attn_workspace_bytes", Hq, Hkv, D, rows)
-        return torch.empty(nb, dtype=torch.uint8, device=device)
+            return _workspace(device, Hq, Hkv, D, rows)
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(_lib.query("mtp_paged_attn_workspace_bytes", Hq, Hkv, D, rows), dtype=torch.uint8,
+                           device=device)
     key = (device.index, _stream(device), Hq, Hkv, D, 0 < rows * (Hq // Hkv) <= 32)
     ws = _SPACES.get(key)
     if ws is None:
-        with torch.cuda.device(device):
-            nb = _lib.query("mtp_paged_attn_workspace_bytes", Hq, Hkv, D, rows)
+        nb = _lib.query("mtp_paged_attn_workspace_bytes", Hq, Hkv, D, rows)
         ws = _SPACES[key] = _lib.WORKSPACES.get(nb, "paged_attn", device)
     return ws

@@ -158,6 +158,8 @@ def _writable(name: str, out: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
 def _int32(name: str, value: Any, device, numel: int | None = None) -> torch.Tensor:
     t = value if isinstance(value, torch.Tensor) else torch.as_tensor(value)
     if t.dtype is not torch.int32 or t.device != device or not t.is_contiguous():
+        if t.numel() and (t.dtype is torch.bool or t.is_floating_point() or t.is_complex()):
+            raise TypeError(f"{name} must hold integers (got {t.dtype})")
         t = t.to(device=device, dtype=torch.int32).contiguous()
     if numel is not None and t.numel() != numel:
         raise ValueError(f"{name} must hold {numel} values (got {t.numel()})")
@@ -214,6 +216,8 @@ def apply_rotary(table: RotaryTable, queries: torch.Tensor, keys: torch.Tensor |
         if Tk != T:
             raise ValueError(f"queries have {T} tokens, keys {Tk}")
         _on(device, "keys", k)
+    if Hq < 1:
+        raise ValueError("queries have no heads")
     if D % 8 or D > 256 or table.dims > D:
         raise ValueError(f"head dim {D} must be a multiple of 8 up to 256 and hold the table's {table.dims} dims")
     pos = _int32("positions", positions, device, T)
@@ -249,7 +253,7 @@ def apply_rotary(table: RotaryTable, queries: torch.Tensor, keys: torch.Tensor |
             raise ValueError("the two outputs overlap")
         qot, qoh = qo.stride()[:2]
         kot, koh = (0, 0) if ko is None else ko.stride()[:2]
-    if T == 0 or Hq == 0:
+    if T == 0:
         return qo, ko
     if not Hkv:
         k = None

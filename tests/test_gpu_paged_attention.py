@@ -350,3 +350,32 @@ def test_captured_steps_at_once(gpu):
         torch.cuda.synchronize()
         for out, w in zip(outs, want):
             assert torch.equal(out, w)
+
+
+def test_two_host_threads_on_one_stream(gpu):
+    """Calls of two threads on the same stream share its workspace; each call's
+    launches stay together."""
+    import threading
+
+    rng = np.random.default_rng(19)
+    H, Hq, D, page = 2, 16, 128, 64
+    table, pages = tables(rng, [6000], page)
+    c = PagedKVCache(pages, H, D, page_size=page, bits=8)
+    c.write(rows(rng, 6000, H, D), rows(rng, 6000, H, D), table, i32([0]))
+    qs = [rows(rng, n, Hq, D) for n in (2, 90)]
+    start = i32([5900])
+    want = [paged_sdpa(q, c, table, start) for q in qs]
+    torch.cuda.synchronize()
+    bad: list = []
+
+    def work(q, w):
+        for _ in range(60):
+            bad.append(paged_sdpa(q, c, table, start).ne(w).any())
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(qs, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert len(bad) == 120 and not any(bool(b) for b in bad)

@@ -155,3 +155,10 @@ def test_streams_and_graph(gpu):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(cap[0], want[0]) and torch.equal(cap[1], want[1])
+
+
+def test_no_query_heads_refused(gpu):
+    rng = np.random.default_rng(5)
+    k = rows(rng, 4, 2, 128)
+    with pytest.raises(ValueError):
+        apply_rotary(rotary_table(128), k[:, :0], k, i32([0, 1, 2, 3]))

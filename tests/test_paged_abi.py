@@ -160,3 +160,13 @@ def test_quantised_rows():
     q, s = O.quantise_rows(x)
     assert q[1].tolist() == [64, -127] and s[1] == np.float32(2) / np.float32(127)   # 63.5 to even
     assert (q[[0, 2]] == 0).all() and (s[[0, 2]] == 0).all() and np.isnan(s[3:]).all()
+
+
+def test_index_arrays_hold_integers():
+    from mtplx_amd.rotary import _int32
+
+    cpu = torch.device("cpu")
+    assert _int32("positions", [3, 4], cpu).dtype is torch.int32 and _int32("positions", [], cpu).numel() == 0
+    for bad in ([0.5], torch.ones(1), torch.ones(1, dtype=torch.bool)):
+        with pytest.raises(TypeError):
+            _int32("positions", bad, cpu)
