@@ -6,11 +6,13 @@
 //
 // f is held as 64-bit fixed point (f 2^64), so p f mod 1 is one wrapping
 // integer product, exact for any int32 position: at position 10^6 a 32-bit
-// float angle is off by up to 0.03 radians, this by 10^-10. The top 32 bits,
-// as a signed fraction of a revolution, go to v_sin_f32 / v_cos_f32, which
-// take revolutions; both are within 2^-20 of the true values over all
-// fractions (bf16 rounds at 2^-9), for 8 issue slots instead of the ~40 that
-// sincosf spends on its own reduction.
+// float angle is off by up to 0.03 radians, this by 10^-13. Cosine and sine are
+// the Taylor polynomials of the nearest quarter turn's rest (at most pi / 4) in
+// fp64, within 2^-40, rounded once to fp32 (v_cos_f32 and v_sin_f32, within
+// 2^-20, put one result in 2000 on the wrong side of its rounding to bf16; this
+// one in 10^5, and a token's angles serve all its heads). The products and
+// their sum are fp32, each rounded, as the formula reads; fp64 products cost
+// the rotation of 8192 tokens 49 us instead of 46.
 #pragma once
 
 #include "common.hpp"
@@ -25,15 +27,35 @@ struct RotSpec {
 
 __device__ __forceinline__ float2 rot_angle(long long pos, unsigned long long f, float gain) {
   const unsigned long long ph = (unsigned long long)pos * f;
-  const float r = (float)(int)(ph >> 32) * 0x1p-32f;   // (-1/2, 1/2] revolutions
-  return make_float2(gain * __builtin_amdgcn_cosf(r), gain * __builtin_amdgcn_sinf(r));
+  const unsigned long long q = (ph + (1ull << 61)) >> 62;   // quarter turns, to the nearest (mod 4)
+  const double x = (double)(long long)(ph - (q << 62)) * (6.283185307179586476925 / 18446744073709551616.0);
+  const double z = x * x;
+  double s = 1.0 / 6227020800.0, c = 1.0 / 479001600.0;
+  s = fma(s, z, -1.0 / 39916800.0);
+  c = fma(c, z, -1.0 / 3628800.0);
+  s = fma(s, z, 1.0 / 362880.0);
+  c = fma(c, z, 1.0 / 40320.0);
+  s = fma(s, z, -1.0 / 5040.0);
+  c = fma(c, z, -1.0 / 720.0);
+  s = fma(s, z, 1.0 / 120.0);
+  c = fma(c, z, 1.0 / 24.0);
+  s = fma(s, z, -1.0 / 6.0);
+  c = fma(c, z, -0.5);
+  s = gain * fma(s * z, x, x);
+  c = gain * fma(c, z, 1.0);
+  const int n = (int)q;
+  const float fs = (float)s, fc = (float)c;
+  const float co = n & 1 ? fs : fc, si = n & 1 ? fc : fs;
+  return make_float2((n + 1) & 2 ? -co : co, n & 2 ? -si : si);
 }
 
 __device__ __forceinline__ float rot_first(float x1, float x2, float2 cs) {
-  return __fmaf_rn(x1, cs.x, -__fmul_rn(x2, cs.y));
+#pragma clang fp contract(off)
+  return x1 * cs.x - x2 * cs.y;
 }
 __device__ __forceinline__ float rot_second(float x1, float x2, float2 cs) {
-  return __fmaf_rn(x1, cs.y, __fmul_rn(x2, cs.x));
+#pragma clang fp contract(off)
+  return x1 * cs.y + x2 * cs.x;
 }
 
 // A head's row falls into items of 8 elements, or, where the halves of the

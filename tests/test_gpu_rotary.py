@@ -1,7 +1,9 @@
 """GPU parity of the rotary positions with the float64 oracle.
 
-Bound: one rounding to bf16 (2^-8 of the value) plus the angle's sine and
-cosine, within 2^-20 each, and two fp32 products: 2^-19 gain (|x1| + |x2|).
+Bound: one rounding to bf16 (2^-8 of the value) plus fp32's: cosine and sine
+(2^-25 gain), the gain itself, the products and their sum (2^-24 of each) make
+less than 2^-22 gain (|x1| + |x2|); the oracle's own angle at position 2^31 is
+off by up to 2^-22, so 2^-21 in all.
 """
 
 import math
@@ -24,7 +26,7 @@ def _check(got, x, pos, t, what):
     h = t.dims // 2
     i1, i2 = (np.arange(0, t.dims, 2), np.arange(1, t.dims, 2)) if t.traditional else (np.arange(h), np.arange(h) + h)
     mate[..., i1], mate[..., i2] = a[..., i2], a[..., i1]
-    bound = HALF * np.abs(want) + abs(t.gain) * 2.0 ** -19 * (a + mate)
+    bound = HALF * np.abs(want) + abs(t.gain) * 2.0 ** -21 * (a + mate)
     bound[..., t.dims:] = 0.0
     check_rows(num(got), want, bound, what)
 
@@ -58,8 +60,8 @@ def test_scaled_and_far(gpu, kw):
 
 def test_sine_and_cosine_of_every_turn(gpu):
     """Unit rows rotated by fractions all around: the outputs are the cosine
-    and sine themselves, within bf16's rounding and 2^-20 of absolute error
-    (seen near their zeros, where rounding is small)."""
+    and sine themselves, within bf16's rounding and fp32's of the angle's
+    functions (2^-25, seen near their zeros, where bf16's is small)."""
     n = 1 << 16
     t = rotary_table(2, frequencies=[2 * math.pi / n * 1.0])
     x = torch.zeros((n, 1, 8), dtype=torch.bfloat16, device="cuda")
@@ -68,7 +70,7 @@ def test_sine_and_cosine_of_every_turn(gpu):
     y = num(apply_rotary(t, x, None, i32(pos))[0])[:, 0, :2]
     a = 2 * math.pi * pos / n
     want = np.stack([np.cos(a), np.sin(a)], -1)
-    assert (np.abs(y - want) <= HALF * np.abs(want) + 2.0 ** -20).all()
+    assert (np.abs(y - want) <= HALF * np.abs(want) + 2.0 ** -24).all()
 
 
 def test_views_in_place_and_outputs(gpu):
