@@ -2,9 +2,8 @@
 // and quantising on the way) and reads. All of them move bytes once, and long
 // calls are bound by that (a large copy reaches 5.17 TB/s on an MI355X):
 //
-//   rotation of 8192 tokens, 40 + 8 heads of 128: 34 us (201 MB, 5.9 TB/s: part
-//     of it stays in the last-level cache);
-//   write of the same at 8 bits, queries rotated: 52 us (218 MB, 4.2 TB/s);
+//   rotation of 8192 tokens, 40 + 8 heads of 128: 46 us (201 MB, 4.4 TB/s);
+//   write of the same at 8 bits, queries rotated: 58 us (218 MB, 3.8 TB/s);
 //   its read back: 11 us (50 MB); eight requests' prefixes: 73 us (349 MB, 4.8).
 //
 // Writes and reads go by blocks of 32 positions of one head. A wave has a block
@@ -226,7 +225,7 @@ __device__ __forceinline__ void turn4(const uint32_t (&a)[4], uint32_t (&t)[4]) 
 // Keys [klo, khi) of a block, few of them (a decode or verify step's): a lane
 // has one 16-byte chunk of a row, its elements go where they belong. Up to two
 // rounds of it; as whole blocks through LDS a decode step of sixteen requests
-// took 10.4 us, this way 5.7.
+// took 10.4 us, this way 5.7 (6.8 with fp64 angles).
 template <int D, int BITS>
 __device__ __forceinline__ void write_few(const WriteParams& p, int h, bool isk, int lane, long long base,
                                           long long first, long long at, int klo, int khi) {
