@@ -632,6 +632,8 @@ typedef struct mtp_paged_attn_args {
   float scale;
   long long q_token, q_head, out_token, out_head;
 } mtp_paged_attn_args;
+/* Two launches share the workspace: calls that may overlap (two streams, two
+ * replayed graphs) need one each. T * Hq < 2^31. */
 size_t mtp_paged_attn_workspace_bytes(int Hq, int Hkv, int D, int max_rows);
 int mtp_paged_attn(const mtp_paged_attn_args* args, void* stream);
 
