@@ -564,7 +564,7 @@ int mtp_rotary(const mtp_rotary_args* args, void* stream);
  * row offsets are clamped to [0, T], pages to the pool.
  *
  * 8 bits, per token and head: A = max |x|, scale = A / 127,
- * q = rint(x * (127 / A)) in fp32; a row below 2^-100 is zeros, one with a NaN
+ * q = rint(x * (127 * (1 / A))) in fp32; a row below 2^-100 is zeros, one with a NaN
  * or an infinity gets a NaN scale and reads as NaN.
  *
  * mtp_paged_write: k, v [T, Hkv, D] into the pages; dims > 0 rotates k at its

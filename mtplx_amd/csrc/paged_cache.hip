@@ -166,11 +166,13 @@ __device__ __forceinline__ void half_row(const uint16_t* rows, int lane, u32x4 (
 }
 
 // 8-bit rows. Largest magnitude A, by the bits of bf16 (m: of each two
-// elements); then 127 / A and A / 127, one correctly rounded division each, and
-// q = rint(x (127 / A)): adding 1.5 2^23 rounds to an integer in the low bits,
-// |x (127 / A)| < 127.5. A row with a NaN or an infinity gets a NaN scale, so it
+// elements); then A / 127 and r = 127 (1 / A), each step rounded once, and
+// q = rint(x r): adding 1.5 2^23 rounds to an integer in the low bits,
+// |x r| < 127.5. (The reciprocal first, as torch computes 127 / A on the GPU:
+// ratios of short mantissas often lie halfway between integers, and rows
+// quantised there and here then hold the same ones.) A row with a NaN or an infinity gets a NaN scale, so it
 // reads as NaN instead of as wrong numbers; one below 2^-100 gets zeros
-// (127 / A would overflow, A / 127 go subnormal).
+// (r would overflow, A / 127 go subnormal).
 __device__ __forceinline__ u16x2 max_bits(u16x2 m, u32x4 x) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, x[j] & 0x7fff7fffu));
@@ -182,7 +184,7 @@ struct RowScale {
 __device__ __forceinline__ RowScale row_scale(int m) {
   const float a = __uint_as_float((uint32_t)m << 16);
   const bool bad = m >= 0x7f80, tiny = a < 0x1p-100f;
-  return {bad || tiny ? 0.f : 127.f / a, bad ? __uint_as_float(0x7fc00000u) : tiny ? 0.f : a / 127.f};
+  return {bad || tiny ? 0.f : __fmul_rn(127.f, 1.f / a), bad ? __uint_as_float(0x7fc00000u) : tiny ? 0.f : a / 127.f};
 }
 __device__ __forceinline__ uint2 bytes8(u32x4 x, float inv) {
 #pragma clang fp contract(off)   // (the product is rounded before the sum)

@@ -31,7 +31,7 @@ def quantise_rows(x: np.ndarray) -> tuple[np.ndarray, np.ndarray]:
     bad = ~np.isfinite(x).all(axis=-1)
     tiny = ~bad & (top < np.float32(2.0) ** -100)
     with np.errstate(all="ignore"):
-        inv = np.where(bad | tiny, np.float32(0), np.float32(127) / top)
+        inv = np.where(bad | tiny, np.float32(0), np.float32(127) * (np.float32(1) / top))
         scale = np.where(bad, np.float32(np.nan), np.where(tiny, np.float32(0), top / np.float32(127)))
         q = np.rint(x * inv[..., None])
     return np.clip(np.nan_to_num(q, nan=0.0), -127, 127).astype(np.int8), scale.astype(np.float32)
