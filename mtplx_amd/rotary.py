@@ -202,6 +202,15 @@ def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a0 < b1 and b0 < a1
 
 
+def _apart(src: torch.Tensor, dst: torch.Tensor, in_place: bool = False) -> bool:
+    """Whether a kernel may write the rows ``dst`` while it reads ``src``: they
+    share no element or, with ``in_place`` (its own source and output), are the
+    same view."""
+    if not _overlaps(dst, src):
+        return True
+    return in_place and dst.data_ptr() == src.data_ptr() and dst.stride() == src.stride() and dst.shape == src.shape
+
+
 def apply_rotary(table: RotaryTable, queries: torch.Tensor, keys: torch.Tensor | None, positions: Any, *,
                  out: tuple | None = None):
     """Rotate ``queries`` [T, Hq, D] and ``keys`` [T, Hkv, D] (or None) bf16 at
@@ -232,23 +241,14 @@ def apply_rotary(table: RotaryTable, queries: torch.Tensor, keys: torch.Tensor |
     else:
         qo = _writable("out[0]", out[0], queries)
         ko = None if k is None else _writable("out[1]", out[1], keys)
-        # The kernel reads a row's parts where it writes them only as far as
-        # the very same view goes.
-        exact = table.traditional or table.dims % 16 == 0
-        for dst in (qo, ko):
-            if dst is None:
-                continue
-            for src in (q, k):
-                if src is not None and _overlaps(dst, src):
-                    same = exact and dst.data_ptr() == src.data_ptr() and dst.stride() == src.stride() \
-                        and dst.shape == src.shape
-                    if not same:
-                        if src is q:
-                            q = q.clone(memory_format=torch.contiguous_format)
-                            qt, qh = Hq * D, D
-                        else:
-                            k = k.clone(memory_format=torch.contiguous_format)
-                            kt, kh = Hkv * D, D
+        # An item of the kernel reads what it stores, unless the halves are no whole chunks; heads go in no order.
+        in_place = table.traditional or table.dims % 16 == 0
+        if not _apart(q, qo, in_place) or (ko is not None and not _apart(q, ko)):
+            q = q.clone(memory_format=torch.contiguous_format)
+            qt, qh = Hq * D, D
+        if k is not None and not (_apart(k, ko, in_place) and _apart(k, qo)):
+            k = k.clone(memory_format=torch.contiguous_format)
+            kt, kh = Hkv * D, D
         if ko is not None and _overlaps(qo, ko) and not _interleaved(qo, ko):
             raise ValueError("the two outputs overlap")
         qot, qoh = qo.stride()[:2]

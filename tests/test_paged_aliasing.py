@@ -1,0 +1,69 @@
+"""What the paged operators hand to their kernels when outputs lie over inputs:
+the argument block of each call, taken instead of a launch (CPU). A kernel reads
+and writes heads in no order, so a source may share memory with an output only
+where it is that output's own and the very same view."""
+
+import itertools
+
+import pytest
+import torch
+
+from mtplx_amd import paged_attention, paged_kv_cache, rotary
+from mtplx_amd.rotary import apply_rotary, rotary_table
+
+T, H, D = 3, 2, 64
+
+
+class OnGpu(torch.Tensor):
+    """A host tensor that the argument checks take for one on the GPU."""
+
+    is_cuda = property(lambda self: True)
+
+
+def held(*shape):
+    return torch.arange(torch.Size(shape).numel()).reshape(shape).to(torch.bfloat16).as_subclass(OnGpu)
+
+
+@pytest.fixture
+def blocks(monkeypatch):
+    """Argument blocks of the calls made, in order."""
+    made = []
+
+    def take(name, block, device):
+        made.append(block)
+
+    for module in (rotary, paged_kv_cache, paged_attention):
+        monkeypatch.setattr(module, "_call", take)
+    monkeypatch.setattr(paged_attention, "_workspace", lambda *a: torch.empty(16, dtype=torch.uint8))
+    return made
+
+
+def _elements(ptr, heads, token, head):
+    return {ptr + 2 * (t * token + h * head + d) for t, h, d in itertools.product(range(T), range(heads), range(D))}
+
+
+def check_block(b, in_place=True):
+    """No source under another's output; its own output apart or the same rows."""
+    src = {"q": (b.q, b.Hq, b.q_token, b.q_head), "k": (b.k, b.Hkv, b.k_token, b.k_head)}
+    dst = {"q": (b.q_out, b.Hq, b.qo_token, b.qo_head), "k": (b.k_out, b.Hkv, b.ko_token, b.ko_head)}
+    for s, d in itertools.product("qk", "qk"):
+        if src[s][0] is None or dst[d][0] is None:
+            continue
+        if s == d and in_place and src[s] == dst[d]:
+            continue
+        assert not _elements(*src[s]) & _elements(*dst[d]), f"{s} is read where {d} is written"
+
+
+def test_a_source_under_another_output_is_copied(blocks):
+    t, pos = rotary_table(D, device="cpu"), torch.arange(T)
+    x, y, z = held(T, H, D), held(T, H, D), held(T, H, D)
+    calls = [(x, x, (x, y)), (x, x, (y, x)), (x, y, (y, x)), (x, y, (z, x)), (x, y, (y, z)), (x, y, (x, y)), (x, x, (y, z))]
+    for q, k, out in calls:
+        got = apply_rotary(t, q, k, pos, out=out)
+        assert got[0] is out[0] and got[1] is out[1]
+        check_block(blocks[-1])
+    b = blocks[-2]   # (x, y) in place: the caller's own rows
+    assert (b.q, b.k) == (b.q_out, b.k_out) == (x.data_ptr(), y.data_ptr())
+    # halves that are no whole chunks: not over the own source either
+    apply_rotary(rotary_table(24, device="cpu"), x, y, pos, out=(x, y))
+    check_block(blocks[-1], in_place=False)
