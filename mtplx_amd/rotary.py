@@ -204,9 +204,9 @@ def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 def _apart(src: torch.Tensor, dst: torch.Tensor, in_place: bool = False) -> bool:
     """Whether a kernel may write the rows ``dst`` while it reads ``src``: they
-    share no element or, with ``in_place`` (its own source and output), are the
+    share no element (rows side by side among them) or, with ``in_place`` (its own source and output), are the
     same view."""
-    if not _overlaps(dst, src):
+    if not _overlaps(dst, src) or _interleaved(dst, src):
         return True
     return in_place and dst.data_ptr() == src.data_ptr() and dst.stride() == src.stride() and dst.shape == src.shape
 

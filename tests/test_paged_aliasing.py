@@ -67,3 +67,31 @@ def test_a_source_under_another_output_is_copied(blocks):
     # halves that are no whole chunks: not over the own source either
     apply_rotary(rotary_table(24, device="cpu"), x, y, pos, out=(x, y))
     check_block(blocks[-1], in_place=False)
+
+
+def _parts(fused, *heads):
+    """Views [T, h, D] side by side in rows of a fused projection."""
+    at, out = 0, []
+    for h in heads:
+        out.append(fused[:, at * D:(at + h) * D].view(T, h, D))
+        at += h
+    return out
+
+
+def test_rotary_in_place_on_a_fused_projection(blocks):
+    """Rows that lie side by side share no element: they are read where they are."""
+    t, pos = rotary_table(D, device="cpu"), torch.arange(T)
+    q, k, _ = _parts(held(T, 8 * D), 4, 2, 2)
+    apply_rotary(t, q, k, pos, out=(q, k))
+    b = blocks[-1]
+    assert (b.q, b.k) == (b.q_out, b.k_out) == (q.data_ptr(), k.data_ptr())
+    check_block(b)
+    # outputs side by side with sources that are not theirs
+    a, x, c, d = _parts(held(T, 8 * D), 2, 2, 2, 2)
+    apply_rotary(t, a, x, pos, out=(d, c))
+    b = blocks[-1]
+    assert (b.q, b.k, b.q_out, b.k_out) == (a.data_ptr(), x.data_ptr(), d.data_ptr(), c.data_ptr())
+    apply_rotary(t, a, x, pos, out=(x, c))   # keys under the queries' output
+    b = blocks[-1]
+    assert b.q == a.data_ptr() and b.k != x.data_ptr()
+    check_block(b)
