@@ -18,7 +18,7 @@ import torch
 
 from . import _lib
 from .paged_kv_cache import PagedKVCache
-from .rotary import _call, _on, _overlaps, _rows, _stream, _writable
+from .rotary import _apart, _call, _on, _rows, _stream, _writable
 
 __all__ = ["paged_sdpa"]
 
@@ -54,7 +54,7 @@ def paged_sdpa(queries: torch.Tensor, cache: PagedKVCache, block_table: Any, q_s
         ot, oh = Hq * D, D
     else:
         out = _writable("out", out, queries)
-        if _overlaps(out, q):
+        if not _apart(q, out):
             q = q.clone(memory_format=torch.contiguous_format)
             qt, qh = Hq * D, D
         ot, oh = out.stride()[:2]

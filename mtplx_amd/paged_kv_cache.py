@@ -24,7 +24,7 @@ from typing import Any
 import torch
 
 from . import _lib
-from .rotary import RotaryTable, _call, _int32, _interleaved, _on, _overlaps, _rows, _writable
+from .rotary import RotaryTable, _apart, _call, _int32, _on, _rows, _writable
 
 __all__ = ["PagedKVCache"]
 
@@ -163,13 +163,11 @@ class PagedKVCache:
             else:
                 qo = _writable("out", out, queries)
                 for name, x in (("keys", k), ("values", v)):
-                    if _overlaps(qo, x) and not _interleaved(qo, x):
+                    if not _apart(x, qo):
                         raise ValueError(f"out overlaps {name}")
-                if _overlaps(qo, q):
-                    same = qo.data_ptr() == q.data_ptr() and qo.stride() == q.stride()
-                    if not same or not (rotary.traditional or rotary.dims % 16 == 0):
-                        q = q.clone(memory_format=torch.contiguous_format)
-                        qt, qh = Hq * D, D
+                if not _apart(q, qo, rotary.traditional or rotary.dims % 16 == 0):
+                    q = q.clone(memory_format=torch.contiguous_format)
+                    qt, qh = Hq * D, D
                 qot, qoh = qo.stride()[:2]
         if T == 0:
             return qo

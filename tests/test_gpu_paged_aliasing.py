@@ -5,8 +5,10 @@ import numpy as np
 import pytest
 import torch
 
+from mtplx_amd.paged_attention import paged_sdpa
+from mtplx_amd.paged_kv_cache import PagedKVCache
 from mtplx_amd.rotary import apply_rotary, rotary_table
-from tests.paged_util import i32, rows
+from tests.paged_util import i32, rows, tables
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +52,29 @@ def test_rotary_on_a_fused_projection(gpu):
     apply_rotary(t, q, k, pos, out=(q, k))
     assert torch.cuda.max_memory_allocated() == before
     assert torch.equal(q, wq) and torch.equal(k, wk) and torch.equal(fused[:, (Hq + H) * D:], keep)
+
+
+def test_write_and_attention_on_fused_rows(gpu):
+    """Queries rotated, then attended, into columns beside them."""
+    rng = np.random.default_rng(33)
+    n, Hq, H, D, keys = 300, 8, 2, 128, 500
+    table, pages = tables(rng, [keys], 64)
+    a, b = (PagedKVCache(pages, H, D, page_size=64) for _ in range(2))
+    rope, start = rotary_table(D, base=1e6), i32([keys - n])
+    old = rows(rng, keys, H, D)
+    for c in (a, b):
+        c.write(old, old, table, i32([0]))
+    fused = rows(rng, n, (2 * Hq + 2 * H) * D)
+    q, k, v, out = (fused[:, lo * D:hi * D].view(n, hi - lo, D) for lo, hi in
+                    ((0, Hq), (Hq, Hq + H), (Hq + H, Hq + 2 * H), (Hq + 2 * H, 2 * (Hq + H))))
+    turned = a.write(k, v, table, start, queries=q, rotary=rope)
+    want = paged_sdpa(turned, a, table, start)
+    q0 = q.clone()
+    assert b.write(k, v, table, start, queries=q, rotary=rope, out=out) is out
+    assert torch.equal(out, turned) and torch.equal(q, q0) and torch.equal(a.k_pages, b.k_pages)
+    b.write(k, v, table, start, queries=q, rotary=rope, out=q)
+    assert torch.equal(q, turned)
+    paged_sdpa(q, b, table, start, out=out)
+    assert torch.equal(out, want) and torch.equal(q, turned)
+    paged_sdpa(q, b, table, start, out=q)
+    assert torch.equal(q, want)

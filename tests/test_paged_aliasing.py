@@ -95,3 +95,22 @@ def test_rotary_in_place_on_a_fused_projection(blocks):
     b = blocks[-1]
     assert b.q == a.data_ptr() and b.k != x.data_ptr()
     check_block(b)
+
+
+def test_write_and_attention_into_rows_side_by_side(blocks):
+    """Queries whose columns only neighbour the output's are read where they are."""
+    cache = paged_kv_cache.PagedKVCache(1, 2, D, device="cpu")
+    table, start = torch.zeros((1, 1), dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    q, k, v, out = _parts(held(T, 12 * D), 4, 2, 2, 4)
+    for rope in (rotary_table(D, device="cpu"), rotary_table(24, device="cpu")):
+        cache.write(k, v, table, start, queries=q, rotary=rope, out=out)
+        assert (blocks[-1].q, blocks[-1].q_out) == (q.data_ptr(), out.data_ptr())
+    assert paged_attention.paged_sdpa(q, cache, table, start, out=out) is out
+    assert (blocks[-1].q, blocks[-1].out) == (q.data_ptr(), out.data_ptr())
+    # over the queries themselves: rotated in place, attended from a copy
+    cache.write(k, v, table, start, queries=q, rotary=rotary_table(D, device="cpu"), out=q)
+    assert blocks[-1].q == blocks[-1].q_out == q.data_ptr()
+    cache.write(k, v, table, start, queries=q, rotary=rotary_table(24, device="cpu"), out=q)
+    assert blocks[-1].q != blocks[-1].q_out == q.data_ptr()
+    paged_attention.paged_sdpa(q, cache, table, start, out=q)
+    assert blocks[-1].q != blocks[-1].out == q.data_ptr()
