@@ -191,13 +191,14 @@ def _call(name: str, block: ctypes.Structure, device) -> None:
 
 
 def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
-    if a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr():
-        return False
-
+    """Whether the address spans of two views meet (two storages may hold the
+    same memory, so storages are not compared)."""
     def span(x):
-        lo = x.storage_offset()
-        return lo, lo + sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1
+        lo = x.data_ptr()
+        return lo, lo + (sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1) * x.element_size()
 
+    if not (a.numel() and b.numel()):
+        return False
     (a0, a1), (b0, b1) = span(a), span(b)
     return a0 < b1 and b0 < a1
 
@@ -269,8 +270,9 @@ def _interleaved(a: torch.Tensor, b: torch.Tensor) -> bool:
     (the parts of a fused projection): equal token strides, disjoint columns."""
     if a.stride(0) != b.stride(0) or a.stride(0) <= 0:
         return False
-    wide = a.stride(0)
-    (a0, an), (b0, bn) = ((x.storage_offset(), (x.shape[1] - 1) * x.stride(1) + x.shape[2]) for x in (a, b))
+    wide = a.stride(0) * a.element_size()
+    (a0, an), (b0, bn) = ((x.data_ptr(), ((x.shape[1] - 1) * x.stride(1) + x.shape[2]) * x.element_size())
+                          for x in (a, b))
     first, n, second = (a0, an, b0) if a0 <= b0 else (b0, bn, a0)
     gap = second - first
     return gap < wide and n <= gap and gap + (bn if first == a0 else an) <= wide

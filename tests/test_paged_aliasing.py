@@ -114,3 +114,27 @@ def test_write_and_attention_into_rows_side_by_side(blocks):
     assert blocks[-1].q != blocks[-1].q_out == q.data_ptr()
     paged_attention.paged_sdpa(q, cache, table, start, out=q)
     assert blocks[-1].q != blocks[-1].out == q.data_ptr()
+
+
+def test_memory_shared_by_two_storages(blocks):
+    """The same rows behind another storage (a tensor passed through dlpack)
+    are found by their addresses."""
+    t, pos = rotary_table(24, device="cpu"), torch.arange(T)
+    x = held(T + 1, H, D)
+    again = torch.from_dlpack(x.as_subclass(torch.Tensor)[1:]).as_subclass(OnGpu)
+    assert again.untyped_storage().data_ptr() != x.untyped_storage().data_ptr() and again.data_ptr() == x[1:].data_ptr()
+    apply_rotary(t, x[:T], None, pos, out=(again, None))
+    check_block(blocks[-1], in_place=False)
+    cache = paged_kv_cache.PagedKVCache(1, H, D, device="cpu")
+    table, start = torch.zeros((1, 1), dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    paged_attention.paged_sdpa(x[:T], cache, table, start, out=again)
+    b = blocks[-1]
+    assert not _elements(b.q, H, b.q_token, b.q_head) & _elements(b.out, H, b.out_token, b.out_head)
+    with pytest.raises(ValueError):
+        cache.write(x[:T], held(T, H, D), table, start, queries=held(T, H, D), rotary=t, out=again)
+    # and rows side by side stay apart
+    q, k = _parts(held(T, 4 * D), 2, 2)
+    k = torch.from_dlpack(k.as_subclass(torch.Tensor)).as_subclass(OnGpu)
+    apply_rotary(rotary_table(D, device="cpu"), q, k, pos, out=(q, k))
+    b = blocks[-1]
+    assert (b.q, b.k) == (b.q_out, b.k_out) == (q.data_ptr(), k.data_ptr())
