@@ -155,11 +155,23 @@ def _writable(name: str, out: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
     return out
 
 
+_INT32 = (-2 ** 31, 2 ** 31 - 1)
+
+
 def _int32(name: str, value: Any, device, numel: int | None = None) -> torch.Tensor:
+    """``value`` as contiguous int32 on ``device``. What int32 cannot hold
+    becomes the nearest that it can: no page of a pool and no position of a
+    table (wrapped, it could be either)."""
     t = value if isinstance(value, torch.Tensor) else torch.as_tensor(value)
     if t.dtype is not torch.int32 or t.device != device or not t.is_contiguous():
         if t.numel() and (t.dtype is torch.bool or t.is_floating_point() or t.is_complex()):
             raise TypeError(f"{name} must hold integers (got {t.dtype})")
+        if t.dtype in (torch.int64, torch.uint32, torch.uint64):
+            top = t.dtype is torch.uint64
+            t = t.to(device=device, dtype=torch.int64)
+            if top:
+                t = torch.where(t < 0, _INT32[1], t)   # (2^63 and on came out negative)
+            t = t.clamp(*_INT32)
         t = t.to(device=device, dtype=torch.int32).contiguous()
     if numel is not None and t.numel() != numel:
         raise ValueError(f"{name} must hold {numel} values (got {t.numel()})")
@@ -215,9 +227,10 @@ def _apart(src: torch.Tensor, dst: torch.Tensor, in_place: bool = False) -> bool
 def apply_rotary(table: RotaryTable, queries: torch.Tensor, keys: torch.Tensor | None, positions: Any, *,
                  out: tuple | None = None):
     """Rotate ``queries`` [T, Hq, D] and ``keys`` [T, Hkv, D] (or None) bf16 at
-    ``positions`` [T] (int32; may stay on the GPU). Returns ``(queries, keys)``
-    rotated, in new tensors or in ``out`` (a pair; the inputs themselves for in
-    place). Views of a fused projection are read where they are."""
+    ``positions`` [T] (int32; may stay on the GPU, where a wider one counts as
+    the nearest that fits). Returns ``(queries, keys)`` rotated, in new tensors or
+    in ``out`` (a pair; the inputs themselves for in place). Views of a fused
+    projection are read, and written, where they are."""
     q, T, Hq, D, qt, qh = _rows("queries", queries)
     device = q.device
     k, Hkv, kt, kh = None, 0, 0, 0
@@ -230,6 +243,11 @@ def apply_rotary(table: RotaryTable, queries: torch.Tensor, keys: torch.Tensor |
         raise ValueError("queries have no heads")
     if D % 8 or D > 256 or table.dims > D:
         raise ValueError(f"head dim {D} must be a multiple of 8 up to 256 and hold the table's {table.dims} dims")
+    if not (isinstance(positions, torch.Tensor) and positions.is_cuda):
+        wide = torch.as_tensor(positions)
+        positions = _int32("positions", wide, wide.device)
+        if not torch.equal(positions.to(torch.int64), wide.to(torch.int64)):
+            raise ValueError("positions must fit int32")
     pos = _int32("positions", positions, device, T)
     _on(device, "table", table.phases)
     ko = None

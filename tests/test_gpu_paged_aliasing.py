@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 import torch
 
+from mtplx_amd._lib import MtpError
 from mtplx_amd.paged_attention import paged_sdpa
 from mtplx_amd.paged_kv_cache import PagedKVCache
 from mtplx_amd.rotary import apply_rotary, rotary_table
@@ -78,3 +79,28 @@ def test_write_and_attention_on_fused_rows(gpu):
     assert torch.equal(out, want) and torch.equal(q, turned)
     paged_sdpa(q, b, table, start, out=q)
     assert torch.equal(q, want)
+
+
+def test_wide_index_arrays_do_not_wrap(gpu):
+    """An int64 table on the GPU whose entries int32 cannot hold: no page of the
+    pool is written or read through them."""
+    rng = np.random.default_rng(34)
+    c = PagedKVCache(4, 1, 64, page_size=32)
+    x = rows(rng, 6, 1, 64)
+    for entry in (2 ** 32, 2 ** 32 + 3, -2 ** 32 + 1):
+        table = torch.tensor([[entry]], device="cuda")
+        c.write(x, x, table, i32([0]))
+        with pytest.raises(MtpError):
+            c.check_status()
+        assert not c.k_pages.any().item() and not c.v_pages.any().item()
+        assert (paged_sdpa(x, c, table, i32([0])) == 0).all()
+        with pytest.raises(MtpError):
+            c.check_status()
+    first = i32([[0]])
+    c.write(x, x, first, torch.tensor([2 ** 32], device="cuda"))   # not position 0
+    with pytest.raises(MtpError):
+        c.check_status()
+    assert not c.k_pages.any().item()
+    c.write(x, x, first, i32([0]), torch.tensor([0, 2 ** 32 + 2], device="cuda"))   # past the rows: all six
+    assert torch.equal(c.read(first, 6)[0][0, 0], x[:, 0])
+    assert torch.equal(c.read(first, 6, lengths=torch.tensor([2 ** 32], device="cuda"))[0][0, 0], x[:, 0])

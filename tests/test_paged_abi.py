@@ -170,3 +170,23 @@ def test_index_arrays_hold_integers():
     for bad in ([0.5], torch.ones(1), torch.ones(1, dtype=torch.bool)):
         with pytest.raises(TypeError):
             _int32("positions", bad, cpu)
+
+
+def test_index_arrays_past_32_bits():
+    """Entries that int32 cannot hold become the nearest it can, which is no page
+    and no position of any cache; they never wrap to one that is."""
+    from mtplx_amd.rotary import _int32
+
+    cpu, top, low = torch.device("cpu"), 2 ** 31 - 1, -2 ** 31
+    wide = [0, 5, -1, top, low, 2 ** 31, low - 1, 2 ** 32, 2 ** 32 + 3, -2 ** 32, 2 ** 63 - 1, -2 ** 63]
+    want = [0, 5, -1, top, low, top, low, top, top, low, top, low]
+    for value in (wide, torch.tensor(wide), torch.tensor(wide).view(2, 6).t()):
+        got = _int32("block_table", value, cpu)
+        assert got.dtype is torch.int32 and got.is_contiguous()
+        assert got.tolist() == (want if got.dim() == 1 else torch.tensor(want).view(2, 6).t().tolist())
+    assert _int32("block_table", torch.tensor([7, 2 ** 32 - 1], dtype=torch.uint32), cpu).tolist() == [7, top]
+    assert _int32("block_table", torch.tensor([7, 255], dtype=torch.uint8), cpu).tolist() == [7, 255]
+    big = torch.tensor([7, 2 ** 63 - 1, 2 ** 63 + 5, 2 ** 64 - 1], dtype=torch.uint64)
+    assert _int32("block_table", big, cpu).tolist() == [7, top, top, top]
+    same = torch.tensor([1, 2], dtype=torch.int32)
+    assert _int32("block_table", same, cpu) is same

@@ -138,3 +138,14 @@ def test_memory_shared_by_two_storages(blocks):
     apply_rotary(rotary_table(D, device="cpu"), q, k, pos, out=(q, k))
     b = blocks[-1]
     assert (b.q, b.k) == (b.q_out, b.k_out) == (q.data_ptr(), k.data_ptr())
+
+
+def test_positions_on_the_host_fit_32_bits(blocks):
+    t, x = rotary_table(D, device="cpu"), held(2, H, D)
+    for bad in ([0, 2 ** 31], [-2 ** 31 - 1, 0], torch.tensor([2 ** 32, 1]),
+                torch.tensor([2 ** 64 - 1, 1], dtype=torch.uint64)):
+        with pytest.raises(ValueError):
+            apply_rotary(t, x, None, bad)
+    assert not blocks
+    apply_rotary(t, x, None, [2 ** 31 - 1, -2 ** 31])
+    assert len(blocks) == 1
