@@ -90,7 +90,10 @@ class PagedKVCache:
 
     def check_status(self) -> None:
         """Raise :class:`MtpError` if a call since the last check met a position
-        without a page (synchronises with the device)."""
+        without a page. Waits for the device, so calls on every stream count;
+        one that another host thread makes meanwhile may go unseen."""
+        if self.device.type == "cuda":
+            torch.cuda.synchronize(self.device)
         if int(self._status.item()) != 0:
             self._status.zero_()
             raise _lib.MtpError("paged_kv_cache", -1, "a position without a page of the pool (status word set)")
