@@ -42,6 +42,8 @@
 #include "paged.hpp"
 #include "qmv_common.hpp"
 
+#include <float.h>
+
 #include <type_traits>
 
 namespace mtp {
@@ -332,6 +334,12 @@ __device__ __forceinline__ void soften(RowState<D>& s, f32x16 (&st)[KB], u32x4 (
     }
   top = max_halves(top);
   if (RAW) top *= scale_log2;
+  // A row that sees a key (of a block the first, then) has a finite maximum, so
+  // it ends with l = 0 and m finite where all its scores are -infinity: NaN.
+  bool sees = !MASK;
+#pragma unroll
+  for (int j = 0; j < KB; ++j) sees = sees || (kt + 32 * j <= s.bound && kt + 32 * j < end[j]);
+  if (sees) top = fmaxf(top, -FLT_MAX);
   if (__any(top > s.m + 8.f)) {
     // Only the rows that passed: the others' bits do not turn on their neighbours.
     const float m_new = top > s.m + 8.f ? top : s.m;
@@ -496,6 +504,9 @@ template <int D>
 __device__ __forceinline__ float4* part_block(const PAttn& p, size_t slot, int RT, int rb, int t) {
   return reinterpret_cast<float4*>(p.part_o) + ((slot * (RT / 32) + rb) * (D / 32) + t) * 256;
 }
+
+// What a row's sums are divided by, as a factor: a row that saw no key is zeros.
+__device__ __forceinline__ float row_factor(float m, float l) { return m == -INFINITY && l == 0.f ? 0.f : 1.f / l; }
 
 // 16 bytes read once per launch (non-temporal, as ld_stream).
 __device__ __forceinline__ u32x4 ld_nt(const void* p) {
@@ -847,7 +858,7 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
     const int ln = fresh(lane);
     if (starts && ends) {
       constexpr int LPR = D / 8, RB = row_bytes<D>();
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv = row_factor(s.m, l);
 #pragma unroll
       for (int t = 0; t < D / 32; ++t)
 #pragma unroll
@@ -1029,7 +1040,7 @@ __global__ __launch_bounds__(kPT, D == 256 ? 1 : 2) void attn_few_kernel(PAttn p
         ls += s_l[w][r] * c;
       }
       if (whole) {
-        const float inv = ls == 0.f ? 0.f : 1.f / ls;
+        const float inv = row_factor(m, ls);
         store4(out_row(p, rq.lo + u.tok, u.h, r + u.off) + d, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
       } else {
         part_block<D>(p, slot, RT, 0, 0)[e] = v;
@@ -1147,7 +1158,7 @@ __global__ __launch_bounds__(kPT) void attn_join_kernel(PAttn p) {
     v.z += __shfl_xor(v.z, off, 64);
     v.w += __shfl_xor(v.w, off, 64);
   }
-  const float l = s_l[row], inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = row_factor(s_m[row], s_l[row]);
   store4(&s_out[row][4 * (tid >> 5)], v.x * inv, v.y * inv, v.z * inv, v.w * inv);
   __syncthreads();
   if (tid >= 128) return;

@@ -1,0 +1,50 @@
+"""paged_sdpa where scores are infinite or weights nothing: what softmax over
+the keys that a row sees gives, at every place of a row's keys (blocks with and
+without a mask, pieces of one tile in several workgroups)."""
+
+import numpy as np
+import pytest
+import torch
+
+from mtplx_amd.paged_attention import paged_sdpa
+from mtplx_amd.paged_kv_cache import PagedKVCache
+from oracle import paged as O
+from tests.paged_util import attention_bound, check_rows, i32, num, rows, stored, tables
+
+pytestmark = pytest.mark.gpu
+
+SHAPES = [(1, 1), (3, 40), (4, 900), (40, 40), (90, 300), (70, 5000)]   # new tokens, keys
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("n,keys", SHAPES)
+def test_scores_of_minus_infinity(gpu, n, keys, D):
+    """Keys of score -infinity have weight 0; a row that sees no other is NaN, as
+    softmax is; a row that sees no key at all is zeros."""
+    rng = np.random.default_rng(n + keys + D)
+    H, Hq = 2, 4
+    for what in ("all", "first", "last", "most"):
+        table, pages = tables(rng, [keys], 64)
+        c = PagedKVCache(pages, H, D, page_size=64)
+        k, v, q = rows(rng, keys, H, D), rows(rng, keys, H, D), rows(rng, n, Hq, D)
+        gone = {"all": slice(0, keys), "first": slice(0, keys - (n + 1) // 2), "last": slice(keys - n // 2 - 1, keys),
+                "most": slice(0, max(keys - 1, 1))}[what]
+        q[..., 5] = 1.0
+        k[gone, :, 5] = float("-inf")
+        c.write(k, v, table, i32([0]))
+        o, spread = np.zeros((n, Hq, D)), np.zeros((n, Hq, D))
+        dead = np.zeros(n, bool)
+        kv = stored(c, table, 0, keys)
+        for i in range(n):   # over the keys whose score is finite
+            seen = np.arange(keys - n + i + 1)
+            seen = seen[(seen < gone.start) | (seen >= gone.stop)]
+            dead[i] = not len(seen)
+            if not dead[i]:
+                r = O.attend(num(q[i:i + 1]), *(x[:, seen] for x in kv), len(seen) - 1)
+                o[i], spread[i] = r[0][0], attention_bound(*r, D)[0]
+        for kw in (dict(), dict(row_off=i32([0, n]))):
+            got = num(paged_sdpa(q, c, table, i32([keys - n]), **kw))
+            check_rows(got[~dead], o[~dead], spread[~dead], f"{what} {kw}")
+            assert np.isnan(got[dead]).all(), f"{what} {kw}"
+        assert (num(paged_sdpa(q, c, table, i32([-n]))) == 0).all()
+        assert (num(paged_sdpa(q, c, torch.full_like(table, -1), i32([keys - n]))) == 0).all()
