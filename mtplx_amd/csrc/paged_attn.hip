@@ -318,6 +318,10 @@ __device__ __forceinline__ void soften(RowState<D>& s, f32x16 (&st)[KB], u32x4 (
   // 16 bits without a mask: the maximum is taken before the scale (positive),
   // and scale and maximum go into one FMA.
   constexpr bool RAW = BITS == 16 && !MASK;
+  auto hidden = [&](int j, int r) {
+    const int key = kt + 32 * j + 8 * (r >> 2) + 4 * h2 + (r & 3);
+    return key > s.bound || key >= end[j];
+  };
   float top = -INFINITY;
 #pragma unroll
   for (int j = 0; j < KB; ++j)
@@ -325,10 +329,7 @@ __device__ __forceinline__ void soften(RowState<D>& s, f32x16 (&st)[KB], u32x4 (
     for (int r = 0; r < 16; ++r) {
       float x = st[j][r];
       if (!RAW) x *= BITS == 8 ? ks(j, r) : scale_log2;
-      if (MASK) {
-        const int key = kt + 32 * j + 8 * (r >> 2) + 4 * h2 + (r & 3);
-        x = key <= s.bound && key < end[j] ? x : -INFINITY;
-      }
+      if (MASK && hidden(j, r)) x = -INFINITY;
       st[j][r] = x;
       top = __builtin_elementwise_maximum(top, x);   // (no quieting of each x; a NaN makes its row NaN)
     }
@@ -366,8 +367,8 @@ __device__ __forceinline__ void soften(RowState<D>& s, f32x16 (&st)[KB], u32x4 (
       sum += a + b;
       if (BITS == 8) {
         const float va = vs(j, r), vb = vs(j, r + 1);
-        a = MASK && a == 0.f ? 0.f : a * va;   // a hidden key's scale may be NaN
-        b = MASK && b == 0.f ? 0.f : b * vb;
+        a = MASK && hidden(j, r) ? 0.f : a * va;   // (a hidden key's scale may be NaN; of one that is seen it shows)
+        b = MASK && hidden(j, r + 1) ? 0.f : b * vb;
       }
       pk[r / 2] = f2bf2(a, b);
     }

@@ -48,3 +48,28 @@ def test_scores_of_minus_infinity(gpu, n, keys, D):
             assert np.isnan(got[dead]).all(), f"{what} {kw}"
         assert (num(paged_sdpa(q, c, table, i32([-n]))) == 0).all()
         assert (num(paged_sdpa(q, c, torch.full_like(table, -1), i32([keys - n]))) == 0).all()
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("n,keys,D", [(4, 140, 128), (40, 140, 128), (70, 300, 64), (40, 140, 256), (4, 140, 256)])
+def test_a_value_that_is_no_number_at_a_weight_of_nothing(gpu, n, keys, D, bits):
+    """NaN in a value whose key's weight underflows: the rows that see it show it
+    (0 times NaN), wherever it lies; those before it keep their bits."""
+    rng = np.random.default_rng(n + D + bits)
+    table, pages = tables(rng, [keys], 64)
+    k, v, q = rows(rng, keys, 1, D, scale=0.1), rows(rng, keys, 1, D), rows(rng, n, 2, D, scale=0.1) + 2
+    for at in (5, 70, keys - n + 1, keys - 2, keys - 1):
+        kk, vv, plain = k.clone(), v.clone(), []
+        kk[at] = -400.0   # scores of -6400 and less
+        for value in (0.0, float("nan")):
+            vv[at, 0, 3] = value
+            c = PagedKVCache(pages, 1, D, page_size=64, bits=bits)
+            c.write(kk, vv, table, i32([0]))
+            for kw in (dict(), dict(row_off=i32([0, n]))):
+                plain.append(num(paged_sdpa(q, c, table, i32([keys - n]), **kw)))
+        first = max(at - (keys - n), 0)
+        for good, got in zip(plain[:2], plain[2:]):
+            assert np.isfinite(good).all() and np.array_equal(got[:first], good[:first])
+            assert np.isnan(got[first:, :, 3]).all(), at
+            if bits == 8:
+                assert np.isnan(got[first:]).all()
