@@ -53,11 +53,10 @@ def paged_sdpa(queries: torch.Tensor, cache: PagedKVCache, block_table: Any, q_s
         out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=device)
         ot, oh = Hq * D, D
     else:
-        out = _writable("out", out, queries)
+        out, ot, oh = _writable("out", out, queries)
         if not _apart(q, out):
             q = q.clone(memory_format=torch.contiguous_format)
             qt, qh = Hq * D, D
-        ot, oh = out.stride()[:2]
     if T == 0:
         return out
     rows = T // B if off is None else 0 if max_rows is None else min(max(0, int(max_rows)), T)

@@ -164,14 +164,13 @@ class PagedKVCache:
                 qo = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=device)
                 qot, qoh = Hq * D, D
             else:
-                qo = _writable("out", out, queries)
+                qo, qot, qoh = _writable("out", out, queries)
                 for name, x in (("keys", k), ("values", v)):
                     if not _apart(x, qo):
                         raise ValueError(f"out overlaps {name}")
                 if not _apart(q, qo, rotary.traditional or rotary.dims % 16 == 0):
                     q = q.clone(memory_format=torch.contiguous_format)
                     qt, qh = Hq * D, D
-                qot, qoh = qo.stride()[:2]
         if T == 0:
             return qo
         a = self._block(_lib.PagedWriteArgs)

@@ -142,17 +142,21 @@ def _rows(name: str, x: torch.Tensor, heads: int | None = None, dim: int | None 
     return x, T, H, D, t, h
 
 
-def _readable(x: torch.Tensor) -> bool:
-    t, h, d = x.stride()
-    return d == 1 and t >= 0 and t % 8 == 0 and h % 8 == 0 and h >= x.shape[2] and x.data_ptr() % 16 == 0
-
-
-def _writable(name: str, out: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
+def _writable(name: str, out: torch.Tensor, like: torch.Tensor):
+    """``(out, token stride, head stride)`` of an output for the rows of ``like``:
+    16-byte aligned rows that do not overlap, tokens or heads outermost."""
     if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
         raise ValueError(f"{name} must be {list(like.shape)} {like.dtype} on {like.device}")
-    if not _readable(out) or out.stride(0) < out.stride(1) * (out.shape[1] - 1) + out.shape[2]:
+    T, H, D = out.shape
+    t, h, d = out.stride()
+    if H < 2:   # (a single one's stride is anything)
+        h = D
+    if T < 2:
+        t = H * h
+    apart = h >= D and t >= h * (H - 1) + D or t >= D and h >= t * (T - 1) + D
+    if d != 1 or t & 7 or h & 7 or out.data_ptr() & 15 or not apart:
         raise ValueError(f"{name} must have 16-byte aligned rows that do not overlap")
-    return out
+    return out, t, h
 
 
 _INT32 = (-2 ** 31, 2 ** 31 - 1)
@@ -258,8 +262,10 @@ def apply_rotary(table: RotaryTable, queries: torch.Tensor, keys: torch.Tensor |
             ko = torch.empty((T, Hkv, D), dtype=torch.bfloat16, device=device)
         kot, koh = Hkv * D, D
     else:
-        qo = _writable("out[0]", out[0], queries)
-        ko = None if k is None else _writable("out[1]", out[1], keys)
+        qo, qot, qoh = _writable("out[0]", out[0], queries)
+        kot = koh = 0
+        if k is not None:
+            ko, kot, koh = _writable("out[1]", out[1], keys)
         # An item of the kernel reads what it stores, unless the halves are no whole chunks; heads go in no order.
         in_place = table.traditional or table.dims % 16 == 0
         if not _apart(q, qo, in_place) or (ko is not None and not _apart(q, ko)):
@@ -270,8 +276,6 @@ def apply_rotary(table: RotaryTable, queries: torch.Tensor, keys: torch.Tensor |
             kt, kh = Hkv * D, D
         if ko is not None and _overlaps(qo, ko) and not _interleaved(qo, ko):
             raise ValueError("the two outputs overlap")
-        qot, qoh = qo.stride()[:2]
-        kot, koh = (0, 0) if ko is None else ko.stride()[:2]
     if T == 0:
         return qo, ko
     if not Hkv:

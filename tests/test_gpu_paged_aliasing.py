@@ -104,3 +104,27 @@ def test_wide_index_arrays_do_not_wrap(gpu):
     c.write(x, x, first, i32([0]), torch.tensor([0, 2 ** 32 + 2], device="cuda"))   # past the rows: all six
     assert torch.equal(c.read(first, 6)[0][0, 0], x[:, 0])
     assert torch.equal(c.read(first, 6, lengths=torch.tensor([2 ** 32], device="cuda"))[0][0, 0], x[:, 0])
+
+
+@pytest.mark.parametrize("n", [1, 4, 90])
+def test_outputs_with_heads_outside_tokens(gpu, n):
+    rng = np.random.default_rng(35)
+    Hq, H, D, keys = 8, 2, 64, 200
+    table, pages = tables(rng, [keys], 32)
+    c = PagedKVCache(pages, H, D, page_size=32)
+    old = rows(rng, keys, H, D)
+    c.write(old, old, table, i32([0]))
+    rope, start, pos = rotary_table(D, base=1e4), i32([keys - n]), i32(np.arange(keys - n, keys))
+    q, k = rows(rng, n, Hq, D), rows(rng, n, H, D)
+    out = lambda: torch.full((Hq, n + 1, D), 3.0, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    for call in (lambda **kw: apply_rotary(rope, q, None, pos, **{a: (b, None) for a, b in kw.items()})[0],
+                 lambda **kw: c.write(k, k, table, start, queries=q, rotary=rope, **kw),
+                 lambda **kw: paged_sdpa(q, c, table, start, **kw),
+                 lambda **kw: paged_sdpa(q, c, table, start, i32([0, n]), **kw)):
+        want, buf = call(), out()
+        got = call(out=buf[:, :n].transpose(0, 1))
+        assert torch.equal(got, want) and torch.equal(buf[:, :n], want.transpose(0, 1)) and (buf[:, n] == 3).all()
+    turned = q.transpose(0, 1).contiguous().transpose(0, 1)
+    want = apply_rotary(rope, q, None, pos)[0]
+    apply_rotary(rope, turned, None, pos, out=(turned, None))
+    assert torch.equal(turned, want)

@@ -149,3 +149,36 @@ def test_positions_on_the_host_fit_32_bits(blocks):
     assert not blocks
     apply_rotary(t, x, None, [2 ** 31 - 1, -2 ** 31])
     assert len(blocks) == 1
+
+
+def test_outputs_in_any_order_of_tokens_and_heads(blocks):
+    """Rows that do not overlap are written where they lie: heads outside tokens,
+    padded rows, a single token or head with any stride."""
+    t, pos = rotary_table(D, device="cpu"), torch.arange(T)
+    cache = paged_kv_cache.PagedKVCache(1, H, D, device="cpu")
+    table, start = torch.zeros((1, 1), dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    x, kv = held(T, H, D), held(T, H, D)
+    outs = [(held(H, T, D).transpose(0, 1), (D, T * D)), (held(H, T, 2 * D)[..., :D].transpose(0, 1), (2 * D, 2 * T * D)),
+            (held(T, 3 * H, D)[:, ::3], (3 * H * D, 3 * D)), (held(T, H, D), (H * D, D))]
+    for out, strides in outs:
+        assert apply_rotary(t, x, None, pos, out=(out, None))[0] is out
+        assert (blocks[-1].qo_token, blocks[-1].qo_head) == strides
+        assert cache.write(kv, kv, table, start, queries=x, rotary=t, out=out) is out
+        assert (blocks[-1].qo_token, blocks[-1].qo_head) == strides
+        assert paged_attention.paged_sdpa(x, cache, table, start, out=out) is out
+        assert (blocks[-1].out_token, blocks[-1].out_head) == strides
+    for n, h in ((1, H), (T, 1), (1, 1)):   # strides of a single token or head are never used
+        out = held(T, H, D)[:n, :h].as_strided((n, h, D), (H * D if n > 1 else 3, D if h > 1 else 5, 1))
+        y = held(n, h, D)
+        assert apply_rotary(t, y, None, pos[:n], out=(out, None))[0] is out
+        b = blocks[-1]
+        assert b.q_out == out.data_ptr() and b.qo_token % 8 == b.qo_head % 8 == 0 and b.qo_head >= D
+    made = len(blocks)
+    room = held(4 * T * H * D)
+    for strides in ((D, D, 1), (D // 2, T * D, 1), (H * D, D // 2, 1), (D, (T - 1) * D, 1), ((H - 1) * D, D, 1), (0, D, 1),
+                    (H * D, 0, 1), (H * D + 4, D, 1), (2 * H * D, 2 * D, 2)):
+        with pytest.raises(ValueError):
+            apply_rotary(t, x, None, pos, out=(room.as_strided((T, H, D), strides), None))
+    with pytest.raises(ValueError):
+        apply_rotary(t, x, None, pos, out=(room[1:].as_strided((T, H, D), (H * D, D, 1)), None))
+    assert len(blocks) == made
