@@ -80,7 +80,7 @@ def rotary_frequencies(dims: int, *, base: float = 10000.0, scale: float = 1.0, 
                          "factor >= 1")
 
     def pair_of(turns: float) -> float:   # index (in dims / 2 pairs) of the pair that makes so many turns
-        return dims * math.log(trained_positions / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
+        return dims * math.log(scale * trained_positions / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
 
     low, high = max(math.floor(pair_of(fast_turns)), 0), min(math.ceil(pair_of(slow_turns)), dims - 1)
     for i, f in enumerate(freqs):

@@ -190,3 +190,14 @@ def test_index_arrays_past_32_bits():
     assert _int32("block_table", big, cpu).tolist() == [7, top, top, top]
     same = torch.tensor([1, 2], dtype=torch.int32)
     assert _int32("block_table", same, cpu) is same
+
+
+def test_yarn_counts_the_turns_that_scaled_positions_make():
+    kw = dict(base=1e6, scaling="yarn", factor=8.0, trained_positions=32768)
+    y, _ = rotary_frequencies(128, scale=0.125, **kw)
+    plain, _ = rotary_frequencies(128, base=1e6, scale=0.125)
+    turns = np.array(plain) * 32768 / (2 * math.pi)
+    ratio = np.array(y) / np.array(plain)
+    # one pair's step is a factor of 1e6^(1/64) = 1.24: whole pairs to either side of 32 and 1 turns
+    assert np.allclose(ratio[turns > 40], 1.0) and np.allclose(ratio[turns < 0.8], 0.125)
+    assert (ratio[(turns < 25) & (turns > 1.3)] < 1.0).all() and (ratio[(turns < 25) & (turns > 1.3)] > 0.125).all()
