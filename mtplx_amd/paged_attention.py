@@ -17,6 +17,7 @@ from typing import Any
 import torch
 
 from . import _lib
+from .attention_context import exact_verify_required
 from .paged_kv_cache import PagedKVCache
 from .rotary import _apart, _call, _on, _rows, _stream, _writable
 
@@ -36,7 +37,12 @@ def paged_sdpa(queries: torch.Tensor, cache: PagedKVCache, block_table: Any, q_s
     Rows past ``row_off[B]`` are not written, so they keep what ``out`` held
     (without ``out``: undefined). Rows that see no key are zeros;
     positions without a page count as absent and set ``cache.status()``.
-    ``scale`` is positive; default ``1 / sqrt(D)``."""
+    ``scale`` is positive; default ``1 / sqrt(D)``. Refused inside
+    ``exact_verify(True)``: how a row's sums are split depends on the lengths of
+    the call's other requests."""
+    if exact_verify_required():
+        raise RuntimeError("paged_sdpa: a row's bits depend on the call's other requests, which a forward inside "
+                           "exact_verify(True) must not (MTPLX_EXACT_T0_GUARD=0 disarms the guard)")
     q, T, Hq, D, qt, qh = _rows("queries", queries, None, cache.head_dim)
     Hkv = cache.n_kv_heads
     if Hq % Hkv or not 1 <= Hq // Hkv <= 32:

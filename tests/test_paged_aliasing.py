@@ -182,3 +182,24 @@ def test_outputs_in_any_order_of_tokens_and_heads(blocks):
     with pytest.raises(ValueError):
         apply_rotary(t, x, None, pos, out=(room[1:].as_strided((T, H, D), (H * D, D, 1)), None))
     assert len(blocks) == made
+
+
+def test_attention_is_refused_where_bits_may_not_depend_on_the_batch(blocks, monkeypatch):
+    """A forward inside exact_verify(True) must give a row the same bits in any
+    batch; paged_sdpa splits by the lengths of all its requests."""
+    from mtplx_amd.attention_context import exact_verify
+
+    monkeypatch.delenv("MTPLX_EXACT_T0_GUARD", raising=False)
+    cache = paged_kv_cache.PagedKVCache(1, H, D, device="cpu")
+    table, start, x = torch.zeros((1, 1), dtype=torch.int32), torch.zeros(1, dtype=torch.int32), held(T, H, D)
+    with exact_verify(True):
+        with pytest.raises(RuntimeError, match="exact_verify"):
+            paged_attention.paged_sdpa(x, cache, table, start)
+        assert not blocks
+        cache.write(x, x, table, start)   # (a row's own values alone)
+        apply_rotary(rotary_table(D, device="cpu"), x, None, torch.arange(T))
+        monkeypatch.setenv("MTPLX_EXACT_T0_GUARD", "0")
+        paged_attention.paged_sdpa(x, cache, table, start)
+    with exact_verify(False):
+        paged_attention.paged_sdpa(x, cache, table, start)
+    assert len(blocks) == 4
