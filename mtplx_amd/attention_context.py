@@ -39,7 +39,7 @@ def exact_t0_guard_armed() -> bool:
 
 def exact_verify_required() -> bool:
     """True inside ``exact_verify(True)`` while the guard is armed."""
-    return exact_t0_guard_armed() and bool(_EXACT_VERIFY_REQUIRED.get())
+    return bool(_EXACT_VERIFY_REQUIRED.get()) and exact_t0_guard_armed()
 
 
 @contextmanager
