@@ -35,8 +35,10 @@ def paged_sdpa(queries: torch.Tensor, cache: PagedKVCache, block_table: Any, q_s
     first, then attend). ``max_rows``: the longest request's rows, if known;
     calls of few rows then take the kernel for them (``row_off`` None: known).
     Rows past ``row_off[B]`` are not written, so they keep what ``out`` held
-    (without ``out``: undefined). Rows that see no key are zeros;
-    positions without a page count as absent and set ``cache.status()``.
+    (without ``out``: undefined). Rows that see no key are zeros; positions of
+    the table without a page count as absent and set ``cache.status()``. A token
+    at or past the table's end (``width * page_size``) sees the positions that the
+    table has and sets nothing here: its ``write`` did.
     ``scale`` is positive; default ``1 / sqrt(D)``. Refused inside
     ``exact_verify(True)``: how a row's sums are split depends on the lengths of
     the call's other requests."""
