@@ -318,10 +318,10 @@ __device__ __forceinline__ void soften(RowState<D>& s, f32x16 (&st)[KB], u32x4 (
   // 16 bits without a mask: the maximum is taken before the scale (positive),
   // and scale and maximum go into one FMA.
   constexpr bool RAW = BITS == 16 && !MASK;
-  auto hidden = [&](int j, int r) {
-    const int key = kt + 32 * j + 8 * (r >> 2) + 4 * h2 + (r & 3);
-    return key > s.bound || key >= end[j];
-  };
+  int last[KB];   // the last key of block j that the row sees, from the block's first on (negative: none)
+#pragma unroll
+  for (int j = 0; j < KB; ++j) last[j] = MASK ? (s.bound < end[j] ? s.bound : end[j] - 1) - kt - 32 * j : 0;
+  auto hidden = [&](int j, int r) { return 8 * (r >> 2) + (r & 3) > last[j] - 4 * h2; };
   float top = -INFINITY;
 #pragma unroll
   for (int j = 0; j < KB; ++j)
@@ -339,7 +339,7 @@ __device__ __forceinline__ void soften(RowState<D>& s, f32x16 (&st)[KB], u32x4 (
   // it ends with l = 0 and m finite where all its scores are -infinity: NaN.
   bool sees = !MASK;
 #pragma unroll
-  for (int j = 0; j < KB; ++j) sees = sees || (kt + 32 * j <= s.bound && kt + 32 * j < end[j]);
+  for (int j = 0; j < KB; ++j) sees = sees || last[j] >= 0;
   if (sees) top = fmaxf(top, -FLT_MAX);
   if (__any(top > s.m + 8.f)) {
     // Only the rows that passed: the others' bits do not turn on their neighbours.
@@ -893,7 +893,7 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
 // -- few rows: one tile of 32 rows, the four waves share a piece by keys ---------
 
 // Blocks go straight from the pages into a wave's registers, the next one asked
-// for as soon as this one's operands are used up (RING 1). Two workgroups a CU
+// for as soon as this one's operands are used up. Two workgroups a CU
 // where their registers allow (D < 256): sixteen requests' verify rows at 8 bits
 // take 120 us, with one 149.
 template <int D, int BITS>
@@ -902,7 +902,6 @@ __global__ __launch_bounds__(kPT, D == 256 ? 1 : 2) void attn_few_kernel(PAttn p
   constexpr int BE = kBlk * D;
   constexpr int LD = D / 16 * (BITS / 8) / 2;   // 16-byte loads of a lane per block
   constexpr int OS = D + 4;                     // padded row: lanes of one store hit distinct banks
-  constexpr int RING = 1;
   __shared__ __attribute__((aligned(16))) float s_o[4][32 * OS];
   __shared__ float s_m[4][32], s_l[4][32];
   const int tid = threadIdx.x, lane = tid & 63, c32 = lane & 31, h2 = lane >> 5;
@@ -935,77 +934,66 @@ __global__ __launch_bounds__(kPT, D == 256 ? 1 : 2) void attn_few_kernel(PAttn p
     const int b0 = (ka >> 5) + nblk * wave / 4, b1 = (ka >> 5) + nblk * (wave + 1) / 4;   // the wave's blocks
     BlockList blocks;
     if (b0 < b1) blocks.fill(p, b, u.h, b0, b1, lane);
-    u32x4 kr[RING][LD], vr[RING][LD];
-    float sc[RING];   // 8 bits: lane l's key's scale, of K (l < 32) and of V
-    auto load = [&](int slot, int blk) {
+    u32x4 kr[LD], vr[LD];
+    float sc = 0.f;   // 8 bits: lane l's key's scale, of K (l < 32) and of V
+    auto load = [&](int blk) {
       const size_t o = (size_t)blocks.get(blk < b1 ? blk : b1 - 1) * BE;   // (past the last: the last again, never used)
       const unsigned char* k = p.k_pages + o * (BITS / 8);
       const unsigned char* v = p.v_pages + o * (BITS / 8);
 #pragma unroll
-      for (int i = 0; i < LD; ++i) kr[slot][i] = ld_nt(k + (uint32_t)(i * 1024 + lane * 16));
+      for (int i = 0; i < LD; ++i) kr[i] = ld_nt(k + (uint32_t)(i * 1024 + lane * 16));
 #pragma unroll
-      for (int i = 0; i < LD; ++i) vr[slot][i] = ld_nt(v + (uint32_t)(i * 1024 + lane * 16));
-      if constexpr (BITS == 8) sc[slot] = (h2 ? p.v_scales : p.k_scales)[o / D + c32];
+      for (int i = 0; i < LD; ++i) vr[i] = ld_nt(v + (uint32_t)(i * 1024 + lane * 16));
+      if constexpr (BITS == 8) sc = (h2 ? p.v_scales : p.k_scales)[o / D + c32];
     };
-    if (b0 < b1) {
-#pragma unroll
-      for (int i = 0; i < RING; ++i) load(i, b0 + i);
-    }
+    if (b0 < b1) load(b0);
     RowState<D> s;
     __syncthreads();   // the previous piece's reads of s_o are done
     take_rows<D>(s, q, p, u, 0, lane, reinterpret_cast<unsigned char*>(s_o[wave]));
     float* const scales = s_o[wave];   // 8 bits: a block's scales, on their way to the lanes that need them
-    auto block = [&](int slot, int blk, auto mask) {
+    auto block = [&](int blk, auto mask) {
       constexpr bool MASK = decltype(mask)::value;
       const int kt = 32 * blk;
-      if constexpr (BITS == 8) scales[lane] = h2 ? sc[slot] : sc[slot] * p.scale_log2;
+      if constexpr (BITS == 8) scales[lane] = h2 ? sc : sc * p.scale_log2;
       auto scale = [&](int r) { return scales[8 * (r >> 2) + 4 * h2 + (r & 3)]; };
       f32x16 st[1];
       u32x4 w[1][2];
       const int end1[1] = {u.nk};
       scores<D, 1>(s, st, [&](int, int i) {
-        if constexpr (BITS == 16) return kr[slot][i];
-        else return (i & 1) ? widen8(kr[slot][i >> 1].z, kr[slot][i >> 1].w) : widen8(kr[slot][i >> 1].x, kr[slot][i >> 1].y);
+        if constexpr (BITS == 16) return kr[i];
+        else return (i & 1) ? widen8(kr[i >> 1].z, kr[i >> 1].w) : widen8(kr[i >> 1].x, kr[i >> 1].y);
       });
       soften<D, BITS, 1, MASK>(
           s, st, w, kt, end1, h2, p.scale_log2, [&](int, int r) { return scale(r); },
           [&](int, int r) { return scale(r + 16); });
       if (BITS == 8) __builtin_amdgcn_sched_barrier(0);   // (V's integers are not widened before their turn)
       add_values<D, BITS, MASK>(s, w[0], kt, u.nk, h2, [&](int t, int jj) {
-        if constexpr (BITS == 16) return vr[slot][2 * t + jj];
-        else return jj ? widen8(vr[slot][t].z, vr[slot][t].w) : widen8(vr[slot][t].x, vr[slot][t].y);
+        if constexpr (BITS == 16) return vr[2 * t + jj];
+        else return jj ? widen8(vr[t].z, vr[t].w) : widen8(vr[t].x, vr[t].y);
       });
     };
-    auto next = [&](int slot, int blk) {   // block blk + RING into the slot that blk leaves
-      if (blk + RING >= blocks.first + 64 && blk + RING < b1) blocks.fill(p, b, u.h, blk + 1, b1, lane);
-      load(slot, blk + RING);
+    auto next = [&](int blk) {   // the block after blk, in its place
+      if (blk + 1 >= blocks.first + 64 && blk + 1 < b1) blocks.fill(p, b, u.h, blk + 1, b1, lane);
+      load(blk + 1);
     };
     // Blocks [b0, bf) hide no key and have their pages.
     int bf = wmin + 1 >= 0 ? (int)((wmin + 1) >> 5) : 0;
     if (bf > b1) bf = b1;
     int blk = b0;
     while (blk < b1) {
-      // As far as this list knows; RING at a time, so each stays in its registers.
+      // As far as this list knows.
       int to = blocks.first + blocks.present();
       if (to > bf) to = bf;
 #pragma unroll 1
-      for (; blk + RING <= to; blk += RING) {
-#pragma unroll
-        for (int i = 0; i < RING; ++i) {
-          block(i, blk + i, std::false_type());
-          next(i, blk + i);
-        }
+      for (; blk < to; ++blk) {
+        block(blk, std::false_type());
+        next(blk);
         to = blocks.first + blocks.present() < bf ? blocks.first + blocks.present() : bf;
       }
       if (blk >= b1) break;
-#pragma unroll
-      for (int i = 0; i < RING; ++i) {
-        if (blk + i < b1) {
-          if (!blocks.absent(blk + i)) block(i, blk + i, std::true_type());
-          next(i, blk + i);
-        }
-      }
-      blk += RING;
+      if (!blocks.absent(blk)) block(blk, std::true_type());
+      next(blk);
+      ++blk;
     }
     // The waves' parts, in wave order.
     const float l = s.l + __shfl_xor(s.l, 32, 64);
