@@ -141,3 +141,29 @@ def test_pages_past_32_bit_offsets(gpu, bits):
         want = paged_sdpa(q, small, tables[1], i32([1000 - n]))
         assert torch.isfinite(want).all() and torch.equal(paged_sdpa(q, big, tables[0], i32([1000 - n])), want)
     big.check_status()
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_hints_that_are_wrong(gpu, bits):
+    """max_rows below or above the longest request: the same rows stored, the
+    same attention within its bound."""
+    rng = np.random.default_rng(80 + bits)
+    n, lengths, Hq, H, D = [300, 1, 40], [900, 200, 40], 8, 2, 128
+    c = _pool(rng, 900, D, H, 64, bits)
+    used = [-(-e // 64) for e in lengths]
+    t = np.full((3, max(used)), -1, np.int32)
+    for b, u in enumerate(used):
+        t[b, :u] = rng.permutation(c.num_pages)[:u]
+    table, off = torch.from_numpy(t).cuda(), i32([0, 300, 301, 341])
+    start = i32([e - m for m, e in zip(n, lengths)])
+    q = rows(rng, 341, Hq, D, scale=0.2)
+    for hint in (1, 2, 4, 7, 299, 5000, 0, -3, None):
+        _check(c, table, q, n, lengths, paged_sdpa(q, c, table, start, off, max_rows=hint), 17)
+    pools = [PagedKVCache(c.num_pages * 3, H, D, page_size=64, bits=bits) for _ in range(3)]
+    apart = (table + i32([[0], [c.num_pages], [2 * c.num_pages]])).masked_fill(table < 0, -1).int()
+    k, v = rows(rng, 341, H, D), rows(rng, 341, H, D)
+    for p, hint in zip(pools, (300, 1, 9000)):
+        p.write(k, v, apart, start, off, max_rows=hint)
+        p.check_status()
+        assert torch.equal(p.k_pages, pools[0].k_pages) and torch.equal(p.v_pages, pools[0].v_pages)
+    c.check_status()
