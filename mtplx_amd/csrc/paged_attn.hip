@@ -318,10 +318,11 @@ __device__ __forceinline__ void soften(RowState<D>& s, f32x16 (&st)[KB], u32x4 (
   // 16 bits without a mask: the maximum is taken before the scale (positive),
   // and scale and maximum go into one FMA.
   constexpr bool RAW = BITS == 16 && !MASK;
-  int last[KB];   // the last key of block j that the row sees, from the block's first on (negative: none)
-#pragma unroll
-  for (int j = 0; j < KB; ++j) last[j] = MASK ? (s.bound < end[j] ? s.bound : end[j] - 1) - kt - 32 * j : 0;
-  auto hidden = [&](int j, int r) { return 8 * (r >> 2) + (r & 3) > last[j] - 4 * h2; };
+  const int bound = s.bound - kt;
+  auto hidden = [&](int j, int r) {   // (one comparison of a constant with what block j's registers share)
+    const int last = (bound < end[j] - 1 - kt ? bound : end[j] - 1 - kt) - 32 * j - 4 * h2;
+    return 8 * (r >> 2) + (r & 3) > last;
+  };
   float top = -INFINITY;
 #pragma unroll
   for (int j = 0; j < KB; ++j)
@@ -339,7 +340,7 @@ __device__ __forceinline__ void soften(RowState<D>& s, f32x16 (&st)[KB], u32x4 (
   // it ends with l = 0 and m finite where all its scores are -infinity: NaN.
   bool sees = !MASK;
 #pragma unroll
-  for (int j = 0; j < KB; ++j) sees = sees || last[j] >= 0;
+  for (int j = 0; j < KB; ++j) sees = sees || (kt + 32 * j <= s.bound && kt + 32 * j < end[j]);
   if (sees) top = fmaxf(top, -FLT_MAX);
   if (__any(top > s.m + 8.f)) {
     // Only the rows that passed: the others' bits do not turn on their neighbours.
