@@ -31,14 +31,17 @@
 //
 // What bounds it, on an MI355X (5.17 TB/s a large copy, 1350 TFLOP/s a large
 // bf16 product), 40 query heads over 8 kv heads of 128:
-//   sixteen requests' four verify rows up to 32k, 8 bits: 124 us, the pages at
+//   sixteen requests' four verify rows up to 32k, 8 bits: 122 us, the pages at
 //     the rate of the copy;
-//   a chunk of 512 over 16k: 184 us, 890 TFLOP/s of what the mask leaves; whole
-//     prompts of 4096: 510 us, 745 (diagonal blocks are computed whole). The
+//   a chunk of 512 over 16k: 190 us, 890 TFLOP/s of what the mask leaves; whole
+//     prompts of 4096: 519 us, 730 (diagonal blocks are computed whole). The
 //     softmax's instructions (an exponential, a product, a maximum, a sum and
 //     half a conversion a score) take as many cycles of a SIMD as the MFMAs,
-//     and the two waves of a SIMD take them in turn;
-//   one token over 4k: 17.6 us, two launches and a chain of dependent loads.
+//     and the two waves of a SIMD take them in turn: in the chunk the matrix
+//     pipes are busy 50% of the CUs' busy cycles, vector issue 49%;
+//   head dim 64: the chunk 117 us, the verify rows 76; head dim 256: 1377 (16
+//     bits: registers spill inside the step) and 531 (8 bits), the verify rows 230;
+//   one token over 4k: 17.7 us, of which the two launches' kernels are 12 and 5.
 #include "paged.hpp"
 #include "qmv_common.hpp"
 

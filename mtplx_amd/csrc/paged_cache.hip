@@ -4,7 +4,7 @@
 //
 //   rotation of 8192 tokens, 40 + 8 heads of 128: 46 us (201 MB, 4.4 TB/s);
 //   write of the same at 8 bits, queries rotated: 58 us (218 MB, 3.8 TB/s);
-//   its read back: 11 us (50 MB); eight requests' prefixes: 73 us (349 MB, 4.8).
+//   its read back: 11 us (50 MB); eight requests' prefixes: 74 us (349 MB, 4.7).
 //
 // Writes and reads go by blocks of 32 positions of one head. A wave has a block
 // to itself (writes: K or V of it, reads both): 8 or 16 KB of loads are under
