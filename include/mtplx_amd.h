@@ -578,10 +578,11 @@ int mtp_rotary(const mtp_rotary_args* args, void* stream);
  * mtp_paged_attn: q, out [T, Hq, D]; out = softmax(scale q k^T) v over
  * positions 0 .. own; a row that sees no key is zeros, one whose scores are all
  * -infinity NaN. A row at or past width * page_size sees the positions that the
- * table has and does not set the status. max_rows as above,
- * it chooses the kernel (at most 32 query rows per kv head and request, or
- * more) and not the result's meaning. A row's result depends on no key behind
- * its own position, whatever its page holds. Hq = 1 to 32 times Hkv. */
+ * table has and does not set the status. A row's result depends on no key
+ * behind its own position, whatever its page holds. Sums are normalised at the
+ * end: finite while the largest |v| times the keys stays below 2^120. max_rows
+ * as above, it chooses the kernel (at most 32 query rows per kv head and
+ * request, or more) and not the result's meaning. Hq = 1 to 32 times Hkv. */
 typedef struct mtp_paged_write_args {
   const void* k;
   const void* v;

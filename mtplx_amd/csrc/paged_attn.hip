@@ -6,8 +6,9 @@
 // in one pass over the keys with the running maximum m and sum l of each row:
 // a block of scores s gives p = 2^(s log2e scale - m), l += sum p, o += p v.
 // m moves only when a block's maximum passes it by 8 (then o and l are scaled
-// by 2^(old - new)): p stays below 2^8 and fp32 carries the rest, and most
-// blocks cost no pass over o.
+// by 2^(old - new)): p stays below 2^8 and fp32 carries the rest (sums are finite
+// while the largest |v| times the keys stays below 2^120), and most blocks cost
+// no pass over o.
 //
 // The query rows of the heads that share a kv head are one list per request
 // (row r = token r / rep, head r % rep), cut into tiles of 32, 128 or 256 rows

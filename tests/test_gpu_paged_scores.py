@@ -73,3 +73,20 @@ def test_a_value_that_is_no_number_at_a_weight_of_nothing(gpu, n, keys, D, bits)
             assert np.isnan(got[first:, :, 3]).all(), at
             if bits == 8:
                 assert np.isnan(got[first:]).all()
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("n", [4, 90])
+def test_large_values(gpu, n, bits):
+    """Sums are not normalised until the end: values of 2^100 over 1000 keys stay
+    within 2^120, and a power of two changes no bit of what it scales."""
+    rng = np.random.default_rng(n + bits)
+    keys, H, D = 1000, 2, 128
+    table, pages = tables(rng, [keys], 64)
+    k, v, q = rows(rng, keys, H, D), rows(rng, keys, H, D), rows(rng, n, 4, D)
+    got = []
+    for scale in (1.0, 2.0 ** 100):
+        c = PagedKVCache(pages, H, D, page_size=64, bits=bits)
+        c.write(k, v * scale, table, i32([0]))
+        got.append(num(paged_sdpa(q, c, table, i32([keys - n]))) / scale)
+    assert np.isfinite(got[0]).all() and np.array_equal(*got)
