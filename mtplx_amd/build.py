@@ -23,7 +23,8 @@ SOURCES = ["qmv.hip", "qmv_xplain.hip", "qmv_xswiglu.hip", "qmv_xpre.hip", "qmv_
            "paged_cache.hip", "paged_attn.hip"]
 
 # Packed fp32 VALU instructions are disabled for every device pass: some
-# of their forms have produced silently wrong results on MI355X. hipcc's host pass warns that it does not know the feature; harmless.
+# of their forms have produced silently wrong results on MI355X. hipcc's host
+# pass warns that it does not know the feature; harmless.
 FLAGS = [
     "--offload-arch=gfx950",
     "-O3",

@@ -511,7 +511,7 @@ __device__ __forceinline__ float4* part_block(const PAttn& p, size_t slot, int R
   return reinterpret_cast<float4*>(p.part_o) + ((slot * (RT / 32) + rb) * (D / 32) + t) * 256;
 }
 
-// What a row's sums are divided by, as a factor: a row that saw no key is zeros.
+// The factor of a row's sums in its output: a row that saw no key is zeros.
 __device__ __forceinline__ float row_factor(float m, float l) { return m == -INFINITY && l == 0.f ? 0.f : 1.f / l; }
 
 // 16 bytes read once per launch (non-temporal, as ld_stream).
@@ -898,9 +898,9 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
 // -- few rows: one tile of 32 rows, the four waves share a piece by keys ---------
 
 // Blocks go straight from the pages into a wave's registers, the next one asked
-// for as soon as this one's operands are used up. Two workgroups a CU
-// where their registers allow (D < 256): sixteen requests' verify rows at 8 bits
-// take 120 us, with one 149.
+// for as soon as this one's operands are used up. Two workgroups a CU where
+// their registers allow (D < 256): sixteen requests' verify rows at 8 bits take
+// 122 us, with one 149.
 template <int D, int BITS>
 __global__ __launch_bounds__(kPT, D == 256 ? 1 : 2) void attn_few_kernel(PAttn p) {
   constexpr int RT = 32;

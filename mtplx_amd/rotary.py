@@ -145,6 +145,8 @@ def _rows(name: str, x: torch.Tensor, heads: int | None = None, dim: int | None 
 def _writable(name: str, out: torch.Tensor, like: torch.Tensor):
     """``(out, token stride, head stride)`` of an output for the rows of ``like``:
     16-byte aligned rows that do not overlap, tokens or heads outermost."""
+    if not isinstance(out, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor (got {type(out).__name__})")
     if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
         raise ValueError(f"{name} must be {list(like.shape)} {like.dtype} on {like.device}")
     T, H, D = out.shape
@@ -221,8 +223,8 @@ def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 def _apart(src: torch.Tensor, dst: torch.Tensor, in_place: bool = False) -> bool:
     """Whether a kernel may write the rows ``dst`` while it reads ``src``: they
-    share no element (rows side by side among them) or, with ``in_place`` (its own source and output), are the
-    same view."""
+    share no element (rows side by side do not) or, with ``in_place`` (an
+    output and its own source), are the same view."""
     if not _overlaps(dst, src) or _interleaved(dst, src):
         return True
     return in_place and dst.data_ptr() == src.data_ptr() and dst.stride() == src.stride() and dst.shape == src.shape
@@ -266,7 +268,8 @@ def apply_rotary(table: RotaryTable, queries: torch.Tensor, keys: torch.Tensor |
         kot = koh = 0
         if k is not None:
             ko, kot, koh = _writable("out[1]", out[1], keys)
-        # An item of the kernel reads what it stores, unless the halves are no whole chunks; heads go in no order.
+        # An item of the kernel reads what it stores, unless the halves are no
+        # whole chunks; tokens and heads go in no order.
         in_place = table.traditional or table.dims % 16 == 0
         if not _apart(q, qo, in_place) or (ko is not None and not _apart(q, ko)):
             q = q.clone(memory_format=torch.contiguous_format)

@@ -203,3 +203,11 @@ def test_attention_is_refused_where_bits_may_not_depend_on_the_batch(blocks, mon
     with exact_verify(False):
         paged_attention.paged_sdpa(x, cache, table, start)
     assert len(blocks) == 4
+
+
+def test_an_output_that_is_missing(blocks):
+    t, pos, x = rotary_table(D, device="cpu"), torch.arange(T), held(T, H, D)
+    for out in ((None, x), (held(T, H, D), None)):
+        with pytest.raises(TypeError, match="out"):
+            apply_rotary(t, x, held(T, H, D), pos, out=out)
+    assert not blocks
