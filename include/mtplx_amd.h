@@ -549,6 +549,26 @@ typedef struct mtp_rotary_args {
 } mtp_rotary_args;
 int mtp_rotary(const mtp_rotary_args* args, void* stream);
 
+/* The same with a norm of each head before it turns and positions of several
+ * axes (time, height and width of an image's or a video's patches):
+ *   x <- w x / sqrt(mean of the head's squares + eps)
+ * over all D elements, in fp32; elements past `dims` are normalised and not
+ * rotated; all is rounded to bf16 once. q_weight / k_weight (fp32 [D]; NULL:
+ * these heads are not normalised). positions int32 [axes][T] (axes 1 to 4):
+ * pair i turns by positions[a][t] with a the two bits at 2 (i % 32) of
+ * axis{i / 32}, which must lie below axes. positions NULL (axes 1):
+ * mtp_rotary_heads reads args->positions, mtp_paged_write_heads rotates at the
+ * positions at which the keys are stored. */
+typedef struct mtp_head_args {
+  const void* q_weight;
+  const void* k_weight;
+  const int32_t* positions;
+  long long axis0, axis1, axis2, axis3;
+  int axes;
+  float eps;
+} mtp_head_args;
+int mtp_rotary_heads(const mtp_rotary_args* args, const mtp_head_args* heads, void* stream);
+
 /* ---- paged KV cache ---------------------------------------------------------
  * A pool of num_pages pages of page_size keys (a multiple of 32) for Hkv heads
  * of D (64, 128, 256): k_pages / v_pages [num_pages][Hkv][page_size / 32]
@@ -602,6 +622,8 @@ typedef struct mtp_paged_write_args {
   long long k_token, k_head, v_token, v_head, q_token, q_head, qo_token, qo_head;
 } mtp_paged_write_args;
 int mtp_paged_write(const mtp_paged_write_args* args, void* stream);
+/* The same with head norms and positions of several axes (dims > 0). */
+int mtp_paged_write_heads(const mtp_paged_write_args* args, const mtp_head_args* heads, void* stream);
 
 typedef struct mtp_paged_read_args {
   const void* k_pages;

@@ -80,7 +80,9 @@ SIGNATURES = {
     "mtp_ragged_gqa_attn_rows_vt": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _vp, _sz, _vp]),
     "mtp_rope_qkv_to_cache_vt": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _vp, _vp]),
     "mtp_rotary": (_i, [_vp, _vp]),
+    "mtp_rotary_heads": (_i, [_vp, _vp, _vp]),
     "mtp_paged_write": (_i, [_vp, _vp]),
+    "mtp_paged_write_heads": (_i, [_vp, _vp, _vp]),
     "mtp_paged_read": (_i, [_vp, _vp]),
     "mtp_paged_attn_workspace_bytes": (_sz, [_i, _i, _i, _i]),
     "mtp_paged_attn": (_i, [_vp, _vp]),
@@ -158,6 +160,8 @@ _ll = C.c_longlong
 RotaryArgs = _block("RotaryArgs", "``mtp_rotary_args`` of include/mtplx_amd.h (same field order).",
                     (_vp, "q k q_out k_out positions table"), (_i, "T Hq Hkv D dims traditional"), (_f, "gain"),
                     (_ll, "q_token q_head k_token k_head qo_token qo_head ko_token ko_head"))
+HeadArgs = _block("HeadArgs", "``mtp_head_args`` (same field order).", (_vp, "q_weight k_weight positions"),
+                  (_ll, "axis0 axis1 axis2 axis3"), (_i, "axes"), (_f, "eps"))
 PagedWriteArgs = _block("PagedWriteArgs", "``mtp_paged_write_args`` (same field order).",
                         (_vp, "k v q q_out table k_pages v_pages k_scales v_scales block_table q_start row_off status"),
                         (_i, "T B width Hq Hkv D page_size num_pages bits dims traditional max_rows"), (_f, "gain"),

@@ -18,6 +18,15 @@ struct mtp_rotary_args {
   long long q_token, q_head, k_token, k_head, qo_token, qo_head, ko_token, ko_head;
 };
 
+struct mtp_head_args {
+  const void* q_weight;
+  const void* k_weight;
+  const int32_t* positions;
+  long long axis0, axis1, axis2, axis3;
+  int axes;
+  float eps;
+};
+
 struct mtp_paged_write_args {
   const void* k;
   const void* v;

@@ -62,6 +62,144 @@ __global__ __launch_bounds__(kNT) void rotary_kernel(RotRows q, RotRows k, const
   }
 }
 
+// Sum over aligned groups of `lanes` (a power of two), neighbours first.
+__device__ __forceinline__ float sum_lanes(float s, int lanes) {
+  for (int off = 1; off < lanes; off <<= 1) s += __shfl_xor(s, off, 64);
+  return s;
+}
+
+// The heads of up to eight tokens, normalised and rotated: `lanes` lanes (a
+// power of two) have a row each round, lane i its item i (rot_item's: a chunk of
+// eight elements, or one and its partner half a rotation on). All of a row is in
+// registers before the norm's factor is known, so it is read once, and the next
+// round's rows are asked for before this one's are turned.
+struct HeadRows {
+  RotRows q, k;
+  int Hq, Hkv, D, lanes;
+};
+template <class Live>
+__device__ __forceinline__ void turn_heads(const HeadRows& rows, const RotSpec& r, const HeadSpec& hs, const float2* cs,
+                                           const float* weights, long long t0, int n, int threads, Live live) {
+  const int heads = rows.Hq + rows.Hkv, D = rows.D, lanes = rows.lanes, half = r.dims / 2;
+  const bool paired = rot_paired(r.dims, r.trad);
+  const int it = threadIdx.x & (lanes - 1), np = paired ? r.dims / 16 : 0;
+  const bool two = it < np, mine = it < rot_items(D, r.dims, r.trad);
+  const int d1 = two ? 8 * it : r.dims * (paired ? 1 : 0) + 8 * (it - np), d2 = d1 + half;
+  const int per = threads / lanes, dt = per / heads, dh = per - dt * heads;
+  const int first = (int)threadIdx.x / lanes;
+  int t = first / heads, h = first - t * heads;
+  auto source = [&](int tt, int hh) {
+    const RotRows& s = hh < rows.Hq ? rows.q : rows.k;
+    return s.src + (t0 + tt) * s.st + (hh < rows.Hq ? hh : hh - rows.Hq) * s.sh;
+  };
+  uint4 a = {}, b = {}, na = {}, nb = {};
+  auto ask = [&](int tt, int hh) {
+    if (tt >= n || !mine) return;
+    const uint16_t* src = source(tt, hh);
+    na = *reinterpret_cast<const uint4*>(src + d1);
+    if (two) nb = *reinterpret_cast<const uint4*>(src + d2);
+  };
+  ask(t, h);
+  while (t < n) {
+    a = na;
+    b = nb;
+    int t1 = t + dt, h1 = h + dh;
+    if (h1 >= heads) {
+      h1 -= heads;
+      ++t1;
+    }
+    ask(t1, h1);
+    const bool isq = h < rows.Hq;
+    const float* w = weights + (isq ? 0 : D);
+    const bool norm = isq ? hs.q_weight != nullptr : hs.k_weight != nullptr;
+    const Chunk8 ca = unpack8(a), cb = unpack8(b);
+    float inv = 1.f;
+    if (norm) {   // (the same for all lanes of a row)
+      float sa = mine ? squares8(ca) : 0.f, sb = two ? squares8(cb) : 0.f;
+      if (paired && r.dims < D) {   // (lanes = the chunks, rounded up: lane j takes chunk j's)
+        const int base = (threadIdx.x & 63) & ~(lanes - 1), j = it;
+        const float up = __shfl(sa, base + (j < np ? j : (j - np) & (lanes - 1)), 64);
+        const float on = __shfl(sb, base + ((j - np) & (lanes - 1)), 64);
+        inv = norm_factor(sum_lanes(8 * j >= D ? 0.f : j >= np && j < 2 * np ? on : up, lanes), D, hs.eps);
+      } else {
+        sa = sum_lanes(sa, lanes);
+        if (paired) sa += sum_lanes(sb, lanes);   // (the whole head turns: the second half's chunks)
+        inv = norm_factor(sa, D, hs.eps);
+      }
+    }
+    const RotRows& to = isq ? rows.q : rows.k;
+    uint16_t* dst = to.dst + (t0 + t) * to.dt + (isq ? h : h - rows.Hq) * to.dh;
+    const float2* c = cs + t * half;
+    auto scale = [&](int d) { return norm ? inv * w[d] : 1.f; };
+    if (mine && live(t)) {
+      if (two) {
+        float y1[8], y2[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float2 z = c[d1 + e];
+          const float x1 = ca.v[e] * scale(d1 + e), x2 = cb.v[e] * scale(d2 + e);
+          y1[e] = rot_first(x1, x2, z);
+          y2[e] = rot_second(x1, x2, z);
+        }
+        *reinterpret_cast<uint4*>(dst + d1) = pack8(y1);
+        *reinterpret_cast<uint4*>(dst + d2) = pack8(y2);
+      } else {
+        float y[8];
+        const uint16_t* row = source(t, h);   // (partners of halves that are no whole chunks)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int d = d1 + e;
+          const float x = ca.v[e] * scale(d);
+          if (paired || d >= r.dims) {
+            y[e] = x;
+          } else if (r.trad) {
+            const float x2 = ca.v[e ^ 1] * scale(d ^ 1);
+            y[e] = e & 1 ? rot_second(x2, x, c[d >> 1]) : rot_first(x, x2, c[d >> 1]);
+          } else if (d < half) {
+            y[e] = rot_first(x, bf2f(row[d + half]) * scale(d + half), c[d]);
+          } else {
+            y[e] = rot_second(bf2f(row[d - half]) * scale(d - half), x, c[d - half]);
+          }
+        }
+        *reinterpret_cast<uint4*>(dst + d1) = pack8(y);
+      }
+    }
+    t = t1;
+    h = h1;
+  }
+}
+
+// Lanes of a row.
+inline int head_lanes(int D, int dims, int trad) {
+  int lanes = 1;
+  while (lanes < rot_items(D, dims, trad)) lanes <<= 1;
+  return lanes;
+}
+
+__device__ __forceinline__ void head_weights(const HeadSpec& hs, int D, float* weights, int threads) {
+  for (int d = threadIdx.x; d < D; d += threads) {
+    if (hs.q_weight) weights[d] = hs.q_weight[d];
+    if (hs.k_weight) weights[D + d] = hs.k_weight[d];
+  }
+}
+
+__global__ __launch_bounds__(kNT) void heads_kernel(HeadRows rows, RotSpec r, HeadSpec hs, int T, int tokens) {
+  __shared__ float2 cs[kRotTokens * kMaxPairs];
+  __shared__ float weights[4 * kMaxPairs];
+  const int half = r.dims / 2;
+  head_weights(hs, rows.D, weights, kNT);
+  for (long long t0 = (long long)blockIdx.x * tokens; t0 < T; t0 += (long long)gridDim.x * tokens) {
+    const int n = T - t0 < tokens ? (int)(T - t0) : tokens;
+    for (int x = threadIdx.x; x < n * half; x += kNT) {
+      const int t = x / half, i = x - t * half;
+      cs[x] = rot_angle(hs.positions[(long long)pair_axis(hs, i) * T + t0 + t], r.table[i], r.gain);
+    }
+    __syncthreads();
+    turn_heads(rows, r, hs, cs, weights, t0, n, kNT, [](int) { return true; });
+    __syncthreads();
+  }
+}
+
 struct WriteParams {
   const uint16_t* k;
   const uint16_t* v;
@@ -79,6 +217,8 @@ struct WriteParams {
   RotRows q;
   int Hq, q_tokens, kv_groups;   // workgroups [0, kv_groups) write K and V, the others rotate q
   int nb_uniform;                // blocks of each request where row_off is null
+  HeadSpec heads;                // (kernels with HEADS)
+  int lanes;
 };
 
 __device__ __forceinline__ long long floor_blk(long long p) { return p >> 5; }   // (blocks of 32)
@@ -228,7 +368,7 @@ __device__ __forceinline__ void turn4(const uint32_t (&a)[4], uint32_t (&t)[4]) 
 // has one 16-byte chunk of a row, its elements go where they belong. Up to two
 // rounds of it; as whole blocks through LDS a decode step of sixteen requests
 // took 10.4 us, this way 5.7 (6.8 with fp64 angles).
-template <int D, int BITS>
+template <int D, int BITS, bool HEADS>
 __device__ __forceinline__ void write_few(const WriteParams& p, int h, bool isk, int lane, long long base,
                                           long long first, long long at, int klo, int khi) {
   constexpr int CPR = D / 8;   // lanes of a row
@@ -243,11 +383,26 @@ __device__ __forceinline__ void write_few(const WriteParams& p, int h, bool isk,
     const int pos = (int)(base + key);
     const uint16_t* row = isk ? p.k + h * p.k_head + token * p.k_token : p.v + h * p.v_head + token * p.v_token;
     u32x4 x;
-    auto angles = [&](int i) { return rot_angle(pos, p.r.table[i], p.r.gain); };
+    TokenPos at_axes;
+    if constexpr (HEADS) {
+      if (isk) at_axes = token_pos(p.heads, p.T, token, pos);
+    }
+    auto angles = [&](int i) {
+      return rot_angle(HEADS ? at_axes.of(pair_axis(p.heads, i)) : pos, p.r.table[i], p.r.gain);
+    };
+    const bool norm = HEADS && isk && p.heads.k_weight;
+    float inv = 1.f;
+    if (norm)
+      inv = norm_factor(sum_lanes(squares8(unpack8(*reinterpret_cast<const uint4*>(row + 8 * c))), CPR), D, p.heads.eps);
+    auto scale = [&](int d) { return norm ? inv * p.heads.k_weight[d] : 1.f; };
+    auto scaled = [&](Chunk8 v, int d) {
+      if constexpr (HEADS) return scaled8(v, d, factors(scale));
+      else return v;
+    };
     if (isk && paired && 8 * c < dims) {
       const int half = dims / 2, d = 8 * c < half ? 8 * c : 8 * c - half;
-      const Chunk8 a = unpack8(*reinterpret_cast<const uint4*>(row + d));
-      const Chunk8 b = unpack8(*reinterpret_cast<const uint4*>(row + d + half));
+      const Chunk8 a = scaled(unpack8(*reinterpret_cast<const uint4*>(row + d)), d);
+      const Chunk8 b = scaled(unpack8(*reinterpret_cast<const uint4*>(row + d + half)), d + half);
       float y[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -256,9 +411,14 @@ __device__ __forceinline__ void write_few(const WriteParams& p, int h, bool isk,
       }
       x = __builtin_bit_cast(u32x4, pack8(y));
     } else if (isk && !paired && 8 * c < dims) {
-      rot_item(c, row, dims, p.r.trad, angles, [&](int, uint4 v) { x = __builtin_bit_cast(u32x4, v); });
+      auto store = [&](int, uint4 v) { x = __builtin_bit_cast(u32x4, v); };
+      if constexpr (HEADS)
+        rot_item(c, row, dims, p.r.trad, angles, store, factors(scale));
+      else
+        rot_item(c, row, dims, p.r.trad, angles, store);
     } else {
       x = *reinterpret_cast<const u32x4*>(row + 8 * c);
+      if (norm) x = __builtin_bit_cast(u32x4, pack8(scaled(unpack8(__builtin_bit_cast(uint4, x)), 8 * c).v));
     }
     unsigned char* dst = (isk ? p.k_pages : p.v_pages) + (size_t)at * (BITS / 8);
     if constexpr (BITS == 16) {
@@ -296,7 +456,7 @@ __device__ __forceinline__ void write_few(const WriteParams& p, int h, bool isk,
 // One unit by one wave, in its own LDS: rows come whole, turn in LDS and leave
 // in the page's order, 16 bytes a lane; keys of a block that is not all new go
 // out element by element (V) or chunk by chunk (K).
-template <int D, int BITS>
+template <int D, int BITS, bool HEADS>
 __device__ __forceinline__ void write_unit(const WriteParams& p, const Unit& w, int h, bool isk, int lane,
                                            uint16_t* rows) {
   constexpr int RS = row16<D>(), NC = D / 16, BS = row8<D>();   // 16-byte loads of a lane
@@ -325,7 +485,7 @@ __device__ __forceinline__ void write_unit(const WriteParams& p, const Unit& w, 
     return;
   }
   if (few) {
-    write_few<D, BITS>(p, h, isk, lane, base, first, at, klo, khi);
+    write_few<D, BITS, HEADS>(p, h, isk, lane, base, first, at, klo, khi);
     return;
   }
 #pragma unroll
@@ -338,19 +498,45 @@ __device__ __forceinline__ void write_unit(const WriteParams& p, const Unit& w, 
   const int key = lane & 31;
   const bool mine = key >= klo && key < khi;   // the lane's row
   if (isk && p.r.dims) {   // in place: an item reads what it stores, or the source
-    const int np = rot_paired(p.r.dims, p.r.trad) ? p.r.dims / 16 : (p.r.dims + 7) / 8;
-    const bool inplace = p.r.trad || rot_paired(p.r.dims, p.r.trad);
-    for (int x = lane; x < 32 * np; x += 64) {
+    const bool paired = rot_paired(p.r.dims, p.r.trad), inplace = p.r.trad || paired;
+    int np = paired ? p.r.dims / 16 : (p.r.dims + 7) / 8;
+    float inv = 1.f;   // of row lane % 32
+    const bool norm = HEADS && p.heads.k_weight;
+    if (norm) {   // every element changes
+      np = rot_items(D, p.r.dims, p.r.trad);
+      half_row<D>(rows, lane, x);
+      float s[NC];
+#pragma unroll
+      for (int i = 0; i < NC; ++i) s[i] = squares8(unpack8(__builtin_bit_cast(uint4, x[i])));
+#pragma unroll
+      for (int off = 1; off < NC; off <<= 1)
+#pragma unroll
+        for (int i = 0; i < NC; i += 2 * off) s[i] += s[i + off];
+      inv = norm_factor(s[0] + __shfl_xor(s[0], 32, 64), D, p.heads.eps);
+      wave_lds();   // read before it changes
+    }
+    for (int x0 = 0; x0 < 32 * np; x0 += 64) {
+      const int x = x0 + lane;
       const int kk = x / np;
+      const float row_inv = HEADS ? __shfl(inv, kk & 31, 64) : 1.f;   // (by all lanes)
       if (kk < klo || kk >= khi) continue;
       const int pos = (int)(base + kk);
       uint16_t* row = rows + kk * RS;
-      auto angles = [&](int i) { return rot_angle(pos, p.r.table[i], p.r.gain); };
+      TokenPos at_axes;
+      if constexpr (HEADS) at_axes = token_pos(p.heads, p.T, first + kk, pos);
+      auto angles = [&](int i) {
+        return rot_angle(HEADS ? at_axes.of(pair_axis(p.heads, i)) : pos, p.r.table[i], p.r.gain);
+      };
       auto store = [&](int d, uint4 v) { *reinterpret_cast<uint4*>(row + d) = v; };
-      if (inplace)
-        rot_item(x % np, row, p.r.dims, p.r.trad, angles, store);
-      else
-        rot_item(x % np, p.k + h * p.k_head + (first + kk) * p.k_token, p.r.dims, p.r.trad, angles, store);
+      const uint16_t* from = inplace ? row : p.k + h * p.k_head + (first + kk) * p.k_token;
+      auto turn = [&](const uint16_t* from) {
+        if constexpr (HEADS)
+          rot_item(x % np, from, p.r.dims, p.r.trad, angles, store,
+                   factors([&](int d) { return norm ? row_inv * p.heads.k_weight[d] : 1.f; }));
+        else
+          rot_item(x % np, from, p.r.dims, p.r.trad, angles, store);
+      };
+      if (inplace) turn(row); else turn(from);
     }
     wave_lds();
   }
@@ -455,8 +641,8 @@ __device__ __forceinline__ int token_request(const WriteParams& p, int t, long l
   return b;
 }
 
-template <int D, int BITS>
-__global__ __launch_bounds__(64 * cache_waves<D>(), D == 256 ? 1 : 4) void paged_write_kernel(WriteParams p) {
+template <int D, int BITS, bool HEADS>
+__global__ __launch_bounds__(64 * cache_waves<D>(), D == 256 ? 1 : HEADS ? 3 : 4) void paged_write_kernel(WriteParams p) {
   constexpr int NT = 64 * cache_waves<D>();
   __shared__ __attribute__((aligned(16))) uint16_t lds[cache_waves<D>()][32 * row16<D>()];
   const int lane = threadIdx.x & 63;
@@ -471,7 +657,24 @@ __global__ __launch_bounds__(64 * cache_waves<D>(), D == 256 ? 1 : 4) void paged
         long long pos = 0;
         const int b = token_request(p, t0 + t, &pos);   // the same in every thread
         if (threadIdx.x == 0) s_live[t] = b >= 0;
-        for (int x = threadIdx.x; x < half; x += NT) cs[t * half + x] = rot_angle(pos, p.r.table[x], p.r.gain);
+        for (int x = threadIdx.x; x < half; x += NT) {
+          if constexpr (HEADS) {
+            if (p.heads.positions) pos = p.heads.positions[(long long)pair_axis(p.heads, x) * p.T + t0 + t];
+          }
+          cs[t * half + x] = rot_angle(pos, p.r.table[x], p.r.gain);
+        }
+      }
+      if constexpr (HEADS) {
+        float* weights = reinterpret_cast<float*>(cs + kRotTokens * kMaxPairs);
+        static_assert(sizeof(lds) >= kRotTokens * kMaxPairs * sizeof(float2) + 2 * D * sizeof(float), "angles, weights");
+        HeadSpec hs = p.heads;
+        hs.k_weight = nullptr;   // (no keys here)
+        head_weights(hs, D, weights, NT);
+        __syncthreads();
+        turn_heads({p.q, p.q, p.Hq, 0, D, p.lanes}, p.r, hs, cs, weights, t0, n, NT, [&](int t) { return s_live[t] != 0; });
+        __syncthreads();
+        if (t0 > p.T - stride) break;
+        continue;
       }
       __syncthreads();
       for (int x = threadIdx.x; x < n * p.Hq * ipr; x += NT) {
@@ -493,7 +696,7 @@ __global__ __launch_bounds__(64 * cache_waves<D>(), D == 256 ? 1 : 4) void paged
     Unit w;
     const long long u = div_pos(x >> 1, p.Hkv);
     if (!find_unit(p, u, lane, w)) return;   // (no barrier follows)
-    write_unit<D, BITS>(p, w, (int)((x >> 1) - u * p.Hkv), (x & 1) == 0, fresh(lane), lds[wave]);
+    write_unit<D, BITS, HEADS>(p, w, (int)((x >> 1) - u * p.Hkv), (x & 1) == 0, fresh(lane), lds[wave]);
   }
 }
 
@@ -652,8 +855,12 @@ inline int check_rotation(const char* who, const void* table, int dims, int D) {
 inline int rot_tokens(int T) { return T >= 8 * 256 ? 8 : T >= 4 * 256 ? 4 : T >= 2 * 256 ? 2 : 1; }
 
 template <int D, int BITS>
-void launch_write(const WriteParams& p, int groups, hipStream_t st) {
-  hipLaunchKernelGGL((paged_write_kernel<D, BITS>), dim3((unsigned)groups), dim3(64 * cache_waves<D>()), 0, st, p);
+void launch_write(const WriteParams& p, bool heads, int groups, hipStream_t st) {
+  const dim3 grid((unsigned)groups), block(64 * cache_waves<D>());
+  if (heads)
+    hipLaunchKernelGGL((paged_write_kernel<D, BITS, true>), grid, block, 0, st, p);
+  else
+    hipLaunchKernelGGL((paged_write_kernel<D, BITS, false>), grid, block, 0, st, p);
 }
 template <int D, int BITS>
 void launch_read(const ReadParams& p, int groups, hipStream_t st) {
@@ -664,8 +871,25 @@ void launch_read(const ReadParams& p, int groups, hipStream_t st) {
 
 using namespace mtp;
 
-MTP_API int mtp_rotary(const mtp_rotary_args* a, void* stream) {
-  const char* who = "mtp_rotary";
+// What a call does to heads, from its argument block; false: refused.
+static bool head_spec(const char* who, const mtp_head_args* a, int dims, HeadSpec& h) {
+  const bool bad = a->axes < 1 || a->axes > 4 || (a->axes > 1 && !a->positions);
+  if (bad || !(a->eps >= 0.f) || !(a->eps < 3.0e38f)) {
+    set_error("%s: 1 to 4 axes (more than one with positions), a norm's eps finite and not negative", who);
+    return false;
+  }
+  const long long axis[4] = {a->axis0, a->axis1, a->axis2, a->axis3};
+  for (int i = 0; i < dims / 2 && i < kMaxPairs; ++i)
+    if ((int)(((unsigned long long)axis[i / 32] >> (2 * (i % 32))) & 3) >= a->axes) {
+      set_error("%s: pair %d turns by an axis past the last of %d", who, i, a->axes);
+      return false;
+    }
+  h = {(const float*)a->q_weight, (const float*)a->k_weight, a->positions, {}, a->axes, a->eps};
+  for (int i = 0; i < 4; ++i) h.axis[i] = (unsigned long long)axis[i];
+  return true;
+}
+
+static int rotary(const char* who, const mtp_rotary_args* a, const mtp_head_args* heads, void* stream) {
   if (!a || !a->q || !a->q_out || !a->positions || a->T < 1 || a->Hq < 1 || a->Hkv < 0 || a->D < 8 || a->D % 8 ||
       a->D > 2 * kMaxPairs || (a->Hkv > 0 && (!a->k || !a->k_out))) {
     set_error("%s: bad arguments (D a multiple of 8 up to 256)", who);
@@ -685,13 +909,30 @@ MTP_API int mtp_rotary(const mtp_rotary_args* a, void* stream) {
   const RotSpec r = {(const unsigned long long*)a->table, a->dims, a->traditional, a->gain};
   const int tokens = rot_tokens(a->T);
   const int groups = cdiv(a->T, tokens);
+  if (heads) {
+    HeadSpec hs;
+    if (!head_spec(who, heads, a->dims, hs)) return MTP_ERR_ARG;
+    if (!hs.positions) hs.positions = a->positions;
+    const HeadRows rows = {q, k, a->Hq, a->Hkv, a->D, head_lanes(a->D, a->dims, a->traditional)};
+    hipLaunchKernelGGL(heads_kernel, dim3((unsigned)groups), dim3(kNT), 0, (hipStream_t)stream, rows, r, hs, a->T, tokens);
+    return launch_check(who);
+  }
   hipLaunchKernelGGL(rotary_kernel, dim3((unsigned)groups), dim3(kNT), 0, (hipStream_t)stream, q, k, a->positions,
                      a->T, a->Hq, a->Hkv, a->D, r, tokens);
   return launch_check(who);
 }
 
-MTP_API int mtp_paged_write(const mtp_paged_write_args* a, void* stream) {
-  const char* who = "mtp_paged_write";
+MTP_API int mtp_rotary(const mtp_rotary_args* a, void* stream) { return rotary("mtp_rotary", a, nullptr, stream); }
+
+MTP_API int mtp_rotary_heads(const mtp_rotary_args* a, const mtp_head_args* heads, void* stream) {
+  if (!heads) {
+    set_error("mtp_rotary_heads: bad arguments");
+    return MTP_ERR_ARG;
+  }
+  return rotary("mtp_rotary_heads", a, heads, stream);
+}
+
+static int paged_write(const char* who, const mtp_paged_write_args* a, const mtp_head_args* heads, void* stream) {
   if (!a || !a->k || !a->v || !a->k_pages || !a->v_pages || !a->block_table || !a->q_start || a->T < 1 ||
       (a->bits == 8 && (!a->k_scales || !a->v_scales)) || (a->q && (!a->q_out || a->Hq < 1))) {
     set_error("%s: bad arguments", who);
@@ -713,6 +954,14 @@ MTP_API int mtp_paged_write(const mtp_paged_write_args* a, void* stream) {
     return MTP_ERR_ARG;
   }
   WriteParams p = {};
+  if (heads) {
+    if (a->dims < 2) {
+      set_error("%s: head norms and positions come with a rotation (dims=%d)", who, a->dims);
+      return MTP_ERR_ARG;
+    }
+    if (!head_spec(who, heads, a->dims, p.heads)) return MTP_ERR_ARG;
+    p.lanes = head_lanes(a->D, a->dims, a->traditional);
+  }
   p.k = (const uint16_t*)a->k;
   p.v = (const uint16_t*)a->v;
   p.k_pages = (unsigned char*)a->k_pages;
@@ -759,14 +1008,26 @@ MTP_API int mtp_paged_write(const mtp_paged_write_args* a, void* stream) {
   hipStream_t st = (hipStream_t)stream;
   const int key = a->D * 100 + a->bits;
   switch (key) {
-    case 6416: launch_write<64, 16>(p, (int)groups, st); break;
-    case 6408: launch_write<64, 8>(p, (int)groups, st); break;
-    case 12816: launch_write<128, 16>(p, (int)groups, st); break;
-    case 12808: launch_write<128, 8>(p, (int)groups, st); break;
-    case 25616: launch_write<256, 16>(p, (int)groups, st); break;
-    default: launch_write<256, 8>(p, (int)groups, st); break;
+    case 6416: launch_write<64, 16>(p, heads != nullptr, (int)groups, st); break;
+    case 6408: launch_write<64, 8>(p, heads != nullptr, (int)groups, st); break;
+    case 12816: launch_write<128, 16>(p, heads != nullptr, (int)groups, st); break;
+    case 12808: launch_write<128, 8>(p, heads != nullptr, (int)groups, st); break;
+    case 25616: launch_write<256, 16>(p, heads != nullptr, (int)groups, st); break;
+    default: launch_write<256, 8>(p, heads != nullptr, (int)groups, st); break;
   }
   return launch_check(who);
+}
+
+MTP_API int mtp_paged_write(const mtp_paged_write_args* a, void* stream) {
+  return paged_write("mtp_paged_write", a, nullptr, stream);
+}
+
+MTP_API int mtp_paged_write_heads(const mtp_paged_write_args* a, const mtp_head_args* heads, void* stream) {
+  if (!heads) {
+    set_error("mtp_paged_write_heads: bad arguments");
+    return MTP_ERR_ARG;
+  }
+  return paged_write("mtp_paged_write_heads", a, heads, stream);
 }
 
 MTP_API int mtp_paged_read(const mtp_paged_read_args* a, void* stream) {

@@ -65,9 +65,54 @@ __host__ __device__ __forceinline__ int rot_items(int D, int dims, int trad) {
   return rot_paired(dims, trad) ? dims / 16 + (D - dims) / 8 : D / 8;
 }
 
+// What a call does to heads beyond one position for all pairs: a norm of each
+// head before it turns, and positions of several axes. Pair i turns by position
+// [axis of i]; the axes are kept in the argument, two bits a pair (a lane reads
+// them without a load).
+struct HeadSpec {
+  const float* q_weight;   // [D], or null: these heads are not normalised
+  const float* k_weight;
+  const int32_t* positions;   // [axes][tokens], or null: a token's own for every pair
+  unsigned long long axis[4];
+  int axes;
+  float eps;
+};
+__device__ __forceinline__ int pair_axis(const HeadSpec& h, int i) {
+  const unsigned long long lo = i & 32 ? h.axis[1] : h.axis[0], hi = i & 32 ? h.axis[3] : h.axis[2];
+  return (int)((i & 64 ? hi : lo) >> (2 * (i & 31))) & 3;
+}
+// A token's positions, in registers.
+struct TokenPos {
+  int p[4];
+  __device__ __forceinline__ int of(int axis) const {
+    const int lo = axis & 1 ? p[1] : p[0], hi = axis & 1 ? p[3] : p[2];
+    return axis & 2 ? hi : lo;
+  }
+};
+__device__ __forceinline__ TokenPos token_pos(const HeadSpec& h, long long tokens, long long token, int own) {
+  TokenPos t;
+#pragma unroll
+  for (int a = 0; a < 4; ++a) t.p[a] = !h.positions ? own : a < h.axes ? h.positions[a * tokens + token] : 0;
+  return t;
+}
+
+// The factor 1 / sqrt(mean of squares + eps) of a head's row. Every kernel adds
+// the squares in one order, eight elements in turn and then the chunks of
+// eight pairwise (neighbours first), so a row's bits do not turn on the call
+// that it comes in.
+__device__ __forceinline__ float norm_factor(float squares, int D, float eps) {
+  return 1.f / sqrtf(squares / (float)D + eps);
+}
+
 struct Chunk8 {
   float v[8];
 };
+__device__ __forceinline__ float squares8(const Chunk8& c) {
+  float s = __fmul_rn(c.v[0], c.v[0]);
+#pragma unroll
+  for (int e = 1; e < 8; ++e) s = __fmaf_rn(c.v[e], c.v[e], s);
+  return s;
+}
 __device__ __forceinline__ Chunk8 unpack8(uint4 r) {
   const uint32_t w[4] = {r.x, r.y, r.z, r.w};
   Chunk8 c;
@@ -82,18 +127,41 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
   return make_uint4(f2bf2(v[0], v[1]), f2bf2(v[2], v[3]), f2bf2(v[4], v[5]), f2bf2(v[6], v[7]));
 }
 
+// What a head's elements are multiplied by before they turn: nothing, or
+// fp32 factors f(d) (a head norm's; an element, its factor and the rotation are
+// rounded to bf16 once, at the end).
+struct NoFactor {
+  static constexpr bool on = false;
+};
+template <class F>
+struct Factor {
+  static constexpr bool on = true;
+  F f;
+};
+template <class F>
+__device__ __forceinline__ Factor<F> factors(F f) { return {f}; }
+template <class X>
+__device__ __forceinline__ Chunk8 scaled8(Chunk8 c, int d, X x) {
+  if constexpr (X::on) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c.v[e] *= x.f(d + e);
+  }
+  return c;
+}
+
 // Item `it` of one head's row (16-byte aligned), cs(i) its token's cos/sin of
 // pair i; store(d, chunk) takes 8 finished elements from d on. An item
 // reads all it needs before it stores, and only what it stores, unless the
 // halves are no whole chunks (then partners are read from other items' rows).
-template <class Angles, class Store>
-__device__ __forceinline__ void rot_item(int it, const uint16_t* row, int dims, int trad, Angles cs, Store store) {
+template <class Angles, class Store, class X = NoFactor>
+__device__ __forceinline__ void rot_item(int it, const uint16_t* row, int dims, int trad, Angles cs, Store store,
+                                         X fx = {}) {
   if (rot_paired(dims, trad)) {
     const int np = dims / 16;
     if (it < np) {
       const int d = 8 * it, half = dims / 2;
-      const Chunk8 a = unpack8(*reinterpret_cast<const uint4*>(row + d));
-      const Chunk8 b = unpack8(*reinterpret_cast<const uint4*>(row + d + half));
+      const Chunk8 a = scaled8(unpack8(*reinterpret_cast<const uint4*>(row + d)), d, fx);
+      const Chunk8 b = scaled8(unpack8(*reinterpret_cast<const uint4*>(row + d + half)), d + half, fx);
       float y1[8], y2[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -105,17 +173,18 @@ __device__ __forceinline__ void rot_item(int it, const uint16_t* row, int dims, 
       store(d + half, pack8(y2));
     } else {
       const int d = dims + 8 * (it - np);
-      store(d, *reinterpret_cast<const uint4*>(row + d));
+      const uint4 raw = *reinterpret_cast<const uint4*>(row + d);
+      store(d, X::on ? pack8(scaled8(unpack8(raw), d, fx).v) : raw);
     }
     return;
   }
   const int d = 8 * it;
   const uint4 raw = *reinterpret_cast<const uint4*>(row + d);
   if (d >= dims) {
-    store(d, raw);
+    store(d, X::on ? pack8(scaled8(unpack8(raw), d, fx).v) : raw);
     return;
   }
-  const Chunk8 a = unpack8(raw);
+  const Chunk8 a = scaled8(unpack8(raw), d, fx);
   float y[8];
   if (trad) {
 #pragma unroll
@@ -127,15 +196,20 @@ __device__ __forceinline__ void rot_item(int it, const uint16_t* row, int dims, 
     }
   } else {
     const int half = dims / 2;
+    auto mate = [&](int i) {
+      const float x = bf2f(row[i]);
+      if constexpr (X::on) return x * fx.f(i);
+      else return x;
+    };
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int dd = d + e;
       if (dd >= dims)
         y[e] = a.v[e];
       else if (dd < half)
-        y[e] = rot_first(a.v[e], bf2f(row[dd + half]), cs(dd));
+        y[e] = rot_first(a.v[e], mate(dd + half), cs(dd));
       else
-        y[e] = rot_second(bf2f(row[dd - half]), a.v[e], cs(dd - half));
+        y[e] = rot_second(mate(dd - half), a.v[e], cs(dd - half));
     }
   }
   store(d, pack8(y));

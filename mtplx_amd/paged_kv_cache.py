@@ -24,7 +24,7 @@ from typing import Any
 import torch
 
 from . import _lib
-from .rotary import RotaryTable, _apart, _call, _int32, _on, _rows, _writable
+from .rotary import HeadNorms, RotaryTable, _apart, _call, _heads, _int32, _on, _positions, _rows, _writable
 
 __all__ = ["PagedKVCache"]
 
@@ -121,6 +121,7 @@ class PagedKVCache:
     # -- writes and reads ------------------------------------------------------------
     def write(self, keys: torch.Tensor, values: torch.Tensor, block_table: Any, q_start: Any, row_off: Any = None, *,
               max_rows: int | None = None, queries: torch.Tensor | None = None, rotary: RotaryTable | None = None,
+              norms: HeadNorms | None = None, positions: Any = None,
               out: torch.Tensor | None = None) -> torch.Tensor | None:
         """Store the new tokens' ``keys`` / ``values`` [T, Hkv, D] bf16.
 
@@ -134,6 +135,11 @@ class PagedKVCache:
         positions on the way, and ``queries`` [T, Hq, D] into the returned
         tensor (or ``out``), as :func:`apply_rotary` would. Without ``rotary``
         ``queries`` has no meaning and is refused.
+
+        ``norms`` (with ``rotary``): keys and queries are normalised by head
+        first, as :func:`apply_rotary` does. ``positions`` [T], or [axes, T] of a
+        table with sections (which needs them): what keys and queries are rotated
+        by, where that is not the position that a key is stored at.
 
         Two tokens of one call must not share a slot. A position without a
         page is skipped and sets :meth:`status`."""
@@ -151,6 +157,14 @@ class PagedKVCache:
             if rotary.dims > D:
                 raise ValueError(f"the rotary table's {rotary.dims} dims exceed the head dim {D}")
             _on(device, "rotary", rotary.phases)
+        elif norms is not None or positions is not None:
+            raise ValueError("norms and positions come with a rotation: give rotary with them")
+        heads = None
+        if rotary is not None:
+            if positions is None and rotary.axes > 1:
+                raise ValueError(f"a table of {rotary.axes} axes needs positions [{rotary.axes}, {T}]")
+            pos = None if positions is None else _positions(rotary, positions, T, device)
+            heads = _heads(rotary, norms, pos, D, device)
         table = self._table(block_table)
         B, width = table.shape
         start, off = self._requests(T, B, q_start, row_off)
@@ -186,7 +200,10 @@ class PagedKVCache:
         if q is not None and Hq:
             a.q, a.q_out, a.Hq = q.data_ptr(), qo.data_ptr(), Hq
             a.q_token, a.q_head, a.qo_token, a.qo_head = qt, qh, qot, qoh
-        _call("mtp_paged_write", a, device)
+        if heads is None:
+            _call("mtp_paged_write", a, device)
+        else:
+            _call("mtp_paged_write_heads", a, device, heads)
         return qo
 
     def read(self, block_table: Any, count: int, *, start: Any = None, lengths: Any = None):

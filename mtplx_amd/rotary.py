@@ -13,7 +13,9 @@ For pair i of position p, with angle ``a = p f_i``::
 
     y1 = gain (x1 cos a - x2 sin a)      y2 = gain (x1 sin a + x2 cos a)
 
-in fp32, rounded once to bf16. The angle is reduced exactly (64-bit
+in fp32, rounded once to bf16. Heads may be normalised on the way
+(:func:`head_norms`), and a token may have several positions, each for its
+own pairs (``sections``). The angle is reduced exactly (64-bit
 fixed-point revolutions), so far positions are as precise as near ones.
 """
 
@@ -28,20 +30,55 @@ import torch
 
 from . import _lib
 
-__all__ = ["RotaryTable", "rotary_table", "apply_rotary"]
+__all__ = ["HeadNorms", "RotaryTable", "apply_rotary", "head_norms", "rotary_table"]
 
 
 @dataclass(frozen=True)
 class RotaryTable:
     """Frequencies of ``dims / 2`` pairs: ``frequencies`` in radians per
     position (host, float64), ``phases`` the same as revolutions times 2^64
-    (device, the bits of a uint64), ``gain`` the factor of the rotated values."""
+    (device, the bits of a uint64), ``gain`` the factor of the rotated values,
+    ``axes`` how many positions a token has and ``axis`` (host) the one that
+    each pair turns by."""
 
     dims: int
     traditional: bool
     gain: float
     frequencies: tuple
     phases: torch.Tensor
+    axes: int = 1
+    axis: tuple = ()
+
+
+@dataclass(frozen=True)
+class HeadNorms:
+    """RMS norms of each head of the queries and keys: fp32 weights ``[D]``
+    (None: that side is not normalised) and the constant beside the mean."""
+
+    queries: torch.Tensor | None
+    keys: torch.Tensor | None
+    eps: float
+
+
+def head_norms(queries: torch.Tensor | None, keys: torch.Tensor | None, *, eps: float = 1e-6) -> HeadNorms:
+    """:class:`HeadNorms` of weights ``[D]`` (any floating type; a copy in fp32
+    is kept, so make it again after a change), for :func:`apply_rotary` and
+    ``PagedKVCache.write``: ``w x / sqrt(mean(x^2) + eps)`` over each head."""
+    eps = float(eps)
+    if not (math.isfinite(eps) and 0.0 <= eps < 3.0e38):
+        raise ValueError(f"eps must be finite and not negative (got {eps})")
+    if queries is None and keys is None:
+        raise ValueError("give the queries' weight, the keys' or both")
+    kept = []
+    for name, w in (("queries", queries), ("keys", keys)):
+        if w is not None:
+            if not isinstance(w, torch.Tensor) or not w.is_floating_point() or w.dim() != 1:
+                raise ValueError(f"the {name}' weight must be one dimension of floats")
+            w = w.detach().to(torch.float32, copy=True).contiguous()
+        kept.append(w)
+    if None not in kept and (kept[0].shape != kept[1].shape or kept[0].device != kept[1].device):
+        raise ValueError("the two weights must have one length and device")
+    return HeadNorms(kept[0], kept[1], eps)
 
 
 def rotary_frequencies(dims: int, *, base: float = 10000.0, scale: float = 1.0, scaling: str | None = None,
@@ -89,13 +126,35 @@ def rotary_frequencies(dims: int, *, base: float = 10000.0, scale: float = 1.0, 
     return freqs, 0.1 * math.log(factor) + 1.0
 
 
+MAX_AXES = 4
+
+
+def _pair_axes(pairs: int, sections: Sequence[int], interleaved: bool) -> tuple:
+    """The axis of each of ``pairs`` pairs."""
+    counts = [int(n) for n in sections]
+    A = len(counts)
+    if not 1 <= A <= MAX_AXES or any(n < 1 for n in counts) or sum(counts) != pairs:
+        raise ValueError(f"sections must be 1 to {MAX_AXES} positive counts of {pairs} pairs in all (got {counts})")
+    if not interleaved:
+        return tuple(a for a, n in enumerate(counts) for _ in range(n))
+    if any(a + A * (n - 1) >= pairs for a, n in enumerate(counts) if a):
+        raise ValueError(f"interleaved sections {counts}: an axis's last pair would lie past the {pairs} pairs")
+    return tuple(i % A if i // A < counts[i % A] else 0 for i in range(pairs))
+
+
 def rotary_table(dims: int, *, base: float = 10000.0, traditional: bool = False, scale: float = 1.0,
                  scaling: str | None = None, factor: float = 1.0, trained_positions: int = 0,
                  fast_turns: float = 32.0, slow_turns: float = 1.0, frequencies: Sequence[float] | None = None,
-                 gain: float | None = None, device: Any = "cuda") -> RotaryTable:
+                 gain: float | None = None, sections: Sequence[int] | None = None, interleaved: bool = False,
+                 device: Any = "cuda") -> RotaryTable:
     """The frequencies of :func:`rotary_frequencies`, or ``frequencies`` as
     given (radians per position, ``dims / 2`` of them, at most pi each), on
-    ``device``. ``gain`` replaces the scaling's own."""
+    ``device``. ``gain`` replaces the scaling's own.
+
+    ``sections``: pairs that turn by each of several positions of a token (up
+    to four axes: time, height and width of images and videos): the first
+    ``sections[0]`` pairs by the first, and so on; ``interleaved``: pair i by
+    axis ``i % axes`` while that axis has pairs left, else by the first."""
     if frequencies is None:
         freqs, own_gain = rotary_frequencies(dims, base=base, scale=scale, scaling=scaling, factor=factor,
                                              trained_positions=trained_positions, fast_turns=fast_turns,
@@ -115,8 +174,49 @@ def rotary_table(dims: int, *, base: float = 10000.0, traditional: bool = False,
         raise ValueError("gain must be finite")
     # At most half a revolution each: the fixed-point value stays below 2^63.
     fixed = [min(round(f / (2.0 * math.pi) * 2.0 ** 64), 2 ** 63 - 1) for f in freqs]
+    if sections is None and interleaved:
+        raise ValueError("interleaved belongs to sections")
+    axis = _pair_axes(dims // 2, sections, interleaved) if sections is not None else ()
     return RotaryTable(int(dims), bool(traditional), gain, tuple(freqs),
-                       torch.tensor(fixed, dtype=torch.int64).to(device))
+                       torch.tensor(fixed, dtype=torch.int64).to(device), len(sections) if axis else 1, axis)
+
+
+def _positions(table: RotaryTable, positions: Any, T: int, device) -> torch.Tensor:
+    """int32 ``[T]``, or ``[axes, T]`` of a table with sections, on ``device``."""
+    if not (isinstance(positions, torch.Tensor) and positions.is_cuda):
+        wide = torch.as_tensor(positions)
+        positions = _int32("positions", wide, wide.device)
+        if not torch.equal(positions.to(torch.int64), wide.to(torch.int64)):
+            raise ValueError("positions must fit int32")
+    pos = _int32("positions", positions, device, table.axes * T)
+    if table.axes > 1 and tuple(pos.shape) != (table.axes, T):
+        raise ValueError(f"positions must be [{table.axes}, {T}], a row for each axis (got {list(pos.shape)})")
+    return pos
+
+
+def _heads(table: RotaryTable, norms: HeadNorms | None, positions: torch.Tensor | None, D: int,
+           device) -> _lib.HeadArgs | None:
+    """The argument block of a call with head norms or several axes (None: one
+    without), its weights checked."""
+    if norms is None and table.axes == 1 and positions is None:
+        return None
+    a = _lib.HeadArgs(axes=table.axes)
+    if norms is not None:
+        if not isinstance(norms, HeadNorms):
+            raise TypeError(f"norms must come from head_norms (got {type(norms).__name__})")
+        for name, w in (("queries", norms.queries), ("keys", norms.keys)):
+            if w is not None:
+                _on(device, f"norms.{name}", w)
+                if w.shape[0] != D:
+                    raise ValueError(f"norms.{name} has {w.shape[0]} weights, heads have {D} elements")
+        a.q_weight, a.k_weight, a.eps = _lib.ptr(norms.queries), _lib.ptr(norms.keys), norms.eps
+    if positions is not None:
+        a.positions = positions.data_ptr()
+    words = [0, 0, 0, 0]
+    for i, axis in enumerate(table.axis):
+        words[i // 32] |= axis << (2 * (i % 32))
+    a.axis0, a.axis1, a.axis2, a.axis3 = (w - (w >> 63 << 64) for w in words)   # (the bits, as signed)
+    return a
 
 
 def _rows(name: str, x: torch.Tensor, heads: int | None = None, dim: int | None = None):
@@ -198,14 +298,14 @@ def _stream(device) -> int:
     return _raw_stream(device.index) if _raw_stream is not None else _lib.stream_handle(device)
 
 
-def _call(name: str, block: ctypes.Structure, device) -> None:
+def _call(name: str, block: ctypes.Structure, device, *more: ctypes.Structure) -> None:
     """Run an argument-block entry point on ``device``'s current stream (the
     kernels of a call go to the current HIP device)."""
     if torch.cuda.current_device() == device.index:
-        _lib.call(name, ctypes.byref(block), _stream(device))
+        _lib.call(name, ctypes.byref(block), *map(ctypes.byref, more), _stream(device))
         return
     with torch.cuda.device(device):
-        _lib.call(name, ctypes.byref(block), _stream(device))
+        _lib.call(name, ctypes.byref(block), *map(ctypes.byref, more), _stream(device))
 
 
 def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -231,12 +331,16 @@ def _apart(src: torch.Tensor, dst: torch.Tensor, in_place: bool = False) -> bool
 
 
 def apply_rotary(table: RotaryTable, queries: torch.Tensor, keys: torch.Tensor | None, positions: Any, *,
-                 out: tuple | None = None):
+                 norms: HeadNorms | None = None, out: tuple | None = None):
     """Rotate ``queries`` [T, Hq, D] and ``keys`` [T, Hkv, D] (or None) bf16 at
-    ``positions`` [T] (int32; may stay on the GPU, where a wider one counts as
-    the nearest that fits). Returns ``(queries, keys)`` rotated, in new tensors or
-    in ``out`` (a pair; the inputs themselves for in place). Views of a fused
-    projection are read, and written, where they are."""
+    ``positions`` [T], or [axes, T] of a table with sections (int32; may stay on
+    the GPU, where a wider one counts as the nearest that fits). Returns
+    ``(queries, keys)`` rotated, in new tensors or in ``out`` (a pair; the inputs
+    themselves for in place). Views of a fused projection are read, and written,
+    where they are.
+
+    ``norms`` (:func:`head_norms`): each head is normalised first, all of it
+    (elements that do not turn too), in the same pass and with one rounding."""
     q, T, Hq, D, qt, qh = _rows("queries", queries)
     device = q.device
     k, Hkv, kt, kh = None, 0, 0, 0
@@ -249,13 +353,9 @@ def apply_rotary(table: RotaryTable, queries: torch.Tensor, keys: torch.Tensor |
         raise ValueError("queries have no heads")
     if D % 8 or D > 256 or table.dims > D:
         raise ValueError(f"head dim {D} must be a multiple of 8 up to 256 and hold the table's {table.dims} dims")
-    if not (isinstance(positions, torch.Tensor) and positions.is_cuda):
-        wide = torch.as_tensor(positions)
-        positions = _int32("positions", wide, wide.device)
-        if not torch.equal(positions.to(torch.int64), wide.to(torch.int64)):
-            raise ValueError("positions must fit int32")
-    pos = _int32("positions", positions, device, T)
+    pos = _positions(table, positions, T, device)
     _on(device, "table", table.phases)
+    heads = _heads(table, norms, None if table.axes == 1 else pos, D, device)
     ko = None
     if out is None:
         qo = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=device)
@@ -283,10 +383,14 @@ def apply_rotary(table: RotaryTable, queries: torch.Tensor, keys: torch.Tensor |
         return qo, ko
     if not Hkv:
         k = None
-    _call("mtp_rotary", _lib.RotaryArgs(
+    block = _lib.RotaryArgs(
         q.data_ptr(), None if k is None else k.data_ptr(), qo.data_ptr(), None if k is None else ko.data_ptr(),
         pos.data_ptr(), table.phases.data_ptr(), T, Hq, Hkv, D, table.dims, table.traditional, table.gain, qt, qh, kt, kh,
-        qot, qoh, kot, koh), device)
+        qot, qoh, kot, koh)
+    if heads is None:
+        _call("mtp_rotary", block, device)
+    else:
+        _call("mtp_rotary_heads", block, device, heads)
     return qo, ko
 
 

@@ -24,6 +24,41 @@ def rotate(x: np.ndarray, positions, frequencies, dims: int, traditional: bool, 
     return y
 
 
+def pair_axes(pairs: int, sections=None, interleaved: bool = False) -> np.ndarray:
+    """The axis that each pair turns by: in runs, or dealt in turn until an
+    axis has its pairs (the first takes the rest)."""
+    if sections is None:
+        return np.zeros(pairs, int)
+    if not interleaved:
+        return np.repeat(np.arange(len(sections)), sections)
+    left = list(sections)
+    axis = np.zeros(pairs, int)
+    for i in range(pairs):
+        a = i % len(sections)
+        if a and left[a]:
+            axis[i] = a
+            left[a] -= 1
+    return axis
+
+
+def norm_heads(x: np.ndarray, weight, eps: float) -> np.ndarray:
+    """``x`` [T, H, D], each head over the root of its mean square, times ``weight``."""
+    x = np.asarray(x, np.float64)
+    with np.errstate(all="ignore"):
+        return x / np.sqrt((x * x).mean(-1, keepdims=True) + eps) * np.asarray(weight, np.float64)
+
+
+def rotate_axes(x: np.ndarray, positions, axis, frequencies, dims: int, traditional: bool, gain: float = 1.0) -> np.ndarray:
+    """:func:`rotate` with ``positions`` [axes, T]: pair i turns by its own axis's."""
+    y = np.array(x, np.float64)
+    for a in range(len(positions)):
+        r = rotate(x, positions[a], frequencies, dims, traditional, gain)
+        for i in np.flatnonzero(np.asarray(axis) == a):
+            for d in ((2 * i, 2 * i + 1) if traditional else (i, i + dims // 2)):
+                y[..., d] = r[..., d]
+    return y
+
+
 def quantise_rows(x: np.ndarray) -> tuple[np.ndarray, np.ndarray]:
     """(int8 values, fp32 scale) of each row (last axis) of float32 ``x``."""
     x = np.asarray(x, np.float32)
