@@ -77,14 +77,21 @@ struct HeadRows {
   RotRows q, k;
   int Hq, Hkv, D, lanes;
 };
-template <class Live>
+
+__device__ __forceinline__ Chunk8 floats8(const float* p) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  return {{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+}
+
+// PAIRED: as rot_paired. weights: the factors of q's elements, then k's (ones
+// where a side is not normalised).
+template <bool PAIRED, bool NORM, class Live>
 __device__ __forceinline__ void turn_heads(const HeadRows& rows, const RotSpec& r, const HeadSpec& hs, const float2* cs,
                                            const float* weights, long long t0, int n, int threads, Live live) {
   const int heads = rows.Hq + rows.Hkv, D = rows.D, lanes = rows.lanes, half = r.dims / 2;
-  const bool paired = rot_paired(r.dims, r.trad);
-  const int it = threadIdx.x & (lanes - 1), np = paired ? r.dims / 16 : 0;
-  const bool two = it < np, mine = it < rot_items(D, r.dims, r.trad);
-  const int d1 = two ? 8 * it : r.dims * (paired ? 1 : 0) + 8 * (it - np), d2 = d1 + half;
+  const int it = threadIdx.x & (lanes - 1), np = PAIRED ? r.dims / 16 : 0;
+  const bool two = PAIRED && it < np, mine = it < np + (D - 16 * np) / 8;
+  const int d1 = two ? 8 * it : 8 * (it + np), d2 = d1 + half;
   const int per = threads / lanes, dt = per / heads, dh = per - dt * heads;
   const int first = (int)threadIdx.x / lanes;
   int t = first / heads, h = first - t * heads;
@@ -92,7 +99,7 @@ __device__ __forceinline__ void turn_heads(const HeadRows& rows, const RotSpec& 
     const RotRows& s = hh < rows.Hq ? rows.q : rows.k;
     return s.src + (t0 + tt) * s.st + (hh < rows.Hq ? hh : hh - rows.Hq) * s.sh;
   };
-  uint4 a = {}, b = {}, na = {}, nb = {};
+  uint4 na = {}, nb = {};
   auto ask = [&](int tt, int hh) {
     if (tt >= n || !mine) return;
     const uint16_t* src = source(tt, hh);
@@ -101,8 +108,7 @@ __device__ __forceinline__ void turn_heads(const HeadRows& rows, const RotSpec& 
   };
   ask(t, h);
   while (t < n) {
-    a = na;
-    b = nb;
+    Chunk8 a = unpack8(na), b = unpack8(nb);
     int t1 = t + dt, h1 = h + dh;
     if (h1 >= heads) {
       h1 -= heads;
@@ -111,55 +117,62 @@ __device__ __forceinline__ void turn_heads(const HeadRows& rows, const RotSpec& 
     ask(t1, h1);
     const bool isq = h < rows.Hq;
     const float* w = weights + (isq ? 0 : D);
-    const bool norm = isq ? hs.q_weight != nullptr : hs.k_weight != nullptr;
-    const Chunk8 ca = unpack8(a), cb = unpack8(b);
     float inv = 1.f;
-    if (norm) {   // (the same for all lanes of a row)
-      float sa = mine ? squares8(ca) : 0.f, sb = two ? squares8(cb) : 0.f;
-      if (paired && r.dims < D) {   // (lanes = the chunks, rounded up: lane j takes chunk j's)
+    if (NORM && (isq ? hs.q_weight : hs.k_weight)) {   // (the same for all lanes of a row)
+      float sa = mine ? squares8(a) : 0.f;
+      const float sb = two ? squares8(b) : 0.f;
+      if (PAIRED && r.dims < D) {   // lane j takes chunk j's (there are lanes enough)
         const int base = (threadIdx.x & 63) & ~(lanes - 1), j = it;
         const float up = __shfl(sa, base + (j < np ? j : (j - np) & (lanes - 1)), 64);
         const float on = __shfl(sb, base + ((j - np) & (lanes - 1)), 64);
-        inv = norm_factor(sum_lanes(8 * j >= D ? 0.f : j >= np && j < 2 * np ? on : up, lanes), D, hs.eps);
+        sa = sum_lanes(8 * j >= D ? 0.f : j >= np && j < 2 * np ? on : up, lanes);
       } else {
         sa = sum_lanes(sa, lanes);
-        if (paired) sa += sum_lanes(sb, lanes);   // (the whole head turns: the second half's chunks)
-        inv = norm_factor(sa, D, hs.eps);
+        if (PAIRED) sa += sum_lanes(sb, lanes);   // (the whole head turns: the second half's chunks)
       }
+      inv = norm_factor(sa, D, hs.eps);
     }
     const RotRows& to = isq ? rows.q : rows.k;
     uint16_t* dst = to.dst + (t0 + t) * to.dt + (isq ? h : h - rows.Hq) * to.dh;
     const float2* c = cs + t * half;
-    auto scale = [&](int d) { return norm ? inv * w[d] : 1.f; };
     if (mine && live(t)) {
+      auto scale = [&](Chunk8& x, int d) {
+        if (!NORM) return;
+        const Chunk8 f = floats8(w + d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x.v[e] *= inv * f.v[e];
+      };
+      scale(a, d1);
       if (two) {
+        scale(b, d2);
         float y1[8], y2[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float2 z = c[d1 + e];
-          const float x1 = ca.v[e] * scale(d1 + e), x2 = cb.v[e] * scale(d2 + e);
-          y1[e] = rot_first(x1, x2, z);
-          y2[e] = rot_second(x1, x2, z);
+        for (int e = 0; e < 8; e += 2) {
+          const float4 z = *reinterpret_cast<const float4*>(c + d1 + e);
+          y1[e] = rot_first(a.v[e], b.v[e], make_float2(z.x, z.y));
+          y2[e] = rot_second(a.v[e], b.v[e], make_float2(z.x, z.y));
+          y1[e + 1] = rot_first(a.v[e + 1], b.v[e + 1], make_float2(z.z, z.w));
+          y2[e + 1] = rot_second(a.v[e + 1], b.v[e + 1], make_float2(z.z, z.w));
         }
         *reinterpret_cast<uint4*>(dst + d1) = pack8(y1);
         *reinterpret_cast<uint4*>(dst + d2) = pack8(y2);
+      } else if (PAIRED) {
+        *reinterpret_cast<uint4*>(dst + d1) = pack8(a.v);
       } else {
         float y[8];
         const uint16_t* row = source(t, h);   // (partners of halves that are no whole chunks)
+        auto mate = [&](int d) { return NORM ? bf2f(row[d]) * (inv * w[d]) : bf2f(row[d]); };
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int d = d1 + e;
-          const float x = ca.v[e] * scale(d);
-          if (paired || d >= r.dims) {
-            y[e] = x;
-          } else if (r.trad) {
-            const float x2 = ca.v[e ^ 1] * scale(d ^ 1);
-            y[e] = e & 1 ? rot_second(x2, x, c[d >> 1]) : rot_first(x, x2, c[d >> 1]);
-          } else if (d < half) {
-            y[e] = rot_first(x, bf2f(row[d + half]) * scale(d + half), c[d]);
-          } else {
-            y[e] = rot_second(bf2f(row[d - half]) * scale(d - half), x, c[d - half]);
-          }
+          if (d >= r.dims)
+            y[e] = a.v[e];
+          else if (r.trad)
+            y[e] = e & 1 ? rot_second(a.v[e ^ 1], a.v[e], c[d >> 1]) : rot_first(a.v[e], a.v[e ^ 1], c[d >> 1]);
+          else if (d < half)
+            y[e] = rot_first(a.v[e], mate(d + half), c[d]);
+          else
+            y[e] = rot_second(mate(d - half), a.v[e], c[d - half]);
         }
         *reinterpret_cast<uint4*>(dst + d1) = pack8(y);
       }
@@ -178,16 +191,17 @@ inline int head_lanes(int D, int dims, int trad) {
 
 __device__ __forceinline__ void head_weights(const HeadSpec& hs, int D, float* weights, int threads) {
   for (int d = threadIdx.x; d < D; d += threads) {
-    if (hs.q_weight) weights[d] = hs.q_weight[d];
-    if (hs.k_weight) weights[D + d] = hs.k_weight[d];
+    weights[d] = hs.q_weight ? hs.q_weight[d] : 1.f;
+    weights[D + d] = hs.k_weight ? hs.k_weight[d] : 1.f;
   }
 }
 
-__global__ __launch_bounds__(kNT) void heads_kernel(HeadRows rows, RotSpec r, HeadSpec hs, int T, int tokens) {
-  __shared__ float2 cs[kRotTokens * kMaxPairs];
-  __shared__ float weights[4 * kMaxPairs];
+template <bool PAIRED, bool NORM>
+__global__ __launch_bounds__(kNT, 4) void heads_kernel(HeadRows rows, RotSpec r, HeadSpec hs, int T, int tokens) {
+  __shared__ __attribute__((aligned(16))) float2 cs[kRotTokens * kMaxPairs];
+  __shared__ __attribute__((aligned(16))) float weights[4 * kMaxPairs];
   const int half = r.dims / 2;
-  head_weights(hs, rows.D, weights, kNT);
+  if (NORM) head_weights(hs, rows.D, weights, kNT);
   for (long long t0 = (long long)blockIdx.x * tokens; t0 < T; t0 += (long long)gridDim.x * tokens) {
     const int n = T - t0 < tokens ? (int)(T - t0) : tokens;
     for (int x = threadIdx.x; x < n * half; x += kNT) {
@@ -195,7 +209,7 @@ __global__ __launch_bounds__(kNT) void heads_kernel(HeadRows rows, RotSpec r, He
       cs[x] = rot_angle(hs.positions[(long long)pair_axis(hs, i) * T + t0 + t], r.table[i], r.gain);
     }
     __syncthreads();
-    turn_heads(rows, r, hs, cs, weights, t0, n, kNT, [](int) { return true; });
+    turn_heads<PAIRED, NORM>(rows, r, hs, cs, weights, t0, n, kNT, [](int) { return true; });
     __syncthreads();
   }
 }
@@ -642,7 +656,7 @@ __device__ __forceinline__ int token_request(const WriteParams& p, int t, long l
 }
 
 template <int D, int BITS, bool HEADS>
-__global__ __launch_bounds__(64 * cache_waves<D>(), D == 256 ? 1 : HEADS ? 3 : 4) void paged_write_kernel(WriteParams p) {
+__global__ __launch_bounds__(64 * cache_waves<D>(), D == 256 ? 1 : 4) void paged_write_kernel(WriteParams p) {
   constexpr int NT = 64 * cache_waves<D>();
   __shared__ __attribute__((aligned(16))) uint16_t lds[cache_waves<D>()][32 * row16<D>()];
   const int lane = threadIdx.x & 63;
@@ -671,7 +685,12 @@ __global__ __launch_bounds__(64 * cache_waves<D>(), D == 256 ? 1 : HEADS ? 3 : 4
         hs.k_weight = nullptr;   // (no keys here)
         head_weights(hs, D, weights, NT);
         __syncthreads();
-        turn_heads({p.q, p.q, p.Hq, 0, D, p.lanes}, p.r, hs, cs, weights, t0, n, NT, [&](int t) { return s_live[t] != 0; });
+        const HeadRows all = {p.q, p.q, p.Hq, 0, D, p.lanes};
+        auto live = [&](int t) { return s_live[t] != 0; };
+        if (rot_paired(p.r.dims, p.r.trad))
+          turn_heads<true, true>(all, p.r, hs, cs, weights, t0, n, NT, live);
+        else
+          turn_heads<false, true>(all, p.r, hs, cs, weights, t0, n, NT, live);
         __syncthreads();
         if (t0 > p.T - stride) break;
         continue;
@@ -907,14 +926,17 @@ static int rotary(const char* who, const mtp_rotary_args* a, const mtp_head_args
   const RotRows q = {(const uint16_t*)a->q, (uint16_t*)a->q_out, a->q_token, a->q_head, a->qo_token, a->qo_head};
   const RotRows k = {(const uint16_t*)a->k, (uint16_t*)a->k_out, a->k_token, a->k_head, a->ko_token, a->ko_head};
   const RotSpec r = {(const unsigned long long*)a->table, a->dims, a->traditional, a->gain};
-  const int tokens = rot_tokens(a->T);
+  const int tokens = heads ? (a->T >= 512 ? 2 : 1) : rot_tokens(a->T);
   const int groups = cdiv(a->T, tokens);
   if (heads) {
     HeadSpec hs;
     if (!head_spec(who, heads, a->dims, hs)) return MTP_ERR_ARG;
     if (!hs.positions) hs.positions = a->positions;
     const HeadRows rows = {q, k, a->Hq, a->Hkv, a->D, head_lanes(a->D, a->dims, a->traditional)};
-    hipLaunchKernelGGL(heads_kernel, dim3((unsigned)groups), dim3(kNT), 0, (hipStream_t)stream, rows, r, hs, a->T, tokens);
+    const bool paired = rot_paired(a->dims, a->traditional), norm = hs.q_weight || hs.k_weight;
+    auto* kernel = paired ? (norm ? heads_kernel<true, true> : heads_kernel<true, false>)
+                          : (norm ? heads_kernel<false, true> : heads_kernel<false, false>);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(kNT), 0, (hipStream_t)stream, rows, r, hs, a->T, tokens);
     return launch_check(who);
   }
   hipLaunchKernelGGL(rotary_kernel, dim3((unsigned)groups), dim3(kNT), 0, (hipStream_t)stream, q, k, a->positions,
