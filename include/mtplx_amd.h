@@ -662,6 +662,16 @@ typedef struct mtp_paged_attn_args {
 size_t mtp_paged_attn_workspace_bytes(int Hq, int Hkv, int D, int max_rows);
 int mtp_paged_attn(const mtp_paged_attn_args* args, void* stream);
 
+/* mtp_paged_attn over part of what a position sees: position p sees the last
+ * `window` (at least 1) of positions 0 .. p, itself among them, and those below
+ * `sinks`. Blocks of 32 positions that no row of a tile sees are not read, and
+ * their pages need not exist (a position without a page sets the status only
+ * where a block that is read holds it). Same workspace. */
+typedef struct mtp_attn_scope {
+  int window, sinks;
+} mtp_attn_scope;
+int mtp_paged_attn_scoped(const mtp_paged_attn_args* args, const mtp_attn_scope* scope, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -78,6 +78,10 @@ struct mtp_paged_attn_args {
   long long q_token, q_head, out_token, out_head;
 };
 
+struct mtp_attn_scope {
+  int window, sinks;
+};
+
 namespace mtp {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));

@@ -25,7 +25,8 @@ __all__ = ["paged_sdpa"]
 
 
 def paged_sdpa(queries: torch.Tensor, cache: PagedKVCache, block_table: Any, q_start: Any, row_off: Any = None, *,
-               max_rows: int | None = None, scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+               max_rows: int | None = None, scale: float | None = None, window: int | None = None, sinks: int = 0,
+               out: torch.Tensor | None = None) -> torch.Tensor:
     """``softmax(scale q k^T) v`` with grouped heads: ``queries`` [T, Hq, D] bf16
     (Hq 1 to 32 times the cache's kv heads) to ``[T, Hq, D]``.
 
@@ -39,6 +40,10 @@ def paged_sdpa(queries: torch.Tensor, cache: PagedKVCache, block_table: Any, q_s
     the table without a page count as absent and set ``cache.status()``. A token
     at or past the table's end (``width * page_size``) sees the positions that the
     table has and sets nothing here: its ``write`` did.
+    ``window``: a token at position p sees positions p - window + 1 to p alone
+    (``window`` of them), and with ``sinks`` the first so many of its request
+    too. What no new token sees is not read: the pages that hold nothing else may
+    have been given back (-1 in the table).
     ``scale`` is positive; default ``1 / sqrt(D)``. Refused inside
     ``exact_verify(True)``: how a row's sums are split depends on the lengths of
     the call's other requests."""
@@ -57,6 +62,7 @@ def paged_sdpa(queries: torch.Tensor, cache: PagedKVCache, block_table: Any, q_s
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError(f"scale must be positive and finite (got {scale})")
+    scope = _scope(window, sinks)
     if out is None:
         out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=device)
         ot, oh = Hq * D, D
@@ -77,8 +83,24 @@ def paged_sdpa(queries: torch.Tensor, cache: PagedKVCache, block_table: Any, q_s
     a.T, a.B, a.width, a.Hq, a.max_rows, a.scale = T, B, width, Hq, rows, scale
     a.q_token, a.q_head, a.out_token, a.out_head = qt, qh, ot, oh
     with _LAUNCH:   # (its launches stay together: host threads may share a stream and so its workspace)
-        _call("mtp_paged_attn", a, device)
+        if scope is None:
+            _call("mtp_paged_attn", a, device)
+        else:
+            _call("mtp_paged_attn_scoped", a, device, scope)
     return out
+
+
+def _scope(window: int | None, sinks: int) -> _lib.AttnScope | None:
+    """What a row sees, as an argument block (None: all up to itself)."""
+    window, sinks = None if window is None else int(window), int(sinks)
+    if sinks < 0 or (window is not None and window < 1):
+        raise ValueError(f"window must be positive and sinks not negative (got {window}, {sinks})")
+    if window is None:
+        if sinks:
+            raise ValueError("sinks belong to a window: without one every earlier token is visible")
+        return None
+    # (no position of a table reaches 2^31: a longer one hides nothing)
+    return _lib.AttnScope(min(window, 2 ** 31 - 1), min(sinks, 2 ** 31 - 1))
 
 
 _SPACES: dict = {}

@@ -88,10 +88,12 @@ def page_order(kind: str, head_dim: int, bits: int) -> np.ndarray:
     return ((t * 2 + jj) * 64 + half * 32 + c) * 8 + e
 
 
-def attend(q: np.ndarray, k: np.ndarray, v: np.ndarray, start: int, scale: float | None = None):
+def attend(q: np.ndarray, k: np.ndarray, v: np.ndarray, start: int, scale: float | None = None,
+           window: int | None = None, sinks: int = 0):
     """``q`` [n, Hq, D] at positions start.. over ``k``, ``v`` [Hkv, keys, D]:
     ``(o, spread, reach)`` float64: the rows, sum_j p_j |v_j| of each element,
-    and per row max_j of sum_d |q_d k_jd| scale and of |score|."""
+    and per row max_j of sum_d |q_d k_jd| scale and of |score|. ``window``: the
+    last so many positions up to a row's own, and the first ``sinks``."""
     q, k, v = (np.asarray(a, np.float64) for a in (q, k, v))
     n, Hq, D = q.shape
     rep = Hq // k.shape[0]
@@ -104,6 +106,12 @@ def attend(q: np.ndarray, k: np.ndarray, v: np.ndarray, start: int, scale: float
             continue
         for h in range(Hq):
             kk, vv = k[h // rep, :seen], v[h // rep, :seen]
+            if window is not None:
+                j = np.arange(seen)
+                j = j[(j > start + i - window) | (j < sinks)]
+                if not len(j):
+                    continue
+                kk, vv = kk[j], vv[j]
             s = kk @ q[i, h] * scale
             p = np.exp(s - s.max())
             p /= p.sum()
