@@ -662,14 +662,21 @@ typedef struct mtp_paged_attn_args {
 size_t mtp_paged_attn_workspace_bytes(int Hq, int Hkv, int D, int max_rows);
 int mtp_paged_attn(const mtp_paged_attn_args* args, void* stream);
 
-/* mtp_paged_attn over part of what a position sees: position p sees the last
- * `window` (at least 1) of positions 0 .. p, itself among them, and those below
- * `sinks`. Blocks of 32 positions that no row of a tile sees are not read, and
- * their pages need not exist (a position without a page sets the status only
- * where a block that is read holds it). Same workspace. */
+/* mtp_paged_attn with one of two additions.
+ * window > 0: position p sees the last `window` (itself among them) of
+ * positions 0 .. p, and those below `sinks`. Blocks of 32 positions that no row
+ * of a tile sees are not read, and their pages need not exist (a position
+ * without a page sets the status only where a block that is read holds it).
+ * shared > 0 (window and sinks 0): the first `shared` positions of all requests
+ * are the same keys, in the pages of the table's first row; whole blocks of 32
+ * of them may be read once for the rows of all requests. The result is
+ * mtp_paged_attn's up to the order of sums; a request that begins inside them
+ * reads its own keys. Workspace: mtp_paged_attn_workspace_bytes, with shared > 0
+ * mtp_paged_attn_shared_workspace_bytes. */
 typedef struct mtp_attn_scope {
-  int window, sinks;
+  int window, sinks, shared;
 } mtp_attn_scope;
+size_t mtp_paged_attn_shared_workspace_bytes(int Hq, int Hkv, int D, int max_rows, int T, int B, int shared);
 int mtp_paged_attn_scoped(const mtp_paged_attn_args* args, const mtp_attn_scope* scope, void* stream);
 
 #ifdef __cplusplus

@@ -86,6 +86,7 @@ SIGNATURES = {
     "mtp_paged_read": (_i, [_vp, _vp]),
     "mtp_paged_attn_workspace_bytes": (_sz, [_i, _i, _i, _i]),
     "mtp_paged_attn": (_i, [_vp, _vp]),
+    "mtp_paged_attn_shared_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
     "mtp_paged_attn_scoped": (_i, [_vp, _vp, _vp]),
 }
 
@@ -174,7 +175,7 @@ PagedAttnArgs = _block("PagedAttnArgs", "``mtp_paged_attn_args`` (same field ord
                        (_vp, "q out k_pages v_pages k_scales v_scales block_table q_start row_off status ws"),
                        (_sz, "ws_bytes"), (_i, "T B width Hq Hkv D page_size num_pages bits max_rows"), (_f, "scale"),
                        (_ll, "q_token q_head out_token out_head"))
-AttnScope = _block("AttnScope", "``mtp_attn_scope`` (same field order).", (_i, "window sinks"))
+AttnScope = _block("AttnScope", "``mtp_attn_scope`` (same field order).", (_i, "window sinks shared"))
 
 
 class MtpError(RuntimeError):

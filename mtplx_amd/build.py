@@ -20,7 +20,8 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 SOURCES = ["qmv.hip", "qmv_xplain.hip", "qmv_xswiglu.hip", "qmv_xpre.hip", "qmv_xrmsnorm.hip", "qmv_rope.hip",
            "qmv_moe.hip", "qmv_generic.hip", "qmv_inplace.hip", "qmm_mfma.hip", "qmm_tiles.hip", "sampler.hip", "attention.hip", "model_ops.hip", "moe.hip",
-           "paged_cache.hip", "paged_attn.hip", "paged_attn_window.hip"]
+           "paged_cache.hip", "paged_attn.hip", "paged_attn_window.hip",
+           "paged_attn_shared.hip"]
 
 # Packed fp32 VALU instructions are disabled for every device pass: some
 # of their forms have produced silently wrong results on MI355X. hipcc's host
@@ -41,7 +42,7 @@ FLAGS = [
 # Sources compiled without that option: the compiler crashes on
 # attn_chunk_kernel<256, 16> with it. Kernels of two waves per SIMD hold 256
 # registers and use no AGPRs either way.
-AGPR_SOURCES = {"paged_attn.hip", "paged_attn_window.hip"}
+AGPR_SOURCES = {"paged_attn.hip", "paged_attn_window.hip", "paged_attn_shared.hip"}
 
 
 def flags_for(src: str) -> list[str]:

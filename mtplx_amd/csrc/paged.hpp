@@ -79,7 +79,7 @@ struct mtp_paged_attn_args {
 };
 
 struct mtp_attn_scope {
-  int window, sinks;
+  int window, sinks, shared;
 };
 
 namespace mtp {

@@ -10,6 +10,18 @@ MTP_API size_t mtp_paged_attn_workspace_bytes(int Hq, int Hkv, int D, int max_ro
   return (size_t)2 * a.G * a.RT * (D + 2) * sizeof(float) + (size_t)a.G * 16;
 }
 
+// Whether the prefix is worth a pass of its own.
+static bool sharing(int Hq, int Hkv, int T, int B, int prefix) {
+  return prefix >= 2 * kStepKeys && B > 1;
+}
+
+MTP_API size_t mtp_paged_attn_shared_workspace_bytes(int Hq, int Hkv, int D, int max_rows, int T, int B, int shared) {
+  const size_t tail = mtp_paged_attn_workspace_bytes(Hq, Hkv, D, max_rows);
+  const int prefix = shared / kBlk * kBlk;
+  if (!tail || T < 1 || B < 1 || shared < 1 || !sharing(Hq, Hkv, T, B, prefix)) return tail;
+  return tail + prefix_plan(Hq, Hkv, D, T, prefix).bytes(Hkv, D);
+}
+
 static int paged_attn(const char* who, const mtp_paged_attn_args* a, const mtp_attn_scope* scope, void* stream) {
   if (!a || !a->q || !a->out || !a->k_pages || !a->v_pages || !a->block_table || !a->q_start || a->T < 1 ||
       a->Hkv < 1 || a->Hq < 1 || (a->bits == 8 && (!a->k_scales || !a->v_scales))) {
@@ -42,7 +54,20 @@ static int paged_attn(const char* who, const mtp_paged_attn_args* a, const mtp_a
   }
   const int max_rows = a->row_off ? a->max_rows : a->T / a->B;
   const AttnPlan plan = attn_plan(a->Hq, a->Hkv, a->D, max_rows);
-  const size_t need = mtp_paged_attn_workspace_bytes(a->Hq, a->Hkv, a->D, max_rows);
+  const size_t tail = mtp_paged_attn_workspace_bytes(a->Hq, a->Hkv, a->D, max_rows);
+  PrefixPlan pre = {};
+  const int prefix = scope ? scope->shared / kBlk * kBlk : 0;
+  if (scope && scope->shared > 0) {
+    if (scope->shared > (long long)a->width * a->page_size) {
+      set_error("%s: %d shared positions are more than the table covers", who, scope->shared);
+      return MTP_ERR_ARG;
+    }
+    if (!sharing(a->Hq, a->Hkv, a->T, a->B, prefix))
+      scope = nullptr;   // each request reads its own keys, as without
+    else
+      pre = prefix_plan(a->Hq, a->Hkv, a->D, a->T, prefix);
+  }
+  const size_t need = tail + pre.bytes(a->Hkv, a->D);
   if (!a->ws || !aligned16(a->ws) || a->ws_bytes < need) {
     set_error("%s: workspace %zu B < required %zu B (or unaligned)", who, a->ws_bytes, need);
     return MTP_ERR_WORKSPACE;
@@ -83,6 +108,12 @@ static int paged_attn(const char* who, const mtp_paged_attn_args* a, const mtp_a
   p.out_head = a->out_head;
   hipStream_t st = (hipStream_t)stream;
   if (!scope) return launch_scope<kCausal>(who, p, plan, a->D, a->bits, st);
+  if (scope->shared > 0) {
+    p.prefix = prefix;
+    p.prefix_o = (const float*)((const unsigned char*)a->ws + tail);
+    p.prefix_ml = p.prefix_o + pre.slots(a->Hkv) * pre.RT * a->D;
+    return launch_shared(who, p, plan, pre, a->D, a->bits, st);
+  }
   p.window = scope->window;
   p.sinks = scope->sinks;
   // A tile's blocks: the sinks', and those of the window of its first row to its last row.
@@ -96,8 +127,9 @@ MTP_API int mtp_paged_attn(const mtp_paged_attn_args* a, void* stream) {
 
 MTP_API int mtp_paged_attn_scoped(const mtp_paged_attn_args* a, const mtp_attn_scope* scope, void* stream) {
   const char* who = "mtp_paged_attn_scoped";
-  if (!scope || scope->window < 1 || scope->sinks < 0) {
-    set_error("%s: bad arguments (a window of at least one position, no negative number of sinks)", who);
+  if (!scope || scope->window < 0 || scope->sinks < 0 || scope->shared < 0 ||
+      (scope->window > 0) == (scope->shared > 0) || (scope->sinks > 0 && !scope->window)) {
+    set_error("%s: bad arguments (a window of at least one position, and its sinks, or shared positions)", who);
     return MTP_ERR_ARG;
   }
   return paged_attn(who, a, scope, stream);

@@ -60,6 +60,8 @@ constexpr int kPT = 256;   // threads: four waves
 enum Scope {
   kCausal,   // every key up to its own position
   kWindow,   // of these the last `window` and the first `sinks`
+  kPrefix,   // rows of all requests as one list: the shared prefix, all of it
+  kTail,     // every key up to its own position, of which the prefix is done
 };
 
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
@@ -88,6 +90,12 @@ struct PAttn {
   int tile_cost;
   int window, sinks;   // kWindow
   long long most;      // kWindow: most line that a tile takes
+  // kPrefix, kTail: keys of the shared prefix (whole blocks), its row tiles of a
+  // kv head, their rows, the pieces that each is cut into by keys; kTail: their
+  // partials, laid out as part_o and part_ml, slot (head, piece, tile).
+  int prefix, prefix_tiles, prefix_rt_log2, prefix_pieces;
+  const float* prefix_o;
+  const float* prefix_ml;
   float scale_log2;
   long long q_token, q_head, out_token, out_head;
 };
@@ -100,6 +108,7 @@ __device__ __forceinline__ int row_token(const PAttn& p, int r) { return (int)((
 
 struct Req {
   int lo, n;          // packed rows
+  int skip;           // kTail: blocks of the prefix (start, keys and lengths count behind them)
   long long start;    // position of the first
   long long base;     // line position where its first head begins
   long long head;     // line length of one head
@@ -157,17 +166,30 @@ __device__ __forceinline__ int div_small(long long a, long long b) {
   return q;
 }
 
+// Tokens whose rows make the prefix's list.
+__device__ __forceinline__ int prefix_tokens(const PAttn& p) {
+  const int n = p.row_off ? p.row_off[p.B] : p.T;
+  return n < 0 ? 0 : n < p.T ? n : p.T;
+}
+
 // A lane's request of the line (64 requests at a time), its rows and length.
 struct LaneReq {
   ReqRows rows;
+  int skip;
   long long start, len;   // len: one head
 };
 template <int SC>
 __device__ __forceinline__ LaneReq lane_req(const PAttn& p, int b) {
-  LaneReq r = {{0, 0}, 0, 0};
+  LaneReq r = {{0, 0}, 0, 0, 0};
   if (b < p.B) {
     r.rows = req_rows(p.row_off, b, p.B, p.T);
     r.start = p.q_start[b];
+    if constexpr (SC == kTail) {
+      // The prefix is done for a request that lies behind it; one that does not
+      // (or whose rows are not among the list's) sees its keys from the first on.
+      if (r.start >= p.prefix && r.rows.lo + r.rows.n <= prefix_tokens(p)) r.skip = p.prefix / kBlk;
+      r.start -= r.skip * kBlk;
+    }
     r.len = head_len<SC>(p, r.start, r.rows.n);
   }
   return r;
@@ -212,6 +234,7 @@ struct Line {
         r.lo = __builtin_amdgcn_readfirstlane(__shfl(q.rows.lo, src, 64));
         r.n = __builtin_amdgcn_readfirstlane(__shfl(q.rows.n, src, 64));
         r.start = uniform64(shfl64(q.start, src));
+        r.skip = SC == kTail ? __builtin_amdgcn_readfirstlane(__shfl(q.skip, src, 64)) : 0;
         r.head = uniform64(shfl64(q.len, src));
         r.base = uniform64(carry + shfl64(end, src)) - p.Hkv * r.head;
         return __builtin_amdgcn_readfirstlane(b0 + src);
@@ -220,6 +243,16 @@ struct Line {
     }
     return -1;   // (not reached: x < W)
   }
+};
+
+// The prefix's list has no line: workgroup g takes piece k of tile t of head h,
+// g = (h pieces + k) tiles + t (tiles that read the same keys are neighbours).
+template <>
+struct Line<kPrefix> {
+  int G;
+  __device__ __forceinline__ Line(const PAttn& p, int) { G = p.Hkv * p.prefix_pieces * p.prefix_tiles; }
+  __device__ __forceinline__ long long lo(int) const { return 0; }
+  __device__ __forceinline__ long long hi(int) const { return 1; }
 };
 
 // One row tile of one head: where it lies on the line and what it is. Tiles are
@@ -248,7 +281,8 @@ __device__ __forceinline__ void set_tile(const PAttn& p, const Req& r, Tile& u) 
   u.len = clamp_start(p, r.start) + (cost < r.n ? cost : r.n);
   if (SC == kWindow && u.len > p.most) u.len = p.most;
   u.pos = r.start + u.tok;
-  const long long cap = (long long)p.width * p.bpp * kBlk;
+  const long long cap = (long long)p.width * p.bpp * kBlk - (SC == kTail ? r.skip * kBlk : 0);
+  if constexpr (SC == kTail) u.gap = r.skip;
   const long long e = u.pos + row_token(p, u.off + u.rows - 1) + 1;
   u.nk = (int)(e < 0 ? 0 : e > cap ? cap : e);
   if constexpr (SC == kWindow) {
@@ -278,6 +312,27 @@ __device__ __forceinline__ Tile tile_at(const PAttn& p, const Req& r, long long 
   return u;
 }
 
+// Workgroup g's piece of the prefix: tile u of the list rq, keys [ka, kb). Its
+// rows are at the prefix's last position, so each sees all of it.
+__device__ __forceinline__ void prefix_piece(const PAttn& p, int g, Req& rq, Tile& u, int& ka, int& kb, int step) {
+  const int v = g / p.prefix_tiles, k = v % p.prefix_pieces;
+  u.h = v / p.prefix_pieces;
+  u.t = g - v * p.prefix_tiles;
+  rq.lo = 0;
+  rq.n = prefix_tokens(p);
+  const int first = u.t << p.rt_log2, left = rq.n * p.rep - first;
+  u.rows = left >> p.rt_log2 > 0 ? 1 << p.rt_log2 : left;
+  u.tok = (int)((uint32_t)first / (uint32_t)p.rep);
+  u.off = first - u.tok * p.rep;
+  const long long cap = (long long)p.width * p.bpp * kBlk;
+  u.nk = p.prefix < cap ? p.prefix : (int)cap;
+  u.pos = u.nk - 1;
+  const int steps = (u.nk + step - 1) / step;
+  ka = (int)((long long)steps * k / p.prefix_pieces) * step;
+  kb = (int)((long long)steps * (k + 1) / p.prefix_pieces) * step;
+  if (kb > u.nk) kb = u.nk;
+}
+
 // The tile after u on the line, in the same request.
 template <int SC>
 __device__ __forceinline__ void next_tile(const PAttn& p, const Req& r, Tile& u) {
@@ -299,8 +354,13 @@ __device__ __forceinline__ int key_at(const Tile& u, long long x, int step) {
   const long long k = x / step * step;
   return k < n ? (int)k : n;
 }
-// kWindow: the place of the v-th counted block.
-__device__ __forceinline__ int block_place(const Tile& u, int v) { return v < u.nsink ? v : v + u.gap; }
+// The place of a tile's v-th counted block.
+template <int SC>
+__device__ __forceinline__ int block_place(const Tile& u, int v) {
+  if constexpr (SC == kWindow) return v < u.nsink ? v : v + u.gap;
+  else if constexpr (SC == kTail) return v + u.gap;
+  else return v;
+}
 
 // Keys of one block that rows may see: a lane's row sees those in
 // [low, bound], of which none at or past end exist. In the sinks' blocks that is
@@ -545,8 +605,8 @@ struct BlockList {
   template <int SC>
   __device__ __forceinline__ void fill(const PAttn& p, int b, const Tile& u, int blk, int end, int lane) {
     first = blk;
-    const int place = SC == kWindow ? block_place(u, blk + lane) : blk + lane;
-    at = blk + lane < end ? (int)page_block(p.table, p.width, b, place, p.bpp, p.num_pages, p.Hkv, u.h, 1) : -1;
+    at = blk + lane < end ? (int)page_block(p.table, p.width, b, block_place<SC>(u, blk + lane), p.bpp, p.num_pages,
+                                            p.Hkv, u.h, 1) : -1;
     if (p.status && blk + lane < end && at < 0) atomicOr(p.status, kStatusPage);
     gone = __ballot(at < 0);
     if (at < 0) at = 0;
@@ -617,6 +677,40 @@ __device__ __forceinline__ float4* part_block(const PAttn& p, size_t slot, int R
   return reinterpret_cast<float4*>(p.part_o) + ((slot * (RT / 32) + rb) * (D / 32) + t) * 256;
 }
 
+// What the prefix left for the lane's row (row0 + lane % 32 of the tile):
+// pieces k0, k0 + dk, .. of it, as the row's state.
+template <int D>
+__device__ __forceinline__ void take_prefix(RowState<D>& s, const PAttn& p, const Req& rq, const Tile& u, int row0,
+                                            int lane, int k0, int dk) {
+  const int h2 = lane >> 5, r = row0 + (lane & 31);
+  if (r >= u.rows) return;
+  const int row = (rq.lo + u.tok) * p.rep + u.off + r, RT = 1 << p.prefix_rt_log2;   // (of the prefix's list)
+  const int t = row >> p.prefix_rt_log2, rr = row & (RT - 1);
+  auto slot = [&](int k) { return (size_t)(u.h * p.prefix_pieces + k) * p.prefix_tiles + t; };
+  auto ml = [&](int k) { return *reinterpret_cast<const float2*>(p.prefix_ml + (slot(k) * RT + rr) * 2); };
+  float m = -INFINITY;
+  for (int k = k0; k < p.prefix_pieces; k += dk) m = fmaxf(m, ml(k).x);
+  float l = 0.f;
+  for (int k = k0; k < p.prefix_pieces; k += dk) {
+    const float2 a = ml(k);
+    const float w = a.x == -INFINITY ? 0.f : exp2_fast(a.x - m);
+    l += a.x == -INFINITY ? a.y : a.y * w;   // (no score: 0 or NaN)
+    const float4* o = reinterpret_cast<const float4*>(p.prefix_o) + (slot(k) * (RT / 32) + (rr >> 5)) * (D / 32) * 256;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float4 v = o[i * 256 + (2 * j + h2) * 32 + (rr & 31)];
+        s.o[i][4 * j] += w == 0.f ? 0.f : v.x * w;
+        s.o[i][4 * j + 1] += w == 0.f ? 0.f : v.y * w;
+        s.o[i][4 * j + 2] += w == 0.f ? 0.f : v.z * w;
+        s.o[i][4 * j + 3] += w == 0.f ? 0.f : v.w * w;
+      }
+  }
+  s.m = m;
+  s.l = h2 == 0 ? l : 0.f;   // (the halves' sums are added at the end)
+}
+
 // The factor of a row's sums in its output: a row that saw no key is zeros.
 __device__ __forceinline__ float row_factor(float m, float l) { return m == -INFINITY && l == 0.f ? 0.f : 1.f / l; }
 
@@ -647,7 +741,7 @@ __device__ __forceinline__ void note_begun(const PAttn& p, const Line<SC>& line,
 // The v-th counted block of a windowed tile; `absent`: it has no page.
 __device__ __forceinline__ Sight block_sight(const PAttn& p, const Tile& u, int v, bool absent) {
   const bool sink = v < u.nsink;
-  const int base = 32 * block_place(u, v);
+  const int base = 32 * block_place<kWindow>(u, v);
   return {base, absent ? base : sink && p.sinks < u.nk ? p.sinks : u.nk, sink};
 }
 
@@ -725,31 +819,47 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
   const int tid = threadIdx.x, lane = tid & 63, h2 = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Line<SC> line(p, lane);
-  if (tid == 0 && (int)blockIdx.x >= line.G) p.begun[blockIdx.x] = make_int4(0, 0, 0, 0);
+  if (SC != kPrefix && tid == 0 && (int)blockIdx.x >= line.G) p.begun[blockIdx.x] = make_int4(0, 0, 0, 0);
   // Neighbours on the line share a head's keys: they go to one XCD (workgroups
   // are dealt to the eight in turn), whose L2 then serves them.
   const int per = cdiv(line.G, 8);
   const int g = ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);
   if ((int)blockIdx.x >> 3 >= per || g >= line.G) return;
-  if (tid == 0) p.begun[g] = make_int4(0, 0, 0, 0);
+  if (SC != kPrefix && tid == 0) p.begun[g] = make_int4(0, 0, 0, 0);
   const long long lo = line.lo(g), hi = line.hi(g);
   const int turn = NW == 8 && wave >= 4 ? 1 : 0;
   const uint32_t klds = lds_addr(lds), vlds = klds + KR * 4 * BE;
   Req rq;
-  int b = line.find(p, lane, lo, rq);
-  Tile u = tile_at<SC>(p, rq, lo);
+  int b;
+  Tile u;
+  int ka, kb;
+  if constexpr (SC == kPrefix) {
+    b = 0;   // (its pages: the first request's)
+    prefix_piece(p, g, rq, u, ka, kb, kStepKeys);
+    if (u.rows <= 0) return;   // (fewer tokens than the launch was sized for)
+  } else {
+    b = line.find(p, lane, lo, rq);
+    u = tile_at<SC>(p, rq, lo);
+  }
   for (long long x = lo; x < hi;) {
-    if (x >= rq.base + p.Hkv * rq.head) {
-      b = line.find(p, lane, x, rq);
-      u = tile_at<SC>(p, rq, x);
-    } else if (x >= u.begin + u.len) {
-      next_tile<SC>(p, rq, u);
+    bool starts = true, ends = false;
+    if constexpr (SC == kPrefix) {
+      x = hi;
+    } else {
+      if (x >= rq.base + p.Hkv * rq.head) {
+        b = line.find(p, lane, x, rq);
+        u = tile_at<SC>(p, rq, x);
+      } else if (x >= u.begin + u.len) {
+        next_tile<SC>(p, rq, u);
+      }
+      const long long end = hi < u.begin + u.len ? hi : u.begin + u.len;
+      ka = key_at<SC>(u, x - u.begin, kStepKeys);
+      kb = key_at<SC>(u, end - u.begin, kStepKeys);
+      starts = x == u.begin;
+      ends = end == u.begin + u.len;
+      x = end;
+      if (starts && !ends && tid == 0) note_begun(p, line, rq, u, g);
     }
-    const long long end = hi < u.begin + u.len ? hi : u.begin + u.len;
-    const int ka = key_at<SC>(u, x - u.begin, kStepKeys), kb = key_at<SC>(u, end - u.begin, kStepKeys);
-    const bool starts = x == u.begin, ends = end == u.begin + u.len;
-    x = end;
-    if (starts && !ends && tid == 0) note_begun(p, line, rq, u, g);
     const int row0 = wave * 32;
     const int rows = u.rows;
     RowLoads<D> ql;
@@ -857,18 +967,26 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
     unsigned char* const mine = lds + wave * (32 * row_bytes<D>());   // (of no step: between pieces)
     RowState<D> s;
     take_rows<D, SC>(s, ql, p, u, row0, lane, mine);
+    if constexpr (SC == kTail) {
+      if (starts && rq.skip) take_prefix(s, p, rq, u, row0, lane, 0, 1);
+    }
     f32x16 st[2];
     u32x4 w[2][2];
-    u32x4 op[2][D / 16];
+    // At D = 256 and 16 bits, eight operands at a time: two blocks' whole ones
+    // (128 registers) beside 192 of accumulators and queries and 64 of tiles on
+    // their way did not fit, and the step spilled.
+    constexpr bool HALVES = D == 256 && BITS == 16;
+    u32x4 op[2][HALVES ? 8 : D / 16];
     // Operands from a ring slot: one address, offsets in the instructions.
     auto operands = [&](uint32_t lds, int ring) {
       uint32_t a = lds + ring * (4 * BE) + lane * 16;
       asm("" : "+v"(a));
       return reinterpret_cast<const lds_u32x4*>(a);
     };
-    auto ask = [&](u32x4 (&to)[D / 16], const lds_u32x4* from, int j) {
+    constexpr int OPS = HALVES ? 8 : D / 16;
+    auto ask = [&](u32x4 (&to)[OPS], const lds_u32x4* from, int j) {   // the j-th so many of a step's
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) to[i] = from[(j * (D / 16) + i) * 64];
+      for (int i = 0; i < OPS; ++i) to[i] = from[(j * OPS + i) * 64];
       __builtin_amdgcn_sched_barrier(0);
     };
     auto keys = [&] {
@@ -893,27 +1011,67 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
     auto products = [&](int n) {
       const lds_u32x4* v = operands(vlds, v0);
       const lds_u32x4* k = operands(klds, k0);
-      auto add = [&](const u32x4 (&from)[D / 16], int j) {
-        add_values<D, BITS, false, false>(s, w[j], 0, 0, Sight{}, h2, [&](int t, int jj) { return from[2 * t + jj]; });
-        __builtin_amdgcn_sched_barrier(0);
-      };
-      auto score = [&](const u32x4 (&from)[D / 16], int j) {
-        f32x16 one[1];
-        scores<D, 1>(s, one, [&](int, int i) { return from[i]; });
-        st[j] = one[0];
-        __builtin_amdgcn_sched_barrier(0);
-      };
-      if (VR == 2) ask(op[0], v, 0);
-      ask(op[1], v, 1);
-      add(op[0], 0);
-      ask(op[0], k, 0);
-      store_k(n + 1);
-      add(op[1], 1);
-      ask(op[1], k, 1);
-      store_v();
-      score(op[0], 0);
-      load_next(n);
-      score(op[1], 1);
+      if constexpr (HALVES) {   // quarters c of the step: half c % 2 of block c / 2's operands
+        auto add = [&](const u32x4 (&from)[OPS], int c) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            f32x16& o = s.o[4 * (c & 1) + i / 2];
+            o = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, from[i]),
+                                                        __builtin_bit_cast(bf16x8, w[c >> 1][i & 1]), o, 0, 0, 0);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        };
+        auto score = [&](const u32x4 (&from)[OPS], int c) {
+          if (!(c & 1)) st[c >> 1] = f32x16{};
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            st[c >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, from[i]),
+                                                                 s.q[8 * (c & 1) + i], st[c >> 1], 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
+        };
+        ask(op[0], v, 0);
+        ask(op[1], v, 1);
+        add(op[0], 0);
+        ask(op[0], v, 2);
+        add(op[1], 1);
+        ask(op[1], v, 3);
+        add(op[0], 2);
+        ask(op[0], k, 0);
+        store_k(n + 1);
+        add(op[1], 3);
+        ask(op[1], k, 1);
+        store_v();
+        score(op[0], 0);
+        ask(op[0], k, 2);
+        score(op[1], 1);
+        ask(op[1], k, 3);
+        load_next(n);
+        score(op[0], 2);
+        score(op[1], 3);
+      }
+      if constexpr (!HALVES) {
+        auto add = [&](const u32x4 (&from)[OPS], int j) {
+          add_values<D, BITS, false, false>(s, w[j], 0, 0, Sight{}, h2, [&](int t, int jj) { return from[2 * t + jj]; });
+          __builtin_amdgcn_sched_barrier(0);
+        };
+        auto score = [&](const u32x4 (&from)[OPS], int j) {
+          f32x16 one[1];
+          scores<D, 1>(s, one, [&](int, int i) { return from[i]; });
+          st[j] = one[0];
+          __builtin_amdgcn_sched_barrier(0);
+        };
+        if (VR == 2) ask(op[0], v, 0);
+        ask(op[1], v, 1);
+        add(op[0], 0);
+        ask(op[0], k, 0);
+        store_k(n + 1);
+        add(op[1], 1);
+        ask(op[1], k, 1);
+        store_v();
+        score(op[0], 0);
+        load_next(n);
+        score(op[1], 1);
+      }
     };
     // Scores to weights. (They are not to be touched before the barrier that ends
     // the products phase: moved ahead of it, the softmax would keep the other
@@ -1061,7 +1219,7 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
           *reinterpret_cast<u32x4*>(out_row(p, rq.lo + u.tok, u.h, row0 + r + u.off) + ln % LPR * 8) = v;
       }
     } else if (row0 < rows) {
-      const size_t slot = 2 * (size_t)g + (starts ? 1 : 0);
+      const size_t slot = SC == kPrefix ? (size_t)g : 2 * (size_t)g + (starts ? 1 : 0);
 #pragma unroll
       for (int t = 0; t < D / 32; ++t)
 #pragma unroll
@@ -1137,6 +1295,9 @@ __global__ __launch_bounds__(kPT, D == 256 ? 1 : 2) void attn_few_kernel(PAttn p
     RowState<D> s;
     __syncthreads();   // the previous piece's reads of s_o are done
     take_rows<D, SC>(s, q, p, u, 0, lane, reinterpret_cast<unsigned char*>(s_o[wave]));
+    if constexpr (SC == kTail) {   // (each wave its share of the prefix's pieces)
+      if (starts && rq.skip) take_prefix(s, p, rq, u, 0, lane, wave, 4);
+    }
     float* const scales = s_o[wave];   // 8 bits: a block's scales, on their way to the lanes that need them
     auto block = [&](int blk, auto mask) {
       constexpr bool MASK = decltype(mask)::value;
@@ -1402,5 +1563,33 @@ int launch_scope(const char* who, const PAttn& p, const AttnPlan& a, int D, int 
   }
 }
 int launch_window(const char* who, const PAttn& p, const AttnPlan& a, int D, int bits, hipStream_t st);
+
+// The shared prefix's row tiles of a kv head, and the pieces of keys that each
+// falls into: about what fills the CUs, whole rounds of them.
+struct PrefixPlan {
+  int RT, tiles, pieces;
+  size_t slots(int Hkv) const { return (size_t)Hkv * tiles * pieces; }
+  size_t bytes(int Hkv, int D) const { return slots(Hkv) * RT * (D + 2) * sizeof(float); }
+};
+inline PrefixPlan prefix_plan(int Hq, int Hkv, int D, int T, int prefix) {
+  PrefixPlan a;
+  a.RT = D == 256 ? 128 : 256;
+  a.tiles = (int)(((long long)T * (Hq / Hkv) + a.RT - 1) / a.RT);
+  a.pieces = 1;
+  const int cus = device_cus() / 8 * 8 > 0 ? device_cus() / 8 * 8 : 8, steps = (prefix + kStepKeys - 1) / kStepKeys;
+  const long long units = (long long)Hkv * a.tiles;
+  double best = 1e30;
+  for (int np = 1; np <= 64 && np <= (steps + 1) / 2; ++np) {
+    // Rounds of workgroups, each its steps and the cost of a start and an end (four
+    // steps'); a piece's partial is read once more (an eighth of a step).
+    const double cost = (double)((units * np + cus - 1) / cus) * ((steps + np - 1) / np + 4) + 0.125 * np;
+    if (cost < best) {
+      best = cost;
+      a.pieces = np;
+    }
+  }
+  return a;
+}
+int launch_shared(const char* who, PAttn p, const AttnPlan& a, const PrefixPlan& pre, int D, int bits, hipStream_t st);
 
 }  // namespace mtp

@@ -26,7 +26,7 @@ __all__ = ["paged_sdpa"]
 
 def paged_sdpa(queries: torch.Tensor, cache: PagedKVCache, block_table: Any, q_start: Any, row_off: Any = None, *,
                max_rows: int | None = None, scale: float | None = None, window: int | None = None, sinks: int = 0,
-               out: torch.Tensor | None = None) -> torch.Tensor:
+               shared: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
     """``softmax(scale q k^T) v`` with grouped heads: ``queries`` [T, Hq, D] bf16
     (Hq 1 to 32 times the cache's kv heads) to ``[T, Hq, D]``.
 
@@ -44,6 +44,11 @@ def paged_sdpa(queries: torch.Tensor, cache: PagedKVCache, block_table: Any, q_s
     (``window`` of them), and with ``sinks`` the first so many of its request
     too. What no new token sees is not read: the pages that hold nothing else may
     have been given back (-1 in the table).
+    ``shared``: the first so many positions of all requests are the same keys, in
+    the same pages (the rows of ``block_table`` begin alike; the first one is
+    read). A batch that shares a long prefix then reads it once instead of once
+    for each request; the result is the same up to the order of sums. Requests
+    that begin inside it are as without. Not together with a window.
     ``scale`` is positive; default ``1 / sqrt(D)``. Refused inside
     ``exact_verify(True)``: how a row's sums are split depends on the lengths of
     the call's other requests."""
@@ -62,7 +67,7 @@ def paged_sdpa(queries: torch.Tensor, cache: PagedKVCache, block_table: Any, q_s
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError(f"scale must be positive and finite (got {scale})")
-    scope = _scope(window, sinks)
+    scope = _scope(window, sinks, int(shared), width * cache.page_size)
     if out is None:
         out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=device)
         ot, oh = Hq * D, D
@@ -74,7 +79,8 @@ def paged_sdpa(queries: torch.Tensor, cache: PagedKVCache, block_table: Any, q_s
     if T == 0:
         return out
     rows = T // B if off is None else 0 if max_rows is None else min(max(0, int(max_rows)), T)
-    ws = _workspace(device, Hq, Hkv, D, rows)
+    ws = _workspace(device, Hq, Hkv, D, rows) if scope is None or not scope.shared else \
+        _shared_workspace(device, Hq, Hkv, D, rows, T, B, scope.shared)
     a = cache._block(_lib.PagedAttnArgs)
     a.q, a.out, a.block_table, a.q_start = q.data_ptr(), out.data_ptr(), table.data_ptr(), start.data_ptr()
     if off is not None:
@@ -90,17 +96,22 @@ def paged_sdpa(queries: torch.Tensor, cache: PagedKVCache, block_table: Any, q_s
     return out
 
 
-def _scope(window: int | None, sinks: int) -> _lib.AttnScope | None:
-    """What a row sees, as an argument block (None: all up to itself)."""
+def _scope(window: int | None, sinks: int, shared: int, covered: int) -> _lib.AttnScope | None:
+    """What a row sees and what requests share, as an argument block (None: all
+    up to itself, and nothing)."""
     window, sinks = None if window is None else int(window), int(sinks)
     if sinks < 0 or (window is not None and window < 1):
         raise ValueError(f"window must be positive and sinks not negative (got {window}, {sinks})")
-    if window is None:
-        if sinks:
-            raise ValueError("sinks belong to a window: without one every earlier token is visible")
-        return None
-    # (no position of a table reaches 2^31: a longer one hides nothing)
-    return _lib.AttnScope(min(window, 2 ** 31 - 1), min(sinks, 2 ** 31 - 1))
+    if sinks and window is None:
+        raise ValueError("sinks belong to a window: without one every earlier token is visible")
+    if not 0 <= shared <= covered:
+        raise ValueError(f"shared must lie in the {covered} positions of the table (got {shared})")
+    if shared and window is not None:
+        raise ValueError("a window and shared positions do not go together")
+    if shared:
+        return _lib.AttnScope(0, 0, shared)
+    # (no position of a table reaches 2^31: a longer window hides nothing)
+    return None if window is None else _lib.AttnScope(min(window, 2 ** 31 - 1), min(sinks, 2 ** 31 - 1), 0)
 
 
 _SPACES: dict = {}
@@ -124,3 +135,14 @@ def _workspace(device, Hq: int, Hkv: int, D: int, rows: int) -> torch.Tensor:
         nb = _lib.query("mtp_paged_attn_workspace_bytes", Hq, Hkv, D, rows)
         ws = _SPACES[key] = _lib.WORKSPACES.get(nb, "paged_attn", device)
     return ws
+
+
+def _shared_workspace(device, Hq: int, Hkv: int, D: int, rows: int, T: int, B: int, shared: int) -> torch.Tensor:
+    """The same for a call with a shared prefix, whose partials grow with its rows."""
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            return _shared_workspace(device, Hq, Hkv, D, rows, T, B, shared)
+    nb = _lib.query("mtp_paged_attn_shared_workspace_bytes", Hq, Hkv, D, rows, T, B, shared)
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nb, dtype=torch.uint8, device=device)
+    return _lib.WORKSPACES.get(nb, "paged_attn_shared", device)

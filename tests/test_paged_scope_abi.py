@@ -21,7 +21,9 @@ def test_argument_block():
     assert _ctypes_fields(_lib.AttnScope) == want
 
 
-@pytest.mark.parametrize("kw", [dict(window=0), dict(window=-5), dict(window=4, sinks=-1)])
+@pytest.mark.parametrize("kw", [dict(window=0), dict(window=-5), dict(window=4, sinks=-1), dict(shared=-1),
+                                dict(shared=32, window=4), dict(shared=32, sinks=4), dict(sinks=4),
+                                dict(shared=193)])   # (the table covers 192)
 def test_bad_scopes(kw):
     assert _run(_attn()[1], _lib.AttnScope(**kw)) == -1
     assert _lib.load().mtp_last_error().decode().startswith("mtp_paged_attn_scoped")
@@ -31,6 +33,15 @@ def test_bad_scopes(kw):
 def test_bad_calls(bad):
     assert _run(_attn(**bad)[1], _lib.AttnScope(window=8, sinks=1)) < 0
     assert _lib.load().mtp_last_error().decode().startswith("mtp_paged_attn_scoped")
+
+
+def test_workspace_bytes():
+    plain = _lib.query("mtp_paged_attn_workspace_bytes", 40, 8, 128, 1)
+    q = lambda *a: _lib.query("mtp_paged_attn_shared_workspace_bytes", *a)  # noqa: E731
+    assert q(40, 8, 128, 1, 16, 16, 8192) > plain and q(40, 8, 128, 1, 16, 16, 0) == plain
+    assert q(40, 8, 128, 1, 1, 1, 8192) == plain and q(3, 2, 128, 1, 16, 16, 8192) == 0   # nobody to share with
+    block = _attn(T=4, B=2, width=100, ws_bytes=_lib.query("mtp_paged_attn_workspace_bytes", 4, 2, 64, 2))[1]
+    assert _run(block, _lib.AttnScope(shared=6400)) == -3
 
 
 def test_null_blocks():
