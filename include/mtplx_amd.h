@@ -671,12 +671,11 @@ int mtp_paged_attn(const mtp_paged_attn_args* args, void* stream);
  * are the same keys, in the pages of the table's first row; whole blocks of 32
  * of them may be read once for the rows of all requests. The result is
  * mtp_paged_attn's up to the order of sums; a request that begins inside them
- * reads its own keys. Workspace: mtp_paged_attn_workspace_bytes, with shared > 0
- * mtp_paged_attn_shared_workspace_bytes. */
+ * reads its own keys. */
 typedef struct mtp_attn_scope {
   int window, sinks, shared;
 } mtp_attn_scope;
-size_t mtp_paged_attn_shared_workspace_bytes(int Hq, int Hkv, int D, int max_rows, int T, int B, int shared);
+size_t mtp_paged_attn_scoped_workspace_bytes(int Hq, int Hkv, int D, int max_rows, int T, int B, int shared);
 int mtp_paged_attn_scoped(const mtp_paged_attn_args* args, const mtp_attn_scope* scope, void* stream);
 
 #ifdef __cplusplus

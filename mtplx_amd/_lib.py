@@ -86,7 +86,7 @@ SIGNATURES = {
     "mtp_paged_read": (_i, [_vp, _vp]),
     "mtp_paged_attn_workspace_bytes": (_sz, [_i, _i, _i, _i]),
     "mtp_paged_attn": (_i, [_vp, _vp]),
-    "mtp_paged_attn_shared_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
+    "mtp_paged_attn_scoped_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
     "mtp_paged_attn_scoped": (_i, [_vp, _vp, _vp]),
 }
 

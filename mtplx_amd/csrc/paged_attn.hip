@@ -15,11 +15,13 @@ static bool sharing(int Hq, int Hkv, int T, int B, int prefix) {
   return prefix >= 2 * kStepKeys && B > 1;
 }
 
-MTP_API size_t mtp_paged_attn_shared_workspace_bytes(int Hq, int Hkv, int D, int max_rows, int T, int B, int shared) {
-  const size_t tail = mtp_paged_attn_workspace_bytes(Hq, Hkv, D, max_rows);
+MTP_API size_t mtp_paged_attn_scoped_workspace_bytes(int Hq, int Hkv, int D, int max_rows, int T, int B, int shared) {
+  const size_t plain = mtp_paged_attn_workspace_bytes(Hq, Hkv, D, max_rows);
+  if (!plain || T < 1 || B < 1) return plain;
+  const size_t own = scoped_bytes(attn_plan(Hq, Hkv, D, max_rows), D, B, Hkv, shared > 0);
   const int prefix = shared / kBlk * kBlk;
-  if (!tail || T < 1 || B < 1 || shared < 1 || !sharing(Hq, Hkv, T, B, prefix)) return tail;
-  return tail + prefix_plan(Hq, Hkv, D, T, prefix).bytes(Hkv, D);
+  if (shared < 1) return own;
+  return sharing(Hq, Hkv, T, B, prefix) ? own + prefix_plan(Hq, Hkv, D, T, prefix).bytes(Hkv, D) : plain;
 }
 
 static int paged_attn(const char* who, const mtp_paged_attn_args* a, const mtp_attn_scope* scope, void* stream) {
@@ -54,7 +56,6 @@ static int paged_attn(const char* who, const mtp_paged_attn_args* a, const mtp_a
   }
   const int max_rows = a->row_off ? a->max_rows : a->T / a->B;
   const AttnPlan plan = attn_plan(a->Hq, a->Hkv, a->D, max_rows);
-  const size_t tail = mtp_paged_attn_workspace_bytes(a->Hq, a->Hkv, a->D, max_rows);
   PrefixPlan pre = {};
   const int prefix = scope ? scope->shared / kBlk * kBlk : 0;
   if (scope && scope->shared > 0) {
@@ -67,7 +68,13 @@ static int paged_attn(const char* who, const mtp_paged_attn_args* a, const mtp_a
     else
       pre = prefix_plan(a->Hq, a->Hkv, a->D, a->T, prefix);
   }
-  const size_t need = tail + pre.bytes(a->Hkv, a->D);
+  if (scope && (long long)a->B * a->Hkv > 1 << 23) {
+    set_error("%s: %d requests of %d kv heads are more than 2^23", who, a->B, a->Hkv);
+    return MTP_ERR_UNSUPPORTED;
+  }
+  const size_t own = scope ? scoped_bytes(plan, a->D, a->B, a->Hkv, scope->shared > 0)
+                           : mtp_paged_attn_workspace_bytes(a->Hq, a->Hkv, a->D, max_rows);
+  const size_t need = own + pre.bytes(a->Hkv, a->D);
   if (!a->ws || !aligned16(a->ws) || a->ws_bytes < need) {
     set_error("%s: workspace %zu B < required %zu B (or unaligned)", who, a->ws_bytes, need);
     return MTP_ERR_WORKSPACE;
@@ -84,8 +91,10 @@ static int paged_attn(const char* who, const mtp_paged_attn_args* a, const mtp_a
   p.row_off = a->row_off;
   p.status = a->status;
   p.part_o = (float*)a->ws;
-  p.part_ml = p.part_o + (size_t)2 * plan.G * plan.RT * a->D;
-  p.begun = reinterpret_cast<int4*>(p.part_ml + (size_t)2 * plan.G * plan.RT * 2);
+  p.splits = scope && plan.few ? dealt_splits(plan, a->B, a->Hkv) : 0;
+  const size_t slots = p.splits ? dealt_slots(plan, a->B, a->Hkv, scope->shared > 0) : (size_t)2 * plan.G;
+  p.part_ml = p.part_o + slots * plan.RT * a->D;
+  p.begun = reinterpret_cast<int4*>(p.part_ml + slots * plan.RT * 2);
   p.T = a->T;
   p.B = a->B;
   p.width = a->width;
@@ -110,7 +119,7 @@ static int paged_attn(const char* who, const mtp_paged_attn_args* a, const mtp_a
   if (!scope) return launch_scope<kCausal>(who, p, plan, a->D, a->bits, st);
   if (scope->shared > 0) {
     p.prefix = prefix;
-    p.prefix_o = (const float*)((const unsigned char*)a->ws + tail);
+    p.prefix_o = (const float*)((const unsigned char*)a->ws + own);
     p.prefix_ml = p.prefix_o + pre.slots(a->Hkv) * pre.RT * a->D;
     return launch_shared(who, p, plan, pre, a->D, a->bits, st);
   }

@@ -90,6 +90,7 @@ struct PAttn {
   int tile_cost;
   int window, sinks;   // kWindow
   long long most;      // kWindow: most line that a tile takes
+  int splits;          // few rows, kWindow and kTail: most pieces of a request's head
   // kPrefix, kTail: keys of the shared prefix (whole blocks), its row tiles of a
   // kv head, their rows, the pieces that each is cut into by keys; kTail: their
   // partials, laid out as part_o and part_ml, slot (head, piece, tile).
@@ -172,6 +173,13 @@ __device__ __forceinline__ int prefix_tokens(const PAttn& p) {
   return n < 0 ? 0 : n < p.T ? n : p.T;
 }
 
+__device__ __forceinline__ bool behind_prefix(const PAttn& p, const ReqRows& rows, long long start) {
+  // (With few rows the join adds the prefix to a request's first tile alone: one
+  // that brings more rows than were announced does without.)
+  return start >= p.prefix && rows.lo + rows.n <= prefix_tokens(p) &&
+         (p.splits == 0 || (long long)rows.n * p.rep <= 1 << p.rt_log2);
+}
+
 // A lane's request of the line (64 requests at a time), its rows and length.
 struct LaneReq {
   ReqRows rows;
@@ -187,7 +195,7 @@ __device__ __forceinline__ LaneReq lane_req(const PAttn& p, int b) {
     if constexpr (SC == kTail) {
       // The prefix is done for a request that lies behind it; one that does not
       // (or whose rows are not among the list's) sees its keys from the first on.
-      if (r.start >= p.prefix && r.rows.lo + r.rows.n <= prefix_tokens(p)) r.skip = p.prefix / kBlk;
+      if (behind_prefix(p, r.rows, r.start)) r.skip = p.prefix / kBlk;
       r.start -= r.skip * kBlk;
     }
     r.len = head_len<SC>(p, r.start, r.rows.n);
@@ -310,6 +318,50 @@ __device__ __forceinline__ Tile tile_at(const PAttn& p, const Req& r, long long 
   u.begin = r.base + u.h * r.head + scope_len<SC>(p, q0, r.n, a);
   set_tile<SC>(p, r, u);
   return u;
+}
+
+// Few rows, kWindow and kTail: no line. Lengths are alike (a window's) or short (a
+// tail's), so every request's head is cut into pieces of the same number of
+// keys, workgroup (request, head, piece) takes one, and what a workgroup has to
+// know of the others is that number. The line's search, a wave's first 1500
+// instructions, took as long as a decode step's keys.
+template <int SC>
+__device__ __forceinline__ long long dealt_keys(const PAttn& p, int b) {
+  const ReqRows rows = req_rows(p.row_off, b, p.B, p.T);
+  long long start = p.q_start[b];
+  const long long cap = (long long)p.width * p.bpp * kBlk;
+  if constexpr (SC == kTail) {
+    if (behind_prefix(p, rows, start)) start -= p.prefix;
+  }
+  long long n = start + rows.n;
+  n = n > cap ? cap : n;
+  if constexpr (SC == kWindow) {
+    const long long most = (long long)p.window + p.sinks + rows.n + 2 * kBlk;
+    n = n < most ? n + kBlk : most;   // (a block may count twice)
+  }
+  return rows.n < 1 || n < 0 ? 0 : n;
+}
+// Keys of a piece: what spreads all keys over the CUs, no less than a block for
+// each wave, and no more pieces than there are workgroups for.
+template <int SC>
+__device__ __forceinline__ int dealt_piece(const PAttn& p, int lane) {
+  long long sum = 0, top = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    const long long n = b0 + lane < p.B ? dealt_keys<SC>(p, b0 + lane) : 0;
+    sum += n;
+    top = n > top ? n : top;
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    sum += __shfl_xor(sum, off, 64);
+    const long long o = __shfl_xor(top, off, 64);
+    top = o > top ? o : top;
+  }
+  sum = uniform64(sum) * p.Hkv;
+  top = uniform64(top);
+  const long long share = div_small(sum, p.G) + 1, least = div_small(top, p.splits) + 1;
+  const long long c = share > least ? share : least;
+  return c <= p.min_share ? p.min_share : (int)((c + kBlk - 1) & -(long long)kBlk);
 }
 
 // Workgroup g's piece of the prefix: tile u of the list rq, keys [ka, kb). Its
@@ -678,34 +730,60 @@ __device__ __forceinline__ float4* part_block(const PAttn& p, size_t slot, int R
 }
 
 // What the prefix left for the lane's row (row0 + lane % 32 of the tile):
-// pieces k0, k0 + dk, .. of it, as the row's state.
+// pieces k0, k0 + dk, .. of it, as the row's state. Lanes without a row (a
+// decode step's tile holds few) take a share of the pieces instead, as in the
+// join, and add theirs to the row's at the end.
+struct PrefixRow {
+  const float4* o;    // of piece 0, its (32 rows, 32 d) blocks from here on
+  const float2* ml;
+  size_t o_step, ml_step;   // to the next piece
+};
+template <int D>
+__device__ __forceinline__ PrefixRow prefix_row(const PAttn& p, int h, int row) {   // row: of the prefix's list
+  const int RT = 1 << p.prefix_rt_log2, t = row >> p.prefix_rt_log2, rr = row & (RT - 1);
+  const size_t slot = (size_t)h * p.prefix_pieces * p.prefix_tiles + t;
+  return {reinterpret_cast<const float4*>(p.prefix_o) + (slot * (RT / 32) + (rr >> 5)) * (D / 32) * 256 + (rr & 31),
+          reinterpret_cast<const float2*>(p.prefix_ml) + slot * RT + rr, (size_t)p.prefix_tiles * RT * D / 4,
+          (size_t)p.prefix_tiles * RT};
+}
 template <int D>
 __device__ __forceinline__ void take_prefix(RowState<D>& s, const PAttn& p, const Req& rq, const Tile& u, int row0,
                                             int lane, int k0, int dk) {
-  const int h2 = lane >> 5, r = row0 + (lane & 31);
+  int NR = 32;
+  while (NR > 4 && u.rows - row0 <= NR / 2) NR >>= 1;
+  const int h2 = lane >> 5, r = row0 + (lane & (NR - 1));
   if (r >= u.rows) return;
-  const int row = (rq.lo + u.tok) * p.rep + u.off + r, RT = 1 << p.prefix_rt_log2;   // (of the prefix's list)
-  const int t = row >> p.prefix_rt_log2, rr = row & (RT - 1);
-  auto slot = [&](int k) { return (size_t)(u.h * p.prefix_pieces + k) * p.prefix_tiles + t; };
-  auto ml = [&](int k) { return *reinterpret_cast<const float2*>(p.prefix_ml + (slot(k) * RT + rr) * 2); };
+  const PrefixRow pr = prefix_row<D>(p, u.h, (rq.lo + u.tok) * p.rep + u.off + r);
+  k0 += dk * ((lane & 31) / NR);
+  dk *= 32 / NR;
   float m = -INFINITY;
-  for (int k = k0; k < p.prefix_pieces; k += dk) m = fmaxf(m, ml(k).x);
+#pragma unroll 4
+  for (int k = k0; k < p.prefix_pieces; k += dk) m = fmaxf(m, pr.ml[k * pr.ml_step].x);
+  for (int off = NR; off < 32; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
   float l = 0.f;
+#pragma unroll 1
   for (int k = k0; k < p.prefix_pieces; k += dk) {
-    const float2 a = ml(k);
+    const float2 a = pr.ml[k * pr.ml_step];
+    const float4* o = pr.o + k * pr.o_step;
+    float4 v[D / 8];
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) v[i] = o[i / 4 * 256 + (2 * (i % 4) + h2) * 32];
     const float w = a.x == -INFINITY ? 0.f : exp2_fast(a.x - m);
     l += a.x == -INFINITY ? a.y : a.y * w;   // (no score: 0 or NaN)
-    const float4* o = reinterpret_cast<const float4*>(p.prefix_o) + (slot(k) * (RT / 32) + (rr >> 5)) * (D / 32) * 256;
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+      s.o[i / 4][i % 4 * 4] += w == 0.f ? 0.f : v[i].x * w;
+      s.o[i / 4][i % 4 * 4 + 1] += w == 0.f ? 0.f : v[i].y * w;
+      s.o[i / 4][i % 4 * 4 + 2] += w == 0.f ? 0.f : v[i].z * w;
+      s.o[i / 4][i % 4 * 4 + 3] += w == 0.f ? 0.f : v[i].w * w;
+    }
+  }
+  for (int off = NR; off < 32; off <<= 1) {
+    l += __shfl_xor(l, off, 64);
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float4 v = o[i * 256 + (2 * j + h2) * 32 + (rr & 31)];
-        s.o[i][4 * j] += w == 0.f ? 0.f : v.x * w;
-        s.o[i][4 * j + 1] += w == 0.f ? 0.f : v.y * w;
-        s.o[i][4 * j + 2] += w == 0.f ? 0.f : v.z * w;
-        s.o[i][4 * j + 3] += w == 0.f ? 0.f : v.w * w;
-      }
+      for (int j = 0; j < 16; ++j) s.o[i][j] += __shfl_xor(s.o[i][j], off, 64);
   }
   s.m = m;
   s.l = h2 == 0 ? l : 0.f;   // (the halves' sums are added at the end)
@@ -730,12 +808,15 @@ __device__ __forceinline__ uint16_t* out_row(const PAttn& p, int token, int h, i
   return p.out + ((long long)token + i) * p.out_token + (long long)(h * p.rep + g) * p.out_head;
 }
 
+constexpr int kWithPrefix = 1 << 30;
+
 // What the join needs to know of the tile that workgroup g begins and others
 // finish (at most one).
 template <int SC>
 __device__ __forceinline__ void note_begun(const PAttn& p, const Line<SC>& line, const Req& rq, const Tile& u, int g) {
   const int last = line.owner(u.begin + u.len - 1);
-  p.begun[g] = make_int4(u.rows | u.off << 16, (last < line.G ? last : line.G - 1) - g + 1, rq.lo + u.tok, u.h);
+  const int pieces = (last < line.G ? last : line.G - 1) - g + 1;
+  p.begun[g] = make_int4(u.rows | u.off << 16, pieces | (SC == kTail && rq.skip ? kWithPrefix : 0), rq.lo + u.tok, u.h);
 }
 
 // The v-th counted block of a windowed tile; `absent`: it has no page.
@@ -968,7 +1049,7 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
     RowState<D> s;
     take_rows<D, SC>(s, ql, p, u, row0, lane, mine);
     if constexpr (SC == kTail) {
-      if (starts && rq.skip) take_prefix(s, p, rq, u, row0, lane, 0, 1);
+      if (starts && ends && rq.skip) take_prefix(s, p, rq, u, row0, lane, 0, 1);   // (else: the join)
     }
     f32x16 st[2];
     u32x4 w[2][2];
@@ -1251,26 +1332,71 @@ __global__ __launch_bounds__(kPT, D == 256 ? 1 : 2) void attn_few_kernel(PAttn p
   __shared__ float s_m[4][32], s_l[4][32];
   const int tid = threadIdx.x, lane = tid & 63, c32 = lane & 31, h2 = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Line<SC> line(p, lane);
+  constexpr bool DEALT = SC != kCausal;
+  const Line<DEALT ? kPrefix : SC> line(p, lane);   // (dealt: none)
   const int g = blockIdx.x;
-  if (tid == 0) p.begun[g] = make_int4(0, 0, 0, 0);
-  if (g >= line.G) return;
-  const long long lo = line.lo(g), hi = line.hi(g);
   Req rq;
-  int b = line.find(p, lane, lo, rq);
-  Tile u = tile_at<SC>(p, rq, lo);
+  int b, piece = 0, share = 0, head = 0;   // dealt: the workgroup's piece, keys of one, (request, kv head)
+  Tile u;
+  long long lo = 0, hi = 0;
+  if constexpr (DEALT) {
+    share = dealt_piece<SC>(p, lane);
+    // First pieces first: the last ones may not be there, and neighbours go to
+    // different XCDs (with a head's pieces as neighbours, some XCDs had none).
+    piece = g / (p.B * p.Hkv);
+    head = g - piece * (p.B * p.Hkv);
+    b = head / p.Hkv;
+    u.h = head - b * p.Hkv;
+    const ReqRows rows = req_rows(p.row_off, b, p.B, p.T);
+    rq.lo = rows.lo;
+    rq.n = rows.n;
+    rq.start = p.q_start[b];
+    rq.skip = SC == kTail && behind_prefix(p, rows, rq.start) ? p.prefix / kBlk : 0;
+    rq.start -= rq.skip * kBlk;
+    hi = tile_count(p, rq.n);   // its tiles: the first in pieces, others (rows that were not announced) whole
+    if (piece == 0 && tid == 0) p.begun[head] = make_int4(0, 0, 0, 0);
+  } else {
+    if (tid == 0) p.begun[g] = make_int4(0, 0, 0, 0);
+    if (g >= line.G) return;
+    lo = line.lo(g);
+    hi = line.hi(g);
+    b = line.find(p, lane, lo, rq);
+    u = tile_at<SC>(p, rq, lo);
+  }
   for (long long x = lo; x < hi;) {
-    if (x >= rq.base + p.Hkv * rq.head) {
-      b = line.find(p, lane, x, rq);
-      u = tile_at<SC>(p, rq, x);
-    } else if (x >= u.begin + u.len) {
-      next_tile<SC>(p, rq, u);
+    int ka, kb;
+    bool starts = true, ends = true;
+    if constexpr (DEALT) {
+      u.t = (int)x++;
+      if (u.t > 0 && u.t % p.splits != piece) continue;
+      set_tile<SC>(p, rq, u);
+      const int n = SC == kWindow ? u.nkeys : u.nk;
+      ka = 0;
+      kb = n;
+      if (u.t == 0) {
+        const int np = n > share ? div_small(n - 1, share) + 1 : 1;
+        if (piece >= np) continue;
+        ka = piece * share;
+        if (piece + 1 < np) kb = ka + share;
+        starts = ends = np == 1 && !rq.skip;   // (else the join has it)
+        if (!ends && piece == 0 && tid == 0)
+          p.begun[head] = make_int4(u.rows | u.off << 16, np | (rq.skip ? kWithPrefix : 0), rq.lo + u.tok, u.h);
+      }
+    } else {
+      if (x >= rq.base + p.Hkv * rq.head) {
+        b = line.find(p, lane, x, rq);
+        u = tile_at<SC>(p, rq, x);
+      } else if (x >= u.begin + u.len) {
+        next_tile<SC>(p, rq, u);
+      }
+      const long long end = hi < u.begin + u.len ? hi : u.begin + u.len;
+      ka = key_at<SC>(u, x - u.begin, kBlk);
+      kb = key_at<SC>(u, end - u.begin, kBlk);
+      starts = x == u.begin;
+      ends = end == u.begin + u.len;
+      x = end;
+      if (starts && !ends && tid == 0) note_begun(p, line, rq, u, g);
     }
-    const long long end = hi < u.begin + u.len ? hi : u.begin + u.len;
-    const int ka = key_at<SC>(u, x - u.begin, kBlk), kb = key_at<SC>(u, end - u.begin, kBlk);
-    const bool starts = x == u.begin, ends = end == u.begin + u.len;
-    x = end;
-    if (starts && !ends && tid == 0) note_begun(p, line, rq, u, g);
     const int rows = u.rows;
     RowLoads<D> q;
     ask_rows<D>(q, p, rq, u, 0, lane);
@@ -1295,9 +1421,6 @@ __global__ __launch_bounds__(kPT, D == 256 ? 1 : 2) void attn_few_kernel(PAttn p
     RowState<D> s;
     __syncthreads();   // the previous piece's reads of s_o are done
     take_rows<D, SC>(s, q, p, u, 0, lane, reinterpret_cast<unsigned char*>(s_o[wave]));
-    if constexpr (SC == kTail) {   // (each wave its share of the prefix's pieces)
-      if (starts && rq.skip) take_prefix(s, p, rq, u, 0, lane, wave, 4);
-    }
     float* const scales = s_o[wave];   // 8 bits: a block's scales, on their way to the lanes that need them
     auto block = [&](int blk, auto mask) {
       constexpr bool MASK = decltype(mask)::value;
@@ -1364,7 +1487,7 @@ __global__ __launch_bounds__(kPT, D == 256 ? 1 : 2) void attn_few_kernel(PAttn p
         *reinterpret_cast<float4*>(&s_o[wave][c32 * OS + 32 * t + 8 * j + 4 * h2]) =
             make_float4(s.o[t][4 * j], s.o[t][4 * j + 1], s.o[t][4 * j + 2], s.o[t][4 * j + 3]);
     __syncthreads();
-    const int slot = 2 * g + (starts ? 1 : 0);
+    const int slot = DEALT ? head * p.splits + piece : 2 * g + (starts ? 1 : 0);
     const bool whole = starts && ends;
     for (int e = tid; e < 8 * D; e += kPT) {   // (row e % 32, d = 4 (e / 32): the partials' order)
       const int r = e & 31, d = e >> 5 << 2;
@@ -1409,7 +1532,10 @@ __global__ __launch_bounds__(kPT, D == 256 ? 1 : 2) void attn_few_kernel(PAttn p
 template <int RT>
 constexpr int join_round() { return RT == 32 ? 64 : 16; }   // pieces whose weights LDS holds
 
-template <int D, int RT>
+// PRE: a tile whose request has the prefix behind it sums the prefix's pieces of
+// its rows too, after its own.
+// DEALT: pieces of few rows that were dealt without a line.
+template <int D, int RT, bool PRE, bool DEALT>
 __global__ __launch_bounds__(kPT) void attn_join_kernel(PAttn p) {
   constexpr int kJoin = join_round<RT>();
   __shared__ float s_w[kJoin][32], s_m[32], s_l[32];
@@ -1417,23 +1543,35 @@ __global__ __launch_bounds__(kPT) void attn_join_kernel(PAttn p) {
   const int tid = threadIdx.x;
   const int g = blockIdx.x;
   const int4 tile = p.begun[g];   // rows (0: none) and first head, pieces, first token, kv head
-  const int rows = tile.x & 0xffff, head0 = tile.x >> 16, np = tile.y;
+  const int rows = tile.x & 0xffff, head0 = tile.x >> 16;
+  const int own = PRE ? tile.y & (kWithPrefix - 1) : tile.y, np = PRE && tile.y & kWithPrefix ? own + p.prefix_pieces : own;
   const int rb = blockIdx.y / (D / 32), t = blockIdx.y % (D / 32);
   const int r0 = 32 * rb;
   if (r0 >= rows) return;
   // Piece k's slot: the one that begins the tile is g's second.
-  auto slot = [&](int k) { return (size_t)(2 * (g + k) + (k == 0 ? 1 : 0)); };
+  auto slot = [&](int k) { return DEALT ? (size_t)g * p.splits + k : (size_t)(2 * (g + k) + (k == 0 ? 1 : 0)); };
   int NR = 32;   // (chunks' tiles: always, so that the loop below is a plain one)
   while (RT == 32 && NR > 4 && rows - r0 <= NR / 2) NR >>= 1;
   const int SP = 32 / NR, row = tid & (NR - 1), share = (tid & 31) / NR;
+  // The prefix's rows: those past the tile's last are its last again (never used).
+  auto list_row = [&](int r) { return tile.z * p.rep + head0 + (r0 + r < rows ? r0 + r : rows - 1); };
+  PrefixRow pr = {}, pw = {};
+  if constexpr (PRE) {
+    pr = prefix_row<D>(p, tile.w, list_row(row));
+    pw = prefix_row<D>(p, tile.w, list_row(tid >> 3));
+  }
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   constexpr int B8 = RT == 32 ? 8 : 4;   // pieces whose blocks are in flight together
   float4 a8[B8];
   auto ask = [&](int k) {   // (the last piece again past the last: never used)
 #pragma unroll
     for (int i = 0; i < B8; ++i) {
-      const int kk = k + SP * i + share;
-      a8[i] = part_block<D>(p, slot(kk < np ? kk : np - 1), RT, rb, t)[(tid & ~31) + row];
+      int kk = k + SP * i + share;
+      kk = kk < np ? kk : np - 1;
+      if (PRE && kk >= own)
+        a8[i] = pr.o[(kk - own) * pr.o_step + t * 256 + (tid & ~31)];
+      else
+        a8[i] = part_block<D>(p, slot(kk), RT, rb, t)[(tid & ~31) + row];
     }
   };
   ask(0);
@@ -1457,7 +1595,12 @@ __global__ __launch_bounds__(kPT) void attn_join_kernel(PAttn p) {
       for (int i = 0; i < kJoin / 8; ++i) {
         const int k = 8 * i + x;
         a[i] = make_float2(-INFINITY, 0.f);
-        if (live && k < n) a[i] = *reinterpret_cast<const float2*>(p.part_ml + (slot(k0 + k) * RT + r0 + rr) * 2);
+        if (live && k < n) {
+          if (PRE && k0 + k >= own)
+            a[i] = pw.ml[(k0 + k - own) * pw.ml_step];
+          else
+            a[i] = *reinterpret_cast<const float2*>(p.part_ml + (slot(k0 + k) * RT + r0 + rr) * 2);
+        }
       }
 #pragma unroll
       for (int i = 0; i < kJoin / 8; ++i) m = fmaxf(m, a[i].x);
@@ -1536,17 +1679,20 @@ inline AttnPlan attn_plan(int Hq, int Hkv, int D, int max_rows) {
 template <int D, int BITS, int SC>
 int launch_attn(const char* who, const PAttn& p, const AttnPlan& a, hipStream_t st) {
   constexpr int NW = chunk_waves<D>();
+  constexpr bool DEALT = SC != kCausal;
+  const unsigned tiles = a.few && DEALT ? (unsigned)(p.B * p.Hkv) : (unsigned)p.G;
   if (a.few)
-    hipLaunchKernelGGL((attn_few_kernel<D, BITS, SC>), dim3((unsigned)p.G), dim3(kPT), 0, st, p);
+    hipLaunchKernelGGL((attn_few_kernel<D, BITS, SC>), dim3(DEALT ? tiles * p.splits : tiles), dim3(kPT), 0, st, p);
   else
-    hipLaunchKernelGGL((attn_chunk_kernel<D, BITS, SC>), dim3((unsigned)p.G), dim3(64 * NW), 0, st, p);
+    hipLaunchKernelGGL((attn_chunk_kernel<D, BITS, SC>), dim3(tiles), dim3(64 * NW), 0, st, p);
   const int rc = launch_check(who);
   if (rc) return rc;
+  if (SC == kWindow && a.few && p.splits == 1) return rc;   // (every head whole)
   const int blocks = a.RT / 32 * (D / 32);
   if (a.few)
-    hipLaunchKernelGGL((attn_join_kernel<D, 32>), dim3((unsigned)p.G, blocks), dim3(kPT), 0, st, p);
+    hipLaunchKernelGGL((attn_join_kernel<D, 32, SC == kTail, DEALT>), dim3(tiles, blocks), dim3(kPT), 0, st, p);
   else
-    hipLaunchKernelGGL((attn_join_kernel<D, 32 * NW>), dim3((unsigned)p.G, blocks), dim3(kPT), 0, st, p);
+    hipLaunchKernelGGL((attn_join_kernel<D, 32 * NW, SC == kTail, false>), dim3(tiles, blocks), dim3(kPT), 0, st, p);
   return launch_check(who);
 }
 
@@ -1563,6 +1709,21 @@ int launch_scope(const char* who, const PAttn& p, const AttnPlan& a, int D, int 
   }
 }
 int launch_window(const char* who, const PAttn& p, const AttnPlan& a, int D, int bits, hipStream_t st);
+
+// Pieces that a request's head may fall into when few rows are dealt: two
+// rounds of workgroups at most (a piece that is not there costs its start).
+inline int dealt_splits(const AttnPlan& a, int B, int Hkv) {
+  const long long n = 2LL * a.G / ((long long)B * Hkv);
+  return n < 1 ? 1 : n > 128 ? 128 : (int)n;
+}
+inline size_t dealt_slots(const AttnPlan& a, int B, int Hkv, bool shared) {
+  const int n = dealt_splits(a, B, Hkv);
+  return n == 1 && !shared ? 0 : (size_t)B * Hkv * n;   // (whole heads leave no partials)
+}
+inline size_t scoped_bytes(const AttnPlan& a, int D, int B, int Hkv, bool shared) {
+  const size_t slots = a.few ? dealt_slots(a, B, Hkv, shared) : 2 * (size_t)a.G;
+  return slots * a.RT * (D + 2) * sizeof(float) + (a.few ? (size_t)B * Hkv : (size_t)a.G) * sizeof(int4);
+}
 
 // The shared prefix's row tiles of a kv head, and the pieces of keys that each
 // falls into: about what fills the CUs, whole rounds of them.

@@ -79,8 +79,8 @@ def paged_sdpa(queries: torch.Tensor, cache: PagedKVCache, block_table: Any, q_s
     if T == 0:
         return out
     rows = T // B if off is None else 0 if max_rows is None else min(max(0, int(max_rows)), T)
-    ws = _workspace(device, Hq, Hkv, D, rows) if scope is None or not scope.shared else \
-        _shared_workspace(device, Hq, Hkv, D, rows, T, B, scope.shared)
+    ws = _workspace(device, Hq, Hkv, D, rows) if scope is None else \
+        _scoped_workspace(device, Hq, Hkv, D, rows, T, B, scope.shared)
     a = cache._block(_lib.PagedAttnArgs)
     a.q, a.out, a.block_table, a.q_start = q.data_ptr(), out.data_ptr(), table.data_ptr(), start.data_ptr()
     if off is not None:
@@ -137,12 +137,13 @@ def _workspace(device, Hq: int, Hkv: int, D: int, rows: int) -> torch.Tensor:
     return ws
 
 
-def _shared_workspace(device, Hq: int, Hkv: int, D: int, rows: int, T: int, B: int, shared: int) -> torch.Tensor:
-    """The same for a call with a shared prefix, whose partials grow with its rows."""
+def _scoped_workspace(device, Hq: int, Hkv: int, D: int, rows: int, T: int, B: int, shared: int) -> torch.Tensor:
+    """The same for a call with a window or a shared prefix, whose partials grow
+    with its requests and rows."""
     if torch.cuda.current_device() != device.index:
         with torch.cuda.device(device):
-            return _shared_workspace(device, Hq, Hkv, D, rows, T, B, shared)
-    nb = _lib.query("mtp_paged_attn_shared_workspace_bytes", Hq, Hkv, D, rows, T, B, shared)
+            return _scoped_workspace(device, Hq, Hkv, D, rows, T, B, shared)
+    nb = _lib.query("mtp_paged_attn_scoped_workspace_bytes", Hq, Hkv, D, rows, T, B, shared)
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(nb, dtype=torch.uint8, device=device)
-    return _lib.WORKSPACES.get(nb, "paged_attn_shared", device)
+    return _lib.WORKSPACES.get(nb, "paged_attn_scoped", device)

@@ -91,6 +91,30 @@ def test_matches_float64(gpu, prefix, tails, n, Hq, H, D, page, bits):
     c.check_status()
 
 
+def test_more_rows_than_announced(gpu):
+    """max_rows costs time, not results: too small for one request, or for all."""
+    rng = np.random.default_rng(41)
+    for D, bits in ((128, 16), (64, 8), (256, 16)):
+        n, tails = [2, 45, 1, 90], [300, 45, 41, 120]
+        c, table, shared = batch(rng, 640, tails, D, 2, 64, bits)
+        lengths = [640 + t for t in tails]
+        q = rows(rng, sum(n), 8, D)
+        start, off = i32([e - m for e, m in zip(lengths, n)]), i32(np.concatenate([[0], np.cumsum(n)]))
+        for max_rows in (1, 2, 8, 45, 1000):
+            got = paged_sdpa(q, c, table, start, off, max_rows=max_rows, shared=shared)
+            check(c, table, q, n, lengths, got, what=f"max_rows={max_rows}")
+
+
+def test_many_requests(gpu):
+    """More heads than workgroups for the tails."""
+    rng = np.random.default_rng(42)
+    tails = [1 + 7 * i % 90 for i in range(300)]
+    c, table, shared = batch(rng, 512, tails, 64, 4, 64, 16, poison=False)
+    q = rows(rng, 300, 4, 64)
+    got = paged_sdpa(q, c, table, i32([511 + t for t in tails]), shared=shared)
+    check(c, table, q, [1] * 300, [512 + t for t in tails], got)
+
+
 @pytest.mark.parametrize("bits", [8, 16])
 def test_long_prefixes(gpu, bits):
     rng = np.random.default_rng(5 + bits)

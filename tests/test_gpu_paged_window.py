@@ -73,6 +73,29 @@ def test_matches_float64(gpu, n, lengths, Hq, H, D, page, bits, window, sinks):
     c.check_status()   # pages given back were not asked for
 
 
+def test_more_rows_than_announced(gpu):
+    """max_rows costs time, not results: too small for one request, or for all."""
+    rng = np.random.default_rng(41)
+    for D, bits, window, sinks in ((128, 16, 70, 5), (64, 8, 300, 0), (256, 16, 40, 33)):
+        n, lengths = [2, 45, 1, 90], [300, 200, 41, 90]
+        c, table = _filled(rng, lengths, D, 2, 64, bits)
+        q = rows(rng, sum(n), 8, D)
+        start, off = i32([e - m for e, m in zip(lengths, n)]), i32(np.concatenate([[0], np.cumsum(n)]))
+        for max_rows in (1, 2, 8, 45, 1000):
+            got = paged_sdpa(q, c, table, start, off, max_rows=max_rows, window=window, sinks=sinks)
+            check(c, table, q, n, lengths, got, window, sinks, what=f"max_rows={max_rows}")
+
+
+def test_many_requests(gpu):
+    """More heads than workgroups: each whole in one."""
+    rng = np.random.default_rng(42)
+    lengths = [1 + 7 * i % 400 for i in range(600)]
+    c, table = _filled(rng, lengths, 64, 4, 64, 16, poison=False)
+    q = rows(rng, 600, 4, 64)
+    got = paged_sdpa(q, c, table, i32([e - 1 for e in lengths]), window=100, sinks=3)
+    check(c, table, q, [1] * 600, lengths, got, 100, 3)
+
+
 @pytest.mark.parametrize("bits", [8, 16])
 def test_long_contexts_and_whole_prompts(gpu, bits):
     rng = np.random.default_rng(77 + bits)

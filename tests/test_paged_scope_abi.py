@@ -29,7 +29,8 @@ def test_bad_scopes(kw):
     assert _lib.load().mtp_last_error().decode().startswith("mtp_paged_attn_scoped")
 
 
-@pytest.mark.parametrize("bad", [dict(q=None), dict(ws=None), dict(ws_bytes=64), dict(Hq=3), dict(D=80), dict(scale=0.0)])
+@pytest.mark.parametrize("bad", [dict(q=None), dict(ws=None), dict(ws_bytes=64), dict(Hq=3), dict(D=80), dict(scale=0.0),
+                                 dict(B=1 << 23, row_off=0x1000)])
 def test_bad_calls(bad):
     assert _run(_attn(**bad)[1], _lib.AttnScope(window=8, sinks=1)) < 0
     assert _lib.load().mtp_last_error().decode().startswith("mtp_paged_attn_scoped")
@@ -37,10 +38,12 @@ def test_bad_calls(bad):
 
 def test_workspace_bytes():
     plain = _lib.query("mtp_paged_attn_workspace_bytes", 40, 8, 128, 1)
-    q = lambda *a: _lib.query("mtp_paged_attn_shared_workspace_bytes", *a)  # noqa: E731
-    assert q(40, 8, 128, 1, 16, 16, 8192) > plain and q(40, 8, 128, 1, 16, 16, 0) == plain
+    q = lambda *a: _lib.query("mtp_paged_attn_scoped_workspace_bytes", *a)  # noqa: E731
+    assert q(40, 8, 128, 1, 16, 16, 8192) > q(40, 8, 128, 1, 16, 16, 0) > 0
     assert q(40, 8, 128, 1, 1, 1, 8192) == plain and q(3, 2, 128, 1, 16, 16, 8192) == 0   # nobody to share with
-    block = _attn(T=4, B=2, width=100, ws_bytes=_lib.query("mtp_paged_attn_workspace_bytes", 4, 2, 64, 2))[1]
+    assert q(40, 8, 128, 1, 2000, 2000, 0) == 2000 * 8 * 16                               # every head whole
+    assert q(40, 8, 128, 1, 2000, 2000, 64) == plain                                      # too short to share
+    block = _attn(T=4, B=2, width=100, ws_bytes=q(4, 2, 64, 2, 4, 2, 0))[1]
     assert _run(block, _lib.AttnScope(shared=6400)) == -3
 
 
