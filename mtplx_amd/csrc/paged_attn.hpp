@@ -341,8 +341,10 @@ __device__ __forceinline__ long long dealt_keys(const PAttn& p, int b) {
   }
   return rows.n < 1 || n < 0 ? 0 : n;
 }
-// Keys of a piece: what spreads all keys over the CUs, no less than a block for
-// each wave, and no more pieces than there are workgroups for.
+// Most keys of a piece: what spreads all keys over the CUs, no less than a block
+// for each wave, and no more pieces than there are workgroups for. Every head
+// ends with a piece that is not whole, half of one on average, and pieces that
+// are one too many for the CUs cost a second round.
 template <int SC>
 __device__ __forceinline__ int dealt_piece(const PAttn& p, int lane) {
   long long sum = 0, top = 0;
@@ -359,7 +361,8 @@ __device__ __forceinline__ int dealt_piece(const PAttn& p, int lane) {
   }
   sum = uniform64(sum) * p.Hkv;
   top = uniform64(top);
-  const long long share = div_small(sum, p.G) + 1, least = div_small(top, p.splits) + 1;
+  const int heads = p.B * p.Hkv, groups = heads < p.G ? p.G - heads / 2 : p.G / 2;
+  const long long share = div_small(sum, groups) + 1, least = div_small(top, p.splits) + 1;
   const long long c = share > least ? share : least;
   return c <= p.min_share ? p.min_share : (int)((c + kBlk - 1) & -(long long)kBlk);
 }
@@ -1374,10 +1377,14 @@ __global__ __launch_bounds__(kPT, D == 256 ? 1 : 2) void attn_few_kernel(PAttn p
       ka = 0;
       kb = n;
       if (u.t == 0) {
-        const int np = n > share ? div_small(n - 1, share) + 1 : 1;
+        int np = n > share ? div_small(n - 1, share) + 1 : 1, size = n;
+        if (np > 1) {   // equal ones
+          size = (div_small(n - 1, np) + kBlk) & -kBlk;
+          np = div_small(n - 1, size) + 1;
+        }
         if (piece >= np) continue;
-        ka = piece * share;
-        if (piece + 1 < np) kb = ka + share;
+        ka = piece * size;
+        if (piece + 1 < np) kb = ka + size;
         starts = ends = np == 1 && !rq.skip;   // (else the join has it)
         if (!ends && piece == 0 && tid == 0)
           p.begun[head] = make_int4(u.rows | u.off << 16, np | (rq.skip ? kWithPrefix : 0), rq.lo + u.tok, u.h);
