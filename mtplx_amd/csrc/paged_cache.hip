@@ -231,6 +231,7 @@ struct WriteParams {
   RotRows q;
   int Hq, q_tokens, kv_groups;   // workgroups [0, kv_groups) write K and V, the others rotate q
   int nb_uniform;                // blocks of each request where row_off is null
+  int k_parts;                   // waves that share a block of K
   HeadSpec heads;                // (kernels with HEADS)
   int lanes;
 };
@@ -471,13 +472,19 @@ __device__ __forceinline__ void write_few(const WriteParams& p, int h, bool isk,
 // in the page's order, 16 bytes a lane; keys of a block that is not all new go
 // out element by element (V) or chunk by chunk (K).
 template <int D, int BITS, bool HEADS>
-__device__ __forceinline__ void write_unit(const WriteParams& p, const Unit& w, int h, bool isk, int lane,
+__device__ __forceinline__ void write_unit(const WriteParams& p, const Unit& w, int h, int part, int lane,
                                            uint16_t* rows) {
+  const bool isk = part < p.k_parts;   // (the part behind K's: V)
   constexpr int RS = row16<D>(), NC = D / 16, BS = row8<D>();   // 16-byte loads of a lane
   const long long base = w.blk * kBlk;
   // Keys [klo, khi) of the block are new; token of key kk: first + kk.
   const KeyRange range = block_keys(base, w.start, w.start + w.rows.n);
-  const int klo = range.lo, khi = range.hi;
+  int klo = range.lo, khi = range.hi;
+  if (isk && p.k_parts > 1) {   // its share of the block's keys
+    const int n = kBlk / p.k_parts;
+    klo = klo > part * n ? klo : part * n;
+    khi = khi < (part + 1) * n ? khi : (part + 1) * n;
+  }
   if (klo >= khi) return;   // (a request of no rows)
   const long long first = w.rows.lo + (base - w.start);
   u32x4 x[NC];
@@ -713,9 +720,9 @@ __global__ __launch_bounds__(64 * cache_waves<D>(), D == 256 ? 1 : 4) void paged
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   for (long long x = (long long)blockIdx.x * cache_waves<D>() + wave;; x += (long long)p.kv_groups * cache_waves<D>()) {
     Unit w;
-    const long long u = div_pos(x >> 1, p.Hkv);
+    const long long v = p.k_parts == 1 ? x >> 1 : div_pos(x, p.k_parts + 1), u = div_pos(v, p.Hkv);
     if (!find_unit(p, u, lane, w)) return;   // (no barrier follows)
-    write_unit<D, BITS, HEADS>(p, w, (int)((x >> 1) - u * p.Hkv), (x & 1) == 0, fresh(lane), lds[wave]);
+    write_unit<D, BITS, HEADS>(p, w, (int)(v - u * p.Hkv), (int)(x - v * (p.k_parts + 1)), fresh(lane), lds[wave]);
   }
 }
 
@@ -1020,7 +1027,13 @@ static int paged_write(const char* who, const mtp_paged_write_args* a, const mtp
     units = (long long)a->B * p.nb_uniform;
   }
   const int waves = a->D == 256 ? cache_waves<256>() : cache_waves<128>();
-  long long groups = (units * 2 * a->Hkv + waves - 1) / waves;
+  // A block of rotated K is turned by one wave (a row's angles are computed once
+  // for both halves) or, where blocks are few and have many new keys, by eight,
+  // four keys each (a lane per chunk, write_few): written and read back, 512 rows
+  // of 8 heads 21 us by eight and 27 by one, 1000 rows 28 and 29, 2000 38 and 32;
+  // decode rows gain nothing.
+  p.k_parts = a->dims > 0 && units * a->Hkv <= 272 && a->T >= 8 * units ? 8 : 1;
+  long long groups = (units * (p.k_parts + 1) * a->Hkv + waves - 1) / waves;
   if (groups > 1 << 20) groups = 1 << 20;
   p.kv_groups = (int)groups;
   if (a->q) {
