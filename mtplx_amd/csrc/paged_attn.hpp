@@ -449,15 +449,22 @@ struct RowState {
 // infinity in any element; the same in every lane.
 template <int D, class VO>
 __device__ __forceinline__ uint32_t odd_keys(VO vop, int h2) {
-  // An exponent of all ones plus one carries into the sign's place, half by half.
+  // Magnitudes by their bits: at or past 0x7f80 there is no number.
+  typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+  u16x8 top = {};
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+    for (int jj = 0; jj < 2; ++jj)
+      top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x8, u32x4(vop(t, jj) & 0x7fff7fffu)));
+  const u32x4 most = __builtin_bit_cast(u32x4, top) + 0x00800080u;   // (a carry into the sign's place, half by half)
+  if (!__any((most.x | most.y | most.z | most.w) & 0x80008000u)) return 0;
   u32x4 a0 = {}, a1 = {};
 #pragma unroll
   for (int t = 0; t < D / 32; ++t) {
     a0 |= (vop(t, 0) & 0x7f807f80u) + 0x00800080u;
     a1 |= (vop(t, 1) & 0x7f807f80u) + 0x00800080u;
   }
-  const u32x4 a = a0 | a1;
-  if (!__any((a.x | a.y | a.z | a.w) & 0x80008000u)) return 0;
   auto two = [&](uint32_t w, int i) {
     return (w >> 15 & 1u) << v_slot_key(h2, 2 * i) | (w >> 31) << v_slot_key(h2, 2 * i + 1);
   };
@@ -512,23 +519,17 @@ __device__ __forceinline__ void soften(RowState<D>& s, f32x16 (&st)[KB], u32x4 (
   // and scale and maximum go into one FMA.
   constexpr bool RAW = BITS == 16 && !MASK;
   const int bound = s.bound - kt;
-  // A row's keys [from, from + span] of a block, from its half's first on.
-  int from[KB];
-  uint32_t span[KB];
+  // WIN: the keys that the row sees, a bit each, from its half's first on.
+  uint32_t vis[KB];
   if constexpr (WIN && MASK) {
 #pragma unroll
     for (int j = 0; j < KB; ++j) {
       const Range k = seen(s, sight[j]);
-      from[j] = k.lo - 4 * h2;
-      span[j] = (uint32_t)(k.hi - k.lo);
-      if (k.hi < k.lo) {   // none: no key's distance from there is 0
-        from[j] = -0x40000000;
-        span[j] = 0;
-      }
+      vis[j] = k.hi < k.lo ? 0u : ((2u << k.hi) - 1u & ~((1u << k.lo) - 1u)) >> (4 * h2);   // (2 << 31 is 0)
     }
   }
+  auto shown = [&](int j, int r) { return (uint32_t)__builtin_amdgcn_sbfe((int)vis[j], 8 * (r >> 2) + (r & 3), 1); };
   auto hidden = [&](int j, int r) {   // (one comparison of a constant with what block j's registers share)
-    if constexpr (WIN && MASK) return (uint32_t)(8 * (r >> 2) + (r & 3) - from[j]) > span[j];
     const int last = (bound < end[j] - 1 - kt ? bound : end[j] - 1 - kt) - 32 * j - 4 * h2;
     return 8 * (r >> 2) + (r & 3) > last;
   };
@@ -539,7 +540,12 @@ __device__ __forceinline__ void soften(RowState<D>& s, f32x16 (&st)[KB], u32x4 (
     for (int r = 0; r < 16; ++r) {
       float x = st[j][r];
       if (!RAW) x *= BITS == 8 ? ks(j, r) : scale_log2;
-      if (MASK && hidden(j, r)) x = -INFINITY;
+      if constexpr (WIN && MASK) {
+        const uint32_t m = shown(j, r);
+        x = __uint_as_float((__float_as_uint(x) & m) | (0xff800000u & ~m));
+      } else {
+        if (MASK && hidden(j, r)) x = -INFINITY;
+      }
       st[j][r] = x;
       top = __builtin_elementwise_maximum(top, x);   // (no quieting of each x; a NaN makes its row NaN)
     }
@@ -580,8 +586,13 @@ __device__ __forceinline__ void soften(RowState<D>& s, f32x16 (&st)[KB], u32x4 (
       sum += a + b;
       if (BITS == 8) {
         const float va = vs(j, r), vb = vs(j, r + 1);
-        a = MASK && hidden(j, r) ? 0.f : a * va;   // (a hidden key's scale may be NaN; of one that is seen it shows)
-        b = MASK && hidden(j, r + 1) ? 0.f : b * vb;
+        if constexpr (WIN && MASK) {
+          a = __uint_as_float(__float_as_uint(a * va) & shown(j, r));
+          b = __uint_as_float(__float_as_uint(b * vb) & shown(j, r + 1));
+        } else {
+          a = MASK && hidden(j, r) ? 0.f : a * va;   // (a hidden key's scale may be NaN; of one that is seen it shows)
+          b = MASK && hidden(j, r + 1) ? 0.f : b * vb;
+        }
       }
       pk[r / 2] = f2bf2(a, b);
     }
