@@ -123,9 +123,13 @@ __device__ __forceinline__ long long tiles_len(long long q0, int n, int P, long 
   const long long f = t < full ? t : full;
   return t * q0 + P * (f * (f + 1) / 2) + (t - f) * n;
 }
-// The same where no tile takes more than `most`.
+// The same where no tile takes more than `most`. Where the first ones, which
+// see less, are few, all count as the others: tiles then end where equal shares
+// of whole tiles do.
+__device__ __forceinline__ bool tiles_alike(long long q0, int n, long long most) { return q0 + n >= 4 * most; }
 __device__ __forceinline__ long long tiles_len(long long q0, int n, int P, long long t, long long most) {
   if (q0 + n <= most) return tiles_len(q0, n, P, t);
+  if (tiles_alike(q0, n, most)) return t * most;
   const long long room = most - q0, under = room > 0 ? (long long)((uint32_t)room / (uint32_t)P) : 0;   // (room < n)
   return t <= under ? tiles_len(q0, n, P, t) : tiles_len(q0, n, P, under) + (t - under) * most;
 }
@@ -225,6 +229,14 @@ struct Line {
     // Equal shares, a whole number of steps each, no shorter than min_share.
     const long long s = W > 0 ? (W - 1) / p.G + 1 : 0;
     S = s > p.min_share ? (s + p.step - 1) & -(long long)p.step : p.min_share;
+    if constexpr (SC == kWindow) {
+      // Three tiles a workgroup and more: whole ones, if at most a tenth of the
+      // workgroups' time is lost that way. A tile cut in two starts twice, and its
+      // partials are written and joined.
+      const long long q = div_small(W, p.G * p.most) + 1, row = p.G * p.most;
+      const long long whole = (q - 1) * row == W ? q - 1 : q;
+      if (whole >= 3 && 10 * whole * row <= 11 * W) S = whole * p.most;
+    }
     G = W > 0 ? div_small(W - 1, S) + 1 : 0;
   }
   __device__ __forceinline__ long long lo(int g) const { return g * S; }
@@ -287,7 +299,7 @@ __device__ __forceinline__ void set_tile(const PAttn& p, const Req& r, Tile& u) 
   u.off = first - u.tok * p.rep;
   const long long cost = (long long)(u.t + 1) * p.P;
   u.len = clamp_start(p, r.start) + (cost < r.n ? cost : r.n);
-  if (SC == kWindow && u.len > p.most) u.len = p.most;
+  if (SC == kWindow && (u.len > p.most || tiles_alike(clamp_start(p, r.start), r.n, p.most))) u.len = p.most;
   u.pos = r.start + u.tok;
   const long long cap = (long long)p.width * p.bpp * kBlk - (SC == kTail ? r.skip * kBlk : 0);
   if constexpr (SC == kTail) u.gap = r.skip;
@@ -610,10 +622,12 @@ __device__ __forceinline__ void soften(RowState<D>& s, f32x16 (&st)[KB], u32x4 (
 // WIN: by `sight`.
 template <int D, int BITS, bool MASK, bool WIN, class VO>
 __device__ __forceinline__ void add_values(RowState<D>& s, const u32x4 (&w)[2], int kt, int end, const Sight& sight,
-                                           int h2, VO vop) {
+                                           int h2, VO vop, bool odd_values = true) {
   u32x4 keep0 = {}, keep1 = {};
   uint32_t odd = 0;
-  if (MASK && BITS == 16) {
+  if (MASK && BITS == 16 && WIN && !odd_values) {   // (known to be finite, all of them)
+    keep0 = keep1 = ~u32x4{};
+  } else if (MASK && BITS == 16) {
     const int n = WIN ? sight.end - sight.base : end - kt;   // keys that exist
     const uint32_t have = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
     odd = odd_keys<D>(vop, h2) & have;
@@ -911,6 +925,11 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
   __shared__ __attribute__((aligned(16))) unsigned char lds[(KR + VR) * 4 * BE];   // K slots, then V's
   static_assert(NW * 32 * row_bytes<D>() <= (KR + VR) * 4 * BE, "a wave's rows turn in the slots' place");
   __shared__ __attribute__((aligned(16))) float ksc[4][kStepKeys], vsc[4][kStepKeys];   // (of step n - 1 to n + 1)
+  // kWindow, 16 bits: whether V of a step's blocks has an element that is no
+  // number, as the waves that stage it see it (each wave that needs to know
+  // looked at all of it: as many instructions as the softmax).
+  constexpr bool FLAGS = SC == kWindow && BITS == 16;
+  __shared__ int s_odd[FLAGS ? 8 : 1][2];   // (of step n % 8; that of n + 4 is cleared with n's)
   const int tid = threadIdx.x, lane = tid & 63, h2 = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Line<SC> line(p, lane);
@@ -1047,6 +1066,28 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
       v1 = VR == 3 ? v2 : v;
       v2 = v;
     };
+    auto flag_v = [&](int n) {   // step n's V, on its way to LDS
+      if constexpr (FLAGS) {
+        typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+        if (tid < 2) s_odd[(n + 4) & 7][tid] = 0;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          u16x8 top = {};
+          bool any = false;
+#pragma unroll
+          for (int i = 0; i < LD; ++i) {
+            const int c = i * NT + wave * 64;
+            if (2 * CB % NT && c >= 2 * CB) break;
+            if ((CB % NT ? c >= CB : i * NT >= CB) != (j == 1)) continue;
+            top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x8, vr[i] & 0x7fff7fffu));
+            any = true;
+          }
+          if (!any) continue;
+          const u32x4 m = __builtin_bit_cast(u32x4, top) + 0x00800080u;
+          if (__any((m.x | m.y | m.z | m.w) & 0x80008000u) && lane == 0) s_odd[n & 7][j] = 1;
+        }
+      }
+    };
     auto store_k = [&](int n) {   // of step n (slot k1 when n is the next step)
       put(klds + k1 * (4 * BE), kr);
       if (BITS == 8 && tid < kStepKeys) {
@@ -1054,7 +1095,10 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
         vsc[n & 3][tid] = vscale;
       }
     };
-    auto store_v = [&] { put(vlds + (VR == 3 ? v2 : v1) * (4 * BE), vr); };   // of step n + 1 (two slots: n)
+    auto store_v = [&](int n) {   // of step n + 1 (two slots: n)
+      put(vlds + (VR == 3 ? v2 : v1) * (4 * BE), vr);
+      flag_v(n + VR - 2);
+    };
     if (nstep > 0) {   // step 0 in LDS (its V on the way, of two slots), step 1 on its way
       load(0, false);
       load(0, true);
@@ -1098,7 +1142,8 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
 #pragma unroll
       for (int j = 0; j < 2; ++j)
         add_values<D, BITS, true, SC == kWindow>(s, w[j], ka + n * kStepKeys + 32 * j, ends2(n, j), sight(n, j), h2,
-                                                 [&](int t, int jj) { return v[(j * (D / 16) + 2 * t + jj) * 64]; });
+                                                 [&](int t, int jj) { return v[(j * (D / 16) + 2 * t + jj) * 64]; },
+                                                 FLAGS ? __builtin_amdgcn_readfirstlane(s_odd[n & 7][j]) != 0 : true);
     };
     // Both products of step n, no key hidden: each eight operands are asked for
     // eight matrix instructions ahead (left alone, the compiler reads one, waits
@@ -1135,7 +1180,7 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
         store_k(n + 1);
         add(op[1], 3);
         ask(op[1], k, 1);
-        store_v();
+        store_v(n);
         score(op[0], 0);
         ask(op[0], k, 2);
         score(op[1], 1);
@@ -1162,7 +1207,7 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
         store_k(n + 1);
         add(op[1], 1);
         ask(op[1], k, 1);
-        store_v();
+        store_v(n);
         score(op[0], 0);
         load_next(n);
         score(op[1], 1);
@@ -1189,6 +1234,7 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
     };
     constexpr std::true_type yes;
     constexpr std::false_type no;
+    if (FLAGS && tid < 16) s_odd[tid >> 1][tid & 1] = 0;
     lds_barrier();   // every wave has its rows
     if (nstep > 0) {
       put(klds, kr);
@@ -1199,12 +1245,13 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
       load(1, false);
       if (VR == 3) {
         put(vlds, vr);
+        flag_v(0);
         load(1, true);
       }
       lds_barrier();
       auto stage = [&](int n) {   // what goes with step n's products
         store_k(n + 1);
-        store_v();
+        store_v(n);
         cover(n > 0 ? n - 1 : 0, n + 2);
         load_next(n);
       };
