@@ -10,18 +10,42 @@ MTP_API size_t mtp_paged_attn_workspace_bytes(int Hq, int Hkv, int D, int max_ro
   return (size_t)2 * a.G * a.RT * (D + 2) * sizeof(float) + (size_t)a.G * 16;
 }
 
-// Whether the prefix is worth a pass of its own.
-static bool sharing(int Hq, int Hkv, int T, int B, int prefix) {
-  return prefix >= 2 * kStepKeys && B > 1;
+// Whether the prefix is worth a pass of its own: calls of few rows alone (a
+// chunk's tile of 256 rows reads K and V once for all of them as it is; tails of
+// many rows lost at every prefix but the longest). One tile of rows a request,
+// 40 heads over 8, 16 bits, tails of 400: two requests behind 1024 keys 20.6 us
+// shared and 19.9 not, behind 2048 20.9 and 22.6; four behind 512 21.0 and 21.8,
+// behind 8192 27 and 38; 32 with four rows each behind 1024 40 and 39, behind
+// 8192 56 and 113. Several tiles: sixteen requests of eight rows behind 1024 48
+// and 36, behind 4096 53 and 61, behind 16384 71 and 161; four of sixteen behind
+// 4096 41 and 37, behind 16384 52 and 64.
+static bool sharing(const AttnPlan& a, int B, int prefix) {
+  if (!a.few || B < 2) return false;
+  if (a.tiles == 1) return prefix >= (B < 4 ? 2048 : 1024);
+  return prefix >= (B < 8 ? 16384 : 4096);
+}
+
+// Whether a windowed call of few rows is dealt (each of its tiles reads the
+// window) or takes chunk tiles of 256 rows, of which it fills few: at most two
+// tiles always, else up to so many keys in all. 40 heads over 8 of 128, 16 bits:
+// sixteen requests of 40 rows a kv head behind 4096 63 us dealt and 67 as chunks
+// (8 bits 46 and 71), four of 240 behind 1024 35 and 35, behind 4096 69 and 44 (8
+// bits 47 and 51); sixteen of 96, head dim 256, behind 4096 124 and 166.
+static bool window_dealt(const AttnPlan& a, int Hkv, int D, int bits, int B, long long keys) {
+  if (!a.few || a.tiles <= 2) return a.few;
+  return (long long)B * Hkv * a.tiles * keys <= (1LL << 18) * (bits == 8 ? 4 : 1) * (D == 256 ? 4 : 1);
 }
 
 MTP_API size_t mtp_paged_attn_scoped_workspace_bytes(int Hq, int Hkv, int D, int max_rows, int T, int B, int shared) {
   const size_t plain = mtp_paged_attn_workspace_bytes(Hq, Hkv, D, max_rows);
   if (!plain || T < 1 || B < 1) return plain;
-  const size_t own = scoped_bytes(attn_plan(Hq, Hkv, D, max_rows), D, B, Hkv, shared > 0);
+  const AttnPlan a = attn_plan(Hq, Hkv, D, max_rows, true);
   const int prefix = shared / kBlk * kBlk;
-  if (shared < 1) return own;
-  return sharing(Hq, Hkv, T, B, prefix) ? own + prefix_plan(Hq, Hkv, D, T, prefix).bytes(Hkv, D) : plain;
+  if (shared > 0)
+    return sharing(a, B, prefix) ? scoped_bytes(a, D, B, Hkv, true) + prefix_plan(Hq, Hkv, D, T, prefix).bytes(Hkv, D)
+                                 : plain;
+  const size_t dealt = scoped_bytes(a, D, B, Hkv, false), chunk = scoped_bytes(attn_plan(Hq, Hkv, D, 0), D, B, Hkv, false);
+  return a.few && a.tiles <= 2 ? dealt : dealt > chunk ? dealt : chunk;   // (the keys decide which, else)
 }
 
 static int paged_attn(const char* who, const mtp_paged_attn_args* a, const mtp_attn_scope* scope, void* stream) {
@@ -55,21 +79,28 @@ static int paged_attn(const char* who, const mtp_paged_attn_args* a, const mtp_a
     return MTP_ERR_ARG;
   }
   const int max_rows = a->row_off ? a->max_rows : a->T / a->B;
-  const AttnPlan plan = attn_plan(a->Hq, a->Hkv, a->D, max_rows);
+  AttnPlan plan = attn_plan(a->Hq, a->Hkv, a->D, max_rows, scope != nullptr);
   PrefixPlan pre = {};
   const int prefix = scope ? scope->shared / kBlk * kBlk : 0;
+  const long long covered = (long long)a->width * a->page_size;
   if (scope && scope->shared > 0) {
-    if (scope->shared > (long long)a->width * a->page_size) {
+    if (scope->shared > covered) {
       set_error("%s: %d shared positions are more than the table covers", who, scope->shared);
       return MTP_ERR_ARG;
     }
-    if (!sharing(a->Hq, a->Hkv, a->T, a->B, prefix))
-      scope = nullptr;   // each request reads its own keys, as without
-    else
+    if (!sharing(plan, a->B, prefix)) {   // each request reads its own keys, as without
+      scope = nullptr;
+      plan = attn_plan(a->Hq, a->Hkv, a->D, max_rows);
+    } else {
       pre = prefix_plan(a->Hq, a->Hkv, a->D, a->T, prefix);
+    }
+  } else if (scope) {
+    const long long keys = (long long)scope->window + scope->sinks;
+    if (!window_dealt(plan, a->Hkv, a->D, a->bits, a->B, keys < covered ? keys : covered))
+      plan = attn_plan(a->Hq, a->Hkv, a->D, 0);
   }
-  if (scope && (long long)a->B * a->Hkv > 1 << 23) {
-    set_error("%s: %d requests of %d kv heads are more than 2^23", who, a->B, a->Hkv);
+  if (scope && (long long)a->B * a->Hkv > 1 << 20) {
+    set_error("%s: %d requests of %d kv heads are more than 2^20", who, a->B, a->Hkv);
     return MTP_ERR_UNSUPPORTED;
   }
   const size_t own = scope ? scoped_bytes(plan, a->D, a->B, a->Hkv, scope->shared > 0)
@@ -91,6 +122,7 @@ static int paged_attn(const char* who, const mtp_paged_attn_args* a, const mtp_a
   p.row_off = a->row_off;
   p.status = a->status;
   p.part_o = (float*)a->ws;
+  p.tiles = scope ? plan.tiles : 0;
   p.splits = scope && plan.few ? dealt_splits(plan, a->B, a->Hkv) : 0;
   const size_t slots = p.splits ? dealt_slots(plan, a->B, a->Hkv, scope->shared > 0) : (size_t)2 * plan.G;
   p.part_ml = p.part_o + slots * plan.RT * a->D;

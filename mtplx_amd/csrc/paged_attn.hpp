@@ -90,7 +90,8 @@ struct PAttn {
   int tile_cost;
   int window, sinks;   // kWindow
   long long most;      // kWindow: most line that a tile takes
-  int splits;          // few rows, kWindow and kTail: most pieces of a request's head
+  int splits;          // few rows, kWindow and kTail: most pieces of a tile
+  int tiles;           // and tiles of a request's head that are dealt
   // kPrefix, kTail: keys of the shared prefix (whole blocks), its row tiles of a
   // kv head, their rows, the pieces that each is cut into by keys; kTail: their
   // partials, laid out as part_o and part_ml, slot (head, piece, tile).
@@ -178,10 +179,10 @@ __device__ __forceinline__ int prefix_tokens(const PAttn& p) {
 }
 
 __device__ __forceinline__ bool behind_prefix(const PAttn& p, const ReqRows& rows, long long start) {
-  // (With few rows the join adds the prefix to a request's first tile alone: one
-  // that brings more rows than were announced does without.)
+  // (The join adds the prefix to the tiles that were dealt: a request that brings
+  // more rows than were announced does without.)
   return start >= p.prefix && rows.lo + rows.n <= prefix_tokens(p) &&
-         (p.splits == 0 || (long long)rows.n * p.rep <= 1 << p.rt_log2);
+         (long long)rows.n * p.rep <= (long long)p.tiles << p.rt_log2;
 }
 
 // A lane's request of the line (64 requests at a time), its rows and length.
@@ -333,8 +334,8 @@ __device__ __forceinline__ Tile tile_at(const PAttn& p, const Req& r, long long 
 }
 
 // Few rows, kWindow and kTail: no line. Lengths are alike (a window's) or short (a
-// tail's), so every request's head is cut into pieces of the same number of
-// keys, workgroup (request, head, piece) takes one, and what a workgroup has to
+// tail's), so every tile is cut into pieces of the same number of keys,
+// workgroup (request, head, tile, piece) takes one, and what a workgroup has to
 // know of the others is that number. The line's search, a wave's first 1500
 // instructions, took as long as a decode step's keys.
 template <int SC>
@@ -354,7 +355,7 @@ __device__ __forceinline__ long long dealt_keys(const PAttn& p, int b) {
   return rows.n < 1 || n < 0 ? 0 : n;
 }
 // Most keys of a piece: what spreads all keys over the CUs, no less than a block
-// for each wave, and no more pieces than there are workgroups for. Every head
+// for each wave, and no more pieces than there are workgroups for. Every tile
 // ends with a piece that is not whole, half of one on average, and pieces that
 // are one too many for the CUs cost a second round.
 template <int SC>
@@ -371,9 +372,9 @@ __device__ __forceinline__ int dealt_piece(const PAttn& p, int lane) {
     const long long o = __shfl_xor(top, off, 64);
     top = o > top ? o : top;
   }
-  sum = uniform64(sum) * p.Hkv;
+  sum = uniform64(sum) * (p.Hkv * p.tiles);
   top = uniform64(top);
-  const int heads = p.B * p.Hkv, groups = heads < p.G ? p.G - heads / 2 : p.G / 2;
+  const int units = p.B * p.Hkv * p.tiles, groups = units < p.G ? p.G - units / 2 : p.G / 2;
   const long long share = div_small(sum, groups) + 1, least = div_small(top, p.splits) + 1;
   const long long c = share > least ? share : least;
   return c <= p.min_share ? p.min_share : (int)((c + kBlk - 1) & -(long long)kBlk);
@@ -757,10 +758,7 @@ __device__ __forceinline__ float4* part_block(const PAttn& p, size_t slot, int R
   return reinterpret_cast<float4*>(p.part_o) + ((slot * (RT / 32) + rb) * (D / 32) + t) * 256;
 }
 
-// What the prefix left for the lane's row (row0 + lane % 32 of the tile):
-// pieces k0, k0 + dk, .. of it, as the row's state. Lanes without a row (a
-// decode step's tile holds few) take a share of the pieces instead, as in the
-// join, and add theirs to the row's at the end.
+// What the prefix left for a row of its list: the pieces' partials.
 struct PrefixRow {
   const float4* o;    // of piece 0, its (32 rows, 32 d) blocks from here on
   const float2* ml;
@@ -774,49 +772,6 @@ __device__ __forceinline__ PrefixRow prefix_row(const PAttn& p, int h, int row) 
           reinterpret_cast<const float2*>(p.prefix_ml) + slot * RT + rr, (size_t)p.prefix_tiles * RT * D / 4,
           (size_t)p.prefix_tiles * RT};
 }
-template <int D>
-__device__ __forceinline__ void take_prefix(RowState<D>& s, const PAttn& p, const Req& rq, const Tile& u, int row0,
-                                            int lane, int k0, int dk) {
-  int NR = 32;
-  while (NR > 4 && u.rows - row0 <= NR / 2) NR >>= 1;
-  const int h2 = lane >> 5, r = row0 + (lane & (NR - 1));
-  if (r >= u.rows) return;
-  const PrefixRow pr = prefix_row<D>(p, u.h, (rq.lo + u.tok) * p.rep + u.off + r);
-  k0 += dk * ((lane & 31) / NR);
-  dk *= 32 / NR;
-  float m = -INFINITY;
-#pragma unroll 4
-  for (int k = k0; k < p.prefix_pieces; k += dk) m = fmaxf(m, pr.ml[k * pr.ml_step].x);
-  for (int off = NR; off < 32; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-  float l = 0.f;
-#pragma unroll 1
-  for (int k = k0; k < p.prefix_pieces; k += dk) {
-    const float2 a = pr.ml[k * pr.ml_step];
-    const float4* o = pr.o + k * pr.o_step;
-    float4 v[D / 8];
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i) v[i] = o[i / 4 * 256 + (2 * (i % 4) + h2) * 32];
-    const float w = a.x == -INFINITY ? 0.f : exp2_fast(a.x - m);
-    l += a.x == -INFINITY ? a.y : a.y * w;   // (no score: 0 or NaN)
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i) {
-      s.o[i / 4][i % 4 * 4] += w == 0.f ? 0.f : v[i].x * w;
-      s.o[i / 4][i % 4 * 4 + 1] += w == 0.f ? 0.f : v[i].y * w;
-      s.o[i / 4][i % 4 * 4 + 2] += w == 0.f ? 0.f : v[i].z * w;
-      s.o[i / 4][i % 4 * 4 + 3] += w == 0.f ? 0.f : v[i].w * w;
-    }
-  }
-  for (int off = NR; off < 32; off <<= 1) {
-    l += __shfl_xor(l, off, 64);
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) s.o[i][j] += __shfl_xor(s.o[i][j], off, 64);
-  }
-  s.m = m;
-  s.l = h2 == 0 ? l : 0.f;   // (the halves' sums are added at the end)
-}
-
 // The factor of a row's sums in its output: a row that saw no key is zeros.
 __device__ __forceinline__ float row_factor(float m, float l) { return m == -INFINITY && l == 0.f ? 0.f : 1.f / l; }
 
@@ -844,7 +799,7 @@ template <int SC>
 __device__ __forceinline__ void note_begun(const PAttn& p, const Line<SC>& line, const Req& rq, const Tile& u, int g) {
   const int last = line.owner(u.begin + u.len - 1);
   const int pieces = (last < line.G ? last : line.G - 1) - g + 1;
-  p.begun[g] = make_int4(u.rows | u.off << 16, pieces | (SC == kTail && rq.skip ? kWithPrefix : 0), rq.lo + u.tok, u.h);
+  p.begun[g] = make_int4(u.rows | u.off << 16, pieces, rq.lo + u.tok, u.h);
 }
 
 // The v-th counted block of a windowed tile; `absent`: it has no page.
@@ -1106,9 +1061,6 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
     unsigned char* const mine = lds + wave * (32 * row_bytes<D>());   // (of no step: between pieces)
     RowState<D> s;
     take_rows<D, SC>(s, ql, p, u, row0, lane, mine);
-    if constexpr (SC == kTail) {
-      if (starts && ends && rq.skip) take_prefix(s, p, rq, u, row0, lane, 0, 1);   // (else: the join)
-    }
     f32x16 st[2];
     u32x4 w[2][2];
     // At D = 256 and 16 bits, eight operands at a time: two blocks' whole ones
@@ -1397,15 +1349,18 @@ __global__ __launch_bounds__(kPT, D == 256 ? 1 : 2) void attn_few_kernel(PAttn p
   const Line<DEALT ? kPrefix : SC> line(p, lane);   // (dealt: none)
   const int g = blockIdx.x;
   Req rq;
-  int b, piece = 0, share = 0, head = 0;   // dealt: the workgroup's piece, keys of one, (request, kv head)
+  int b, piece = 0, share = 0, unit = 0, tile0 = 0;   // dealt: piece, most keys of one, (request, kv head, tile)
   Tile u;
   long long lo = 0, hi = 0;
   if constexpr (DEALT) {
     share = dealt_piece<SC>(p, lane);
     // First pieces first: the last ones may not be there, and neighbours go to
     // different XCDs (with a head's pieces as neighbours, some XCDs had none).
-    piece = g / (p.B * p.Hkv);
-    head = g - piece * (p.B * p.Hkv);
+    const int units = p.B * p.Hkv * p.tiles;
+    piece = g / units;
+    unit = g - piece * units;
+    const int head = unit / p.tiles;
+    tile0 = unit - head * p.tiles;
     b = head / p.Hkv;
     u.h = head - b * p.Hkv;
     const ReqRows rows = req_rows(p.row_off, b, p.B, p.T);
@@ -1414,8 +1369,12 @@ __global__ __launch_bounds__(kPT, D == 256 ? 1 : 2) void attn_few_kernel(PAttn p
     rq.start = p.q_start[b];
     rq.skip = SC == kTail && behind_prefix(p, rows, rq.start) ? p.prefix / kBlk : 0;
     rq.start -= rq.skip * kBlk;
-    hi = tile_count(p, rq.n);   // its tiles: the first in pieces, others (rows that were not announced) whole
-    if (piece == 0 && tid == 0) p.begun[head] = make_int4(0, 0, 0, 0);
+    // Its tile; the first one's workgroups take those of rows that were not
+    // announced too, whole.
+    lo = tile0;
+    hi = tile_count(p, rq.n);
+    if (tile0 > 0 && hi > tile0) hi = tile0 + 1;
+    if (piece == 0 && tid == 0) p.begun[unit] = make_int4(0, 0, 0, 0);
   } else {
     if (tid == 0) p.begun[g] = make_int4(0, 0, 0, 0);
     if (g >= line.G) return;
@@ -1429,12 +1388,12 @@ __global__ __launch_bounds__(kPT, D == 256 ? 1 : 2) void attn_few_kernel(PAttn p
     bool starts = true, ends = true;
     if constexpr (DEALT) {
       u.t = (int)x++;
-      if (u.t > 0 && u.t % p.splits != piece) continue;
+      if (u.t != tile0 && (u.t < p.tiles || u.t % p.splits != piece)) continue;
       set_tile<SC>(p, rq, u);
       const int n = SC == kWindow ? u.nkeys : u.nk;
       ka = 0;
       kb = n;
-      if (u.t == 0) {
+      if (u.t == tile0) {
         int np = n > share ? div_small(n - 1, share) + 1 : 1, size = n;
         if (np > 1) {   // equal ones
           size = (div_small(n - 1, np) + kBlk) & -kBlk;
@@ -1445,7 +1404,7 @@ __global__ __launch_bounds__(kPT, D == 256 ? 1 : 2) void attn_few_kernel(PAttn p
         if (piece + 1 < np) kb = ka + size;
         starts = ends = np == 1 && !rq.skip;   // (else the join has it)
         if (!ends && piece == 0 && tid == 0)
-          p.begun[head] = make_int4(u.rows | u.off << 16, np | (rq.skip ? kWithPrefix : 0), rq.lo + u.tok, u.h);
+          p.begun[unit] = make_int4(u.rows | u.off << 16, np | (rq.skip ? kWithPrefix : 0), rq.lo + u.tok, u.h);
       }
     } else {
       if (x >= rq.base + p.Hkv * rq.head) {
@@ -1552,7 +1511,7 @@ __global__ __launch_bounds__(kPT, D == 256 ? 1 : 2) void attn_few_kernel(PAttn p
         *reinterpret_cast<float4*>(&s_o[wave][c32 * OS + 32 * t + 8 * j + 4 * h2]) =
             make_float4(s.o[t][4 * j], s.o[t][4 * j + 1], s.o[t][4 * j + 2], s.o[t][4 * j + 3]);
     __syncthreads();
-    const int slot = DEALT ? head * p.splits + piece : 2 * g + (starts ? 1 : 0);
+    const int slot = DEALT ? unit * p.splits + piece : 2 * g + (starts ? 1 : 0);
     const bool whole = starts && ends;
     for (int e = tid; e < 8 * D; e += kPT) {   // (row e % 32, d = 4 (e / 32): the partials' order)
       const int r = e & 31, d = e >> 5 << 2;
@@ -1726,11 +1685,16 @@ __global__ __launch_bounds__(kPT) void attn_join_kernel(PAttn p) {
 struct AttnPlan {
   bool few;
   int RT, P, G, min_share, step, tile_cost;
+  int tiles;   // dealt: of a request's head
 };
-inline AttnPlan attn_plan(int Hq, int Hkv, int D, int max_rows) {
+// `dealt`: a call with a window or a shared prefix, whose few rows go without a
+// line: up to eight tiles of 32 rows of a request's head.
+inline AttnPlan attn_plan(int Hq, int Hkv, int D, int max_rows, bool dealt = false) {
   const int rep = Hq / Hkv;
+  const long long rows = (long long)max_rows * rep;
   AttnPlan a;
-  a.few = max_rows > 0 && (long long)max_rows * rep <= 32;
+  a.few = rows > 0 && rows <= (dealt ? 256 : 32);
+  a.tiles = a.few ? (int)(rows + 31) / 32 : 0;
   a.RT = a.few ? 32 : D == 256 ? 128 : 256;   // chunk_waves<D>() * 32
   a.P = (a.RT + rep - 2) / rep + 1;
   a.G = a.few ? device_cus() * (D < 256 ? 2 : 1) : device_cus() / 8 * 8;   // (chunks: dealt to eight XCDs)
@@ -1745,19 +1709,19 @@ template <int D, int BITS, int SC>
 int launch_attn(const char* who, const PAttn& p, const AttnPlan& a, hipStream_t st) {
   constexpr int NW = chunk_waves<D>();
   constexpr bool DEALT = SC != kCausal;
-  const unsigned tiles = a.few && DEALT ? (unsigned)(p.B * p.Hkv) : (unsigned)p.G;
-  if (a.few)
-    hipLaunchKernelGGL((attn_few_kernel<D, BITS, SC>), dim3(DEALT ? tiles * p.splits : tiles), dim3(kPT), 0, st, p);
-  else
-    hipLaunchKernelGGL((attn_chunk_kernel<D, BITS, SC>), dim3(tiles), dim3(64 * NW), 0, st, p);
-  const int rc = launch_check(who);
-  if (rc) return rc;
-  if (SC == kWindow && a.few && p.splits == 1) return rc;   // (every head whole)
+  const unsigned tiles = a.few && DEALT ? (unsigned)(p.B * p.Hkv * p.tiles) : (unsigned)p.G;
   const int blocks = a.RT / 32 * (D / 32);
-  if (a.few)
+  if (a.few) {
+    hipLaunchKernelGGL((attn_few_kernel<D, BITS, SC>), dim3(DEALT ? tiles * p.splits : tiles), dim3(kPT), 0, st, p);
+    const int rc = launch_check(who);
+    if (rc || (SC == kWindow && p.splits == 1)) return rc;   // (every tile whole)
     hipLaunchKernelGGL((attn_join_kernel<D, 32, SC == kTail, DEALT>), dim3(tiles, blocks), dim3(kPT), 0, st, p);
-  else
-    hipLaunchKernelGGL((attn_join_kernel<D, 32 * NW, SC == kTail, false>), dim3(tiles, blocks), dim3(kPT), 0, st, p);
+  } else if constexpr (SC != kTail) {   // (a tail's rows are few)
+    hipLaunchKernelGGL((attn_chunk_kernel<D, BITS, SC>), dim3(tiles), dim3(64 * NW), 0, st, p);
+    const int rc = launch_check(who);
+    if (rc) return rc;
+    hipLaunchKernelGGL((attn_join_kernel<D, 32 * NW, false, false>), dim3(tiles, blocks), dim3(kPT), 0, st, p);
+  }
   return launch_check(who);
 }
 
@@ -1775,19 +1739,19 @@ int launch_scope(const char* who, const PAttn& p, const AttnPlan& a, int D, int 
 }
 int launch_window(const char* who, const PAttn& p, const AttnPlan& a, int D, int bits, hipStream_t st);
 
-// Pieces that a request's head may fall into when few rows are dealt: two
-// rounds of workgroups at most (a piece that is not there costs its start).
+// Pieces that a tile may fall into when few rows are dealt: two rounds of
+// workgroups at most (a piece that is not there costs its start).
 inline int dealt_splits(const AttnPlan& a, int B, int Hkv) {
-  const long long n = 2LL * a.G / ((long long)B * Hkv);
+  const long long n = 2LL * a.G / ((long long)B * Hkv * a.tiles);
   return n < 1 ? 1 : n > 128 ? 128 : (int)n;
 }
 inline size_t dealt_slots(const AttnPlan& a, int B, int Hkv, bool shared) {
   const int n = dealt_splits(a, B, Hkv);
-  return n == 1 && !shared ? 0 : (size_t)B * Hkv * n;   // (whole heads leave no partials)
+  return n == 1 && !shared ? 0 : (size_t)B * Hkv * a.tiles * n;   // (whole tiles leave no partials)
 }
 inline size_t scoped_bytes(const AttnPlan& a, int D, int B, int Hkv, bool shared) {
   const size_t slots = a.few ? dealt_slots(a, B, Hkv, shared) : 2 * (size_t)a.G;
-  return slots * a.RT * (D + 2) * sizeof(float) + (a.few ? (size_t)B * Hkv : (size_t)a.G) * sizeof(int4);
+  return slots * a.RT * (D + 2) * sizeof(float) + (a.few ? (size_t)B * Hkv * a.tiles : (size_t)a.G) * sizeof(int4);
 }
 
 // The shared prefix's row tiles of a kv head, and the pieces of keys that each

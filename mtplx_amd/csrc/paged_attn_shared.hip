@@ -25,7 +25,6 @@ int launch_shared(const char* who, PAttn p, const AttnPlan& a, const PrefixPlan&
   p.prefix_rt_log2 = pre.RT == 128 ? 7 : 8;
   PAttn q = p;
   q.rt_log2 = p.prefix_rt_log2;
-  q.splits = 0;
   q.part_o = const_cast<float*>(p.prefix_o);
   q.part_ml = const_cast<float*>(p.prefix_ml);
   const int groups = (int)((pre.slots(p.Hkv) + 7) / 8 * 8);

@@ -60,14 +60,17 @@ def check(c, table, q, n, lengths, got, what="", rows_of=None):
 
 
 CASES = [  # prefix, tail of each (its new tokens among it), new tokens; query heads, kv heads, head dim, page, bits
-    (512, [1, 1], [1, 1], 8, 8, 128, 64, 16), (640, [5, 40, 300], [1, 1, 1], 40, 8, 128, 64, 8),
-    (513, [4, 9, 100, 33], [4, 1, 0, 3], 10, 2, 128, 32, 16), (1000, [7, 1, 2], [2, 1, 2], 5, 1, 64, 32, 8),
-    (2000, [3] * 33, [1] * 33, 4, 1, 64, 64, 16), (544, [8, 600], [8, 8], 4, 1, 256, 32, 16),
-    (700, [2, 5, 64], [2, 5, 1], 6, 1, 256, 64, 8), (600, [20] * 70, [4] * 70, 10, 2, 128, 32, 16),
+    (2048, [1, 1], [1, 1], 8, 8, 128, 64, 16), (2240, [5, 40, 300], [1, 1, 1], 40, 8, 128, 64, 8),
+    (1025, [4, 9, 100, 33], [4, 1, 0, 3], 10, 2, 128, 32, 16), (1100, [7, 1, 2, 90], [2, 1, 2, 1], 5, 1, 64, 32, 8),
+    (2000, [3] * 33, [1] * 33, 4, 1, 64, 64, 16), (2080, [8, 600], [8, 8], 4, 1, 256, 32, 16),
+    (1100, [2, 5, 64, 33], [2, 5, 1, 1], 6, 1, 256, 64, 8), (1056, [20] * 70, [4] * 70, 10, 2, 128, 32, 16),
     (3000, [6, 9], [1, 1], 32, 1, 128, 128, 16), (4500, [90, 1, 31, 32, 33], [1, 1, 1, 1, 1], 2, 2, 128, 96, 8),
-    # more rows than the few-row kernel takes
-    (512, [50, 9], [50, 9], 5, 1, 128, 64, 16), (576, [200, 64, 1], [200, 33, 1], 4, 2, 64, 64, 8),
-    (608, [90, 300], [90, 100], 8, 2, 256, 32, 16), (800, [41, 41], [41, 41], 32, 1, 128, 32, 8),
+    # several tiles of 32 rows a request
+    (4128, [50, 9, 8, 300, 31, 32, 33, 100], [8, 9, 8, 1, 0, 10, 12, 7], 5, 1, 128, 64, 16),
+    (4100, [200, 64, 1, 70, 33, 40, 41, 42, 50], [30, 33, 1, 20, 33, 4, 5, 6, 7], 4, 1, 64, 64, 8),
+    (4096, [41] * 8, [8] * 8, 32, 1, 128, 32, 8), (4160, [90, 300, 20, 20, 20, 20, 20, 20], [17] * 8, 2, 2, 256, 32, 16),
+    # too short, or too many rows, to be worth a pass of its own
+    (512, [50, 9], [50, 9], 5, 1, 128, 64, 16), (576, [200, 64, 1], [1, 3, 1], 4, 2, 64, 64, 8),
 ]
 
 
@@ -96,8 +99,8 @@ def test_more_rows_than_announced(gpu):
     rng = np.random.default_rng(41)
     for D, bits in ((128, 16), (64, 8), (256, 16)):
         n, tails = [2, 45, 1, 90], [300, 45, 41, 120]
-        c, table, shared = batch(rng, 640, tails, D, 2, 64, bits)
-        lengths = [640 + t for t in tails]
+        c, table, shared = batch(rng, 1024, tails, D, 2, 64, bits)
+        lengths = [1024 + t for t in tails]
         q = rows(rng, sum(n), 8, D)
         start, off = i32([e - m for e, m in zip(lengths, n)]), i32(np.concatenate([[0], np.cumsum(n)]))
         for max_rows in (1, 2, 8, 45, 1000):
@@ -109,16 +112,16 @@ def test_many_requests(gpu):
     """More heads than workgroups for the tails."""
     rng = np.random.default_rng(42)
     tails = [1 + 7 * i % 90 for i in range(300)]
-    c, table, shared = batch(rng, 512, tails, 64, 4, 64, 16, poison=False)
+    c, table, shared = batch(rng, 1024, tails, 64, 4, 64, 16, poison=False)
     q = rows(rng, 300, 4, 64)
-    got = paged_sdpa(q, c, table, i32([511 + t for t in tails]), shared=shared)
-    check(c, table, q, [1] * 300, [512 + t for t in tails], got)
+    got = paged_sdpa(q, c, table, i32([1023 + t for t in tails]), shared=shared)
+    check(c, table, q, [1] * 300, [1024 + t for t in tails], got)
 
 
 @pytest.mark.parametrize("bits", [8, 16])
 def test_long_prefixes(gpu, bits):
     rng = np.random.default_rng(5 + bits)
-    for prefix, tails, n, Hq, H in ((20000, [700, 3, 40, 1], [1, 1, 1, 1], 10, 2), (9000, [64] * 40, [4] * 40, 16, 2)):
+    for prefix, tails, n, Hq, H in ((20000, [700, 30, 40, 1], [1, 9, 1, 1], 10, 2), (9000, [64] * 40, [4] * 40, 16, 2)):
         c, table, shared = batch(rng, prefix, tails, 128, H, 64, bits)
         lengths = [prefix + t for t in tails]
         q = rows(rng, sum(n), Hq, 128)
@@ -167,62 +170,63 @@ def test_requests_that_begin_inside(gpu):
 @pytest.mark.parametrize("bits", [8, 16])
 def test_absent_pages_and_odd_values(gpu, bits):
     rng = np.random.default_rng(8)
-    c, table, shared = batch(rng, 1024, [40, 40], 128, 1, 64, bits)
+    c, table, shared = batch(rng, 2048, [40, 40], 128, 1, 64, bits)
     q = rows(rng, 2, 4, 128)
     t = table.clone()
     t[:, 3] = -1   # keys 192..255 of the prefix
-    got = paged_sdpa(q, c, t, i32([1063, 1063]), shared=shared)
+    got = paged_sdpa(q, c, t, i32([2087, 2087]), shared=shared)
     assert int(c.status().item()) == 1
     c.status().zero_()
-    keep = np.r_[0:192, 256:1064]
+    keep = np.r_[0:192, 256:2088]
     for b in range(2):
-        k, v = (x[:, keep] for x in stored(c, table, b, 1064))
+        k, v = (x[:, keep] for x in stored(c, table, b, 2088))
         o, spread, reach = O.attend(num(q[b:b + 1]), k, v, len(keep) - 1)
         check_rows(num(got[b:b + 1]), o, attention_bound(o, spread, reach, 128), f"request {b}")
     t[:] = -1
-    assert (paged_sdpa(q, c, t, i32([1063, 1063]), shared=shared) == 0).all()
+    assert (paged_sdpa(q, c, t, i32([2087, 2087]), shared=shared) == 0).all()
     c.status().zero_()
     # a value that is not a number: in the prefix all rows show it, in a tail its own
     bad = rows(rng, 1, 1, 128)
     bad[0, 0, 3] = float("nan")
-    want = paged_sdpa(q, c, table, i32([1063, 1063]), shared=shared)
-    c.write(torch.zeros_like(bad), bad, table[1:].contiguous(), i32([1050]))
-    got = paged_sdpa(q, c, table, i32([1063, 1063]), shared=shared)
+    want = paged_sdpa(q, c, table, i32([2087, 2087]), shared=shared)
+    c.write(torch.zeros_like(bad), bad, table[1:].contiguous(), i32([2074]))
+    got = paged_sdpa(q, c, table, i32([2087, 2087]), shared=shared)
     assert torch.equal(got[0], want[0]) and torch.isnan(got[1, :, 3]).all()
     c.write(torch.zeros_like(bad), bad, table[:1].contiguous(), i32([100]))
-    got = paged_sdpa(q, c, table, i32([1063, 1063]), shared=shared)
+    got = paged_sdpa(q, c, table, i32([2087, 2087]), shared=shared)
     assert torch.isnan(got[..., 3]).all()
 
 
 def test_scores_of_minus_infinity(gpu):
     rng = np.random.default_rng(9)
-    c, table, shared = batch(rng, 512, [3, 3], 64, 1, 64, 16, poison=False)
-    low = rows(rng, 512, 1, 64)
+    c, table, shared = batch(rng, 2048, [3, 3], 64, 1, 64, 16, poison=False)
+    low = rows(rng, 2048, 1, 64)
     low[:, 0, 0] = float("-inf")
     q = rows(rng, 2, 2, 64).abs() + 0.5
-    before = paged_sdpa(q, c, table, i32([514, 514]), shared=shared)
-    c.write(low, rows(rng, 512, 1, 64), table[:1].contiguous(), i32([0]))
-    got = paged_sdpa(q, c, table, i32([514, 514]), shared=shared)
+    before = paged_sdpa(q, c, table, i32([2050, 2050]), shared=shared)
+    c.write(low, rows(rng, 2048, 1, 64), table[:1].contiguous(), i32([0]))
+    got = paged_sdpa(q, c, table, i32([2050, 2050]), shared=shared)
     for b in range(2):   # the prefix counts for nothing
-        k, v = (x[:, 512:] for x in stored(c, table, b, 515))
+        k, v = (x[:, 2048:] for x in stored(c, table, b, 2051))
         o, spread, reach = O.attend(num(q[b:b + 1]), k, v, 2)
         check_rows(num(got[b:b + 1]), o, attention_bound(o, spread, reach, 64), f"request {b}")
-    c.write(low[:3], low[:3], table[:1].contiguous(), i32([512]))
-    got = paged_sdpa(q, c, table, i32([514, 514]), shared=shared)
+    c.write(low[:3], low[:3], table[:1].contiguous(), i32([2048]))
+    got = paged_sdpa(q, c, table, i32([2050, 2050]), shared=shared)
     assert torch.isnan(got[0]).all() and torch.isfinite(got[1]).all() and torch.isfinite(before).all()
 
 
-@pytest.mark.parametrize("few", [True, False])
-def test_scores_of_every_size(gpu, few):
+@pytest.mark.parametrize("n,B", [(2, 2), (11, 8)])
+def test_scores_of_every_size(gpu, n, B):
     """One key of the prefix or of the tail takes all; a maximum that rises or
     falls from the prefix to the tail."""
     rng = np.random.default_rng(10)
-    n = 2 if few else 40
+    prefix = 2048 if B == 2 else 4096
+    tails = [100, 60, 33, 20, 64, 12, 99, 40][:B]
     for kind in ("large", "rising", "falling"):
-        c, table, shared = batch(rng, 1500 // 32 * 32, [100, 60], 128, 1, 32, 16, poison=False)
-        keys = 1472 + 100
+        c, table, shared = batch(rng, prefix, tails, 128, 1, 32, 16, poison=False)
+        keys = prefix + 100
         k, v = rows(rng, keys, 1, 128), rows(rng, keys, 1, 128)
-        q = rows(rng, 2 * n, 4, 128)
+        q = rows(rng, B * n, 4, 128)
         if kind == "large":
             k *= 20
             q *= 4
@@ -230,11 +234,11 @@ def test_scores_of_every_size(gpu, few):
             ramp = torch.linspace(0, 30, keys, device="cuda")
             k[:, 0, 0] = (ramp if kind == "rising" else 30 - ramp).to(k.dtype)
             q[..., 0] = 40.0
-        for b, t in enumerate((100, 60)):
-            c.write(k[:1472 + t], v[:1472 + t], table[b:b + 1].contiguous(), i32([0]))
-        lengths = [1572, 1532]
+        for b, t in enumerate(tails):
+            c.write(k[:prefix + t], v[:prefix + t], table[b:b + 1].contiguous(), i32([0]))
+        lengths = [prefix + t for t in tails]
         got = paged_sdpa(q, c, table, i32([e - n for e in lengths]), shared=shared)
-        check(c, table, q, [n, n], lengths, got, what=kind)
+        check(c, table, q, [n] * B, lengths, got, what=kind)
 
 
 def test_decode_steps_and_graphs(gpu):
@@ -299,10 +303,10 @@ def test_decode_steps_and_graphs(gpu):
 def test_views_and_outputs(gpu):
     rng = np.random.default_rng(14)
     for n in (3, 50):
-        c, table, shared = batch(rng, 512, [80, 90], 64, 2, 32, 16)
+        c, table, shared = batch(rng, 2048, [80, 90], 64, 2, 32, 16)
         fused = rows(rng, 2 * n, 8 * 64)
         q = fused[:, :256].view(2 * n, 4, 64)
-        start = i32([592 - n, 602 - n])
+        start = i32([2128 - n, 2138 - n])
         want = paged_sdpa(q.contiguous(), c, table, start, scale=0.3, shared=shared)
         assert torch.equal(paged_sdpa(q, c, table.long(), start.cpu(), scale=0.3, shared=shared), want)
         wide = torch.zeros((2 * n, 8 * 64), dtype=torch.bfloat16, device="cuda")

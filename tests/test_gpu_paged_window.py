@@ -118,10 +118,12 @@ def test_a_window_over_everything_is_none(gpu, n, keys, Hq, bits):
     rng = np.random.default_rng(keys + n)
     c, table = _filled(rng, [keys], 128, 2, 64, bits)
     q = rows(rng, n, Hq, 128)
-    want = paged_sdpa(q, c, table, i32([keys - n]))
-    for window in (keys, keys + 1, 2 ** 31 - 1, 2 ** 40):
-        assert torch.equal(paged_sdpa(q, c, table, i32([keys - n]), window=window), want)
-    # and so are sinks that reach every row, up to the order of sums
+    want = paged_sdpa(q, c, table, i32([keys - n]), window=keys)
+    check(c, table, q, [n], [keys], want, None, 0)
+    for window in (keys + 1, 2 ** 31 - 1, 2 ** 40):
+        got = paged_sdpa(q, c, table, i32([keys - n]), window=window)
+        check(c, table, q, [n], [keys], got, None, 0, what=f"window={window}")
+    # and so are sinks that reach every row
     got = paged_sdpa(q, c, table, i32([keys - n]), window=3, sinks=2 ** 31 - 1)
     check(c, table, q, [n], [keys], got, None, 0)
 
