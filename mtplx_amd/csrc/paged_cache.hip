@@ -662,6 +662,48 @@ __device__ __forceinline__ int token_request(const WriteParams& p, int t, long l
   return b;
 }
 
+// Queries of tokens [t0, t0 + n), normalised and rotated; live: whether each
+// belongs to a request (rows behind the last one stay as they are).
+template <bool PAIRED>
+__device__ __forceinline__ void turn_queries(const WriteParams& p, int D, int t0, int n, float2* cs, float* weights,
+                                             int* s_live, int threads) {
+  const int half = p.r.dims / 2;
+  for (int t = 0; t < n; ++t) {
+    long long pos = 0;
+    const int b = token_request(p, t0 + t, &pos);   // the same in every thread
+    if (threadIdx.x == 0) s_live[t] = b >= 0;
+    for (int x = threadIdx.x; x < half; x += threads) {
+      if (p.heads.positions) pos = p.heads.positions[(long long)pair_axis(p.heads, x) * p.T + t0 + t];
+      cs[t * half + x] = rot_angle(pos, p.r.table[x], p.r.gain);
+    }
+  }
+  HeadSpec hs = p.heads;
+  hs.k_weight = nullptr;   // (no keys here)
+  head_weights(hs, D, weights, threads);
+  __syncthreads();
+  const HeadRows all = {p.q, p.q, p.Hq, 0, D, p.lanes};
+  turn_heads<PAIRED, true>(all, p.r, hs, cs, weights, t0, n, threads, [&](int t) { return s_live[t] != 0; });
+  __syncthreads();
+}
+
+// The same by a launch of their own: at head dim 256 the writes' workgroups are
+// two waves with 33 KB of LDS, which leaves eight waves a CU to turn long calls'
+// queries (6000 tokens, 24 heads over 4, written and read back: 95 us, 122 in one
+// launch; at head dim 128, four waves, 8192 tokens of 40 over 8 take 92 either way
+// and shorter calls 10 us more).
+template <bool PAIRED>
+__global__ __launch_bounds__(kNT, 4) void queries_kernel(WriteParams p, int D) {
+  __shared__ __attribute__((aligned(16))) float2 cs[2 * kMaxPairs];
+  __shared__ __attribute__((aligned(16))) float weights[4 * kMaxPairs];
+  __shared__ int s_live[2];
+  const int stride = (int)gridDim.x * p.q_tokens;
+  for (int t0 = (int)blockIdx.x * p.q_tokens; t0 < p.T; t0 += stride) {
+    const int n = p.T - t0 < p.q_tokens ? p.T - t0 : p.q_tokens;
+    turn_queries<PAIRED>(p, D, t0, n, cs, weights, s_live, kNT);
+    if (t0 > p.T - stride) break;   // (t0 + stride could pass 2^31)
+  }
+}
+
 template <int D, int BITS, bool HEADS>
 __global__ __launch_bounds__(64 * cache_waves<D>(), D == 256 ? 1 : 4) void paged_write_kernel(WriteParams p) {
   constexpr int NT = 64 * cache_waves<D>();
@@ -674,33 +716,21 @@ __global__ __launch_bounds__(64 * cache_waves<D>(), D == 256 ? 1 : 4) void paged
     const int stride = ((int)gridDim.x - p.kv_groups) * p.q_tokens;
     for (int t0 = ((int)blockIdx.x - p.kv_groups) * p.q_tokens; t0 < p.T; t0 += stride) {
       const int n = p.T - t0 < p.q_tokens ? p.T - t0 : p.q_tokens;
+      if constexpr (HEADS) {
+        float* weights = reinterpret_cast<float*>(cs + kRotTokens * kMaxPairs);
+        static_assert(sizeof(lds) >= kRotTokens * kMaxPairs * sizeof(float2) + 2 * D * sizeof(float), "angles, weights");
+        if (rot_paired(p.r.dims, p.r.trad))
+          turn_queries<true>(p, D, t0, n, cs, weights, s_live, NT);
+        else
+          turn_queries<false>(p, D, t0, n, cs, weights, s_live, NT);
+        if (t0 > p.T - stride) break;
+        continue;
+      }
       for (int t = 0; t < n; ++t) {
         long long pos = 0;
         const int b = token_request(p, t0 + t, &pos);   // the same in every thread
         if (threadIdx.x == 0) s_live[t] = b >= 0;
-        for (int x = threadIdx.x; x < half; x += NT) {
-          if constexpr (HEADS) {
-            if (p.heads.positions) pos = p.heads.positions[(long long)pair_axis(p.heads, x) * p.T + t0 + t];
-          }
-          cs[t * half + x] = rot_angle(pos, p.r.table[x], p.r.gain);
-        }
-      }
-      if constexpr (HEADS) {
-        float* weights = reinterpret_cast<float*>(cs + kRotTokens * kMaxPairs);
-        static_assert(sizeof(lds) >= kRotTokens * kMaxPairs * sizeof(float2) + 2 * D * sizeof(float), "angles, weights");
-        HeadSpec hs = p.heads;
-        hs.k_weight = nullptr;   // (no keys here)
-        head_weights(hs, D, weights, NT);
-        __syncthreads();
-        const HeadRows all = {p.q, p.q, p.Hq, 0, D, p.lanes};
-        auto live = [&](int t) { return s_live[t] != 0; };
-        if (rot_paired(p.r.dims, p.r.trad))
-          turn_heads<true, true>(all, p.r, hs, cs, weights, t0, n, NT, live);
-        else
-          turn_heads<false, true>(all, p.r, hs, cs, weights, t0, n, NT, live);
-        __syncthreads();
-        if (t0 > p.T - stride) break;
-        continue;
+        for (int x = threadIdx.x; x < half; x += NT) cs[t * half + x] = rot_angle(pos, p.r.table[x], p.r.gain);
       }
       __syncthreads();
       for (int x = threadIdx.x; x < n * p.Hq * ipr; x += NT) {
@@ -1036,11 +1066,20 @@ static int paged_write(const char* who, const mtp_paged_write_args* a, const mtp
   long long groups = (units * (p.k_parts + 1) * a->Hkv + waves - 1) / waves;
   if (groups > 1 << 20) groups = 1 << 20;
   p.kv_groups = (int)groups;
-  if (a->q) {
+  const bool apart = heads && a->q && a->D == 256 && a->T >= 2048;
+  if (a->q && !apart) {
     p.q_tokens = rot_tokens(a->T);
     groups += cdiv(a->T, p.q_tokens) < (1 << 20) ? cdiv(a->T, p.q_tokens) : 1 << 20;
   }
   hipStream_t st = (hipStream_t)stream;
+  if (apart) {
+    p.q_tokens = 2;
+    const int n = cdiv(a->T, 2) < (1 << 20) ? cdiv(a->T, 2) : 1 << 20;
+    auto* kernel = rot_paired(a->dims, a->traditional) ? queries_kernel<true> : queries_kernel<false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(kNT), 0, st, p, a->D);
+    rc = launch_check(who);
+    if (rc) return rc;
+  }
   const int key = a->D * 100 + a->bits;
   switch (key) {
     case 6416: launch_write<64, 16>(p, heads != nullptr, (int)groups, st); break;

@@ -159,6 +159,8 @@ WRITES = [   # rows of each request, start of each, Hq, Hkv, D, bits, dims, trad
     ([45, 2], [0, 17], 4, 2, 128, 16, 24, False, (6, 3, 3), True, 128),
     ([45, 2], [0, 17], 4, 2, 256, 8, 256, True, None, False, 128),
     ([333], [0], 3, 3, 64, 8, 24, False, None, False, 32),
+    ([2049, 3], [5, 0], 2, 1, 256, 16, 64, False, (12, 10, 10), True, 64),   # queries by a launch of their own
+    ([2100], [0], 2, 1, 256, 8, 24, False, None, False, 64),
 ]
 
 
