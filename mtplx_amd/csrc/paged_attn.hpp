@@ -462,22 +462,15 @@ struct RowState {
 // infinity in any element; the same in every lane.
 template <int D, class VO>
 __device__ __forceinline__ uint32_t odd_keys(VO vop, int h2) {
-  // Magnitudes by their bits: at or past 0x7f80 there is no number.
-  typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
-  u16x8 top = {};
-#pragma unroll
-  for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-    for (int jj = 0; jj < 2; ++jj)
-      top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x8, u32x4(vop(t, jj) & 0x7fff7fffu)));
-  const u32x4 most = __builtin_bit_cast(u32x4, top) + 0x00800080u;   // (a carry into the sign's place, half by half)
-  if (!__any((most.x | most.y | most.z | most.w) & 0x80008000u)) return 0;
+  // An exponent of all ones plus one carries into the sign's place, half by half.
   u32x4 a0 = {}, a1 = {};
 #pragma unroll
   for (int t = 0; t < D / 32; ++t) {
     a0 |= (vop(t, 0) & 0x7f807f80u) + 0x00800080u;
     a1 |= (vop(t, 1) & 0x7f807f80u) + 0x00800080u;
   }
+  const u32x4 a = a0 | a1;
+  if (!__any((a.x | a.y | a.z | a.w) & 0x80008000u)) return 0;
   auto two = [&](uint32_t w, int i) {
     return (w >> 15 & 1u) << v_slot_key(h2, 2 * i) | (w >> 31) << v_slot_key(h2, 2 * i + 1);
   };
