@@ -143,7 +143,18 @@ def _scoped_workspace(device, Hq: int, Hkv: int, D: int, rows: int, T: int, B: i
     if torch.cuda.current_device() != device.index:
         with torch.cuda.device(device):
             return _scoped_workspace(device, Hq, Hkv, D, rows, T, B, shared)
-    nb = _lib.query("mtp_paged_attn_scoped_workspace_bytes", Hq, Hkv, D, rows, T, B, shared)
+    def size() -> int:
+        return _lib.query("mtp_paged_attn_scoped_workspace_bytes", Hq, Hkv, D, rows, T, B, shared)
+
     if torch.cuda.is_current_stream_capturing():
-        return torch.empty(nb, dtype=torch.uint8, device=device)
-    return _lib.WORKSPACES.get(nb, "paged_attn_scoped", device)
+        return torch.empty(size(), dtype=torch.uint8, device=device)
+    key = (device.index, _stream(device), Hq, Hkv, D, rows, B, shared and T, shared)
+    ws = _SCOPED_SPACES.get(key)
+    if ws is None:
+        if len(_SCOPED_SPACES) >= 1024:   # (batches come in many shapes)
+            _SCOPED_SPACES.clear()
+        ws = _SCOPED_SPACES[key] = _lib.WORKSPACES.get(size(), "paged_attn_scoped", device)
+    return ws
+
+
+_SCOPED_SPACES: dict = {}

@@ -23,7 +23,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Any, Sequence
 
 import torch
@@ -39,7 +39,7 @@ class RotaryTable:
     position (host, float64), ``phases`` the same as revolutions times 2^64
     (device, the bits of a uint64), ``gain`` the factor of the rotated values,
     ``axes`` how many positions a token has and ``axis`` (host) the one that
-    each pair turns by."""
+    each pair turns by (``axis_words``: as the kernels read it)."""
 
     dims: int
     traditional: bool
@@ -48,6 +48,7 @@ class RotaryTable:
     phases: torch.Tensor
     axes: int = 1
     axis: tuple = ()
+    axis_words: tuple = (0, 0, 0, 0)
 
 
 @dataclass(frozen=True)
@@ -58,6 +59,7 @@ class HeadNorms:
     queries: torch.Tensor | None
     keys: torch.Tensor | None
     eps: float
+    args: Any = field(default=None, repr=False, compare=False)   # what every call with them passes
 
 
 def head_norms(queries: torch.Tensor | None, keys: torch.Tensor | None, *, eps: float = 1e-6) -> HeadNorms:
@@ -78,7 +80,7 @@ def head_norms(queries: torch.Tensor | None, keys: torch.Tensor | None, *, eps: 
         kept.append(w)
     if None not in kept and (kept[0].shape != kept[1].shape or kept[0].device != kept[1].device):
         raise ValueError("the two weights must have one length and device")
-    return HeadNorms(kept[0], kept[1], eps)
+    return HeadNorms(kept[0], kept[1], eps, _lib.HeadArgs(_lib.ptr(kept[0]), _lib.ptr(kept[1]), axes=1, eps=eps))
 
 
 def rotary_frequencies(dims: int, *, base: float = 10000.0, scale: float = 1.0, scaling: str | None = None,
@@ -177,8 +179,12 @@ def rotary_table(dims: int, *, base: float = 10000.0, traditional: bool = False,
     if sections is None and interleaved:
         raise ValueError("interleaved belongs to sections")
     axis = _pair_axes(dims // 2, sections, interleaved) if sections is not None else ()
+    words = [0, 0, 0, 0]
+    for i, a in enumerate(axis):   # two bits a pair
+        words[i // 32] |= a << (2 * (i % 32))
     return RotaryTable(int(dims), bool(traditional), gain, tuple(freqs),
-                       torch.tensor(fixed, dtype=torch.int64).to(device), len(sections) if axis else 1, axis)
+                       torch.tensor(fixed, dtype=torch.int64).to(device), len(sections) if axis else 1, axis,
+                       tuple(w - (w >> 63 << 64) for w in words))   # (the bits, as signed)
 
 
 def _positions(table: RotaryTable, positions: Any, T: int, device) -> torch.Tensor:
@@ -198,24 +204,24 @@ def _heads(table: RotaryTable, norms: HeadNorms | None, positions: torch.Tensor 
            device) -> _lib.HeadArgs | None:
     """The argument block of a call with head norms or several axes (None: one
     without), its weights checked."""
-    if norms is None and table.axes == 1 and positions is None:
-        return None
-    a = _lib.HeadArgs(axes=table.axes)
-    if norms is not None:
-        if not isinstance(norms, HeadNorms):
+    if norms is None:
+        if table.axes == 1 and positions is None:
+            return None
+        a = _lib.HeadArgs(axes=1)
+    else:
+        if not isinstance(norms, HeadNorms) or norms.args is None:
             raise TypeError(f"norms must come from head_norms (got {type(norms).__name__})")
         for name, w in (("queries", norms.queries), ("keys", norms.keys)):
             if w is not None:
                 _on(device, f"norms.{name}", w)
                 if w.shape[0] != D:
                     raise ValueError(f"norms.{name} has {w.shape[0]} weights, heads have {D} elements")
-        a.q_weight, a.k_weight, a.eps = _lib.ptr(norms.queries), _lib.ptr(norms.keys), norms.eps
+        a = _lib.HeadArgs.from_buffer_copy(norms.args)
     if positions is not None:
         a.positions = positions.data_ptr()
-    words = [0, 0, 0, 0]
-    for i, axis in enumerate(table.axis):
-        words[i // 32] |= axis << (2 * (i % 32))
-    a.axis0, a.axis1, a.axis2, a.axis3 = (w - (w >> 63 << 64) for w in words)   # (the bits, as signed)
+    if table.axes > 1:
+        a.axes = table.axes
+        a.axis0, a.axis1, a.axis2, a.axis3 = table.axis_words
     return a
 
 
