@@ -99,6 +99,10 @@ static int paged_attn(const char* who, const mtp_paged_attn_args* a, const mtp_a
     if (!window_dealt(plan, a->Hkv, a->D, a->bits, a->B, keys < covered ? keys : covered))
       plan = attn_plan(a->Hq, a->Hkv, a->D, 0);
   }
+  if (scope && covered > 0x7fffffffLL - 2 * kBlk) {   // (a block that counts twice would pass 2^31)
+    set_error("%s: a table of %lld positions is more than 2^31 - 65", who, covered);
+    return MTP_ERR_UNSUPPORTED;
+  }
   if (scope && (long long)a->B * a->Hkv > 1 << 20) {
     set_error("%s: %d requests of %d kv heads are more than 2^20", who, a->B, a->Hkv);
     return MTP_ERR_UNSUPPORTED;

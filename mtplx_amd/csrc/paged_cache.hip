@@ -156,8 +156,19 @@ __device__ __forceinline__ void turn_heads(const HeadRows& rows, const RotSpec& 
         }
         *reinterpret_cast<uint4*>(dst + d1) = pack8(y1);
         *reinterpret_cast<uint4*>(dst + d2) = pack8(y2);
-      } else if (PAIRED) {
+      } else if (PAIRED || d1 >= r.dims) {
         *reinterpret_cast<uint4*>(dst + d1) = pack8(a.v);
+      } else if (r.trad && d1 + 8 <= r.dims && half % 2 == 0) {   // (angles of four pairs: 16-byte aligned)
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+          const float4 z = *reinterpret_cast<const float4*>(c + (d1 + e) / 2);
+          y[e] = rot_first(a.v[e], a.v[e + 1], make_float2(z.x, z.y));
+          y[e + 1] = rot_second(a.v[e], a.v[e + 1], make_float2(z.x, z.y));
+          y[e + 2] = rot_first(a.v[e + 2], a.v[e + 3], make_float2(z.z, z.w));
+          y[e + 3] = rot_second(a.v[e + 2], a.v[e + 3], make_float2(z.z, z.w));
+        }
+        *reinterpret_cast<uint4*>(dst + d1) = pack8(y);
       } else {
         float y[8];
         const uint16_t* row = source(t, h);   // (partners of halves that are no whole chunks)

@@ -288,6 +288,51 @@ def test_captured_steps(gpu):
             assert torch.equal(out, w), i
 
 
+def test_two_host_threads_on_one_stream(gpu):
+    """Windowed calls of two threads on the same stream share its workspace."""
+    import threading
+
+    rng = np.random.default_rng(19)
+    H, Hq, D, page = 2, 16, 128, 64
+    table, pages = tables(rng, [6000], page)
+    c = PagedKVCache(pages, H, D, page_size=page, bits=8)
+    c.write(rows(rng, 6000, H, D), rows(rng, 6000, H, D), table, i32([0]))
+    qs = [rows(rng, n, Hq, D) for n in (2, 90)]
+    start, kw = i32([5900]), dict(window=3000, sinks=4)
+    want = [paged_sdpa(q, c, table, start, **kw) for q in qs]
+    torch.cuda.synchronize()
+    bad: list = []
+
+    def work(q, w):
+        for _ in range(40):
+            bad.append(paged_sdpa(q, c, table, start, **kw).ne(w).any())
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(qs, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert len(bad) == 80 and not any(bool(b) for b in bad)
+
+
+def test_views_and_outputs(gpu):
+    rng = np.random.default_rng(14)
+    for n in (3, 50, 300):
+        c, table = _filled(rng, [400], 64, 2, 32, 16)
+        fused = rows(rng, n, 8 * 64)
+        q = fused[:, :256].view(n, 4, 64)
+        start, kw = i32([400 - n]), dict(scale=0.3, window=90, sinks=3)
+        want = paged_sdpa(q.contiguous(), c, table, start, **kw)
+        assert torch.equal(paged_sdpa(q, c, table.long(), torch.tensor([400 - n]), **kw), want)
+        wide = torch.zeros((n, 8 * 64), dtype=torch.bfloat16, device="cuda")
+        out = wide[:, 128:384].view(n, 4, 64)
+        paged_sdpa(q, c, table, start, out=out, **kw)
+        assert torch.equal(out, want) and (wide[:, :128] == 0).all() and (wide[:, 384:] == 0).all()
+        paged_sdpa(q, c, table, start, out=q, **kw)   # over its own queries
+        assert torch.equal(q, want)
+
+
 def test_refusals(gpu):
     c = PagedKVCache(2, 2, 64, page_size=32)
     q = torch.zeros((4, 4, 64), dtype=torch.bfloat16, device="cuda")

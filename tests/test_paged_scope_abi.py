@@ -30,7 +30,7 @@ def test_bad_scopes(kw):
 
 
 @pytest.mark.parametrize("bad", [dict(q=None), dict(ws=None), dict(ws_bytes=64), dict(Hq=3), dict(D=80), dict(scale=0.0),
-                                 dict(B=1 << 20, row_off=0x1000)])
+                                 dict(B=1 << 20, row_off=0x1000), dict(width=(1 << 25) - 1)])
 def test_bad_calls(bad):
     assert _run(_attn(**bad)[1], _lib.AttnScope(window=8, sinks=1)) < 0
     assert _lib.load().mtp_last_error().decode().startswith("mtp_paged_attn_scoped")
