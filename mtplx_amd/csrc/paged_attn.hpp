@@ -30,6 +30,19 @@
 // workgroup, and attn_join adds them in the line's order. The split depends on
 // lengths alone, so results do not depend on timing.
 //
+// Two more scopes share the kernels (each compiled in a source of its own):
+//
+// A window, with sinks: position p sees j > p - W and j < S. A tile's key blocks
+// are those that hold sinks and those from its first row's window on, counted
+// through without the gap between them; what is counted is dealt, loaded and
+// masked as before, and what is not is never read. Every row's keys of a block are
+// one range, so a mask is a word of bits per row and block.
+//
+// A shared prefix: paged_attn_shared.hip.
+//
+// Few rows (a request's up to 256 per kv head) of both are dealt in equal pieces
+// without a line (dealt_piece).
+//
 // What bounds it, on an MI355X (5.17 TB/s a large copy, 1350 TFLOP/s a large
 // bf16 product), 40 query heads over 8 kv heads of 128:
 //   sixteen requests' four verify rows up to 32k, 8 bits: 122 us, the pages at
@@ -40,9 +53,16 @@
 //     half a conversion a score) take as many cycles of a SIMD as the MFMAs,
 //     and the two waves of a SIMD take them in turn: in the chunk the matrix
 //     pipes are busy 50% of the CUs' busy cycles, vector issue 49%;
-//   head dim 64: the chunk 117 us, the verify rows 76; head dim 256: 1377 (16
-//     bits: registers spill inside the step) and 531 (8 bits), the verify rows 230;
-//   one token over 4k: 17.7 us, of which the two launches' kernels are 12 and 5.
+//   head dim 64: the chunk 115 us, the verify rows 76; head dim 256: 1041 (16
+//     bits: registers spill inside the step) and 529 (8 bits), the verify rows 230;
+//   one token over 4k: 17.3 us, of which the two launches' kernels are 12 and 5;
+//   behind a window of 4096 one token at 32k 15 us (kernels 11.7 and 4.2), sixteen
+//     requests' four verify rows 37 (8 bits, 140 MB in 31 us of the first kernel);
+//   a prompt of 8192 behind a window of 1024: 230 us, 700 TFLOP/s of what the
+//     window leaves. A step of 64 keys is 2 us, as in the chunk, and a tile of 18
+//     steps costs about 10 more: its rows' and first keys' way from memory, 1700
+//     instructions of addresses, and three or four steps at the window's ends
+//     whose masks are as many instructions as the softmax.
 #pragma once
 
 #include "paged.hpp"
@@ -178,9 +198,11 @@ __device__ __forceinline__ int prefix_tokens(const PAttn& p) {
   return n < 0 ? 0 : n < p.T ? n : p.T;
 }
 
+// The prefix is done for a request that lies behind it; one that does not, or
+// whose rows are not among the list's, sees its keys from the first on. (The
+// join adds the prefix to the tiles that were dealt: a request that brings more
+// rows than were announced does without, too.)
 __device__ __forceinline__ bool behind_prefix(const PAttn& p, const ReqRows& rows, long long start) {
-  // (The join adds the prefix to the tiles that were dealt: a request that brings
-  // more rows than were announced does without.)
   return start >= p.prefix && rows.lo + rows.n <= prefix_tokens(p) &&
          (long long)rows.n * p.rep <= (long long)p.tiles << p.rt_log2;
 }
@@ -188,21 +210,14 @@ __device__ __forceinline__ bool behind_prefix(const PAttn& p, const ReqRows& row
 // A lane's request of the line (64 requests at a time), its rows and length.
 struct LaneReq {
   ReqRows rows;
-  int skip;
   long long start, len;   // len: one head
 };
 template <int SC>
 __device__ __forceinline__ LaneReq lane_req(const PAttn& p, int b) {
-  LaneReq r = {{0, 0}, 0, 0, 0};
+  LaneReq r = {{0, 0}, 0, 0};
   if (b < p.B) {
     r.rows = req_rows(p.row_off, b, p.B, p.T);
     r.start = p.q_start[b];
-    if constexpr (SC == kTail) {
-      // The prefix is done for a request that lies behind it; one that does not
-      // (or whose rows are not among the list's) sees its keys from the first on.
-      if (behind_prefix(p, r.rows, r.start)) r.skip = p.prefix / kBlk;
-      r.start -= r.skip * kBlk;
-    }
     r.len = head_len<SC>(p, r.start, r.rows.n);
   }
   return r;
@@ -255,7 +270,6 @@ struct Line {
         r.lo = __builtin_amdgcn_readfirstlane(__shfl(q.rows.lo, src, 64));
         r.n = __builtin_amdgcn_readfirstlane(__shfl(q.rows.n, src, 64));
         r.start = uniform64(shfl64(q.start, src));
-        r.skip = SC == kTail ? __builtin_amdgcn_readfirstlane(__shfl(q.skip, src, 64)) : 0;
         r.head = uniform64(shfl64(q.len, src));
         r.base = uniform64(carry + shfl64(end, src)) - p.Hkv * r.head;
         return __builtin_amdgcn_readfirstlane(b0 + src);
@@ -337,7 +351,9 @@ __device__ __forceinline__ Tile tile_at(const PAttn& p, const Req& r, long long 
 // tail's), so every tile is cut into pieces of the same number of keys,
 // workgroup (request, head, tile, piece) takes one, and what a workgroup has to
 // know of the others is that number. The line's search, a wave's first 1500
-// instructions, took as long as a decode step's keys.
+// instructions, took as long as a decode step's keys: one token behind a window
+// of 4096 20.5 us by the line and 15.1 dealt, sixteen requests' verify rows 44 and
+// 36, sixteen tails of up to 600 keys 26 and 18 (kernel).
 template <int SC>
 __device__ __forceinline__ long long dealt_keys(const PAttn& p, int b) {
   const ReqRows rows = req_rows(p.row_off, b, p.B, p.T);

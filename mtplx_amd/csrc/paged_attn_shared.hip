@@ -4,11 +4,19 @@
 //
 // A row's softmax falls into keys [0, P) and [P, its own position]. The first
 // part's keys are the same for all requests, so their rows make one list per kv
-// head, cut into tiles of 256 (D = 256: 128) as a long chunk's, and K and V of the prefix
-// are read once per tile instead of once per request. Every piece of keys leaves
-// (o, m, l) of its rows; the second part's kernel begins a row with what the
-// pieces give together, m = max m_k, l = sum 2^(m_k - m) l_k, o alike, as if it had
-// seen the prefix itself, and goes on over the request's own keys.
+// head, cut into tiles of 256 (D = 256: 128) as a long chunk's, and K and V of the
+// prefix are read once per tile instead of once per request. Every piece of keys
+// leaves (o, m, l) of its rows, and so does every piece of a request's own keys;
+// the join adds both, m = max m_k, l = sum 2^(m_k - m) l_k, o alike. (The prefix's
+// state as the first of a tail's kernel cost 50 us of dependent loads for a wave's
+// eight pieces, a join of everything 6.)
+//
+// What bounds it (40 heads over 8 of 128): 32 requests' four verify rows behind
+// 32768 keys, 8 bits: 116 us, of which the prefix 78 (640 rows in tiles of 256:
+// 635 TFLOP/s of what there is, 760 with the empty half tile; the chunk kernel's
+// 830), the tails 33 (86 MB; 12 us before the first key) and the join 12 (27 MB of
+// partials). Without sharing 345. One row of sixteen requests behind 8192 keys, 16
+// bits: 39 us (98 without), of 15, 18 and 6.5, each mostly the way of its first loads.
 #include "paged_attn.hpp"
 
 namespace mtp {

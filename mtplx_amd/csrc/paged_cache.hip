@@ -4,7 +4,15 @@
 //
 //   rotation of 8192 tokens, 40 + 8 heads of 128: 46 us (201 MB, 4.4 TB/s);
 //   write of the same at 8 bits, queries rotated: 58 us (218 MB, 3.8 TB/s);
-//   its read back: 11 us (50 MB); eight requests' prefixes: 74 us (349 MB, 4.7).
+//   its read back: 11 us (50 MB); eight requests' prefixes: 74 us (349 MB, 4.7);
+//   rotation with head norms of 8192 tokens: 44 us (40 the kernel, 5.0 TB/s: a row
+//     is read once, its factor comes from three exchanges between eight lanes);
+//     by three axes without norms 30 us (32 heads over 4, 151 MB); 2000 tokens of
+//     24 heads over 4 of 256, a quarter of each turned, 19 us (57 MB): a round is
+//     16 bytes a lane, and seven rounds wait one after another; traditional pairs
+//     57 us (twice the lanes for a row, and as many sums and exchanges each);
+//   norms, rotation and write of 8192 tokens, 16 bits: 67 us (235 MB, 3.5 TB/s; a
+//     key's angles are computed for each head's block).
 //
 // Writes and reads go by blocks of 32 positions of one head. A wave has a block
 // to itself (writes: K or V of it, reads both): 8 or 16 KB of loads are under
