@@ -5,7 +5,9 @@
 ``ragged_causal_mask``, ``mtplx/ragged_attention.py:42``): the rule
 ``j <= q_start[b] + i`` applied implicitly. Requests of one call may bring one
 token or thousands each: decode rows, verify rows, prompt chunks and whole
-prompts run together.
+prompts run together. A row may see a sliding window of its positions and the
+first few (``window``, ``sinks``), and a batch whose requests share a long prefix
+reads that once (``shared``).
 """
 
 from __future__ import annotations

@@ -7,6 +7,10 @@ the pages that its row of a block table names, so requests of any length come
 and go without copies and may share the pages of a common prefix. Which page
 belongs to whom is the caller's: the cache stores, it does not allocate.
 
+The write rotates keys and queries on their way, and normalises their heads
+where the model does (``norms``); a token's rotation may go by several positions
+(``positions``), the slot that it is stored in by one.
+
 Pages lie in the order in which :func:`mtplx_amd.paged_attention.paged_sdpa`
 loads them (``include/mtplx_amd.h``); :meth:`PagedKVCache.read` gives rows
 back in the reference's ``[B, Hkv, count, D]``.

@@ -102,6 +102,17 @@ def test_equal_axes_are_one_position(gpu):
             assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+def test_a_table_that_does_not_turn(gpu):
+    rng = np.random.default_rng(6)
+    D = 128
+    t = rotary_table(D, frequencies=[0.0] * (D // 2))
+    x, w = rows(rng, 40, 3, D), weight(rng, D)
+    got = apply_rotary(t, x, None, i32(range(40)), norms=head_norms(w, None))[0]
+    want = O.norm_heads(num(x), num(w), 1e-6)
+    check_rows(num(got), want, HALF * np.abs(want) + 2.0 ** -20 * np.abs(want), "norms alone")
+    assert torch.equal(apply_rotary(t, x, None, i32(range(40)))[0], x)
+
+
 def test_rows_of_odd_values(gpu):
     """Zeros, tiny and huge rows, one with a NaN, one with an infinity: each row
     alone decides its result."""
