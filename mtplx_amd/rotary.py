@@ -59,7 +59,7 @@ class HeadNorms:
     queries: torch.Tensor | None
     keys: torch.Tensor | None
     eps: float
-    args: Any = field(default=None, repr=False, compare=False)   # what every call with them passes
+    args: Any = field(default=None, init=False, repr=False, compare=False)   # what every call with them passes
 
 
 def head_norms(queries: torch.Tensor | None, keys: torch.Tensor | None, *, eps: float = 1e-6) -> HeadNorms:
@@ -80,7 +80,9 @@ def head_norms(queries: torch.Tensor | None, keys: torch.Tensor | None, *, eps: 
         kept.append(w)
     if None not in kept and (kept[0].shape != kept[1].shape or kept[0].device != kept[1].device):
         raise ValueError("the two weights must have one length and device")
-    return HeadNorms(kept[0], kept[1], eps, _lib.HeadArgs(_lib.ptr(kept[0]), _lib.ptr(kept[1]), axes=1, eps=eps))
+    norms = HeadNorms(kept[0], kept[1], eps)
+    object.__setattr__(norms, "args", _lib.HeadArgs(_lib.ptr(kept[0]), _lib.ptr(kept[1]), axes=1, eps=eps))
+    return norms
 
 
 def rotary_frequencies(dims: int, *, base: float = 10000.0, scale: float = 1.0, scaling: str | None = None,

@@ -2,12 +2,13 @@
 launch, the axes of a table's pairs."""
 
 import ctypes
+import dataclasses
 
 import pytest
 import torch
 
 from mtplx_amd import _lib
-from mtplx_amd.rotary import _heads, _pair_axes, head_norms, rotary_table
+from mtplx_amd.rotary import HeadNorms, _heads, _pair_axes, head_norms, rotary_table
 from oracle import paged as O
 from tests.test_capi_symbols import HEADER, ROOT, _ctypes_fields, _struct_fields
 from tests.test_paged_abi import _rotary, _write
@@ -83,3 +84,13 @@ def test_norms_keep_a_copy():
                 dict(queries=w, keys=None, eps=float("nan")), dict(queries=w, keys=None, eps=1e39)):
         with pytest.raises(ValueError):
             head_norms(**bad)
+
+
+def test_norms_from_elsewhere_are_refused():
+    """What a call passes holds the weights' addresses: others do not inherit it."""
+    n = head_norms(torch.ones(8), None)
+    t = rotary_table(8, device="cpu")
+    assert _heads(t, n, None, 8, CPU).q_weight == n.queries.data_ptr()
+    for other in (dataclasses.replace(n, eps=0.5), dataclasses.replace(n, queries=torch.ones(8)), HeadNorms(n.queries, None, 1e-6)):
+        with pytest.raises(TypeError):
+            _heads(t, other, None, 8, CPU)
