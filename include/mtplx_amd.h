@@ -667,11 +667,14 @@ int mtp_paged_attn(const mtp_paged_attn_args* args, void* stream);
  * positions 0 .. p, and those below `sinks`. Blocks of 32 positions that no row
  * of a tile sees are not read, and their pages need not exist (a position
  * without a page sets the status only where a block that is read holds it).
- * shared > 0 (window and sinks 0): the first `shared` positions of all requests
- * are the same keys, in the pages of the table's first row; whole blocks of 32
- * of them may be read once for the rows of all requests. The result is
- * mtp_paged_attn's up to the order of sums; a request that begins inside them
- * reads its own keys. */
+ * shared > 0 (window and sinks 0): all requests that begin behind the first
+ * `shared` positions hold the same keys there, in the same pages; whole blocks of
+ * 32 of them may be read once for the rows of all, by the table's row of the first
+ * such request that has tokens. The result is mtp_paged_attn's up to the order of
+ * sums; a request that begins inside them reads its own keys.
+ * Workspace: mtp_paged_attn_scoped_workspace_bytes of the call's sizes (max_rows
+ * as in the arguments, without row_off T / B). At most 2^20 requests times kv
+ * heads and tables of 2^31 - 65 positions. */
 typedef struct mtp_attn_scope {
   int window, sinks, shared;
 } mtp_attn_scope;

@@ -198,6 +198,18 @@ __device__ __forceinline__ int prefix_tokens(const PAttn& p) {
   return n < 0 ? 0 : n < p.T ? n : p.T;
 }
 
+// The request whose pages the prefix is read from: the first that has rows and
+// lies behind it (a free slot of a batch has neither keys nor pages); -1: none.
+__device__ __forceinline__ int prefix_request(const PAttn& p, int lane) {
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    const int b = b0 + lane;
+    const bool has = b < p.B && req_rows(p.row_off, b, p.B, p.T).n > 0 && p.q_start[b] >= p.prefix;
+    const unsigned long long m = __ballot(has);
+    if (m) return b0 + __ffsll((long long)m) - 1;
+  }
+  return -1;
+}
+
 // The prefix is done for a request that lies behind it; one that does not, or
 // whose rows are not among the list's, sees its keys from the first on. (The
 // join adds the prefix to the tiles that were dealt: a request that brings more
@@ -912,9 +924,9 @@ __global__ __launch_bounds__(64 * chunk_waves<D>()) void attn_chunk_kernel(PAttn
   Tile u;
   int ka, kb;
   if constexpr (SC == kPrefix) {
-    b = 0;   // (its pages: the first request's)
+    b = prefix_request(p, lane);
     prefix_piece(p, g, rq, u, ka, kb, kStepKeys);
-    if (u.rows <= 0) return;   // (fewer tokens than the launch was sized for)
+    if (b < 0 || u.rows <= 0) return;   // (nobody reads it; fewer tokens than the launch was sized for)
   } else {
     b = line.find(p, lane, lo, rq);
     u = tile_at<SC>(p, rq, lo);

@@ -16,7 +16,8 @@
 // 635 TFLOP/s of what there is, 760 with the empty half tile; the chunk kernel's
 // 830), the tails 33 (86 MB; 12 us before the first key) and the join 12 (27 MB of
 // partials). Without sharing 345. One row of sixteen requests behind 8192 keys, 16
-// bits: 39 us (98 without), of 15, 18 and 6.5, each mostly the way of its first loads.
+// bits: 40 us (98 without), of 16, 18 and 6.5, each mostly the way of its first loads
+// (1 us of the first launch: which request's pages to read).
 #include "paged_attn.hpp"
 
 namespace mtp {

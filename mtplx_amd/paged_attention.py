@@ -46,11 +46,12 @@ def paged_sdpa(queries: torch.Tensor, cache: PagedKVCache, block_table: Any, q_s
     (``window`` of them), and with ``sinks`` the first so many of its request
     too. What no new token sees is not read: the pages that hold nothing else may
     have been given back (-1 in the table).
-    ``shared``: the first so many positions of all requests are the same keys, in
-    the same pages (the rows of ``block_table`` begin alike; the first one is
-    read). A batch that shares a long prefix then reads it once instead of once
+    ``shared``: all requests that begin behind so many first positions hold the
+    same keys there, in the same pages (their rows of ``block_table`` begin
+    alike). A batch that shares a long prefix then reads it once instead of once
     for each request; the result is the same up to the order of sums. Requests
-    that begin inside it are as without. Not together with a window.
+    that begin inside it, free slots among them, are as without. Not together
+    with a window.
     ``scale`` is positive; default ``1 / sqrt(D)``. Refused inside
     ``exact_verify(True)``: how a row's sums are split depends on the lengths of
     the call's other requests."""
@@ -111,7 +112,7 @@ def _scope(window: int | None, sinks: int, shared: int, covered: int) -> _lib.At
     if shared and window is not None:
         raise ValueError("a window and shared positions do not go together")
     if shared:
-        return _lib.AttnScope(0, 0, shared)
+        return _lib.AttnScope(0, 0, min(shared, 2 ** 31 - 1))
     # (no position of a table reaches 2^31: a longer window hides nothing)
     return None if window is None else _lib.AttnScope(min(window, 2 ** 31 - 1), min(sinks, 2 ** 31 - 1), 0)
 

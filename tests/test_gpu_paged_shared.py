@@ -300,6 +300,41 @@ def test_decode_steps_and_graphs(gpu):
             assert torch.equal(out, w)
 
 
+def test_free_slots(gpu):
+    """Slots of a batch without a request, the first one's among them: no rows, or
+    a row of padding at position 0, and no pages."""
+    rng = np.random.default_rng(15)
+    for bits, B in ((16, 6), (8, 6), (16, 90)):
+        busy = [2, 4, 5] if B == 6 else [70, 71, 89]
+        c, own, shared = batch(rng, 2048, [40, 70, 9], 128, 2, 64, bits)
+        table = torch.full((B, own.shape[1]), -1, dtype=torch.int32, device="cuda")
+        table[busy] = own
+        starts = np.zeros(B, np.int32)
+        starts[busy] = [2087, 2117, 2056]
+        q = rows(rng, B, 8, 128)
+        for padded in (True, False):
+            n = np.ones(B, np.int32) if padded else np.isin(np.arange(B), busy).astype(np.int32)
+            off = np.concatenate([[0], np.cumsum(n)])
+            out = paged_sdpa(q[:off[-1]], c, table, i32(starts), i32(off), max_rows=1, shared=shared)
+            for i, b in enumerate(busy):
+                k, v = stored(c, own, i, int(starts[b]) + 1)
+                r = slice(off[b], off[b] + 1)
+                o, spread, reach = O.attend(num(q[r]), k, v, int(starts[b]))
+                check_rows(num(out[r]), o, attention_bound(o, spread, reach, 128), f"slot {b} of {B}")
+            assert (out[off[:-1][np.isin(np.arange(B), busy, invert=True) & (n > 0)]] == 0).all()
+            assert int(c.status().item()) == int(padded)   # (the padding's own positions have no page)
+            c.status().zero_()
+        # nobody lies behind it
+        starts[:] = 5
+        out = paged_sdpa(q, c, table, i32(starts), shared=shared)
+        assert (out[[b for b in range(B) if b not in busy]] == 0).all()
+        for i, b in enumerate(busy):
+            k, v = stored(c, own, i, 6)
+            o, spread, reach = O.attend(num(q[b:b + 1]), k, v, 5)
+            check_rows(num(out[b:b + 1]), o, attention_bound(o, spread, reach, 128), f"inside, slot {b}")
+        c.status().zero_()
+
+
 def test_views_and_outputs(gpu):
     rng = np.random.default_rng(14)
     for n in (3, 50):
