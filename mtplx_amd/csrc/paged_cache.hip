@@ -129,7 +129,7 @@ __device__ __forceinline__ void turn_heads(const HeadRows& rows, const RotSpec& 
     if (NORM && (isq ? hs.q_weight : hs.k_weight)) {   // (the same for all lanes of a row)
       float sa = mine ? squares8(a) : 0.f;
       const float sb = two ? squares8(b) : 0.f;
-      if (PAIRED && r.dims < D) {   // lane j takes chunk j's (there are lanes enough)
+      if (PAIRED && r.dims < D) {   // lane j takes chunk j's (head_lanes: there are lanes enough)
         const int base = (threadIdx.x & 63) & ~(lanes - 1), j = it;
         const float up = __shfl(sa, base + (j < np ? j : (j - np) & (lanes - 1)), 64);
         const float on = __shfl(sb, base + ((j - np) & (lanes - 1)), 64);
@@ -201,10 +201,14 @@ __device__ __forceinline__ void turn_heads(const HeadRows& rows, const RotSpec& 
   }
 }
 
-// Lanes of a row.
-inline int head_lanes(int D, int dims, int trad) {
+// Lanes of a row: one for each item and, where a norm's sum takes a chunk a lane,
+// for each chunk (items of a head partly turned are fewer: 8 of 12 chunks at 64 of
+// 96 elements).
+inline int head_lanes(int D, int dims, int trad, bool norm) {
+  const int items = rot_items(D, dims, trad);
+  const int least = norm && rot_paired(dims, trad) && dims < D ? D / 8 : items;
   int lanes = 1;
-  while (lanes < rot_items(D, dims, trad)) lanes <<= 1;
+  while (lanes < least) lanes <<= 1;
   return lanes;
 }
 
@@ -988,8 +992,8 @@ static int rotary(const char* who, const mtp_rotary_args* a, const mtp_head_args
     HeadSpec hs;
     if (!head_spec(who, heads, a->dims, hs)) return MTP_ERR_ARG;
     if (!hs.positions) hs.positions = a->positions;
-    const HeadRows rows = {q, k, a->Hq, a->Hkv, a->D, head_lanes(a->D, a->dims, a->traditional)};
     const bool paired = rot_paired(a->dims, a->traditional), norm = hs.q_weight || hs.k_weight;
+    const HeadRows rows = {q, k, a->Hq, a->Hkv, a->D, head_lanes(a->D, a->dims, a->traditional, norm)};
     auto* kernel = paired ? (norm ? heads_kernel<true, true> : heads_kernel<true, false>)
                           : (norm ? heads_kernel<false, true> : heads_kernel<false, false>);
     hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(kNT), 0, (hipStream_t)stream, rows, r, hs, a->T, tokens);
@@ -1038,7 +1042,7 @@ static int paged_write(const char* who, const mtp_paged_write_args* a, const mtp
       return MTP_ERR_ARG;
     }
     if (!head_spec(who, heads, a->dims, p.heads)) return MTP_ERR_ARG;
-    p.lanes = head_lanes(a->D, a->dims, a->traditional);
+    p.lanes = head_lanes(a->D, a->dims, a->traditional, true);
   }
   p.k = (const uint16_t*)a->k;
   p.v = (const uint16_t*)a->v;
