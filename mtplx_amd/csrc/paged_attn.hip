@@ -154,6 +154,7 @@ static int paged_attn(const char* who, const mtp_paged_attn_args* a, const mtp_a
   hipStream_t st = (hipStream_t)stream;
   if (!scope) return launch_scope<kCausal>(who, p, plan, a->D, a->bits, st);
   if (scope->shared > 0) {
+    p.shared = scope->shared;
     p.prefix = prefix;
     p.prefix_o = (const float*)((const unsigned char*)a->ws + own);
     p.prefix_ml = p.prefix_o + pre.slots(a->Hkv) * pre.RT * a->D;

@@ -112,10 +112,11 @@ struct PAttn {
   long long most;      // kWindow: most line that a tile takes
   int splits;          // few rows, kWindow and kTail: most pieces of a tile
   int tiles;           // and tiles of a request's head that are dealt
-  // kPrefix, kTail: keys of the shared prefix (whole blocks), its row tiles of a
-  // kv head, their rows, the pieces that each is cut into by keys; kTail: their
-  // partials, laid out as part_o and part_ml, slot (head, piece, tile).
-  int prefix, prefix_tiles, prefix_rt_log2, prefix_pieces;
+  // kPrefix, kTail: positions that requests which begin behind them share, keys of
+  // the prefix (the whole blocks of these), its row tiles of a kv head, their rows,
+  // the pieces that each is cut into by keys; kTail: their partials, laid out as
+  // part_o and part_ml, slot (head, piece, tile).
+  int shared, prefix, prefix_tiles, prefix_rt_log2, prefix_pieces;
   const float* prefix_o;
   const float* prefix_ml;
   float scale_log2;
@@ -199,23 +200,25 @@ __device__ __forceinline__ int prefix_tokens(const PAttn& p) {
 }
 
 // The request whose pages the prefix is read from: the first that has rows and
-// lies behind it (a free slot of a batch has neither keys nor pages); -1: none.
+// begins behind what is shared (a free slot of a batch has neither keys nor pages,
+// and one that begins inside, if only in the block that is cut, may hold other
+// keys); -1: none.
 __device__ __forceinline__ int prefix_request(const PAttn& p, int lane) {
   for (int b0 = 0; b0 < p.B; b0 += 64) {
     const int b = b0 + lane;
-    const bool has = b < p.B && req_rows(p.row_off, b, p.B, p.T).n > 0 && p.q_start[b] >= p.prefix;
+    const bool has = b < p.B && req_rows(p.row_off, b, p.B, p.T).n > 0 && p.q_start[b] >= p.shared;
     const unsigned long long m = __ballot(has);
     if (m) return b0 + __ffsll((long long)m) - 1;
   }
   return -1;
 }
 
-// The prefix is done for a request that lies behind it; one that does not, or
-// whose rows are not among the list's, sees its keys from the first on. (The
+// The prefix is done for a request that begins behind what is shared; one that does
+// not, or whose rows are not among the list's, sees its keys from the first on. (The
 // join adds the prefix to the tiles that were dealt: a request that brings more
 // rows than were announced does without, too.)
 __device__ __forceinline__ bool behind_prefix(const PAttn& p, const ReqRows& rows, long long start) {
-  return start >= p.prefix && rows.lo + rows.n <= prefix_tokens(p) &&
+  return start >= p.shared && rows.lo + rows.n <= prefix_tokens(p) &&
          (long long)rows.n * p.rep <= (long long)p.tiles << p.rt_log2;
 }
 
