@@ -61,6 +61,18 @@ class HeadNorms:
     eps: float
     args: Any = field(default=None, init=False, repr=False, compare=False)   # what every call with them passes
 
+    def _take_args(self) -> None:
+        object.__setattr__(self, "args", _lib.HeadArgs(_lib.ptr(self.queries), _lib.ptr(self.keys), axes=1, eps=self.eps))
+
+    # A copy's calls pass the addresses of its own weights.
+    def __getstate__(self):
+        return {"queries": self.queries, "keys": self.keys, "eps": self.eps, "args": self.args is not None}
+
+    def __setstate__(self, state) -> None:
+        self.__dict__.update(state, args=None)
+        if state["args"]:
+            self._take_args()
+
 
 def head_norms(queries: torch.Tensor | None, keys: torch.Tensor | None, *, eps: float = 1e-6) -> HeadNorms:
     """:class:`HeadNorms` of weights ``[D]`` (any floating type; a copy in fp32
@@ -81,7 +93,7 @@ def head_norms(queries: torch.Tensor | None, keys: torch.Tensor | None, *, eps: 
     if None not in kept and (kept[0].shape != kept[1].shape or kept[0].device != kept[1].device):
         raise ValueError("the two weights must have one length and device")
     norms = HeadNorms(kept[0], kept[1], eps)
-    object.__setattr__(norms, "args", _lib.HeadArgs(_lib.ptr(kept[0]), _lib.ptr(kept[1]), axes=1, eps=eps))
+    norms._take_args()
     return norms
 
 
