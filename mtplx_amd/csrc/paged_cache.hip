@@ -1082,10 +1082,16 @@ static int paged_write(const char* who, const mtp_paged_write_args* a, const mtp
   const int waves = a->D == 256 ? cache_waves<256>() : cache_waves<128>();
   // A block of rotated K is turned by one wave (a row's angles are computed once
   // for both halves) or, where blocks are few and have many new keys, by eight,
-  // four keys each (a lane per chunk, write_few): written and read back, 512 rows
-  // of 8 heads 21 us by eight and 27 by one, 1000 rows 28 and 29, 2000 38 and 32;
-  // decode rows gain nothing.
-  p.k_parts = a->dims > 0 && units * a->Hkv <= 272 && a->T >= 8 * units ? 8 : 1;
+  // four keys each (a lane per chunk, write_few); decode rows gain nothing. One wave
+  // and eight, by blocks of all heads, replayed, of 1 to 16 heads: head dim 128,
+  // normalised, 17.2 and 8.9 us at 64 blocks, 17.6 and 13 at 220, 18.7 and 16.4 at
+  // 264, 21.6 and 26.4 at 512; rotated alone 9.3 and 6.4 at 158, 9.6 and 10.3 at 252
+  // (8 bits: 10.4 and 11.4 at 240). Head dim 256, normalised, 30 and 14 at 64, 34 and
+  // 35 at 256. Head dim 64, where a row is eight lanes' and few waves are enough:
+  // rotated 7.0 and 6.6 at 160, 6.4 and 7.3 at 240; normalised 11.4 and 8.8 at 128,
+  // 10.7 and 14.7 at 189.
+  const int few = a->D == 64 ? 160 : heads ? 272 : 208;
+  p.k_parts = a->dims > 0 && units * a->Hkv <= few && a->T >= 8 * units ? 8 : 1;
   long long groups = (units * (p.k_parts + 1) * a->Hkv + waves - 1) / waves;
   if (groups > 1 << 20) groups = 1 << 20;
   p.kv_groups = (int)groups;
