@@ -710,10 +710,15 @@ __device__ __forceinline__ void turn_queries(const WriteParams& p, int D, int t0
 }
 
 // The same by a launch of their own: at head dim 256 the writes' workgroups are
-// two waves with 33 KB of LDS, which leaves eight waves a CU to turn long calls'
-// queries (6000 tokens, 24 heads over 4, written and read back: 95 us, 122 in one
-// launch; at head dim 128, four waves, 8192 tokens of 40 over 8 take 92 either way
-// and shorter calls 10 us more).
+// two waves with 33 KB of LDS, which leaves eight waves a CU to turn many queries. In
+// one launch and apart, 16 bits, a quarter turned: 24 heads over 4 31 and 27 us at 1000
+// tokens, 84 and 44 at 2048, 73 and 77 at 2500, 76 and 86 at 4000, 134 and 101 at 6000;
+// 32 over 8 65 and 76 at 1500, 93 and 79 at 2048, 149 and 99 at 4000; 32 over 2 50 and
+// 33 at 1500, 89 and 37 at 2048; few queries a token lose by it: 4 over 1 19 and 20 at
+// 2048 (all turned: 15 and 19), 8 over 8 61 and 67 at 2048, 122 and 136 at 6000, 162
+// and 149 at 8192. (Head dim 128, four waves: 8192 tokens of 40 over 8 take 92 either
+// way and shorter calls 10 us more.)
+constexpr long long kApartRows = 24 * 2048;
 template <bool PAIRED>
 __global__ __launch_bounds__(kNT, 4) void queries_kernel(WriteParams p, int D) {
   __shared__ __attribute__((aligned(16))) float2 cs[2 * kMaxPairs];
@@ -1095,7 +1100,7 @@ static int paged_write(const char* who, const mtp_paged_write_args* a, const mtp
   long long groups = (units * (p.k_parts + 1) * a->Hkv + waves - 1) / waves;
   if (groups > 1 << 20) groups = 1 << 20;
   p.kv_groups = (int)groups;
-  const bool apart = heads && a->q && a->D == 256 && a->T >= 2048;
+  const bool apart = heads && a->q && a->D == 256 && (long long)a->T * a->Hq >= kApartRows;
   if (a->q && !apart) {
     p.q_tokens = rot_tokens(a->T);
     groups += cdiv(a->T, p.q_tokens) < (1 << 20) ? cdiv(a->T, p.q_tokens) : 1 << 20;

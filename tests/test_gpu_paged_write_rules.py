@@ -45,6 +45,6 @@ def test_blocks_of_keys(gpu, D, Hkv, n, bits, normed):
 @pytest.mark.parametrize("T", [2000, 2100])
 @pytest.mark.parametrize("dims,trad", [(64, False), (256, False), (256, True), (24, False)])
 def test_queries_of_wide_heads(gpu, T, dims, trad):
-    """24 heads of 256: 2048 tokens' queries and more have a launch of their own;
+    """24 heads of 256: 48 Ki rows of queries and more have a launch of their own;
     rows behind the last request stay as they are."""
     written(np.random.default_rng(T + dims), [T - 40, 3, 0, 30], [5, 90, 7, 0], 24, 4, 256, 16, dims, True, trad, padded=7)
