@@ -254,7 +254,6 @@ struct WriteParams {
   RotRows q;
   int Hq, q_tokens, kv_groups;   // workgroups [0, kv_groups) write K and V, the others rotate q
   int nb_uniform;                // blocks of each request where row_off is null
-  int k_parts;                   // waves that share a block of K
   HeadSpec heads;                // (kernels with HEADS)
   int lanes;
 };
@@ -493,25 +492,28 @@ __device__ __forceinline__ void write_few(const WriteParams& p, int h, bool isk,
 
 // One unit by one wave, in its own LDS: rows come whole, turn in LDS and leave
 // in the page's order, 16 bytes a lane; keys of a block that is not all new go
-// out element by element (V) or chunk by chunk (K).
-template <int D, int BITS, bool HEADS>
+// out element by element (V) or chunk by chunk (K). PARTS: waves that share a block
+// of K (in the argument instead it cost every write 0.2 to 0.5 us, a decode step's of
+// 8 bits 5.7 instead of 5.2).
+template <int D, int BITS, bool HEADS, int PARTS>
 __device__ __forceinline__ void write_unit(const WriteParams& p, const Unit& w, int h, int part, int lane,
                                            uint16_t* rows) {
-  const bool isk = part < p.k_parts;   // (the part behind K's: V)
+  static_assert(PARTS == 1 || kBlk / PARTS <= 1024 / D, "a share of a block is few keys");
+  const bool isk = part < PARTS;   // (the part behind K's: V)
   constexpr int RS = row16<D>(), NC = D / 16, BS = row8<D>();   // 16-byte loads of a lane
   const long long base = w.blk * kBlk;
   // Keys [klo, khi) of the block are new; token of key kk: first + kk.
   const KeyRange range = block_keys(base, w.start, w.start + w.rows.n);
   int klo = range.lo, khi = range.hi;
-  if (isk && p.k_parts > 1) {   // its share of the block's keys
-    const int n = kBlk / p.k_parts;
+  if (PARTS > 1 && isk) {   // its share of the block's keys
+    constexpr int n = kBlk / PARTS;
     klo = klo > part * n ? klo : part * n;
     khi = khi < (part + 1) * n ? khi : (part + 1) * n;
   }
   if (klo >= khi) return;   // (a request of no rows)
   const long long first = w.rows.lo + (base - w.start);
   u32x4 x[NC];
-  const bool few = khi - klo <= 1024 / D;
+  const bool few = (PARTS > 1 && isk) || khi - klo <= 1024 / D;
   if (!few) {
     const uint16_t* src = isk ? p.k + h * p.k_head : p.v + h * p.v_head;
     const long long st = isk ? p.k_token : p.v_token;
@@ -732,7 +734,7 @@ __global__ __launch_bounds__(kNT, 4) void queries_kernel(WriteParams p, int D) {
   }
 }
 
-template <int D, int BITS, bool HEADS>
+template <int D, int BITS, bool HEADS, int PARTS>
 __global__ __launch_bounds__(64 * cache_waves<D>(), D == 256 ? 1 : 4) void paged_write_kernel(WriteParams p) {
   constexpr int NT = 64 * cache_waves<D>();
   __shared__ __attribute__((aligned(16))) uint16_t lds[cache_waves<D>()][32 * row16<D>()];
@@ -778,9 +780,9 @@ __global__ __launch_bounds__(64 * cache_waves<D>(), D == 256 ? 1 : 4) void paged
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   for (long long x = (long long)blockIdx.x * cache_waves<D>() + wave;; x += (long long)p.kv_groups * cache_waves<D>()) {
     Unit w;
-    const long long v = p.k_parts == 1 ? x >> 1 : div_pos(x, p.k_parts + 1), u = div_pos(v, p.Hkv);
+    const long long v = PARTS == 1 ? x >> 1 : div_pos(x, PARTS + 1), u = div_pos(v, p.Hkv);
     if (!find_unit(p, u, lane, w)) return;   // (no barrier follows)
-    write_unit<D, BITS, HEADS>(p, w, (int)(v - u * p.Hkv), (int)(x - v * (p.k_parts + 1)), fresh(lane), lds[wave]);
+    write_unit<D, BITS, HEADS, PARTS>(p, w, (int)(v - u * p.Hkv), (int)(x - v * (PARTS + 1)), fresh(lane), lds[wave]);
   }
 }
 
@@ -938,13 +940,13 @@ inline int check_rotation(const char* who, const void* table, int dims, int D) {
 // once there is a workgroup for every CU that way, else fewer.
 inline int rot_tokens(int T) { return T >= 8 * 256 ? 8 : T >= 4 * 256 ? 4 : T >= 2 * 256 ? 2 : 1; }
 
+constexpr int kKeyWaves = 8;   // of a block of K, where blocks are few
+
 template <int D, int BITS>
-void launch_write(const WriteParams& p, bool heads, int groups, hipStream_t st) {
-  const dim3 grid((unsigned)groups), block(64 * cache_waves<D>());
-  if (heads)
-    hipLaunchKernelGGL((paged_write_kernel<D, BITS, true>), grid, block, 0, st, p);
-  else
-    hipLaunchKernelGGL((paged_write_kernel<D, BITS, false>), grid, block, 0, st, p);
+void launch_write(const WriteParams& p, bool heads, bool shared, int groups, hipStream_t st) {
+  auto* kernel = heads ? (shared ? paged_write_kernel<D, BITS, true, kKeyWaves> : paged_write_kernel<D, BITS, true, 1>)
+                       : (shared ? paged_write_kernel<D, BITS, false, kKeyWaves> : paged_write_kernel<D, BITS, false, 1>);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(64 * cache_waves<D>()), 0, st, p);
 }
 template <int D, int BITS>
 void launch_read(const ReadParams& p, int groups, hipStream_t st) {
@@ -1088,16 +1090,17 @@ static int paged_write(const char* who, const mtp_paged_write_args* a, const mtp
   // A block of rotated K is turned by one wave (a row's angles are computed once
   // for both halves) or, where blocks are few and have many new keys, by eight,
   // four keys each (a lane per chunk, write_few); decode rows gain nothing. One wave
-  // and eight, by blocks of all heads, replayed, of 1 to 16 heads: head dim 128,
-  // normalised, 17.2 and 8.9 us at 64 blocks, 17.6 and 13 at 220, 18.7 and 16.4 at
-  // 264, 21.6 and 26.4 at 512; rotated alone 9.3 and 6.4 at 158, 9.6 and 10.3 at 252
-  // (8 bits: 10.4 and 11.4 at 240). Head dim 256, normalised, 30 and 14 at 64, 34 and
-  // 35 at 256. Head dim 64, where a row is eight lanes' and few waves are enough:
-  // rotated 7.0 and 6.6 at 160, 6.4 and 7.3 at 240; normalised 11.4 and 8.8 at 128,
-  // 10.7 and 14.7 at 189.
+  // and eight, by blocks of all heads, replayed: head dim 128, normalised, 17.6 and
+  // 8.6 us at 64 blocks, 17.5 and 12.0 at 220, 17.6 and 15.2 at 264, 18.3 and 18.6 at
+  // 384; rotated alone 9.2 and 7.8 at 158, 9.5 and 8.8 at 256, 8 bits 9.8 and 9.0 at
+  // 208 and 9.8 and 10.6 at 240. Head dim 256, normalised, 27 and 13 at 64, 32.5 and
+  // 32.1 at 240, 33 and 36 at 252; rotated 14.1 and 12.2 at 208, 14.3 and 15.5 at 240.
+  // Head dim 64, where a row is eight lanes' and few waves are enough: rotated 6.8 and
+  // 6.3 at 160, 6.2 and 6.8 at 240; normalised 11.5 and 9.2 at 160 and, of one head,
+  // 10.6 and 14.4 at 189.
   const int few = a->D == 64 ? 160 : heads ? 272 : 208;
-  p.k_parts = a->dims > 0 && units * a->Hkv <= few && a->T >= 8 * units ? 8 : 1;
-  long long groups = (units * (p.k_parts + 1) * a->Hkv + waves - 1) / waves;
+  const bool shared = a->dims > 0 && units * a->Hkv <= few && a->T >= 8 * units;
+  long long groups = (units * (shared ? kKeyWaves + 1 : 2) * a->Hkv + waves - 1) / waves;
   if (groups > 1 << 20) groups = 1 << 20;
   p.kv_groups = (int)groups;
   const bool apart = heads && a->q && a->D == 256 && (long long)a->T * a->Hq >= kApartRows;
@@ -1116,12 +1119,12 @@ static int paged_write(const char* who, const mtp_paged_write_args* a, const mtp
   }
   const int key = a->D * 100 + a->bits;
   switch (key) {
-    case 6416: launch_write<64, 16>(p, heads != nullptr, (int)groups, st); break;
-    case 6408: launch_write<64, 8>(p, heads != nullptr, (int)groups, st); break;
-    case 12816: launch_write<128, 16>(p, heads != nullptr, (int)groups, st); break;
-    case 12808: launch_write<128, 8>(p, heads != nullptr, (int)groups, st); break;
-    case 25616: launch_write<256, 16>(p, heads != nullptr, (int)groups, st); break;
-    default: launch_write<256, 8>(p, heads != nullptr, (int)groups, st); break;
+    case 6416: launch_write<64, 16>(p, heads != nullptr, shared, (int)groups, st); break;
+    case 6408: launch_write<64, 8>(p, heads != nullptr, shared, (int)groups, st); break;
+    case 12816: launch_write<128, 16>(p, heads != nullptr, shared, (int)groups, st); break;
+    case 12808: launch_write<128, 8>(p, heads != nullptr, shared, (int)groups, st); break;
+    case 25616: launch_write<256, 16>(p, heads != nullptr, shared, (int)groups, st); break;
+    default: launch_write<256, 8>(p, heads != nullptr, shared, (int)groups, st); break;
   }
   return launch_check(who);
 }
