@@ -70,7 +70,9 @@ def paged_sdpa(queries: torch.Tensor, cache: PagedKVCache, block_table: Any, q_s
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError(f"scale must be positive and finite (got {scale})")
-    scope = _scope(window, sinks, int(shared), width * cache.page_size)
+    scope = None
+    if window is not None or sinks or shared:
+        scope = _scope(window, sinks, int(shared), width * cache.page_size)
     if out is None:
         out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=device)
         ot, oh = Hq * D, D

@@ -161,10 +161,10 @@ class PagedKVCache:
             if rotary.dims > D:
                 raise ValueError(f"the rotary table's {rotary.dims} dims exceed the head dim {D}")
             _on(device, "rotary", rotary.phases)
-        elif norms is not None or positions is not None:
-            raise ValueError("norms and positions come with a rotation: give rotary with them")
         heads = None
-        if rotary is not None:
+        if norms is not None or positions is not None or (rotary is not None and rotary.axes > 1):
+            if rotary is None:
+                raise ValueError("norms and positions come with a rotation: give rotary with them")
             if positions is None and rotary.axes > 1:
                 raise ValueError(f"a table of {rotary.axes} axes needs positions [{rotary.axes}, {T}]")
             pos = None if positions is None else _positions(rotary, positions, T, device)

@@ -215,12 +215,10 @@ def _positions(table: RotaryTable, positions: Any, T: int, device) -> torch.Tens
 
 
 def _heads(table: RotaryTable, norms: HeadNorms | None, positions: torch.Tensor | None, D: int,
-           device) -> _lib.HeadArgs | None:
-    """The argument block of a call with head norms or several axes (None: one
-    without), its weights checked."""
+           device) -> _lib.HeadArgs:
+    """The argument block of a call with head norms, several axes or positions
+    of its own, its weights checked."""
     if norms is None:
-        if table.axes == 1 and positions is None:
-            return None
         a = _lib.HeadArgs(axes=1)
     else:
         if not isinstance(norms, HeadNorms) or norms.args is None:
@@ -318,14 +316,17 @@ def _stream(device) -> int:
     return _raw_stream(device.index) if _raw_stream is not None else _lib.stream_handle(device)
 
 
-def _call(name: str, block: ctypes.Structure, device, *more: ctypes.Structure) -> None:
-    """Run an argument-block entry point on ``device``'s current stream (the
-    kernels of a call go to the current HIP device)."""
-    if torch.cuda.current_device() == device.index:
-        _lib.call(name, ctypes.byref(block), *map(ctypes.byref, more), _stream(device))
-        return
-    with torch.cuda.device(device):
-        _lib.call(name, ctypes.byref(block), *map(ctypes.byref, more), _stream(device))
+def _call(name: str, block: ctypes.Structure, device, more: ctypes.Structure | None = None) -> None:
+    """Run an argument-block entry point, one of a single block or with ``more``,
+    on ``device``'s current stream (the kernels of a call go to the current HIP
+    device)."""
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            _call(name, block, device, more)
+    elif more is None:
+        _lib.call(name, ctypes.byref(block), _stream(device))
+    else:
+        _lib.call(name, ctypes.byref(block), ctypes.byref(more), _stream(device))
 
 
 def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -375,7 +376,9 @@ def apply_rotary(table: RotaryTable, queries: torch.Tensor, keys: torch.Tensor |
         raise ValueError(f"head dim {D} must be a multiple of 8 up to 256 and hold the table's {table.dims} dims")
     pos = _positions(table, positions, T, device)
     _on(device, "table", table.phases)
-    heads = _heads(table, norms, None if table.axes == 1 else pos, D, device)
+    heads = None   # (the plain call pays for no part of it)
+    if norms is not None or table.axes > 1:
+        heads = _heads(table, norms, None if table.axes == 1 else pos, D, device)
     ko = None
     if out is None:
         qo = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=device)
