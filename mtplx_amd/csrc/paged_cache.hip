@@ -1092,13 +1092,14 @@ static int paged_write(const char* who, const mtp_paged_write_args* a, const mtp
   // four keys each (a lane per chunk, write_few); decode rows gain nothing. One wave
   // and eight, by blocks of all heads, replayed: head dim 128, normalised, 17.6 and
   // 8.6 us at 64 blocks, 17.5 and 12.0 at 220, 17.6 and 15.2 at 264, 18.3 and 18.6 at
-  // 384; rotated alone 9.2 and 7.8 at 158, 9.5 and 8.8 at 256, 8 bits 9.8 and 9.0 at
-  // 208 and 9.8 and 10.6 at 240. Head dim 256, normalised, 27 and 13 at 64, 32.5 and
-  // 32.1 at 240, 33 and 36 at 252; rotated 14.1 and 12.2 at 208, 14.3 and 15.5 at 240.
-  // Head dim 64, where a row is eight lanes' and few waves are enough: rotated 6.8 and
-  // 6.3 at 160, 6.2 and 6.8 at 240; normalised 11.5 and 9.2 at 160 and, of one head,
-  // 10.6 and 14.4 at 189.
-  const int few = a->D == 64 ? 160 : heads ? 272 : 208;
+  // 384; rotated, with four query heads a kv head, 9.9 and 8.5 at 136, 10.1 and 7.8 at
+  // 184, 10.3 and 10.8 at 189 of one head. Head dim 256, normalised, 27 and 13 at 64,
+  // 32.5 and 32.1 at 240, 33 and 36 at 252; rotated 14.9 and 14.2 at 136, 15.8 and 16.6
+  // at 184, 16.2 and 17.8 at 208 (the queries wait behind so many workgroups; without
+  // any 14.1 and 12.2). Head dim 64, where a row is eight lanes' and few waves are
+  // enough: rotated 6.8 and 6.5 at 132, 6.2 and 6.8 at 240; normalised 11.5 and 9.2 at
+  // 160 and, of one head, 10.6 and 14.4 at 189.
+  const int few = heads ? (a->D == 64 ? 160 : a->D == 128 ? 272 : 240) : (a->D == 128 ? 184 : 136);
   const bool shared = a->dims > 0 && units * a->Hkv <= few && a->T >= 8 * units;
   long long groups = (units * (shared ? kKeyWaves + 1 : 2) * a->Hkv + waves - 1) / waves;
   if (groups > 1 << 20) groups = 1 << 20;
