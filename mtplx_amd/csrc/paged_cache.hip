@@ -23,6 +23,8 @@
 #include "paged.hpp"
 #include "rotary.hpp"
 
+#include <type_traits>
+
 namespace mtp {
 
 constexpr int kNT = 256;
@@ -561,29 +563,33 @@ __device__ __forceinline__ void write_unit(const WriteParams& p, const Unit& w, 
       inv = norm_factor(s[0] + __shfl_xor(s[0], 32, 64), D, p.heads.eps);
       wave_lds();   // read before it changes
     }
-    for (int x0 = 0; x0 < 32 * np; x0 += 64) {
-      const int x = x0 + lane;
-      const int kk = x / np;
-      const float row_inv = HEADS ? __shfl(inv, kk & 31, 64) : 1.f;   // (by all lanes)
-      if (kk < klo || kk >= khi) continue;
-      const int pos = (int)(base + kk);
-      uint16_t* row = rows + kk * RS;
-      TokenPos at_axes;
-      if constexpr (HEADS) at_axes = token_pos(p.heads, p.T, first + kk, pos);
-      auto angles = [&](int i) {
-        return rot_angle(HEADS ? at_axes.of(pair_axis(p.heads, i)) : pos, p.r.table[i], p.r.gain);
-      };
-      auto store = [&](int d, uint4 v) { *reinterpret_cast<uint4*>(row + d) = v; };
-      const uint16_t* from = inplace ? row : p.k + h * p.k_head + (first + kk) * p.k_token;
-      auto turn = [&](const uint16_t* from) {
+    auto turn = [&](auto here) {   // from the rows in LDS, or from their source
+      constexpr bool HERE = decltype(here)::value;
+      for (int x0 = 0; x0 < 32 * np; x0 += 64) {
+        const int x = x0 + lane;
+        const int kk = x / np;
+        const float row_inv = HEADS ? __shfl(inv, kk & 31, 64) : 1.f;   // (by all lanes)
+        if (kk < klo || kk >= khi) continue;
+        const int pos = (int)(base + kk);
+        uint16_t* row = rows + kk * RS;
+        TokenPos at_axes;
+        if constexpr (HEADS) at_axes = token_pos(p.heads, p.T, first + kk, pos);
+        auto angles = [&](int i) {
+          return rot_angle(HEADS ? at_axes.of(pair_axis(p.heads, i)) : pos, p.r.table[i], p.r.gain);
+        };
+        auto store = [&](int d, uint4 v) { *reinterpret_cast<uint4*>(row + d) = v; };
+        const uint16_t* from = HERE ? row : p.k + h * p.k_head + (first + kk) * p.k_token;
         if constexpr (HEADS)
           rot_item(x % np, from, p.r.dims, p.r.trad, angles, store,
                    factors([&](int d) { return norm ? row_inv * p.heads.k_weight[d] : 1.f; }));
         else
           rot_item(x % np, from, p.r.dims, p.r.trad, angles, store);
-      };
-      if (inplace) turn(row); else turn(from);
-    }
+      }
+    };
+    if (inplace)
+      turn(std::true_type());
+    else
+      turn(std::false_type());
     wave_lds();
   }
   uint32_t q[D / 8];   // 8 bits: the lane's half row
