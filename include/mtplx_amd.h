@@ -552,8 +552,9 @@ int mtp_rotary(const mtp_rotary_args* args, void* stream);
 /* The same with a norm of each head before it turns and positions of several
  * axes (time, height and width of an image's or a video's patches):
  *   x <- w x / sqrt(mean of the head's squares + eps)
- * over all D elements, in fp32; elements past `dims` are normalised and not
- * rotated; all is rounded to bf16 once. q_weight / k_weight (fp32 [D]; NULL:
+ * over all D elements, in fp32 (a head whose squares sum to 2^128 or more comes
+ * out as zeros, as an infinite mean makes it); elements past `dims` are normalised
+ * and not rotated; all is rounded to bf16 once. q_weight / k_weight (fp32 [D]; NULL:
  * these heads are not normalised). positions int32 [axes][T] (axes 1 to 4):
  * pair i turns by positions[a][t] with a the two bits at 2 (i % 32) of
  * axis{i / 32}, which must lie below axes. positions NULL (axes 1):
@@ -578,7 +579,8 @@ int mtp_rotary_heads(const mtp_rotary_args* args, const mtp_head_args* heads, vo
  * (i + 1) * page_size) are in page block_table[b * width + i]; an entry
  * outside [0, num_pages) is no page. Packed tokens: request b's are rows
  * [row_off[b], row_off[b + 1]) (row_off NULL: T / B each), the first at
- * position q_start[b]. Rows of no request are neither read nor written.
+ * position q_start[b]. Rows of no request are not written, and what they hold
+ * changes nothing.
  * `status` (int32 [1], may be NULL) gets bit 0 set where a position has no
  * page; that row is skipped. Device arrays are never trusted with an access:
  * row offsets are clamped to [0, T], pages to the pool.
@@ -671,7 +673,8 @@ int mtp_paged_attn(const mtp_paged_attn_args* args, void* stream);
  * `shared` positions hold the same keys there, in the same pages; whole blocks of
  * 32 of them may be read once for the rows of all, by the table's row of the first
  * such request that has tokens. The result is mtp_paged_attn's up to the order of
- * sums; a request that begins inside them reads its own keys.
+ * sums; a request that begins inside the first `shared` positions, if only behind
+ * their last whole block, reads its own keys.
  * Workspace: mtp_paged_attn_scoped_workspace_bytes of the call's sizes (max_rows
  * as in the arguments, without row_off T / B). At most 2^20 requests times kv
  * heads and tables of 2^31 - 65 positions. */

@@ -21,7 +21,12 @@
 //
 // 8-bit pages: integers are exact in bf16, so K and V enter the products as
 // they are stored and their rows' scales multiply scores and weights in fp32.
-// P is rounded to bf16 (as the values of V are), l sums it before that.
+// P is rounded to bf16 (as the values of V are; times their scale at 8 bits), l
+// sums it before that: a weight is off by up to half a step, 2^-8 of it, each its
+// own way, so a row over many keys by nearly as much as its output's own rounding
+// (relative error against 64 bits 0.0022 where weights of 32 bits give 0.0017; 0.0026
+// and 0.0020 at 8 bits). A P of two bf16 parts would keep it, for half as many matrix
+// instructions again.
 //
 // Work is dealt by keys: every (request, kv head, row tile) is as long as the
 // keys it sees plus a fixed cost, and workgroup g takes the g-th equal share
@@ -56,8 +61,14 @@
 //   head dim 64: the chunk 115 us, the verify rows 76; head dim 256: 1041 (16
 //     bits: registers spill inside the step) and 529 (8 bits), the verify rows 230;
 //   one token over 4k: 17.3 us, of which the two launches' kernels are 12 and 5;
-//   behind a window of 4096 one token at 32k 15 us (kernels 11.7 and 4.2), sixteen
-//     requests' four verify rows 37 (8 bits, 140 MB in 31 us of the first kernel);
+//   behind a window of 4096 one token at 32k 14.8 us replayed (kernels 11.7 and
+//     4.2, of which the keys' bytes are 3.2: a wave has one block of 32 keys, and
+//     positions, queries, block table, keys, the waves' join, the partials and the
+//     second launch's come one after another), sixteen requests' four verify rows 37
+//     (8 bits, 140 MB in 31 us of the first kernel);
+//   two requests of 256 rows behind a window of 2048: 48 and 10 us. 80 tiles over
+//     256 CUs are twelve steps a workgroup, 23 us; the rest is their starts and 54 MB
+//     of partials, which the join reads again (MFMAs 24% of the busy cycles);
 //   a prompt of 8192 behind a window of 1024: 230 us, 700 TFLOP/s of what the
 //     window leaves. A step of 64 keys is 2 us, as in the chunk, and a tile of 18
 //     steps costs about 10 more: its rows' and first keys' way from memory, 1700

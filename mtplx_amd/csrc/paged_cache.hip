@@ -7,10 +7,16 @@
 //   its read back: 11 us (50 MB); eight requests' prefixes: 74 us (349 MB, 4.7);
 //   rotation with head norms of 8192 tokens: 44 us (40 the kernel, 5.0 TB/s: a row
 //     is read once, its factor comes from three exchanges between eight lanes);
-//     by three axes without norms 30 us (32 heads over 4, 151 MB); 2000 tokens of
-//     24 heads over 4 of 256, a quarter of each turned, 19 us (57 MB): a round is
-//     16 bytes a lane, and seven rounds wait one after another; traditional pairs
-//     57 us (twice the lanes for a row, and as many sums and exchanges each);
+//     by three axes without norms 30 us (32 heads over 4, 151 MB); traditional
+//     pairs 57 us (twice the lanes for a row, and as many sums and exchanges each);
+//     halves that are no whole chunks (24 elements) 130 us (an element's partner is
+//     a load of its own);
+//   the same where part of a wide head turns, a quarter of 256, 24 heads over 4:
+//     2000 tokens 19 us (57 MB), 6000 48: vector issue. 29.3 M instructions of 4
+//     cycles are 48 us of the chip's 1024 SIMDs: 44 an element of a lane's, 24 where
+//     the whole head turns (8192 tokens as above, 31 of 40 us). Of a row's 32
+//     lanes four turn two chunks and 24 pass one, and a wave issues both branches
+//     (all of the 256 turned, 6000 tokens take 33 us, 5.2 TB/s);
 //   norms, rotation and write of 8192 tokens, 16 bits: 67 us (235 MB, 3.5 TB/s; a
 //     key's angles are computed for each head's block).
 //

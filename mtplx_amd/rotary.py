@@ -77,7 +77,8 @@ class HeadNorms:
 def head_norms(queries: torch.Tensor | None, keys: torch.Tensor | None, *, eps: float = 1e-6) -> HeadNorms:
     """:class:`HeadNorms` of weights ``[D]`` (any floating type; a copy in fp32
     is kept, so make it again after a change), for :func:`apply_rotary` and
-    ``PagedKVCache.write``: ``w x / sqrt(mean(x^2) + eps)`` over each head."""
+    ``PagedKVCache.write``: ``w x / sqrt(mean(x^2) + eps)`` over each head, in
+    fp32 (a head whose squares sum to 2^128 or more comes out as zeros)."""
     eps = float(eps)
     if not (math.isfinite(eps) and 0.0 <= eps < 3.0e38):
         raise ValueError(f"eps must be finite and not negative (got {eps})")

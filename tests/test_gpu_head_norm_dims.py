@@ -48,3 +48,24 @@ def test_many_tokens_and_axes(gpu, D, dims):
     apply_rotary(t, q, k, i32(pos), norms=head_norms(w, w, eps=1e-5), out=(q, k))
     check(q, want_q, w, 1e-5, pos, t, "q")
     check(k, want_k, w, 1e-5, pos, t, "k")
+
+
+def test_large_rows(gpu):
+    """Squares that sum to nearly 2^128 are as any others; from there on the mean is
+    infinite and the head zeros, its neighbours as they were."""
+    rng = np.random.default_rng(3)
+    D, T = 128, 4
+    x = rows(rng, T, 2, D)
+    x /= x.abs().amax(-1, keepdim=True)
+    x[1] *= 2.0 ** 60
+    x[2, 0] *= 2.0 ** 66
+    x[3] *= 2.0 ** 100
+    w = weight(rng, D)
+    pos = np.arange(T, dtype=np.int32)
+    for dims in (128, 64, 24):
+        t = rotary_table(dims, base=1e6)
+        got = apply_rotary(t, x, x[:, :1], i32(pos), norms=head_norms(w, w, eps=1e-5))
+        check(got[0][:2], x[:2], w, 1e-5, pos[:2], t, "q")
+        check(got[0][2:3, 1:], x[2:3, 1:], w, 1e-5, pos[2:3], t, "beside")
+        check(got[1][:2], x[:2, :1], w, 1e-5, pos[:2], t, "k")
+        assert (got[0][2, 0] == 0).all() and (got[0][3] == 0).all() and (got[1][2:] == 0).all()
