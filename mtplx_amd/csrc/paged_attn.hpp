@@ -272,12 +272,18 @@ struct Line {
     const long long s = W > 0 ? (W - 1) / p.G + 1 : 0;
     S = s > p.min_share ? (s + p.step - 1) & -(long long)p.step : p.min_share;
     if constexpr (SC == kWindow) {
-      // Three tiles a workgroup and more: whole ones, if at most a tenth of the
-      // workgroups' time is lost that way. A tile cut in two starts twice, and its
-      // partials are written and joined.
+      // Whole tiles, if at most a twentieth of the workgroups' time is lost that way: a
+      // tile cut in two starts twice, and its partials are written and joined. Prompts,
+      // cut and whole, by tiles a workgroup and what is lost: 40 heads over 8 of 128,
+      // 8192 rows behind 512 (5, nothing) 179 and 162 us, behind 1024 247 and 228; 16000
+      // behind 1024 (10, 2%) 484 and 475; 5000 (3, 9%) 190 and 197; 12000 behind 4096 (7,
+      // 15%) 998 and 1057; 4000 (3, 39%) 153 and 185. 16 over 4 of 64, 4000 behind 256
+      // (1, 2%) 37 and 23, 8192 behind 512 (2, nothing) 62 and 49, 4000 behind 1024 (1,
+      // 16%) 57 and 62. 24 over 4 of 256, 8192 behind 512 (6, nothing) 568 and 533, 6000
+      // behind 2000 (4, 7%) 1059 and 1102.
       const long long q = div_small(W, p.G * p.most) + 1, row = p.G * p.most;
       const long long whole = (q - 1) * row == W ? q - 1 : q;
-      if (whole >= 3 && 10 * whole * row <= 11 * W) S = whole * p.most;
+      if (whole > 0 && 20 * whole * row <= 21 * W) S = whole * p.most;
     }
     G = W > 0 ? div_small(W - 1, S) + 1 : 0;
   }
