@@ -1005,7 +1005,11 @@ static int rotary(const char* who, const mtp_rotary_args* a, const mtp_head_args
   const RotRows q = {(const uint16_t*)a->q, (uint16_t*)a->q_out, a->q_token, a->q_head, a->qo_token, a->qo_head};
   const RotRows k = {(const uint16_t*)a->k, (uint16_t*)a->k_out, a->k_token, a->k_head, a->ko_token, a->ko_head};
   const RotSpec r = {(const unsigned long long*)a->table, a->dims, a->traditional, a->gain};
-  const int tokens = heads ? (a->T >= 512 ? 2 : 1) : rot_tokens(a->T);
+  // Head rows: one token a workgroup, two from 1536 on. One and two, replayed: 40 heads
+  // over 8 of 128, 6.7 and 7.8 us at 512 tokens, 10.5 and 10.9 at 1280, 12.3 and 11.2 at
+  // 1536, 47 and 43 at 8192; 24 over 4 of 256, a quarter turned, 13.1 and 15.0 at 1024,
+  // 17.6 and 17.4 at 1536, 73 and 67 at 8192. (Four: 11.5 us at 512 of the first, 44 at 8192.)
+  const int tokens = heads ? (a->T >= 1536 ? 2 : 1) : rot_tokens(a->T);
   const int groups = cdiv(a->T, tokens);
   if (heads) {
     HeadSpec hs;

@@ -38,7 +38,7 @@ def test_many_tokens_and_axes(gpu, D, dims):
     """Workgroups of two tokens, more heads than a round takes, in place, and
     positions of three axes."""
     rng = np.random.default_rng(D + dims)
-    T = 601
+    T = 1601
     fused = rows(rng, T, 14 * D)
     q, k = fused[:, :11 * D].view(T, 11, D), fused[:, 11 * D:].view(T, 3, D)
     w = weight(rng, D)
