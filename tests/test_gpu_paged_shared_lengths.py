@@ -5,6 +5,7 @@ in the block that the length cuts."""
 
 import numpy as np
 import pytest
+import torch
 
 from mtplx_amd.paged_attention import paged_sdpa
 from mtplx_amd.paged_kv_cache import PagedKVCache
@@ -61,3 +62,34 @@ def test_requests_that_begin_in_the_cut_block(gpu, shared, starts, n, Hq, H, D, 
         check(cache, table, q, n, lengths, paged_sdpa(q, cache, table, i32(starts), shared=shared), what="equal rows",
               rows_of=lambda m: [0])
     cache.check_status()
+
+
+def test_captured_steps_across_the_cut_block(gpu):
+    """A captured step replayed as batches change under it: who shares is read from the
+    positions, so a slot may hold a request of its own keys in one replay and one that
+    shares in the next."""
+    rng = np.random.default_rng(12)
+    shared, n, Hq, H, D, page = 2050, 2, 8, 2, 128, 64
+    batches = [[2048, 2060, 2100], [2300, 2049, 2050], [2047, 2048, 2049], [2050, 2051, 2100]]
+    made = []
+    for starts in batches:
+        made.append(batch(rng, shared, [*starts, 2300], [n] * 4, D, H, page, 16))   # (the fourth: one width for all)
+    cache = PagedKVCache(made[0][0].num_pages, H, D, page_size=page)
+    table, start, q = made[0][1][:3].clone(), i32(batches[0]), rows(rng, 3 * n, Hq, D)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        out = paged_sdpa(q, cache, table, start, shared=shared)
+    for _ in range(2):
+        for (c, t), starts in zip(made, batches):
+            cache.k_pages.copy_(c.k_pages)
+            cache.v_pages.copy_(c.v_pages)
+            table.copy_(t[:3])
+            start.copy_(i32(starts))
+            q.copy_(rows(rng, 3 * n, Hq, D))
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            check(c, table, q, [n] * 3, [s + n for s in starts], out, what=str(starts))
+            assert torch.equal(out, paged_sdpa(q, c, t[:3].contiguous(), start, shared=shared))
